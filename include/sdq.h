@@ -386,6 +386,126 @@ int sdq_qlinear_host(const sdq_weight* w, const float* A, int64_t M, int64_t K,
  * Row-major output: aq [M,K] int8, as [M] f32 (src/core/qgemm.cpp:82-96). */
 int sdq_act_quant(const float* A, int64_t M, int64_t K, int8_t* aq, float* as, void* stream);
 
+/* The inverse: y[i, k] = aq[i, k] * as[i], one rounding; y [M,K] contiguous. */
+int sdq_dequant(const int8_t* aq, const float* as, int64_t M, int64_t K, float* y, void* stream);
+
+/* sdq_qlinear on rows that are quantized already: Y = epilogue(aq . W as
+ * sdq_qlinear computes it from these codes and scales), for callers that
+ * quantize once and run several Linears on the result. After sdq_act_quant(A)
+ * the same bits as sdq_qlinear(A). aq [M,K] int8 with codes in -127..127, as
+ * [M] f32, both contiguous; Y must not overlap them. Workspace and graph
+ * capture as sdq_qlinear. */
+int sdq_qlinear_codes(const sdq_weight* w, const int8_t* aq, const float* as, int64_t M, int64_t K,
+                      const sdq_epilogue* epi, void* Y, void* stream);
+
+/* Residual addition, root-mean-square norm and int8 codes in one pass:
+ *   h = fl(x + d)                                 (d NULL: h = x)
+ *   y = fl( h / sqrt(mean_k(h^2) + eps) * w )     (w NULL: 1), 64-bit sums and
+ *       products, one rounding to fp32
+ *   aq, as = sdq_act_quant(y), bit for bit
+ * For the Linears that read a normalized copy of a residual stream (pre-norm
+ * layers with RMS norms: a text encoder's; sdq_qlinear_lnmod is the DiT's
+ * layernorm form). x, d and sum have row strides ldx, ldd, ldsum (floats, >= K);
+ * sum (nullable) receives h and may be x or d itself; no other output may
+ * overlap anything. aq [M,K] and as [M] contiguous; w [K]. A row of NaN or
+ * infinities follows the same steps (NaN codes are -127). eps >= 0.
+ * Stream-ordered, no scratch: it can be captured without a call before. No
+ * counterpart in the reference's DiT; its text encoder normalizes this way
+ * (src/model/t5enc.cpp). */
+int sdq_rmsnorm_quant(const float* x, int64_t ldx, const float* d, int64_t ldd, int64_t M,
+                      int64_t K, const float* w, float eps, float* sum, int64_t ldsum, int8_t* aq,
+                      float* as, void* stream);
+
+/* ---- Linears with 4-bit weights ----------------------------------------
+ * Weight-only quantization for the Linears of few rows, which are bound by
+ * reading the weight (the time MLP, the modulation projection, single tokens):
+ *   W[n,k] = scale[n, k / group] * (u[n,k] - zero[n, k / group])
+ *   Y = epilogue(A . W^T (+ bias))
+ * u: 4-bit codes, two to a byte, the even k in the low half; row n starts at byte
+ * n * ceil(K/2). group 32, 64 or 128, G = ceil(K / group) groups a row. scale
+ * [N,G] f32; zero [N,G] bytes 0..15, or NULL: 8 everywhere. The handle owns a
+ * copy in the kernels' layout; the sources may be freed after the call.
+ * N at most 2^20, K at most 2^22, both at least 1.
+ * No counterpart in the reference (its packs hold int8). */
+typedef struct sdq_weight4 sdq_weight4;
+/* From HOST memory. */
+int sdq_weight4_upload(const uint8_t* u, const float* scale, const uint8_t* zero, int64_t N,
+                       int64_t K, int group, void* stream, sdq_weight4** out);
+/* From DEVICE memory. */
+int sdq_weight4_upload_device(const uint8_t* u, const float* scale, const uint8_t* zero, int64_t N,
+                              int64_t K, int group, void* stream, sdq_weight4** out);
+int sdq_weight4_free(sdq_weight4* w);
+int sdq_weight4_dims(const sdq_weight4* w, int64_t* N, int64_t* K, int* group);
+/* A [M,K] and Y [M,N] device pointers, row-major, contiguous; epilogues as
+ * sdq_qlinear except SDQ_EPI_ACC, which has no meaning here. Activations are
+ * not quantized: each row's values enter as 24-bit integers with a power of two
+ * per group, exact int32 sums per group, fp32 sums over the groups (errors of
+ * a few 1e-7 of the row's norm times the weight's). A row that holds a NaN or an infinity
+ * gives NaN. Built for few rows: 1 to 32 read the weight once, more run in
+ * blocks of 32. Y must not overlap A (resid may be Y). Stream-ordered; scratch
+ * from the stream's workspace as sdq_qlinear (none for the fewest rows). */
+int sdq_q4linear(const sdq_weight4* w, const float* A, int64_t M, int64_t K,
+                 const sdq_epilogue* epi, float* Y, void* stream);
+
+/* ---- paged cache of keys and values, int8 ------------------------------
+ * Keys and values that many calls read again: a prompt's context over all
+ * denoising steps, the frames already made for a chunk of new ones. Device
+ * memory of the caller, a pool of pages of page_size tokens:
+ *   k, v   [pages, kv_heads, page_size, 128] int8 codes, 16-byte aligned
+ *   ks, vs [pages, kv_heads, page_size] f32, the scale of each token and head
+ * A value is code * scale; the codes of 128 values are sdq_act_quant's.
+ * page_size: a power of two from 16 to 32768; head_dim 128. */
+typedef struct sdq_kv_cache {
+  int8_t* k;
+  float* ks;
+  int8_t* v;
+  float* vs;
+  int64_t pages;
+  int page_size;
+  int kv_heads;
+} sdq_kv_cache;
+/* A batch of ragged sequences over the pool, device arrays read when the call
+ * runs on the stream. Sequence s holds lens[s] tokens, token p in row
+ * p % page_size of page table[s * max_pages + p / page_size]; rows
+ * [q_start[s], q_start[s+1]) of a call's tensors are its last tokens, row i the
+ * token at position lens[s] - (q_start[s+1] - q_start[s]) + i - q_start[s].
+ * q_start must not fall and starts at 0 or more; rows before q_start[0] and from
+ * q_start[nseq] on belong to no sequence and are left as they are. Lengths past
+ * max_pages * page_size count as that, negative ones as 0. A page id outside the pool names no page: nothing
+ * is written there, its tokens read back as 0 and are not attended to. Rows
+ * whose position is negative have no place: treated the same way. */
+typedef struct sdq_kv_batch {
+  const int32_t* q_start; /* [nseq + 1] */
+  const int32_t* lens;    /* [nseq] */
+  const int32_t* table;   /* [nseq, max_pages] */
+  int nseq;               /* 0 .. 65535 */
+  int64_t max_pages;      /* max_pages * page_size at most 2^30 */
+} sdq_kv_batch;
+/* Quantizes the rows of k and v ([T, kv_heads*128], row strides ldk, ldv in
+ * floats, 16-byte aligned rows) into their sequences' places. lens counts the
+ * new tokens already. Two rows of one call must not share a place (pages may be
+ * shared where they are only read). Stream-ordered, no scratch. */
+int sdq_kv_write(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* k, int64_t ldk,
+                 const float* v, int64_t ldv, int64_t T, void* stream);
+/* Reads the same places back: the values code * scale as fp32. */
+int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t ldk, float* v,
+                int64_t ldv, int64_t T, void* stream);
+/* Attention of each sequence's new tokens over its cached ones (themselves
+ * among them, once written): for row i at position p, head h,
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / (heads/kv_heads)]) v[j, ...]
+ * over j < lens[s], and j <= p where causal != 0. q and out [T, heads*128] with
+ * row strides (16-byte aligned rows), heads a multiple of kv_heads; out must not
+ * overlap q. Rows that see no key get 0. The cached codes enter exactly, q and the
+ * softmax weights as two fp16 parts each (22 bits), fp32 sums and statistics:
+ * errors of about 1e-6 of the values' scale, whatever the scales of keys and
+ * values between 2^-60 and 2^60. Few rows cut the keys into shares joined by a second kernel, their
+ * scratch from the stream's workspace: a capture needs one call of the same shape
+ * before it (SDQ_ERR_INVALID otherwise, the capture stays usable).
+ * Results do not depend on the other sequences' contents, nor on timing. */
+int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
+                     float* out, int64_t ldo, int64_t T, int heads, float scale, int causal,
+                     void* stream);
+
 /* ---- device memory, for host code that reaches HIP only through this ABI */
 #define SDQ_H2D 0
 #define SDQ_D2H 1

@@ -28,6 +28,7 @@
 #include <vector>
 
 #include "sdq_internal.h"
+#include "sdq_kv.h"
 #include "sdq_sdpa_plan.h"
 
 // Scratch memory of sdq_qlinear_noalloc: a file-scope device array, one copy
@@ -42,6 +43,15 @@ struct sdq_weight {
   int64_t N, K, Np, KFp;
   int8_t* frags;  // (Np/32) * KFp * 1024 bytes
   float* scale;   // Np floats, zero padded
+};
+
+struct sdq_weight4 {
+  int device;
+  int64_t N, K;
+  int group;
+  uint8_t* codes;
+  float* scale;
+  int8_t* zero;  // nullptr: 8 everywhere
 };
 
 namespace sdq {
@@ -363,17 +373,24 @@ struct LnMod {
   float eps;
 };
 
+// Rows that are quantized already (sdq_qlinear_codes): row-major codes, scales.
+struct Codes {
+  const int8_t* aq;
+  const float* as;
+};
+
 // Core device-pointer path shared by the entry points. `pre` (nullable):
 // A's row maxima are known; `rmax_out` (nullable, GELU): write Y's; `lnmod`
-// (nullable): quantize mod_rows(layernorm(A)) instead of A.
+// (nullable): quantize mod_rows(layernorm(A)) instead of A. `codes` (nullable):
+// the rows' codes are given, A is not read.
 // `fixed` (nullable): the no-alloc mode, all scratch carved from this
 // device's static scratch array instead of the grown workspace (nothing is
 // allocated; no profiling events are made).
 int qlinear_device(const sdq_weight* w, const float* A, int64_t M, int64_t K,
                    const sdq_epilogue* epi, void* Y, hipStream_t s, const RowMax* pre = nullptr,
                    RowMax* rmax_out = nullptr, const LnMod* lnmod = nullptr,
-                   char* fixed = nullptr) {
-  if (fixed && (pre || rmax_out || lnmod))
+                   char* fixed = nullptr, const Codes* codes = nullptr) {
+  if (fixed && (pre || rmax_out || lnmod || codes))
     return set_error(SDQ_ERR_INVALID, "no-alloc mode covers the plain qlinear only");
   const bool prof = t_prof && !fixed;
   int rc = check_weight(w, K);
@@ -381,7 +398,7 @@ int qlinear_device(const sdq_weight* w, const float* A, int64_t M, int64_t K,
   if ((rc = validate_epi(epi))) return rc;
   if (M < 0) return set_error(SDQ_ERR_INVALID, "negative M");
   if (M == 0 || w->N == 0) return SDQ_OK;
-  if (!A && K > 0) return set_error(SDQ_ERR_INVALID, "null A");
+  if (!A && K > 0 && !codes) return set_error(SDQ_ERR_INVALID, "null A");
   if (!Y) return set_error(SDQ_ERR_INVALID, "null Y");
   if ((rc = ensure_device(w->device))) return rc;
   const int64_t N = w->N;
@@ -391,7 +408,7 @@ int qlinear_device(const sdq_weight* w, const float* A, int64_t M, int64_t K,
                                   g_dev[w->device].cu_count);
   if (lnmod && (!lnmod->shift || !lnmod->scale || K == 0))
     return set_error(SDQ_ERR_INVALID, "layernorm+modulation needs shift, scale and K > 0");
-  if (!lnmod && cfg == kCfgSkinny && qin_fits(M, K, w->KFp) && !std::getenv("SDQ_NO_QIN")) {
+  if (!lnmod && !codes && cfg == kCfgSkinny && qin_fits(M, K, w->KFp) && !std::getenv("SDQ_NO_QIN")) {
     // a few rows: the GEMM quantizes them itself (SDQ_NO_QIN: the two-launch
     // path, for comparisons)
     const EpiArgs ea = make_epi(epi, K);
@@ -479,7 +496,8 @@ int qlinear_device(const sdq_weight* w, const float* A, int64_t M, int64_t K,
 
   hipEvent_t p0 = prof ? prof_mark(s) : nullptr;
   hipError_t e =
-      lnrows ? launch_act_quant_frags_lnmod_rows(A, M, K, Mp, w->KFp, ws->at, ws->as, cc,
+      codes ? launch_codes_frags(codes->aq, codes->as, M, K, Mp, w->KFp, ws->at, ws->as, cc, s)
+      : lnrows ? launch_act_quant_frags_lnmod_rows(A, M, K, Mp, w->KFp, ws->at, ws->as, cc,
                                                  lnmod->shift, lnmod->scale, lnmod->eps, s)
       : lnmod ? launch_act_quant_frags_lnmod(A, M, K, Mp, w->KFp, ws->at, ws->as, cc, lnmod->shift,
                                            lnmod->scale, lnmod->eps, ws->st, s)
@@ -528,7 +546,11 @@ int qlinear_device(const sdq_weight* w, const float* A, int64_t M, int64_t K,
   if (prof) {
     hipEvent_t p2 = prof_mark(s);
     if (p0 && p1 && p2 && (!tail || pmid)) {
-      t_recs.push_back({lnmod ? "ln_mod_quant" : premax ? "act_quant_premax" : "act_quant", p0, p1});
+      t_recs.push_back({lnmod    ? "ln_mod_quant"
+                        : premax ? "act_quant_premax"
+                        : codes  ? "codes_frags"
+                                 : "act_quant",
+                        p0, p1});
       const std::string g = std::string("qgemm_") + gemm_cfg_name(cfg) + (splitk > 1 ? "_splitk" : "");
       if (tail) {
         // the 256x256 launch over the full rounds' rows, then the 128x128
@@ -900,6 +922,82 @@ int64_t host_piece_rows(int64_t M, size_t row_bytes) {
 bool bytes_overlap(const void* a, size_t na, const void* b, size_t nb) {
   const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return a && b && na && nb && x < y + nb && y < x + na;
+}
+
+// One timed launch: a record of its own between sdq_profile_begin / _end.
+template <class F>
+int timed(const char* name, hipStream_t s, F launch) {
+  hipEvent_t p0 = t_prof ? prof_mark(s) : nullptr;
+  const hipError_t e = launch();
+  if (e != hipSuccess) {
+    drop_events({p0});
+    return hip_error(e, name);
+  }
+  if (t_prof) {
+    hipEvent_t p1 = prof_mark(s);
+    if (p0 && p1)
+      t_recs.push_back({name, p0, p1});
+    else
+      drop_events({p0, p1});
+  }
+  return SDQ_OK;
+}
+
+int check_weight4(const uint8_t* u, const float* scale, int64_t N, int64_t K, int group) {
+  if (N < 1 || K < 1 || N > kMaxWeightN || K > kMaxWeightK)
+    return set_error(SDQ_ERR_INVALID, "4-bit weight: N 1 .. 2^20, K 1 .. 2^22 (N=" +
+                                          std::to_string(N) + ", K=" + std::to_string(K) + ")");
+  if (group != 32 && group != 64 && group != 128)
+    return set_error(SDQ_ERR_INVALID, "4-bit weight: group must be 32, 64 or 128");
+  if (!u || !scale) return set_error(SDQ_ERR_INVALID, "null weight data");
+  return SDQ_OK;
+}
+
+// The kernels' view of a cache and a batch, checked.
+int kv_view(const sdq_kv_cache* c, const sdq_kv_batch* b, int64_t T, const std::string& tag,
+            kv::View* out) {
+  if (!c || !b) return set_error(SDQ_ERR_INVALID, tag + ": null cache or batch");
+  int log2 = 0;
+  while (log2 < 15 && (1 << log2) < c->page_size) log2++;
+  if (c->page_size < 16 || c->page_size != 1 << log2)
+    return set_error(SDQ_ERR_INVALID, tag + ": page_size must be a power of two from 16 to 32768");
+  if (c->kv_heads < 1 || c->kv_heads > 65535)
+    return set_error(SDQ_ERR_INVALID, tag + ": kv_heads must be 1 .. 65535");
+  if (c->pages < 0 || c->pages > (int64_t(1) << 31))
+    return set_error(SDQ_ERR_INVALID, tag + ": pages must be 0 .. 2^31");
+  if (T < 0 || T > kMaxRows) return set_error(SDQ_ERR_INVALID, tag + ": T must be 0 .. 2^30 rows");
+  if (b->nseq < 0 || b->nseq > 65535)
+    return set_error(SDQ_ERR_INVALID, tag + ": nseq must be 0 .. 65535");
+  if (b->max_pages < 0 || b->max_pages > (kMaxRows >> log2))
+    return set_error(SDQ_ERR_INVALID, tag + ": max_pages * page_size must be 0 .. 2^30");
+  if (T * 2 * c->kv_heads > (int64_t(1) << 34))
+    return set_error(SDQ_ERR_INVALID, tag + ": T * kv_heads must be at most 2^33");
+  *out = kv::View{c->k,       c->ks,   c->v,     c->vs,   c->pages,     log2, c->kv_heads,
+                  b->q_start, b->lens, b->table, b->nseq, b->max_pages, T};
+  if (b->nseq == 0) out->T = 0;
+  if (out->T == 0) return SDQ_OK;
+  if (c->pages > 0 && (!c->k || !c->ks || !c->v || !c->vs))
+    return set_error(SDQ_ERR_INVALID, tag + ": null cache memory");
+  if (!aligned16(c->k) || !aligned16(c->v))
+    return set_error(SDQ_ERR_INVALID, tag + ": the cache's codes must be 16-byte aligned");
+  if (!b->q_start || !b->lens || (b->max_pages > 0 && !b->table))
+    return set_error(SDQ_ERR_INVALID, tag + ": null batch arrays");
+  return SDQ_OK;
+}
+
+int usable_device(int* dev) {
+  const int rc = current_device(dev);
+  return rc ? rc : ensure_device(*dev);
+}
+
+int kv_rows(const std::string& tag, const char* name, const float* p, int64_t ld, int64_t C) {
+  if (!p) return set_error(SDQ_ERR_INVALID, tag + ": null " + name);
+  if (ld < C || ld > (int64_t(1) << 32))
+    return set_error(SDQ_ERR_INVALID,
+                     tag + ": the row stride of " + name + " must cover its heads * 128");
+  if (!aligned16(p) || ld % 4)
+    return set_error(SDQ_ERR_INVALID, tag + ": " + name + " needs 16-byte aligned rows");
+  return SDQ_OK;
 }
 
 // Host -> device through the first two slots' pinned buffers, on the first
@@ -2058,6 +2156,260 @@ int sdq_act_quant(const float* A, int64_t M, int64_t K, int8_t* aq, float* as, v
   hipError_t e = launch_act_quant_rowmajor(A, M, K, aq, as, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_error(e, "act_quant launch");
   return SDQ_OK;
+}
+
+int sdq_dequant(const int8_t* aq, const float* as, int64_t M, int64_t K, float* y, void* stream) {
+  if (M < 0 || K < 0) return set_error(SDQ_ERR_INVALID, "dequant: negative dims");
+  if (M > kMaxRows || K > kMaxWeightK)
+    return set_error(SDQ_ERR_INVALID, "dequant: at most 2^30 rows of at most 2^22 values");
+  if (M == 0 || K == 0) return SDQ_OK;
+  if (!aq || !as || !y) return set_error(SDQ_ERR_INVALID, "dequant: null pointer");
+  const size_t n = (size_t)(M * K);
+  if (bytes_overlap(y, n * 4, aq, n) || bytes_overlap(y, n * 4, as, (size_t)M * 4))
+    return set_error(SDQ_ERR_INVALID, "dequant: y overlaps an input");
+  int dev = -1;
+  int rc = current_device(&dev);
+  if (rc || (rc = ensure_device(dev))) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return timed("dequant", s, [&] { return launch_dequant(aq, as, M, K, y, s); });
+}
+
+int sdq_qlinear_codes(const sdq_weight* w, const int8_t* aq, const float* as, int64_t M, int64_t K,
+                      const sdq_epilogue* epi, void* Y, void* stream) {
+  if (w && K == w->K && M > 0 && M <= kMaxRows && w->N > 0) {
+    if (!as || (K > 0 && !aq)) return set_error(SDQ_ERR_INVALID, "qlinear_codes: null pointer");
+    const size_t ny = (size_t)M * (size_t)w->N * 4;
+    if (bytes_overlap(Y, ny, aq, (size_t)M * (size_t)K) || bytes_overlap(Y, ny, as, (size_t)M * 4))
+      return set_error(SDQ_ERR_INVALID, "qlinear_codes: Y overlaps an input");
+  }
+  const Codes codes{aq, as};
+  return qlinear_device(w, nullptr, M, K, epi, Y, static_cast<hipStream_t>(stream), nullptr,
+                        nullptr, nullptr, nullptr, &codes);
+}
+
+int sdq_rmsnorm_quant(const float* x, int64_t ldx, const float* d, int64_t ldd, int64_t M,
+                      int64_t K, const float* w, float eps, float* sum, int64_t ldsum, int8_t* aq,
+                      float* as, void* stream) {
+  if (M < 0 || K < 1) return set_error(SDQ_ERR_INVALID, "rmsnorm_quant: negative M or K < 1");
+  if (M > kMaxRows || K > kMaxWeightK)
+    return set_error(SDQ_ERR_INVALID, "rmsnorm_quant: at most 2^30 rows of at most 2^22 values");
+  if (!(eps >= 0.f) || eps > 3.4e38f)
+    return set_error(SDQ_ERR_INVALID, "rmsnorm_quant: eps must be finite and not negative");
+  if (M == 0) return SDQ_OK;
+  if (!x || !aq || !as) return set_error(SDQ_ERR_INVALID, "rmsnorm_quant: null pointer");
+  constexpr int64_t kMaxLd = int64_t(1) << 32;
+  if (ldx < K || (d && ldd < K) || (sum && ldsum < K) || ldx > kMaxLd || (d && ldd > kMaxLd) ||
+      (sum && ldsum > kMaxLd))
+    return set_error(SDQ_ERR_INVALID, "rmsnorm_quant: row strides must cover K (and stay under 2^32)");
+  auto span = [&](int64_t ld) { return (size_t)((M - 1) * ld + K) * 4; };
+  const size_t nx = span(ldx), nd = d ? span(ldd) : 0, ns = sum ? span(ldsum) : 0;
+  const size_t nq = (size_t)M * (size_t)K, na = (size_t)M * 4, nw = (size_t)K * 4;
+  const bool bad_sum =
+      sum && ((bytes_overlap(sum, ns, x, nx) && !(sum == x && ldsum == ldx)) ||
+              (bytes_overlap(sum, ns, d, nd) && !(sum == d && ldsum == ldd)) ||
+              bytes_overlap(sum, ns, w, nw));
+  auto bad_out = [&](const void* p, size_t n) {
+    return bytes_overlap(p, n, x, nx) || bytes_overlap(p, n, d, nd) ||
+           bytes_overlap(p, n, sum, ns) || bytes_overlap(p, n, w, nw);
+  };
+  if (bad_sum || bad_out(aq, nq) || bad_out(as, na) || bytes_overlap(aq, nq, as, na))
+    return set_error(SDQ_ERR_INVALID,
+                     "rmsnorm_quant: an output overlaps another array (sum may be x or d as a whole)");
+  int dev = -1;
+  int rc = current_device(&dev);
+  if (rc || (rc = ensure_device(dev))) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return timed("rmsnorm_quant", s, [&] {
+    return launch_rmsnorm_quant(x, ldx, d, ldd, M, K, w, eps, sum, ldsum, aq, as,
+                                g_dev[dev].cu_count, s);
+  });
+}
+
+// ---- 4-bit weights ----
+
+int sdq_weight4_upload_device(const uint8_t* u, const float* scale, const uint8_t* zero, int64_t N,
+                              int64_t K, int group, void* stream, sdq_weight4** out) {
+  if (!out) return set_error(SDQ_ERR_INVALID, "null out");
+  *out = nullptr;
+  int rc = check_weight4(u, scale, N, K, group);
+  if (rc) return rc;
+  int dev = -1;
+  if ((rc = current_device(&dev)) || (rc = ensure_device(dev))) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (capturing(s))
+    return set_error(SDQ_ERR_INVALID, "a weight cannot be uploaded while the stream captures a graph");
+  sdq_weight4* w = new (std::nothrow) sdq_weight4{dev, N, K, group, nullptr, nullptr, nullptr};
+  if (!w) return set_error(SDQ_ERR_NOMEM, "host allocation failed");
+  const size_t blocks = (size_t)(ceil_div(N, 16) * ceil_div(K, 128));
+  const size_t groups = blocks * (size_t)(128 / group) * 16;
+  hipError_t e = hipMalloc(&w->codes, blocks * 1024);
+  if (e == hipSuccess) e = hipMalloc(&w->scale, groups * 4);
+  if (e == hipSuccess && zero) e = hipMalloc(&w->zero, groups);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    sdq_weight4_free(w);
+    return set_error(SDQ_ERR_NOMEM, "weight allocation of " +
+                                        std::to_string(blocks * 1024 + groups * 5) +
+                                        " bytes failed");
+  }
+  e = launch_w4_repack(u, scale, zero, N, K, group, w->codes, w->scale, w->zero, s);
+  if (e == hipSuccess) e = hipStreamSynchronize(s);
+  if (e != hipSuccess) {
+    sdq_weight4_free(w);
+    return hip_error(e, "4-bit weight repack");
+  }
+  *out = w;
+  return SDQ_OK;
+}
+
+int sdq_weight4_upload(const uint8_t* u, const float* scale, const uint8_t* zero, int64_t N,
+                       int64_t K, int group, void* stream, sdq_weight4** out) {
+  if (!out) return set_error(SDQ_ERR_INVALID, "null out");
+  *out = nullptr;
+  int rc = check_weight4(u, scale, N, K, group);
+  if (rc) return rc;
+  int dev = -1;
+  if ((rc = current_device(&dev)) || (rc = ensure_device(dev))) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (capturing(s))
+    return set_error(SDQ_ERR_INVALID, "a weight cannot be uploaded while the stream captures a graph");
+  const size_t nu = (size_t)N * (size_t)((K + 1) / 2), ng = (size_t)(N * ceil_div(K, group));
+  const size_t at_s = (size_t)round_up((int64_t)nu, 256), at_z = at_s + (size_t)round_up((int64_t)ng * 4, 256);
+  char* tmp = nullptr;
+  hipError_t e = hipMalloc(&tmp, at_z + ng);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    return set_error(SDQ_ERR_NOMEM, "staging allocation of " + std::to_string(at_z + ng) +
+                                        " bytes failed");
+  }
+  e = hipMemcpy(tmp, u, nu, hipMemcpyHostToDevice);
+  if (e == hipSuccess) e = hipMemcpy(tmp + at_s, scale, ng * 4, hipMemcpyHostToDevice);
+  if (e == hipSuccess && zero) e = hipMemcpy(tmp + at_z, zero, ng, hipMemcpyHostToDevice);
+  if (e != hipSuccess)
+    rc = hip_error(e, "4-bit weight copy");
+  else
+    rc = sdq_weight4_upload_device(reinterpret_cast<uint8_t*>(tmp),
+                                   reinterpret_cast<float*>(tmp + at_s),
+                                   zero ? reinterpret_cast<uint8_t*>(tmp + at_z) : nullptr, N, K,
+                                   group, stream, out);
+  (void)hipFree(tmp);
+  return rc;
+}
+
+int sdq_weight4_free(sdq_weight4* w) {
+  if (!w) return SDQ_OK;
+  if (w->codes) (void)hipFree(w->codes);
+  if (w->scale) (void)hipFree(w->scale);
+  if (w->zero) (void)hipFree(w->zero);
+  delete w;
+  return SDQ_OK;
+}
+
+int sdq_weight4_dims(const sdq_weight4* w, int64_t* N, int64_t* K, int* group) {
+  if (!w) return set_error(SDQ_ERR_INVALID, "null weight handle");
+  if (N) *N = w->N;
+  if (K) *K = w->K;
+  if (group) *group = w->group;
+  return SDQ_OK;
+}
+
+int sdq_q4linear(const sdq_weight4* w, const float* A, int64_t M, int64_t K,
+                 const sdq_epilogue* epi, float* Y, void* stream) {
+  if (!w) return set_error(SDQ_ERR_INVALID, "null weight handle");
+  if (K != w->K)
+    return set_error(SDQ_ERR_INVALID, "K mismatch: activations have K=" + std::to_string(K) +
+                                          ", weight has K=" + std::to_string(w->K));
+  int dev = -1;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  if (dev != w->device)
+    return set_error(SDQ_ERR_INVALID, "weight lives on device " + std::to_string(w->device) +
+                                          ", current device is " + std::to_string(dev));
+  if ((rc = validate_epi(epi))) return rc;
+  if (epi && epi->kind == SDQ_EPI_ACC)
+    return set_error(SDQ_ERR_INVALID, "q4linear has no integer accumulators to return");
+  if (M < 0) return set_error(SDQ_ERR_INVALID, "negative M");
+  if (M == 0) return SDQ_OK;
+  if (!A || !Y) return set_error(SDQ_ERR_INVALID, "q4linear: null pointer");
+  if ((rc = check_rows(M, w->N, ""))) return rc;
+  const size_t ny = (size_t)M * (size_t)w->N * 4;
+  const float* resid = epi && (epi->kind == SDQ_EPI_GATED || epi->kind == SDQ_EPI_RESID) ? epi->resid : nullptr;
+  const float* gate = epi && epi->kind == SDQ_EPI_GATED ? epi->gate : nullptr;
+  if (bytes_overlap(Y, ny, A, (size_t)M * (size_t)K * 4) ||
+      (resid != Y && bytes_overlap(Y, ny, resid, ny)) ||
+      bytes_overlap(Y, ny, gate, (size_t)w->N * 4) ||
+      bytes_overlap(Y, ny, epi ? epi->bias : nullptr, (size_t)w->N * 4))
+    return set_error(SDQ_ERR_INVALID, "q4linear: Y overlaps an input (resid may be Y as a whole)");
+  if ((rc = ensure_device(dev))) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const W4View view{w->N, w->K, w->group, w->codes, w->scale, w->zero};
+  const EpiArgs ea = make_epi(epi, K);
+  return timed("q4linear", s, [&] { return launch_w4(view, A, M, ea, Y, s); });
+}
+
+// ---- the paged cache ----
+
+int sdq_kv_write(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* k, int64_t ldk,
+                 const float* v, int64_t ldv, int64_t T, void* stream) {
+  kv::View view;
+  int rc = kv_view(c, b, T, "kv_write", &view);
+  if (rc || view.T == 0) return rc;
+  const int64_t C = (int64_t)c->kv_heads * kv::kHd;
+  if ((rc = kv_rows("kv_write", "k", k, ldk, C)) || (rc = kv_rows("kv_write", "v", v, ldv, C)))
+    return rc;
+  int dev = -1;
+  if ((rc = usable_device(&dev))) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return timed("kv_write", s, [&] { return launch_kv_write(view, k, ldk, v, ldv, s); });
+}
+
+int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t ldk, float* v,
+                int64_t ldv, int64_t T, void* stream) {
+  kv::View view;
+  int rc = kv_view(c, b, T, "kv_read", &view);
+  if (rc || view.T == 0) return rc;
+  const int64_t C = (int64_t)c->kv_heads * kv::kHd;
+  if ((rc = kv_rows("kv_read", "k", k, ldk, C)) || (rc = kv_rows("kv_read", "v", v, ldv, C)))
+    return rc;
+  // k and v may be column blocks of one array: rows apart or side by side
+  if (bytes_overlap(k, (size_t)((T - 1) * ldk + C) * 4, v, (size_t)((T - 1) * ldv + C) * 4)) {
+    const int64_t by = k < v ? v - k : k - v;
+    if (ldk != ldv || by % ldk < C || by % ldk > ldk - C)
+      return set_error(SDQ_ERR_INVALID, "kv_read: k and v overlap");
+  }
+  int dev = -1;
+  if ((rc = usable_device(&dev))) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return timed("kv_read", s, [&] { return launch_kv_read(view, k, ldk, v, ldv, s); });
+}
+
+int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
+                     float* out, int64_t ldo, int64_t T, int heads, float scale, int causal,
+                     void* stream) {
+  kv::View view;
+  int rc = kv_view(c, b, T, "kv_attention", &view);
+  if (rc) return rc;
+  if (heads < 1 || heads > 65535 || heads % c->kv_heads)
+    return set_error(SDQ_ERR_INVALID,
+                     "kv_attention: heads must be a multiple of the cache's kv_heads, at most 65535");
+  if (!(scale >= -3.4e38f && scale <= 3.4e38f))
+    return set_error(SDQ_ERR_INVALID, "kv_attention: scale must be finite");
+  if (view.T == 0) return SDQ_OK;
+  const int64_t C = (int64_t)heads * kv::kHd;
+  if ((rc = kv_rows("kv_attention", "q", q, ldq, C)) ||
+      (rc = kv_rows("kv_attention", "out", out, ldo, C)))
+    return rc;
+  if (bytes_overlap(out, (size_t)((T - 1) * ldo + C) * 4, q, (size_t)((T - 1) * ldq + C) * 4)) {
+    const int64_t by = q < out ? out - q : q - out;
+    if (ldq != ldo || by % ldq < C || by % ldq > ldq - C)
+      return set_error(SDQ_ERR_INVALID, "kv_attention: out overlaps q");
+  }
+  int dev = -1;
+  if ((rc = usable_device(&dev))) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return timed("kv_attention", s, [&] {
+    return launch_kv_attn(view, q, ldq, out, ldo, heads, scale, causal != 0, s);
+  });
 }
 
 int sdq_device_alloc(size_t bytes, void** out) {

@@ -225,6 +225,43 @@ hipError_t launch_repack_weight(const int8_t* q, const float* scale, int64_t N, 
 hipError_t launch_unpack_weight(const int8_t* frags, int64_t N, int64_t K, int64_t KFp,
                                 int8_t* q, hipStream_t s);
 
+// h = x (+ d) with its rows' RMS norm as int8 row codes (sdq_rmsnorm_quant).
+hipError_t launch_rmsnorm_quant(const float* x, int64_t ldx, const float* d, int64_t ldd,
+                                int64_t M, int64_t K, const float* w, float eps, float* sum,
+                                int64_t ldsum, int8_t* aq, float* as, int cu_count,
+                                hipStream_t s);
+// y[i, k] = aq[i, k] * as[i].
+hipError_t launch_dequant(const int8_t* aq, const float* as, int64_t M, int64_t K, float* y,
+                          hipStream_t s);
+// Row-major codes and scales in the place of the quantizer's output: the
+// fragments of Mp rows, as[Mp] and the padded column copies.
+hipError_t launch_codes_frags(const int8_t* aq, const float* as, int64_t M, int64_t K, int64_t Mp,
+                              int64_t KFp, int8_t* at, float* as_out, const ColCopy& cc,
+                              hipStream_t s);
+// 4-bit weights: blocks of 16 outputs, units of 128 values (sdq_w4.hip).
+struct W4View {
+  int64_t N, K;
+  int group;
+  const uint8_t* codes;  // ceil(N/16) * ceil(K/128) * 1024 bytes
+  const float* scale;    // [ceil(N/16)][ceil(K/128) * 128 / group][16]
+  const int8_t* zero;    // the same, zero - 8; nullptr: 0
+};
+hipError_t launch_w4_repack(const uint8_t* u, const float* scale, const uint8_t* zero, int64_t N,
+                            int64_t K, int group, uint8_t* codes, float* scale_out,
+                            int8_t* zero_out, hipStream_t s);
+hipError_t launch_w4(const W4View& w, const float* x, int64_t M, const EpiArgs& epi, float* y,
+                     hipStream_t s);
+// The paged cache (kv::View: sdq_kv.h).
+namespace kv {
+struct View;
+}
+hipError_t launch_kv_write(const kv::View& c, const float* k, int64_t ldk, const float* v,
+                           int64_t ldv, hipStream_t s);
+hipError_t launch_kv_read(const kv::View& c, float* k, int64_t ldk, float* v, int64_t ldv,
+                          hipStream_t s);
+hipError_t launch_kv_attn(const kv::View& c, const float* q, int64_t ldq, float* out, int64_t ldo,
+                          int heads, float scale, int causal, hipStream_t s);
+
 // GEMM tile configurations.
 enum GemmCfg : int {
   kCfgSkinny = 0,   // M <= kSkinnyMaxM: 32-row activation blocks, split-K waves

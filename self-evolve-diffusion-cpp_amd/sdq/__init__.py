@@ -60,6 +60,18 @@ class GemmPlan(ctypes.Structure):
                 ("rows", ctypes.c_int64 * 2)]
 
 
+class KvCacheView(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("vs", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_size", ctypes.c_int),
+                ("kv_heads", ctypes.c_int)]
+
+
+class KvBatchView(ctypes.Structure):
+    _fields_ = [("q_start", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("nseq", ctypes.c_int),
+                ("max_pages", ctypes.c_int64)]
+
+
 class KernelTime(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 48), ("launches", ctypes.c_int),
                 ("total_ms", ctypes.c_double)]
@@ -107,6 +119,26 @@ SIGNATURES = {
                                      ctypes.c_int, _vp, _vp]),
     "sdq_qlinear_host": (ctypes.c_int, [_vp, _vp, _i64, _i64, ctypes.POINTER(Epilogue), _vp]),
     "sdq_act_quant": (ctypes.c_int, [_vp, _i64, _i64, _vp, _vp, _vp]),
+    "sdq_dequant": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _vp]),
+    "sdq_qlinear_codes": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, ctypes.POINTER(Epilogue), _vp,
+                                         _vp]),
+    "sdq_rmsnorm_quant": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, ctypes.c_float, _vp,
+                                         _i64, _vp, _vp, _vp]),
+    "sdq_weight4_upload": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, ctypes.c_int, _vp,
+                                          ctypes.POINTER(_vp)]),
+    "sdq_weight4_upload_device": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, ctypes.c_int, _vp,
+                                                 ctypes.POINTER(_vp)]),
+    "sdq_weight4_free": (ctypes.c_int, [_vp]),
+    "sdq_weight4_dims": (ctypes.c_int, [_vp, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
+                                        ctypes.POINTER(ctypes.c_int)]),
+    "sdq_q4linear": (ctypes.c_int, [_vp, _vp, _i64, _i64, ctypes.POINTER(Epilogue), _vp, _vp]),
+    "sdq_kv_write": (ctypes.c_int, [ctypes.POINTER(KvCacheView), ctypes.POINTER(KvBatchView), _vp,
+                                    _i64, _vp, _i64, _i64, _vp]),
+    "sdq_kv_read": (ctypes.c_int, [ctypes.POINTER(KvCacheView), ctypes.POINTER(KvBatchView), _vp,
+                                   _i64, _vp, _i64, _i64, _vp]),
+    "sdq_kv_attention": (ctypes.c_int, [ctypes.POINTER(KvCacheView), ctypes.POINTER(KvBatchView),
+                                        _vp, _i64, _vp, _i64, _i64, ctypes.c_int, ctypes.c_float,
+                                        ctypes.c_int, _vp]),
     "sdq_device_alloc": (ctypes.c_int, [ctypes.c_size_t, ctypes.POINTER(_vp)]),
     "sdq_device_free": (ctypes.c_int, [_vp]),
     "sdq_memcpy": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, ctypes.c_int, _vp]),
@@ -678,6 +710,225 @@ def act_quant(A, aq, asc, stream=None):
     load_library()
     c.done()
     _check(_lib.sdq_act_quant(pa, M, K, pq, ps, _stream(stream)))
+
+
+def dequant(aq, asc, y, stream=None):
+    """y = aq * asc[:, None]: row codes (act_quant, rmsnorm_quant) back to float32."""
+    c = _Args()
+    pq = c(aq, "aq", "i8", (None, None))
+    M, K = aq.shape
+    ps, py = c(asc, "as", "f32", (M,)), c(y, "y", "f32", (M, K))
+    load_library()
+    c.done()
+    _check(_lib.sdq_dequant(pq, ps, M, K, py, _stream(stream)))
+    return y
+
+
+def qlinear_codes(w: Weight, aq, asc, out, kind="none", bias=None, gate=None, resid=None,
+                  gate_fma=True, stream=None):
+    """qlinear on rows that are quantized already: codes aq [M, K] int8 and their
+    scales asc [M] (act_quant, rmsnorm_quant)."""
+    c = _Args()
+    h = _weight(w)
+    pq = c(aq, "aq", "i8", (None, w.K))
+    M = aq.shape[0]
+    ps = c(asc, "as", "f32", (M,))
+    e = _epilogue_args(c, kind, M, w.N, out, bias, gate, resid, gate_fma)
+    c.done()
+    _check(_lib.sdq_qlinear_codes(h, pq, ps, M, w.K, ctypes.byref(e), _ptr(out), _stream(stream)))
+    return out
+
+
+def rmsnorm_quant(x, aq, asc, w=None, delta=None, sum_out=None, eps=1e-6, stream=None):
+    """h = x + delta, then rmsnorm(h, w, eps) as int8 codes aq [M, K] and row
+    scales asc [M]; sum_out (x or delta itself allowed) receives h. x, delta and
+    sum_out: 2-D, rows may be strided."""
+    c = _Args()
+    px = c(x, "x", "f32", (None, None), contig=False)
+    M, K = x.shape
+    pd = c(delta, "delta", "f32", (M, K), contig=False, optional=True)
+    ph = c(sum_out, "sum_out", "f32", (M, K), contig=False, optional=True)
+    pw = c(w, "w", "f32", (K,), optional=True)
+    pq, ps = c(aq, "aq", "i8", (M, K)), c(asc, "as", "f32", (M,))
+    load_library()
+    c.done()
+    ld = lambda t: 0 if t is None else _ld(t)  # noqa: E731
+    _check(_lib.sdq_rmsnorm_quant(px, _ld(x), pd, ld(delta), M, K, pw, eps, ph, ld(sum_out), pq, ps,
+                                  _stream(stream)))
+    return aq, asc
+
+
+class Weight4:
+    """Device copy of a weight in 4-bit codes with group scales (and zero
+    points) in the layout of sdq_q4linear. u: uint8 [N, ceil(K/2)], the even k in
+    a byte's low half; scale float32 [N, ceil(K/group)]; zero uint8 of the same
+    shape, or None: 8 everywhere."""
+
+    def __init__(self, handle, N, K, group):
+        self.h = handle
+        self.N, self.K, self.group = int(N), int(K), int(group)
+
+    @staticmethod
+    def _shape(u, k, group):
+        if group not in (32, 64, 128):
+            raise _bad(f"group: {group}, expected 32, 64 or 128")
+        if len(u.shape) != 2:
+            raise _bad(f"u: shape {tuple(u.shape)}, expected (N, ceil(K/2))")
+        N = int(u.shape[0])
+        K = 2 * int(u.shape[1]) if k is None else int(k)
+        if K < 1 or (K + 1) // 2 != u.shape[1]:
+            raise _bad(f"k: {K} values do not take {u.shape[1]} bytes a row")
+        return N, K, -(-K // group)
+
+    @classmethod
+    def from_host(cls, u, scale, zero=None, k=None, group=128, stream=None):
+        """numpy arrays; k: the row length where it is odd (default: 2 per byte)."""
+        u = np.ascontiguousarray(u, np.uint8)
+        N, K, G = cls._shape(u, k, group)
+        scale = np.ascontiguousarray(scale, np.float32)
+        zero = None if zero is None else np.ascontiguousarray(zero, np.uint8)
+        for name, a in (("scale", scale), ("zero", zero)):
+            if a is not None and a.shape != (N, G):
+                raise _bad(f"{name}: shape {a.shape}, expected {(N, G)}")
+        lib = load_library()
+        h = ctypes.c_void_p()
+        _check(lib.sdq_weight4_upload(_ptr(u), _ptr(scale), _ptr(zero), N, K, group,
+                                      _stream(stream) if stream is not None else None,
+                                      ctypes.byref(h)))
+        return cls(h, N, K, group)
+
+    @classmethod
+    def from_device(cls, u, scale, zero=None, k=None, group=128, stream=None):
+        """Device tensors; they may be freed after the call."""
+        c = _Args()
+        pu = c(u, "u", "u8", (None, None))
+        N, K, G = cls._shape(u, k, group)
+        ps = c(scale, "scale", "f32", (N, G))
+        pz = c(zero, "zero", "u8", (N, G), optional=True)
+        lib = load_library()
+        c.done()
+        h = ctypes.c_void_p()
+        _check(lib.sdq_weight4_upload_device(pu, ps, pz, N, K, group, _stream(stream),
+                                             ctypes.byref(h)))
+        return cls(h, N, K, group)
+
+    def free(self):
+        if self.h is not None and self.h.value:
+            _lib.sdq_weight4_free(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:  # pragma: no cover - interpreter shutdown
+            pass
+
+
+def q4linear(w: Weight4, A, out, kind="none", bias=None, gate=None, resid=None, gate_fma=True,
+             stream=None):
+    """out = epilogue(A . W^T + bias) with 4-bit weights (sdq_q4linear): A [M, K],
+    out [M, N] float32, kinds none, gelu, gated and resid as qlinear's."""
+    if not isinstance(w, Weight4) or w.h is None or not w.h.value:
+        raise _bad("w: not a live Weight4")
+    c = _Args()
+    pa = c(A, "A", "f32", (None, w.K))
+    M = A.shape[0]
+    e = _epilogue_args(c, kind, M, w.N, out, bias, gate, resid, gate_fma)
+    c.done()
+    _check(_lib.sdq_q4linear(w.h, pa, M, w.K, ctypes.byref(e), _ptr(out), _stream(stream)))
+    return out
+
+
+class KvCache:
+    """A pool of pages of int8 keys and values (sdq_kv_cache): device tensors k, v
+    int8 [pages, kv_heads, page_size, 128] and their scales ks, vs float32
+    [pages, kv_heads, page_size], all contiguous."""
+
+    def __init__(self, k, ks, v, vs):
+        if k.dim() != 4 or k.shape[3] != 128:
+            raise _bad(f"k: shape {tuple(k.shape)}, expected (pages, kv_heads, page_size, 128)")
+        self.pages, self.kv_heads, self.page_size = (int(n) for n in k.shape[:3])
+        if self.page_size not in (1 << i for i in range(4, 16)):
+            raise _bad(f"page_size: {self.page_size}, expected a power of two from 16 to 32768")
+        self.k, self.ks, self.v, self.vs = k, ks, v, vs
+
+    @classmethod
+    def empty(cls, pages, page_size, kv_heads, device="cuda"):
+        """A zeroed pool on `device`."""
+        import torch
+
+        shape = (pages, kv_heads, page_size)
+        return cls(torch.zeros(shape + (128,), dtype=torch.int8, device=device),
+                   torch.zeros(shape, device=device),
+                   torch.zeros(shape + (128,), dtype=torch.int8, device=device),
+                   torch.zeros(shape, device=device))
+
+    def _view(self, c):
+        shape = (self.pages, self.kv_heads, self.page_size)
+        return KvCacheView(c(self.k, "cache.k", "i8", shape + (128,)).value,
+                           c(self.ks, "cache.ks", "f32", shape).value,
+                           c(self.v, "cache.v", "i8", shape + (128,)).value,
+                           c(self.vs, "cache.vs", "f32", shape).value,
+                           self.pages, self.page_size, self.kv_heads)
+
+
+class KvBatch:
+    """A batch of ragged sequences over a KvCache (sdq_kv_batch): int32 device
+    tensors q_start [nseq + 1] (rows of a call's tensors), lens [nseq] (tokens the
+    cache holds, new ones counted) and table [nseq, max_pages] (page ids)."""
+
+    def __init__(self, q_start, lens, table):
+        self.q_start, self.lens, self.table = q_start, lens, table
+
+    def _view(self, c):
+        pt = c(self.table, "table", "i32", (None, None))
+        nseq, most = (int(n) for n in self.table.shape)
+        return KvBatchView(c(self.q_start, "q_start", "i32", (nseq + 1,)).value,
+                           c(self.lens, "lens", "i32", (nseq,)).value, pt.value, nseq, most)
+
+
+def _kv_args(cache, batch, rows, heads):
+    """The checked views of a paged call, and the addresses of its row tensors
+    ((name, tensor) pairs of heads * 128 columns, rows may be strided)."""
+    if not isinstance(cache, KvCache) or not isinstance(batch, KvBatch):
+        raise _bad("expected a KvCache and a KvBatch")
+    c = _Args()
+    vc, vb = cache._view(c), batch._view(c)
+    T = None
+    ptrs = []
+    for name, t in rows:
+        p = c(t, name, "f32", (T, heads * 128), contig=False)
+        T = t.shape[0]
+        ptrs += [p, _ld(t)]
+    c.done()
+    load_library()
+    return vc, vb, ptrs, T
+
+
+def kv_write(cache: KvCache, batch: KvBatch, k, v, stream=None):
+    """Quantizes the rows of k and v [T, kv_heads*128] into the last places of
+    their sequences (sdq_kv_write); rows may be strided."""
+    vc, vb, p, T = _kv_args(cache, batch, (("k", k), ("v", v)), cache.kv_heads)
+    _check(_lib.sdq_kv_write(ctypes.byref(vc), ctypes.byref(vb), *p, T, _stream(stream)))
+
+
+def kv_read(cache: KvCache, batch: KvBatch, k, v, stream=None):
+    """Reads the same places back into k and v (sdq_kv_read)."""
+    vc, vb, p, T = _kv_args(cache, batch, (("k", k), ("v", v)), cache.kv_heads)
+    _check(_lib.sdq_kv_read(ctypes.byref(vc), ctypes.byref(vb), *p, T, _stream(stream)))
+    return k, v
+
+
+def kv_attention(cache: KvCache, batch: KvBatch, q, out, heads, causal=True, scale=None,
+                 stream=None):
+    """out = attention of the batch's new tokens over the cache
+    (sdq_kv_attention): q and out [T, heads*128], rows may be strided; scale
+    defaults to 1/sqrt(128). Rows of no sequence are left as they are."""
+    vc, vb, p, T = _kv_args(cache, batch, (("q", q), ("out", out)), int(heads))
+    scale = 128 ** -0.5 if scale is None else float(scale)
+    _check(_lib.sdq_kv_attention(ctypes.byref(vc), ctypes.byref(vb), *p, T, int(heads), scale,
+                                 1 if causal else 0, _stream(stream)))
+    return out
 
 
 def qlinear_plan(w: Weight, M: int, kind="none") -> list:

@@ -1,0 +1,451 @@
+"""The paged int8 cache: sdq_kv_write / sdq_kv_read against the quantizer's steps
+(exact), sdq_kv_attention against the softmax in 64 bits over the values that the
+cache holds.
+
+Attention's tolerance, per row, from its arithmetic: a logit (in units of log2)
+is off by the q parts' 2^-22 and 136 fp32 roundings of the sum of |q k| products,
+plus two roundings of itself and of the running maximum; a weight by its logit's
+error times ln 2, exp2's 2^-22 and the parts' 2^-21; the sums over n keys by
+(n / 8 + 64) 2^-24. Numerator and denominator each, so twice that, of max |v|."""
+import numpy as np
+import pytest
+
+from conftest import assert_bitexact
+from test_gpu_rmsnorm_quant import codes_of
+
+pytestmark = pytest.mark.gpu
+
+F = np.float32
+HD = 128
+
+
+class Case:
+    """A pool of shuffled pages and a ragged batch over it, host and device."""
+
+    def __init__(self, dev, new, lens, kv_heads, page, seed=0, extra=2, first=0, behind=0,
+                 kscale=0.012, vscale=0.02):
+        import torch
+
+        import sdq
+
+        rng = np.random.default_rng(seed)
+        self.new, self.lens, self.kvh, self.page = list(new), list(lens), kv_heads, page
+        need = [-(-max(n, 0) // page) for n in lens]
+        self.pages = sum(need) + extra
+        ids = rng.permutation(self.pages).astype(np.int32)
+        self.most = max(need + [1])
+        self.table = np.full((len(lens), self.most), -1, np.int32)
+        at = 0
+        for s, n in enumerate(need):
+            self.table[s, :n] = ids[at:at + n]
+            at += n
+        self.free = ids[at:]
+        shape = (self.pages, kv_heads, page)
+        self.k = rng.integers(-127, 128, shape + (HD,)).astype(np.int8)
+        self.v = rng.integers(-127, 128, shape + (HD,)).astype(np.int8)
+        self.ks = (kscale * rng.uniform(0.5, 1.5, shape)).astype(F)
+        self.vs = (vscale * rng.uniform(0.5, 1.5, shape)).astype(F)
+        self.start = first + np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        self.T = int(self.start[-1]) + behind
+        self.dev, self.rng = dev, rng
+        self.sdq, self.torch = sdq, torch
+        self.up()
+
+    def t(self, a):
+        return self.torch.from_numpy(np.ascontiguousarray(a)).to(self.dev)
+
+    def up(self):
+        self.cache = self.sdq.KvCache(self.t(self.k), self.t(self.ks), self.t(self.v),
+                                      self.t(self.vs))
+        self.batch = self.sdq.KvBatch(self.t(self.start), self.t(np.array(self.lens, np.int32)),
+                                      self.t(self.table))
+
+    def values(self, s, h):
+        """K and V of sequence s, head h in 64 bits, and which tokens have a page."""
+        p = np.arange(max(0, min(self.lens[s], self.most * self.page)))
+        page = self.table[s, p // self.page]
+        ok = (page >= 0) & (page < self.pages)
+        at = np.where(ok, page, 0), h, p % self.page
+        f = lambda c, sc: c[at].astype(np.float64) * sc[at].astype(np.float64)[:, None]  # noqa: E731
+        with np.errstate(invalid="ignore"):
+            return f(self.k, self.ks), f(self.v, self.vs), ok
+
+    def attend(self, q, heads, scale, causal, fill=0.0):
+        """The definition in 64 bits, and the tolerance of each row and head."""
+        out = np.full((self.T, heads * HD), fill)
+        tol = np.zeros((self.T, heads * HD))
+        G = heads // self.kvh
+        for s, n in enumerate(self.new):
+            L = max(0, min(self.lens[s], self.most * self.page))
+            pos = L - n + np.arange(n)
+            for h in range(heads):
+                k, v, ok = self.values(s, h // G)
+                x = q[self.start[s]:self.start[s + 1], h * HD:(h + 1) * HD].astype(np.float64)
+                t = x @ k.T * scale
+                size = np.abs(x) @ np.abs(k).T * abs(scale)
+                see = ok[None] & (pos[:, None] >= 0) & np.ones((n, len(k)), bool)
+                if causal:
+                    see &= np.arange(len(k))[None] <= pos[:, None]
+                t = np.where(see, t, -np.inf)
+                top = t.max(1, initial=-np.inf, keepdims=True)
+                w = np.exp(t - np.where(np.isinf(top), 0, top)) * see
+                z = w.sum(1, keepdims=True)
+                w = w / np.where(z == 0, 1, z)
+                rows = slice(self.start[s], self.start[s + 1]), slice(h * HD, (h + 1) * HD)
+                out[rows] = w @ np.where(ok[:, None], v, 0)
+                # of a key far below the maximum the weight itself bounds the error
+                err = ((2.0**-22 + 136 * 2.0**-24) * size + 2.0**-21 * np.abs(np.where(see, t, 0))
+                       + 2.0**-21 * np.abs(np.where(np.isinf(top), 0, top)))
+                rel = (w * (err + 2.0**-20)).sum(1, keepdims=True) + (len(k) / 8 + 64) * 2.0**-24
+                tol[rows] = 2 * rel * np.abs(v[ok]).max(initial=0)
+        return out, tol
+
+    def check(self, heads, causal, scale=None, q=None, fill=-3.0, slack=1.0):
+        q = self.rng.standard_normal((self.T, heads * HD)).astype(F) * F(1.5) if q is None else q
+        out = self.torch.full((self.T, heads * HD), fill, device=self.dev)
+        self.sdq.kv_attention(self.cache, self.batch, self.t(q), out, heads, causal=causal,
+                              scale=scale)
+        got = out.cpu().numpy()
+        want, tol = self.attend(q, heads, HD**-0.5 if scale is None else scale, causal, fill)
+        bad = ~(np.abs(got - want) <= tol * slack)
+        assert not bad.any(), (np.argwhere(bad)[:3], got[bad][:3], want[bad][:3], tol[bad][:3])
+        return got
+
+
+# ---- writes and reads ----
+
+@pytest.mark.parametrize("new,lens,kvh,page", [
+    ([1], [1], 1, 16), ([1, 1, 1], [40, 1, 17], 3, 16), ([5, 0, 33, 1], [5, 9, 70, 256], 2, 32),
+    ([300], [300], 24, 256), ([17, 16, 15], [17, 48, 1000], 5, 64)])
+@pytest.mark.parametrize("strided", [False, True])
+def test_write_and_read(sdq_dev, new, lens, kvh, page, strided):
+    import torch
+
+    c = Case(sdq_dev, new, lens, kvh, page, first=2, behind=3)
+    C = kvh * HD
+    kv = c.rng.standard_normal((c.T, 2 * C)).astype(F) * 3
+    kv[0, :HD] = 0
+    kv[2, 5] = np.nan
+    kv[3 if c.T > 3 else 2, C + 7] = np.inf
+    kv[2 + sum(new) - 1, C:C + HD] = 0
+    t = c.t(kv)
+    k, v = (t[:, :C], t[:, C:]) if strided else (t[:, :C].contiguous(), t[:, C:].contiguous())
+    before = [a.copy() for a in (c.k, c.ks, c.v, c.vs)]
+    c.sdq.kv_write(c.cache, c.batch, k, v)
+    want = before
+    for s, n in enumerate(new):
+        for i in range(n):
+            p = lens[s] - n + i
+            at = c.table[s, p // page], slice(None), p % page
+            for x, codes, scales in ((kv[c.start[s] + i, :C], want[0], want[1]),
+                                     (kv[c.start[s] + i, C:], want[2], want[3])):
+                codes[at], scales[at] = codes_of(x.reshape(kvh, HD))
+    for got, w, name in zip((c.cache.k, c.cache.ks, c.cache.v, c.cache.vs), want,
+                            ("k", "ks", "v", "vs")):
+        assert_bitexact(got.cpu().numpy(), w, name)  # the whole pool: nothing else moved
+    o = torch.full((c.T, 2 * C), -9.0, device=sdq_dev)
+    c.sdq.kv_read(c.cache, c.batch, o[:, :C], o[:, C:])
+    got = o.cpu().numpy()
+    assert (got[:2] == -9).all() and (got[2 + sum(new):] == -9).all()
+    for s, n in enumerate(new):
+        for i in range(n):
+            p = lens[s] - n + i
+            at = c.table[s, p // page], slice(None), p % page
+            with np.errstate(invalid="ignore"):
+                y = np.concatenate([(want[0][at] * want[1][at][:, None]).ravel(),
+                                    (want[2][at] * want[3][at][:, None]).ravel()])
+            np.testing.assert_array_equal(got[c.start[s] + i], y)
+
+
+def test_rows_without_a_place(sdq_dev):
+    """Page ids outside the pool, lengths past the table and below the rows: nothing
+    is written there, reads give 0, and attention leaves the tokens out."""
+    import torch
+
+    c = Case(sdq_dev, [4, 6, 3], [40, 4, 30], 2, 16, behind=1)
+    c.table[0, 2] = c.pages  # tokens 32..39 of the first sequence have no page
+    c.table[2, 1] = -7
+    c.up()
+    x = c.t(c.rng.standard_normal((c.T, 256)).astype(F))
+    pool = [a.clone() for a in (c.cache.k, c.cache.v, c.cache.ks, c.cache.vs)]
+    c.sdq.kv_write(c.cache, c.batch, x, x)
+    k, v = torch.full((c.T, 256), 5.0, device=sdq_dev), torch.full((c.T, 256), 5.0, device=sdq_dev)
+    c.sdq.kv_read(c.cache, c.batch, k, v)
+    rows = k.cpu().numpy()
+    assert (rows[:4] == 0).all() and (rows[4:6] == 0).all() and (rows[6:10] != 0).any(1).all()
+    assert (rows[10:13] == 0).all() and (rows[13] == 5).all()
+    for a, b in zip(pool, (c.cache.k, c.cache.v, c.cache.ks, c.cache.vs)):
+        a[c.table[1, 0]] = b[c.table[1, 0]]
+        assert torch.equal(a, b)
+    c.k, c.v = c.cache.k.cpu().numpy(), c.cache.v.cpu().numpy()
+    c.ks, c.vs = c.cache.ks.cpu().numpy(), c.cache.vs.cpu().numpy()
+    for causal in (False, True):
+        c.check(4, causal)
+    c.lens[0] = 10**6  # past the table: as long as the table
+    c.up()
+    c.check(2, True)
+
+
+# ---- attention ----
+
+@pytest.mark.parametrize("lens", [[1], [2], [15], [16], [17], [31], [33], [64], [65], [127], [500],
+                                  [1025], [4099], [3, 0, 700, 64, 1, 129, 0, 2050]])
+@pytest.mark.parametrize("heads,kvh", [(1, 1), (6, 2), (8, 1), (20, 1), (3, 3)])
+def test_single_tokens(sdq_dev, lens, heads, kvh):
+    c = Case(sdq_dev, [1] * len(lens), lens, kvh, 16 if len(lens) > 1 else 64, seed=len(lens))
+    c.check(heads, True)
+
+
+@pytest.mark.parametrize("new,lens", [([2], [2]), ([16], [16]), ([17], [40]), ([33], [100]),
+                                      ([64], [64]), ([65], [1000]), ([130], [131]), ([257], [700]),
+                                      ([5, 40, 0, 100], [5, 300, 50, 99]), ([300, 7], [300, 2000]),
+                                      ([31, 1, 128, 2], [0, 1, 500, 77])])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kvh", [(2, 2), (4, 1), (5, 1)])
+def test_chunks(sdq_dev, new, lens, causal, heads, kvh):
+    """Ragged chunks; new tokens beyond the cache's length (rows without a
+    position: 0) and empty sequences among them."""
+    c = Case(sdq_dev, new, lens, kvh, (16, 32, 128)[len(new) % 3], seed=sum(new), first=1, behind=2)
+    c.check(heads, causal)
+
+
+@pytest.mark.parametrize("new,L,heads,kvh", [(1, 30011, 4, 1), (1, 9000, 3, 3), (40, 20000, 2, 1),
+                                             (700, 5000, 2, 2)])
+def test_long(sdq_dev, new, L, heads, kvh):
+    c = Case(sdq_dev, [new], [L], kvh, 256, seed=7)
+    c.check(heads, True)
+    c.check(heads, False)
+
+
+@pytest.mark.parametrize("new", [1, 40, 300])
+def test_scale_and_strides(sdq_dev, new):
+    import torch
+
+    c = Case(sdq_dev, [new], [333], 2, 32, seed=3)
+    c.check(4, True, scale=0.3)
+    c.check(4, False, scale=-0.05)
+    c.check(4, True, scale=0.0)
+    # columns of wider rows, in and out; the columns beside them stay
+    wide = torch.full((new, 1536), -2.0, device=sdq_dev)
+    q = c.rng.standard_normal((new, 512)).astype(F)
+    wide[:, 256:768] = c.t(q)
+    c.sdq.kv_attention(c.cache, c.batch, wide[:, 256:768], wide[:, 896:1408], 4, causal=True)
+    want, tol = c.attend(q, 4, HD**-0.5, True)
+    got = wide.cpu().numpy()
+    assert (np.abs(got[:, 896:1408] - want) <= tol).all()
+    assert (got[:, :256] == -2).all() and (got[:, 768:896] == -2).all() and (got[:, 1408:] == -2).all()
+    assert_bitexact(got[:, 256:768], q, "q")
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_sharp_and_far_apart(sdq_dev, new):
+    """Logits of hundreds; scales of keys and values far apart, weights the other
+    way round, so that small values of heavy keys stand beside large ones of light
+    keys: each output to its own scale."""
+    c = Case(sdq_dev, [new], [600], 1, 64, seed=4, kscale=0.4)
+    c.check(2, True)
+    c = Case(sdq_dev, [new], [600], 1, 64, seed=5)
+    p = c.table[0, np.arange(600) // 64], 0, np.arange(600) % 64
+    heavy = np.arange(600) % 50 == 3
+    c.vs[p] = np.where(heavy, F(2.0**-24), F(1.0))
+    c.ks[p] = np.where(heavy, F(0.02), F(1e-6))
+    q = np.zeros((new, HD), F)
+    k0 = c.k[p][3].astype(F)
+    q[:] = k0 / np.linalg.norm(k0) * 60
+    for i in np.arange(600)[heavy]:
+        c.k[c.table[0, i // 64], 0, i % 64] = c.k[p][3]
+    c.up()
+    c.check(1, False, q=q)
+    c.vs[p] = F(2.0) ** c.rng.integers(-40, 40, 600)
+    c.ks[p] = F(0.05) * F(2.0) ** c.rng.integers(-20, 2, 600)
+    c.up()
+    c.check(2, True)
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_nan_stays_where_it_is(sdq_dev, new):
+    """NaN and infinite scales behind a sequence's end, in pages that are not its
+    own, and in another sequence change nothing; a NaN query its own row only."""
+    c = Case(sdq_dev, [new, new], [new + 37, new + 90], 2, 16, seed=6)
+    clean = c.check(4, True)
+    q = c.rng.standard_normal((c.T, 512)).astype(F)
+    first = c.check(4, True, q=q)
+    for f in c.free:
+        c.ks[f], c.vs[f] = np.nan, np.inf
+    for s in range(2):
+        end = c.lens[s]
+        if end % 16:
+            c.ks[c.table[s, end // 16], :, end % 16:] = np.nan
+            c.vs[c.table[s, end // 16], :, end % 16:] = np.inf
+    c.up()
+    assert_bitexact(c.check(4, True, q=q), first, "masked NaN")
+    bad = q.copy()
+    bad[0, 3] = np.nan
+    bad[new, 130] = np.inf
+    out = c.torch.zeros((c.T, 512), device=sdq_dev)
+    c.sdq.kv_attention(c.cache, c.batch, c.t(bad), out, 4, causal=True)
+    got = out.cpu().numpy()
+    assert np.isnan(got[0, :HD]).all() and not np.isfinite(got[new, HD:2 * HD]).all()
+    want, tol = c.attend(q, 4, HD**-0.5, True)
+    keep = np.ones((c.T, 512), bool)
+    keep[0, :HD] = keep[new, HD:2 * HD] = False
+    assert (np.abs(got - want) <= tol)[keep].all()
+    c.vs[c.table[1, 0]] = np.nan
+    c.up()
+    out.zero_()
+    c.sdq.kv_attention(c.cache, c.batch, c.t(q), out, 4, causal=True)
+    got = out.cpu().numpy()
+    assert_bitexact(got[:new], first[:new], "the other sequence")
+    assert np.isnan(got[new:]).all() and np.isfinite(clean).all()
+
+
+def test_shared_pages_and_independence(sdq_dev):
+    """Two sequences that share their first pages; a batch's rows do not depend on
+    who else is in it, bit for bit where the call's sizes are the same."""
+    c = Case(sdq_dev, [3, 3], [50, 60], 2, 16, seed=8)
+    c.table[1, :2] = c.table[0, :2]
+    c.up()
+    q = c.rng.standard_normal((c.T, 256)).astype(F)
+    both = c.check(2, True, q=q)
+    c.k[c.table[1, 3]] = 5
+    c.up()
+    assert_bitexact(c.check(2, True, q=q)[:3], both[:3], "first sequence")
+
+
+def test_empty_calls(sdq_dev):
+    import torch
+
+    c = Case(sdq_dev, [1], [0], 2, 16)
+    got = c.check(2, True)
+    assert (got == 0).all()
+    none = torch.empty((0, 256), device=sdq_dev)
+    c.sdq.kv_attention(c.cache, c.batch, none, none, 2)
+    c.sdq.kv_write(c.cache, c.batch, none, none)
+    empty = c.sdq.KvBatch(torch.zeros(1, dtype=torch.int32, device=sdq_dev),
+                          torch.zeros(0, dtype=torch.int32, device=sdq_dev),
+                          torch.zeros((0, 1), dtype=torch.int32, device=sdq_dev))
+    x = torch.full((2, 256), 3.0, device=sdq_dev)
+    o = torch.full((2, 256), 3.0, device=sdq_dev)
+    c.sdq.kv_attention(c.cache, empty, x, o, 2)
+    assert (o == 3).all()
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_captured_and_two_streams(sdq_dev, new):
+    """Write and attention captured (after one eager call) and replayed with growing
+    sequences; two batches at once on two streams."""
+    import torch
+
+    c = Case(sdq_dev, [new, new], [new, new], 2, 16, seed=9)
+    most = 6 * new + 400
+    need = -(-most // 16)
+    c.pages = 2 * need
+    c.table = np.arange(2 * need, dtype=np.int32)[::-1].reshape(2, need).copy()
+    c.most = need
+    shape = (c.pages, 2, 16)
+    c.k, c.v = np.zeros(shape + (HD,), np.int8), np.zeros(shape + (HD,), np.int8)
+    c.ks, c.vs = np.ones(shape, F), np.ones(shape, F)
+    c.up()
+    qkv = torch.empty((c.T, 512 + 512), device=sdq_dev)
+    out = torch.empty((c.T, 512), device=sdq_dev)
+
+    def step(o):
+        c.sdq.kv_write(c.cache, c.batch, qkv[:, 512:768], qkv[:, 768:])
+        c.sdq.kv_attention(c.cache, c.batch, qkv[:, :512], o, 4)
+
+    side = torch.cuda.Stream()
+    qkv.normal_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step(out)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step(out)
+    for i in range(4):
+        c.lens = [new * (i + 1), new * (i + 1) + 100 * i]
+        c.batch.lens.copy_(torch.tensor(c.lens, dtype=torch.int32))
+        qkv.copy_(torch.from_numpy(np.random.default_rng(i).standard_normal((c.T, 1024)).astype(F)))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        again = torch.empty_like(out)
+        step(again)
+        torch.cuda.synchronize()
+        assert torch.equal(got, again), i
+        c.k, c.v = c.cache.k.cpu().numpy(), c.cache.v.cpu().numpy()
+        c.ks, c.vs = c.cache.ks.cpu().numpy(), c.cache.vs.cpu().numpy()
+        want, tol = c.attend(qkv[:, :512].cpu().numpy(), 4, HD**-0.5, True)
+        assert (np.abs(got.cpu().numpy() - want) <= tol).all(), i
+    others = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(out) for _ in others]
+    for _ in range(3):
+        for st, o in zip(others, outs):
+            with torch.cuda.stream(st):
+                c.sdq.kv_attention(c.cache, c.batch, qkv[:, :512], o, 4)
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o, again)
+
+
+# ---- a serving step out of all of them ----
+
+def test_serving_step(sdq_dev, oracle):
+    """Residual + norm + codes -> q|k|v -> cache -> attention -> 4-bit output Linear
+    into the residual, over a prompt and three single tokens, against the same
+    steps in 64 bits on the GPU's own codes and cache."""
+    import torch
+
+    import sdq
+    from test_gpu_q4linear import expected, make
+
+    D, H = 512, 4
+    rng = np.random.default_rng(12)
+    qw, qs = oracle.quant_rows((rng.standard_normal((3 * D, D)) * 0.04).astype(F))
+    wqkv = sdq.Weight.from_host(qw, qs)
+    u, sc, z = make(D, D, 64, True, 13)
+    sc *= F(0.1)
+    wo = sdq.Weight4.from_host(u, sc, z, group=64)
+    nw = (1 + 0.1 * rng.standard_normal(D)).astype(F)
+    cache = sdq.KvCache.empty(8, 16, H, sdq_dev)
+    table = torch.tensor([[5, 2, 7, 0]], dtype=torch.int32, device=sdq_dev)
+    total = 0
+    for n in (21, 1, 1, 1):
+        total += n
+        batch = sdq.KvBatch(torch.tensor([0, n], dtype=torch.int32, device=sdq_dev),
+                            torch.tensor([total], dtype=torch.int32, device=sdq_dev), table)
+        x, d = (rng.standard_normal((n, D)).astype(F) for _ in range(2))
+        tx, td = (torch.from_numpy(a).to(sdq_dev) for a in (x, d))
+        aq = torch.empty((n, D), dtype=torch.int8, device=sdq_dev)
+        asc = torch.empty(n, device=sdq_dev)
+        qkv, att = torch.empty((n, 3 * D), device=sdq_dev), torch.empty((n, D), device=sdq_dev)
+        sdq.rmsnorm_quant(tx, aq, asc, w=torch.from_numpy(nw).to(sdq_dev), delta=td, sum_out=tx)
+        sdq.qlinear_codes(wqkv, aq, asc, qkv)
+        sdq.kv_write(cache, batch, qkv[:, D:2 * D], qkv[:, 2 * D:])
+        sdq.kv_attention(cache, batch, qkv[:, :D], att, H)
+        h = tx.clone()
+        sdq.q4linear(wo, att, tx, kind="resid", resid=tx)
+        torch.cuda.synchronize()
+        want_h, want_q, want_s = __import__("test_gpu_rmsnorm_quant").oracle_norm(x, d, nw, 1e-6)
+        assert_bitexact(h.cpu().numpy(), want_h, "sum")
+        assert_bitexact(aq.cpu().numpy(), want_q, "codes")
+        acc = want_q.astype(np.int64) @ qw.astype(np.int64).T
+        y = acc.astype(F) * (want_s[:, None] * qs[None]).astype(F)
+        assert_bitexact(qkv.cpu().numpy(), y, "q|k|v")
+        c = Case.__new__(Case)
+        c.new, c.lens, c.kvh, c.page, c.most, c.pages = [n], [total], H, 16, 4, 8
+        c.table, c.start, c.T = table.cpu().numpy(), np.array([0, n]), n
+        c.k, c.v = cache.k.cpu().numpy(), cache.v.cpu().numpy()
+        c.ks, c.vs = cache.ks.cpu().numpy(), cache.vs.cpu().numpy()
+        place = c.table[0, (total - n + np.arange(n)) // 16], slice(None), (total - n + np.arange(n)) % 16
+        for got, cols in ((c.k, slice(D, 2 * D)), (c.v, slice(2 * D, 3 * D))):
+            codes, _ = codes_of(y[:, cols].reshape(n * H, HD))
+            assert_bitexact(got[place], codes.reshape(n, H, HD), "cache")
+        want, tol = c.attend(y[:, :D], H, HD**-0.5, True)
+        a = att.cpu().numpy()
+        assert (np.abs(a - want) <= tol).all()
+        o, tol = expected(a, u, sc, z, 64)
+        o = want_h + o
+        assert (np.abs(tx.cpu().numpy() - o) <= tol + 2.0**-24 * np.abs(o)).all()
