@@ -29,6 +29,7 @@
 
 #include "sdq_internal.h"
 #include "sdq_kv.h"
+#include "sdq_kv_plan.h"
 #include "sdq_sdpa_plan.h"
 
 // Scratch memory of sdq_qlinear_noalloc: a file-scope device array, one copy
@@ -92,7 +93,7 @@ struct Workspace {
   size_t rinv_bytes = 0;
   char* grp = nullptr;  // sdq_qlinear_group's per-item scratch
   size_t grp_bytes = 0;
-  float* sdpa = nullptr;  // attention: packed K and V, shares' partial outputs
+  float* sdpa = nullptr;  // attention, paged or not: packed K and V, shares' partial outputs
   size_t sdpa_bytes = 0;
   std::mutex sdpa_mu;  // held from its lookup to the last launch that uses it
 };
@@ -973,7 +974,9 @@ int kv_view(const sdq_kv_cache* c, const sdq_kv_batch* b, int64_t T, const std::
   if (T * 2 * c->kv_heads > (int64_t(1) << 34))
     return set_error(SDQ_ERR_INVALID, tag + ": T * kv_heads must be at most 2^33");
   *out = kv::View{c->k,       c->ks,   c->v,     c->vs,   c->pages,     log2, c->kv_heads,
-                  b->q_start, b->lens, b->table, b->nseq, b->max_pages, T};
+                  b->q_start, b->lens, b->table, b->nseq,
+                  c->pages > 0 ? b->max_pages : 0,  // an empty pool: sequences without keys
+                  T};
   if (b->nseq == 0) out->T = 0;
   if (out->T == 0) return SDQ_OK;
   if (c->pages > 0 && (!c->k || !c->ks || !c->v || !c->vs))
@@ -2407,8 +2410,26 @@ int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* 
   int dev = -1;
   if ((rc = usable_device(&dev))) return rc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const kvplan::Plan plan =
+      kvplan::plan(T, view.nseq, heads / c->kv_heads, c->kv_heads,
+                   view.max_pages << view.page_log2, g_dev[dev].cu_count);
+  // Threads that share the stream queue their calls' launches one after the
+  // other, so that each call's scratch is its own until the next begins.
+  float* scratch = nullptr;
+  std::unique_lock<std::mutex> turn;
+  if (plan.scratch_bytes > 0) {
+    std::unique_lock<std::mutex> lk(g_mu);
+    Workspace& ws = ws_of(dev, s);
+    lk.unlock();
+    turn = std::unique_lock<std::mutex>(ws.sdpa_mu);
+    lk.lock();
+    if ((rc = grow(s, reinterpret_cast<void**>(&ws.sdpa), &ws.sdpa_bytes,
+                   (size_t)plan.scratch_bytes)))
+      return rc;
+    scratch = ws.sdpa;
+  }
   return timed("kv_attention", s, [&] {
-    return launch_kv_attn(view, q, ldq, out, ldo, heads, scale, causal != 0, s);
+    return launch_kv_attn(view, q, ldq, out, ldo, heads, scale, causal != 0, plan, scratch, s);
   });
 }
 

@@ -255,12 +255,17 @@ hipError_t launch_w4(const W4View& w, const float* x, int64_t M, const EpiArgs& 
 namespace kv {
 struct View;
 }
+namespace kvplan {
+struct Plan;
+}
 hipError_t launch_kv_write(const kv::View& c, const float* k, int64_t ldk, const float* v,
                            int64_t ldv, hipStream_t s);
 hipError_t launch_kv_read(const kv::View& c, float* k, int64_t ldk, float* v, int64_t ldv,
                           hipStream_t s);
+// plan: kvplan::plan's for this call; scratch: its scratch_bytes.
 hipError_t launch_kv_attn(const kv::View& c, const float* q, int64_t ldq, float* out, int64_t ldo,
-                          int heads, float scale, int causal, hipStream_t s);
+                          int heads, float scale, int causal, const kvplan::Plan& plan,
+                          void* scratch, hipStream_t s);
 
 // GEMM tile configurations.
 enum GemmCfg : int {

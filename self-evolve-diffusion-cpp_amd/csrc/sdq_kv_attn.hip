@@ -1,12 +1,33 @@
 // Attention of new tokens over the paged int8 cache (gfx950).
 //
-// Per row (token i at position p, head h): logits t_j = scale q . k_j over the
-// sequence's keys (j <= p where causal), out = sum_j 2^(t_j - m) v_j / sum_j
-// 2^(t_j - m) with t in units of log2 and m the running maximum.
+// Per row (token i at position p, head h), over the keys j that it sees, with
+// s_j = scale log2(e) q . k_j:   out = sum_j 2^s_j v_j / sum_j 2^s_j.
+//
+// Numbers. A cached value is code * scale; the codes are exact in fp16, so each
+// fp32 product costs two fp16 MFMA products: q = (hi + lo) 2^-r, r one power of
+// two for a tile of rows that puts its largest element into [2^14, 2^15), and
+// the softmax weight = hi + lo below. hi + lo hold 22 bits, and an absolute
+// 2^-40 of the largest beneath them. The key's scale multiplies the finished
+// sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in [1/2, 1), E0 the exponent of
+// the sequence's first value: its exponent goes into the softmax,
+//   t_j = s_j + e_j,  X_j = 2^(t_j - m), m the running maximum of t,
+//   out = 2^E0 sum_j X_j f_j code_j / sum_j X_j 2^-e_j,
+// one exponential a key as before, and the weights that are split into parts
+// are those that count: no value is lost beside another, however far apart the
+// scales of heavy and light keys are (e_j is held to -60 .. 60).
+//
+// Scores are computed transposed, S^T = K Q^T (16x16x32): a lane then holds one
+// query's scores for keys 4 g + 0..3 (g = lane / 16) of two 16-key tiles, which
+// is the B operand of out^T = V^T P^T with no exchange between lanes, where the
+// eight k slots of lane group g stand for keys 4 g .. 4 g + 3 of either tile.
+// Dims: k slot 8 g + i of step kb is dim 64 (kb / 2) + 16 g + 8 (kb % 2) + i (16
+// bytes of a cached row a lane), and row c of V's tile e is dim 8 c + e (8
+// bytes), so that lane group g ends with dims 32 g .. 32 g + 31 of its query.
 #include <algorithm>
 
 #include "sdq_device.h"
 #include "sdq_kv.h"
+#include "sdq_kv_plan.h"
 
 #pragma clang fp contract(off)
 
@@ -15,50 +36,725 @@ namespace {
 
 using kv::kHd;
 using kv::View;
+using dev::v4f;
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-// One wave a row and head; lane l holds dims 2l and 2l + 1.
-__global__ void __launch_bounds__(64)
-kv_attn_simple_kernel(View c, const float* __restrict__ q, int64_t ldq, float* __restrict__ out,
-                      int64_t ldo, int heads, float scale2, int causal) {
-  const int64_t t = blockIdx.x;
-  const int h = blockIdx.y, l = threadIdx.x;
-  const int s = kv::seq_of(c, t);
-  if (s < 0) return;
-  const int64_t len = kv::length_of(c, s);
-  const int64_t p = len - kv::row_of(c, s + 1) + t;
-  const int64_t end = causal ? (p + 1 < len ? p + 1 : len) : len;
-  const int kvh = h / (heads / c.kv_heads);
-  const float2 a = reinterpret_cast<const float2*>(q + t * ldq + (int64_t)h * kHd)[l];
-  float m = -INFINITY, z = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int64_t j = 0; p >= 0 && j < end; j++) {
-    const int64_t at = kv::place_of(c, s, j, kvh);
-    if (at < 0) continue;
-    const uint16_t kk = reinterpret_cast<const uint16_t*>(c.k + at * kHd)[l];
-    const uint16_t vv = reinterpret_cast<const uint16_t*>(c.v + at * kHd)[l];
-    float dot = a.x * (float)(int8_t)kk + a.y * (float)(int8_t)(kk >> 8);
+constexpr int kTop = 15;      // largest q of a tile below 2^kTop
+constexpr int kWeight = 13;   // weights X f enter as X f 2^kWeight
+constexpr int kFar = 60;      // e_j is held to -kFar .. kFar
+
+struct Args {
+  View c;
+  const float* q;
+  int64_t ldq;
+  float* out;
+  int64_t ldo;
+  int heads, group;  // query heads, query heads per cached head
+  float scale2;      // scale * log2(e)
+  int causal;
+  int splits;
+  int64_t tile0;     // first tile of this launch
+  float* part;       // [tile][kv head][split][row][128], unscaled sums
+  float2* part_ml;   // the same without dims: maximum, denominator
+};
+
+// A tile of rows: rows [r0, r0 + RT) of sequence s, row r = token r / group,
+// query head r % group of the tile's cached head.
+struct Tile {
+  int s;          // -1: none
+  int64_t r0;
+  int64_t rows;   // of the sequence
+  int64_t row0;   // the sequence's first row in q
+  int64_t len;    // keys
+  int64_t first;  // position of the sequence's first row
+};
+
+// The tile with number `tile` when every sequence is cut into tiles of RT rows:
+// a scan over the sequences, 64 at a time. The same in every wave.
+template <int RT>
+__device__ __forceinline__ Tile find_tile(const View& c, int group, int64_t tile) {
+  const int l = threadIdx.x & 63;
+  Tile t{-1, 0, 0, 0, 0, 0};
+  int64_t base = 0;
+  for (int s0 = 0; s0 < c.nseq; s0 += 64) {
+    const int s = s0 + l;
+    const int64_t n = s < c.nseq ? kv::row_of(c, s + 1) - kv::row_of(c, s) : 0;
+    const int64_t rows = n > 0 ? n * group : 0;
+    const int64_t count = (rows + RT - 1) / RT;
+    int64_t upto = count;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
-    const float x = dot * c.ks[at] * scale2;
-    const float top = m < x ? x : m;
-    const float f = m == top ? 1.f : __builtin_exp2f(m - top);
-    const float e = __builtin_exp2f(x - top);
-    const float w = e * c.vs[at];
-    z = z * f + e;
-    o0 = o0 * f + w * (float)(int8_t)vv;
-    o1 = o1 * f + w * (float)(int8_t)(vv >> 8);
-    m = top;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t u = __shfl_up(upto, o);
+      upto += l >= o ? u : 0;
+    }
+    const uint64_t past = __ballot(base + upto > tile);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      t.s = __builtin_amdgcn_readfirstlane(s0 + at);
+      t.r0 = (tile - base - __shfl(upto - count, at)) * RT;
+      t.rows = __shfl(rows, at);
+      t.row0 = kv::row_of(c, t.s);
+      t.len = kv::length_of(c, t.s);
+      t.first = t.len - t.rows / group;
+      return t;
+    }
+    base += __shfl(upto, 63);
   }
-  const float inv = z == 0.f ? 0.f : 1.f / z;
-  reinterpret_cast<float2*>(out + t * ldo + (int64_t)h * kHd)[l] = float2{o0 * inv, o1 * inv};
+  return t;
+}
+
+// Keys that the rows [r, r + n) of a tile see at most (0: none).
+__device__ __forceinline__ int64_t keys_of(const Tile& t, int64_t r, int n, int group, int causal) {
+  if (r >= t.rows) return 0;
+  const int64_t last = (r + n < t.rows ? r + n : t.rows) - 1;
+  const int64_t p = t.first + last / group;
+  return p < 0 ? 0 : causal ? (p + 1 < t.len ? p + 1 : t.len) : t.len;
+}
+
+// Eight codes (two dwords) as fp16: 0x6400 | u is 1024 + u, with u = code + 128.
+__device__ __forceinline__ v2h less1152(uint32_t x) {
+  return __builtin_bit_cast(v2h, x) + v2h{(_Float16)-1152.f, (_Float16)-1152.f};
+}
+__device__ __forceinline__ v8h codes8(uint32_t a, uint32_t b) {
+  a ^= 0x80808080u;
+  b ^= 0x80808080u;
+  const v2h x = less1152(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u));
+  const v2h y = less1152(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u));
+  const v2h z = less1152(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u));
+  const v2h w = less1152(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u));
+  return v8h{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
+}
+// Byte I of two dwords (codes xor 0x80) as a pair of fp16.
+template <int I>
+__device__ __forceinline__ v2h pair_of(uint32_t a, uint32_t b) {
+  constexpr uint32_t sel = 0x0c000c00u | (uint32_t)I | ((uint32_t)(I + 4) << 16);
+  return less1152(__builtin_amdgcn_perm(b, a, sel) | 0x64006400u);
+}
+
+__device__ __forceinline__ float xor_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float xor_sum(float v) {
+  v = v + __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// fp32 to two fp16 parts.
+__device__ __forceinline__ void parts8(const float x[8], v8h& hi, v8h& lo) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    hi[i] = (_Float16)x[i];
+    lo[i] = (_Float16)(x[i] - (float)hi[i]);
+  }
+}
+
+// The lane's slice of a query row (head of a token), zeros where it is none.
+__device__ __forceinline__ void load_q(const Args& a, const Tile& t, int h, int64_t r, int g,
+                                       float x[4][8]) {
+  const bool ok = r < t.rows;
+  const int64_t rr = ok ? r : 0;
+  const int64_t tok = rr / a.group;
+  const float* p =
+      a.q + (t.row0 + tok) * a.ldq + (int64_t)(h * a.group + (int)(rr - tok * a.group)) * kHd;
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const float4 v =
+          ok ? *reinterpret_cast<const float4*>(p + 64 * (kb >> 1) + 16 * g + 8 * (kb & 1) + 4 * j)
+             : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[kb][4 * j] = v.x;
+      x[kb][4 * j + 1] = v.y;
+      x[kb][4 * j + 2] = v.z;
+      x[kb][4 * j + 3] = v.w;
+    }
+}
+__device__ __forceinline__ float amax_finite(const float x[4][8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float v = fabsf(x[kb][i]);
+      m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
+    }
+  return m;
+}
+// Exponent that scales a tile's largest |q| below 2^kTop; within what a float's
+// power of two can hold.
+__device__ __forceinline__ int q_exp(float m) {
+  const int e = m > 0.f ? kTop - __builtin_amdgcn_frexp_expf(m) : 0;
+  return e > 100 ? 100 : e;
+}
+
+// What a key contributes: c (score to log2 units), e, 2^-e and f 2^kWeight. One
+// that is not there (masked, no page) gives zeros, so that whatever its memory
+// holds stays out.
+struct KeyTerms {
+  float c, e, w, f;
+};
+__device__ __forceinline__ KeyTerms key_terms(float ks, float vs, bool ok, float qk, int e0) {
+  KeyTerms k;
+  int e = vs != 0.f ? __builtin_amdgcn_frexp_expf(vs) - e0 : 0;
+  e = e < -kFar ? -kFar : e > kFar ? kFar : e;
+  k.c = ok ? ks * qk : 0.f;
+  k.e = ok ? (float)e : 0.f;
+  k.w = ok ? __builtin_ldexpf(1.f, -e) : 0.f;
+  k.f = ok ? __builtin_ldexpf(vs, kWeight - e - e0) : 0.f;
+  return k;
+}
+// E0: the exponent of the sequence's first value scale.
+__device__ __forceinline__ int first_exp(const View& c, const Tile& t, int h) {
+  if (t.len <= 0) return 0;
+  const int64_t at = kv::place_of(c, t.s, 0, h);
+  const float v = at >= 0 ? c.vs[at] : 0.f;
+  return v != 0.f ? __builtin_amdgcn_frexp_expf(v) : 0;
+}
+
+// One query's softmax state in a lane: the maximum is the same in the query's
+// four lanes, the denominator is the lane's own share.
+struct State {
+  float m, l;
+};
+
+// A 32-key block's scores of one query tile (tiles kt, elements i: key 16 kt +
+// 4 g + i) to the two parts of its weights. seen(kt, i): the row sees that key.
+// Returns the factor that the sums so far shrink by.
+template <bool MASK, class Seen>
+__device__ __forceinline__ float soft_step(const v4f s[2], const KeyTerms k[2][4], State& st,
+                                           Seen seen, v8h& hi, v8h& lo) {
+  float t[8];
+  float mx = -INFINITY;
+#pragma unroll
+  for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float v = __builtin_fmaf(s[kt][i], k[kt][i].c, k[kt][i].e);
+      if (MASK && !seen(kt, i)) v = -INFINITY;
+      t[4 * kt + i] = v;
+      mx = fmaxf(mx, v);
+    }
+  mx = fmaxf(st.m, xor_max(mx));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  const float shrink = __builtin_amdgcn_exp2f(st.m - ref);
+  st.m = mx;
+  float l = st.l * shrink;
+  float p[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float x = __builtin_amdgcn_exp2f(t[j] - ref);
+    l = __builtin_fmaf(x, k[j >> 2][j & 3].w, l);
+    p[j] = x * k[j >> 2][j & 3].f;
+    if (MASK && !seen(j >> 2, j & 3)) p[j] = 0.f;  // its scale may be NaN
+  }
+  st.l = l;
+  parts8(p, hi, lo);
+  return shrink;
+}
+
+// ---- few rows: a tile of 16, the workgroup's waves share out the keys ----
+
+constexpr int kFewRows = kvplan::kFewRows;
+constexpr int kFewWaves = kvplan::kFewWaves;
+constexpr int kFewStride = kHd + 4;  // LDS row of a merged sum (bank spread)
+
+__global__ void __launch_bounds__(64 * kFewWaves) kv_attn_few_kernel(Args a) {
+  const View& c = a.c;
+  const int w = threadIdx.x >> 6, l = threadIdx.x & 63, r16 = l & 15, g = l >> 4;
+  const int z = (int)(blockIdx.x % a.splits);
+  const int64_t th = blockIdx.x / a.splits;
+  const int h = (int)(th % c.kv_heads);
+  const int64_t tile = a.tile0 + th / c.kv_heads;
+  const Tile t = find_tile<kFewRows>(c, a.group, tile);
+  if (t.s < 0) return;
+
+  float x[4][8];
+  load_q(a, t, h, t.r0 + r16, g, x);
+  float qm = amax_finite(x);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) qm = fmaxf(qm, __shfl_xor(qm, o));
+  const int qe = q_exp(qm);
+  v8h qh[4], ql[4];
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[kb][i] = __builtin_ldexpf(x[kb][i], qe);
+    parts8(x[kb], qh[kb], ql[kb]);
+  }
+  const float qk = __builtin_ldexpf(a.scale2, -qe);
+  const int e0 = first_exp(c, t, h);
+
+  const int64_t keys = keys_of(t, t.r0, kFewRows, a.group, a.causal);
+  const int64_t blocks = (keys + 31) / 32;
+  const int64_t b0 = blocks * z / a.splits, b1 = blocks * (z + 1) / a.splits;
+  // what this lane's row sees, and what every row of the tile does
+  const int64_t pos = t.first + (t.r0 + r16) / a.group;
+  const int64_t mine = t.r0 + r16 >= t.rows || pos < 0 ? 0
+                       : a.causal                      ? (pos + 1 < t.len ? pos + 1 : t.len)
+                                                       : t.len;
+  int64_t all = mine;
+  if (t.r0 + r16 >= t.rows) all = keys;
+#pragma unroll
+  for (int o = 8; o; o >>= 1) {
+    const int64_t u = __shfl_xor(all, o);
+    all = u < all ? u : all;
+  }
+
+  State st{-INFINITY, 0.f};
+  v4f acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) acc[e] = v4f{0.f, 0.f, 0.f, 0.f};
+
+  const int32_t* table = c.table + t.s * c.max_pages;
+  for (int64_t b = b0 + w; b < b1; b += kFewWaves) {
+    uint4 kr[2][2];
+    uint2 vr[2][4];
+    float4 ks[2], vs[2];
+    bool there[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; kt++) {
+      const int64_t p = b * 32 + 16 * kt;
+      int64_t page = p < keys ? table[p >> c.page_log2] : -1;
+      there[kt] = page >= 0 && page < c.pages;
+      if (!there[kt]) page = 0;
+      const int64_t at =
+          ((page * c.kv_heads + h) << c.page_log2) + (p & ((1 << c.page_log2) - 1));
+      const int8_t* kp = c.k + (at + r16) * kHd + 16 * g;
+      kr[kt][0] = *reinterpret_cast<const uint4*>(kp);
+      kr[kt][1] = *reinterpret_cast<const uint4*>(kp + 64);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        vr[kt][i] = *reinterpret_cast<const uint2*>(c.v + (at + 4 * g + i) * kHd + 8 * r16);
+      ks[kt] = *reinterpret_cast<const float4*>(c.ks + at + 4 * g);
+      vs[kt] = *reinterpret_cast<const float4*>(c.vs + at + 4 * g);
+    }
+    v4f s[2];
+    KeyTerms kk[2][4];
+#pragma unroll
+    for (int kt = 0; kt < 2; kt++) {
+      s[kt] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < 4; kb++) {
+        const uint4 r = kr[kt][kb >> 1];
+        const v8h ka = kb & 1 ? codes8(r.z, r.w) : codes8(r.x, r.y);
+        s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[kb], s[kt], 0, 0, 0);
+        s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[kb], s[kt], 0, 0, 0);
+      }
+      const float ksv[4] = {ks[kt].x, ks[kt].y, ks[kt].z, ks[kt].w};
+      const float vsv[4] = {vs[kt].x, vs[kt].y, vs[kt].z, vs[kt].w};
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        kk[kt][i] = key_terms(ksv[i], vsv[i],
+                              there[kt] && b * 32 + 16 * kt + 4 * g + i < t.len, qk, e0);
+    }
+    v8h ph, pl;
+    float shrink;
+    if (b * 32 + 32 <= all && there[0] && there[1]) {
+      shrink = soft_step<false>(s, kk, st, [](int, int) { return true; }, ph, pl);
+    } else {
+      const int64_t k0 = b * 32 + 4 * g;
+      shrink = soft_step<true>(
+          s, kk, st,
+          [&](int kt, int i) { return there[kt] && k0 + 16 * kt + i < mine; }, ph, pl);
+    }
+    uint32_t va[8], vb[8];  // dims 0-3 and 4-7 of the lane's eight, keys in slot order
+#pragma unroll
+    for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        va[4 * kt + i] = vr[kt][i].x ^ 0x80808080u;
+        vb[4 * kt + i] = vr[kt][i].y ^ 0x80808080u;
+      }
+    auto tile_e = [&](auto I, const uint32_t (&v)[8], v4f& o) {
+      constexpr int i = decltype(I)::value;
+      const v2h p0 = pair_of<i>(v[0], v[1]), p1 = pair_of<i>(v[2], v[3]);
+      const v2h p2 = pair_of<i>(v[4], v[5]), p3 = pair_of<i>(v[6], v[7]);
+      const v8h vv{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+      o = o * shrink;
+      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o, 0, 0, 0);
+      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph, o, 0, 0, 0);
+    };
+    tile_e(std::integral_constant<int, 0>{}, va, acc[0]);
+    tile_e(std::integral_constant<int, 1>{}, va, acc[1]);
+    tile_e(std::integral_constant<int, 2>{}, va, acc[2]);
+    tile_e(std::integral_constant<int, 3>{}, va, acc[3]);
+    tile_e(std::integral_constant<int, 0>{}, vb, acc[4]);
+    tile_e(std::integral_constant<int, 1>{}, vb, acc[5]);
+    tile_e(std::integral_constant<int, 2>{}, vb, acc[6]);
+    tile_e(std::integral_constant<int, 3>{}, vb, acc[7]);
+  }
+
+  // Join the waves: common maximum, then sums.
+  __shared__ float2 ml[kFewWaves][kFewRows];
+  __shared__ __attribute__((aligned(16))) float sums[kFewWaves][kFewRows][kFewStride];
+  st.l = xor_sum(st.l);
+  if (g == 0) ml[w][r16] = float2{st.m, st.l};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {  // dims 32 g + 8 i + e
+    float* o = &sums[w][r16][32 * g + 8 * i];
+    *reinterpret_cast<v4f*>(o) = v4f{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+    *reinterpret_cast<v4f*>(o + 4) = v4f{acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
+  }
+  __syncthreads();
+  constexpr int kPer = kFewRows * kHd / (64 * kFewWaves);  // dims a thread
+  const int row = threadIdx.x * kPer / kHd, d0 = threadIdx.x * kPer % kHd;
+  const int64_t r = t.r0 + row;
+  if (r >= t.rows) return;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; i++) m = fmaxf(m, ml[i][row].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float den = 0.f, o[kPer] = {};
+#pragma unroll
+  for (int i = 0; i < kFewWaves; i++) {
+    const float f = __builtin_amdgcn_exp2f(ml[i][row].x - ref);
+    den = __builtin_fmaf(ml[i][row].y, f, den);
+#pragma unroll
+    for (int d = 0; d < kPer; d++) o[d] = __builtin_fmaf(sums[i][row][d0 + d], f, o[d]);
+  }
+  float* dst;
+  if (a.splits == 1) {
+    const float f = den == 0.f ? 0.f : __builtin_ldexpf(1.f, e0 - kWeight) / den;
+#pragma unroll
+    for (int d = 0; d < kPer; d++) o[d] = o[d] * f;
+    const int64_t tok = r / a.group;
+    dst = a.out + (t.row0 + tok) * a.ldo +
+          (int64_t)(h * a.group + (int)(r - tok * a.group)) * kHd + d0;
+  } else {
+    const int64_t at = (th * a.splits + z) * kFewRows + row;
+    if (d0 == 0) a.part_ml[at] = float2{m, den};
+    dst = a.part + at * kHd + d0;
+  }
+#pragma unroll
+  for (int d = 0; d < kPer; d += 4)
+    *reinterpret_cast<v4f*>(dst + d) = v4f{o[d], o[d + 1], o[d + 2], o[d + 3]};
+}
+
+// ---- joining the shares of cut keys: one wave a row ----
+
+template <int RT>
+__global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
+  const int l = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t th = i / RT;
+  const int row = (int)(i % RT), h = (int)(th % a.c.kv_heads);
+  const Tile t = find_tile<RT>(a.c, a.group, a.tile0 + th / a.c.kv_heads);
+  if (t.s < 0 || t.r0 + row >= t.rows) return;
+  const int64_t at = th * a.splits * RT + row;
+  float m = -INFINITY;
+  for (int z = 0; z < a.splits; z++) m = fmaxf(m, a.part_ml[at + (int64_t)z * RT].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float den = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int z = 0; z < a.splits; z++) {
+    const float2 ml = a.part_ml[at + (int64_t)z * RT];
+    const float2 v = reinterpret_cast<const float2*>(a.part + (at + (int64_t)z * RT) * kHd)[l];
+    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+    den = __builtin_fmaf(ml.y, f, den);
+    o0 = __builtin_fmaf(v.x, f, o0);
+    o1 = __builtin_fmaf(v.y, f, o1);
+  }
+  const float f =
+      den == 0.f ? 0.f : __builtin_ldexpf(1.f, first_exp(a.c, t, h) - kWeight) / den;
+  const int64_t r = t.r0 + row, tok = r / a.group;
+  float* dst = a.out + (t.row0 + tok) * a.ldo +
+               (int64_t)(h * a.group + (int)(r - tok * a.group)) * kHd;
+  reinterpret_cast<float2*>(dst)[l] = float2{o0 * f, o1 * f};
+}
+
+// ---- chunks: NW waves of 16 QT rows over the same keys ----
+//
+// A block of 8 NW keys is loaded as codes, two blocks ahead, turned to fp16 once
+// by the whole workgroup in the order of the MFMA operands and read by every
+// wave from LDS (two buffers, one barrier a block).
+
+template <int NW>
+struct Block {
+  static constexpr int kKeys = 8 * NW;
+  static constexpr int kSubs = kKeys / 32;
+  __attribute__((aligned(16))) char k[kSubs][2][4][1024];  // [sub][kt][kb][lane 16 B]
+  __attribute__((aligned(16))) char v[kSubs][8][1024];     // [sub][e][lane 16 B]
+  __attribute__((aligned(16))) float c[kKeys], e[kKeys], w[kKeys], f[kKeys];
+};
+
+template <int NW, int QT>
+__global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
+  constexpr int kRows = 16 * QT * NW;
+  using Blk = Block<NW>;
+  constexpr int KB = Blk::kKeys;
+  __shared__ Blk buf[2];
+  __shared__ float wave_max[NW];
+  const View& c = a.c;
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, r16 = l & 15, g = l >> 4;
+  const int z = (int)(blockIdx.x % a.splits);
+  const int64_t th = blockIdx.x / a.splits;
+  const int h = (int)(th % c.kv_heads);
+  const Tile t = find_tile<kRows>(c, a.group, a.tile0 + th / c.kv_heads);
+  if (t.s < 0) return;
+
+  v8h qh[QT][4], ql[QT][4];
+  int64_t mine[QT];
+  float qk;
+  int e0;
+  {
+    float x[QT][4][8];
+    float qm = 0.f;
+#pragma unroll
+    for (int qt = 0; qt < QT; qt++) {
+      const int64_t r = t.r0 + (w * QT + qt) * 16 + r16;
+      load_q(a, t, h, r, g, x[qt]);
+      qm = fmaxf(qm, amax_finite(x[qt]));
+      const int64_t pos = t.first + r / a.group;
+      mine[qt] = r >= t.rows || pos < 0 ? 0 : a.causal ? (pos + 1 < t.len ? pos + 1 : t.len) : t.len;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) qm = fmaxf(qm, __shfl_xor(qm, o));
+    if (l == 0) wave_max[w] = qm;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; i++) qm = fmaxf(qm, wave_max[i]);
+    const int qe = q_exp(qm);
+#pragma unroll
+    for (int qt = 0; qt < QT; qt++)
+#pragma unroll
+      for (int kb = 0; kb < 4; kb++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[qt][kb][i] = __builtin_ldexpf(x[qt][kb][i], qe);
+        parts8(x[qt][kb], qh[qt][kb], ql[qt][kb]);
+      }
+    qk = __builtin_ldexpf(a.scale2, -qe);
+    e0 = first_exp(c, t, h);
+  }
+  const int64_t keys = keys_of(t, t.r0, kRows, a.group, a.causal);
+  const int64_t blocks = (keys + KB - 1) / KB;
+  const int64_t b0 = blocks * z / a.splits, b1 = blocks * (z + 1) / a.splits;
+  // keys that the wave's rows see at most, and all of them see
+  int64_t most = 0, all = keys;
+#pragma unroll
+  for (int qt = 0; qt < QT; qt++) {
+    most = mine[qt] > most ? mine[qt] : most;
+    if (t.r0 + (w * QT + qt) * 16 + r16 < t.rows) all = mine[qt] < all ? mine[qt] : all;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    const int64_t u = __shfl_xor(most, o), v = __shfl_xor(all, o);
+    most = u > most ? u : most;
+    all = v < all ? v : all;
+  }
+  // uniform over the wave, so that the branches on them are scalar
+  const int64_t wmost = ((int64_t)__builtin_amdgcn_readfirstlane((int)(most >> 32)) << 32) |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
+  const int64_t wall = ((int64_t)__builtin_amdgcn_readfirstlane((int)(all >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
+
+  State st[QT];
+  v4f acc[QT][8];
+#pragma unroll
+  for (int qt = 0; qt < QT; qt++) {
+    st[qt] = State{-INFINITY, 0.f};
+#pragma unroll
+    for (int e = 0; e < 8; e++) acc[qt][e] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // The thread's part of a block: 16 dims of a key, 4 dims of four values' rows,
+  // one key's scales (the first KB threads).
+  const int32_t* table = c.table + t.s * c.max_pages;
+  const int k_key = 16 * (tid >> 7) + (tid & 15), k_j = (tid >> 4) & 7;   // dims 16 k_j ..
+  const int v_row = 4 * (tid >> 5), v_d = 4 * (tid & 31);                 // keys, dims
+  uint4 kr;
+  uint32_t vr[4];
+  float ksr = 0.f, vsr = 0.f;
+  bool ok = false;
+  auto place = [&](int64_t p, bool& there) -> int64_t {
+    int64_t page = p < keys ? table[p >> c.page_log2] : -1;
+    there = page >= 0 && page < c.pages;
+    return (((there ? page : 0) * c.kv_heads + h) << c.page_log2) +
+           (p & ((1 << c.page_log2) - 1));
+  };
+  auto fetch = [&](int64_t b) {
+    bool there;
+    int64_t at = place(b * KB + k_key, there);
+    kr = *reinterpret_cast<const uint4*>(c.k + at * kHd + 16 * k_j);
+    at = place(b * KB + v_row, there);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      vr[i] = *reinterpret_cast<const uint32_t*>(c.v + (at + i) * kHd + v_d);
+    if (tid < KB) {
+      at = place(b * KB + tid, there);
+      ksr = c.ks[at];
+      vsr = c.vs[at];
+      ok = there && b * KB + tid < t.len;
+    }
+  };
+  auto stage = [&](Blk& d) {
+    const int kt = tid >> 7;  // 16-key tile of the block
+    char* kd = d.k[kt >> 1][kt & 1][2 * (k_j >> 2)] + (16 * (k_j & 3) + (tid & 15)) * 16;
+    *reinterpret_cast<v8h*>(kd) = codes8(kr.x, kr.y);
+    *reinterpret_cast<v8h*>(kd + 1024) = codes8(kr.z, kr.w);
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = vr[i] ^ 0x80808080u;
+    // keys v_row .. + 3: tile (v_row / 16) % 2 of sub-block v_row / 32, lane group (v_row / 4) % 4
+    char* vd = d.v[v_row >> 5][v_d & 7] + (16 * ((v_row >> 2) & 3) + (v_d >> 3)) * 16 +
+               8 * ((v_row >> 4) & 1);
+    auto put = [&](auto I) {
+      constexpr int i = decltype(I)::value;
+      const v2h p = pair_of<i>(x[0], x[1]), q = pair_of<i>(x[2], x[3]);
+      typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<v4h*>(vd + 1024 * i) = v4h{p[0], p[1], q[0], q[1]};
+    };
+    put(std::integral_constant<int, 0>{});
+    put(std::integral_constant<int, 1>{});
+    put(std::integral_constant<int, 2>{});
+    put(std::integral_constant<int, 3>{});
+    if (tid < KB) {
+      const KeyTerms k = key_terms(ksr, vsr, ok, qk, e0);
+      d.c[tid] = ok ? k.c : 0.f;
+      d.e[tid] = ok ? k.e : -INFINITY;  // no key: its logit is -inf in every row
+      d.w[tid] = k.w;
+      d.f[tid] = k.f;
+    }
+  };
+  auto compute = [&](const Blk& d, int64_t b) {
+#pragma unroll
+    for (int sub = 0; sub < Blk::kSubs; sub++) {
+      const int64_t k0 = b * KB + 32 * sub;
+      if (k0 >= wmost) break;
+      v4f s[QT][2];
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++) {
+#pragma unroll
+        for (int qt = 0; qt < QT; qt++) s[qt][kt] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++) {
+          const v8h ka = *reinterpret_cast<const v8h*>(d.k[sub][kt][kb] + l * 16);
+#pragma unroll
+          for (int qt = 0; qt < QT; qt++) {
+            s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[qt][kb], s[qt][kt], 0, 0, 0);
+            s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[qt][kb], s[qt][kt], 0, 0, 0);
+          }
+        }
+      }
+      KeyTerms kk[2][4];
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++) {
+        const int at = 32 * sub + 16 * kt + 4 * g;
+        const v4f vc = *reinterpret_cast<const v4f*>(d.c + at);
+        const v4f ve = *reinterpret_cast<const v4f*>(d.e + at);
+        const v4f vw = *reinterpret_cast<const v4f*>(d.w + at);
+        const v4f vf = *reinterpret_cast<const v4f*>(d.f + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) kk[kt][i] = KeyTerms{vc[i], ve[i], vw[i], vf[i]};
+      }
+      v8h ph[QT], pl[QT];
+      float shrink[QT];
+#pragma unroll
+      for (int qt = 0; qt < QT; qt++) {
+        if (k0 + 32 <= wall) {
+          shrink[qt] = soft_step<false>(s[qt], kk, st[qt], [](int, int) { return true; }, ph[qt],
+                                        pl[qt]);
+        } else {
+          const int64_t kg = k0 + 4 * g, end = mine[qt];
+          shrink[qt] = soft_step<true>(
+              s[qt], kk, st[qt], [&](int kt, int i) { return kg + 16 * kt + i < end; }, ph[qt],
+              pl[qt]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const v8h va = *reinterpret_cast<const v8h*>(d.v[sub][e] + l * 16);
+#pragma unroll
+        for (int qt = 0; qt < QT; qt++) {
+          v4f o = acc[qt][e] * shrink[qt];
+          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[qt], o, 0, 0, 0);
+          acc[qt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[qt], o, 0, 0, 0);
+        }
+      }
+    }
+  };
+
+  if (b0 < b1) {
+    fetch(b0);
+    stage(buf[b0 & 1]);
+    if (b0 + 1 < b1) fetch(b0 + 1);
+    __syncthreads();
+    for (int64_t b = b0; b < b1; b++) {
+      if (b + 1 < b1) stage(buf[(b + 1) & 1]);
+      if (b + 2 < b1) fetch(b + 2);
+      compute(buf[b & 1], b);
+      __syncthreads();
+    }
+  }
+
+#pragma unroll
+  for (int qt = 0; qt < QT; qt++) {
+    const int row = (w * QT + qt) * 16 + r16;
+    const int64_t r = t.r0 + row;
+    if (r >= t.rows) continue;
+    const float den = xor_sum(st[qt].l);
+    float f = 1.f;
+    float* dst;
+    if (a.splits == 1) {
+      f = den == 0.f ? 0.f : __builtin_ldexpf(1.f, e0 - kWeight) / den;
+      const int64_t tok = r / a.group;
+      dst = a.out + (t.row0 + tok) * a.ldo +
+            (int64_t)(h * a.group + (int)(r - tok * a.group)) * kHd + 32 * g;
+    } else {
+      const int64_t at = (th * a.splits + z) * kRows + row;
+      if (g == 0) a.part_ml[at] = float2{st[qt].m, den};
+      dst = a.part + at * kHd + 32 * g;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      *reinterpret_cast<v4f*>(dst + 8 * i) =
+          v4f{acc[qt][0][i] * f, acc[qt][1][i] * f, acc[qt][2][i] * f, acc[qt][3][i] * f};
+      *reinterpret_cast<v4f*>(dst + 8 * i + 4) =
+          v4f{acc[qt][4][i] * f, acc[qt][5][i] * f, acc[qt][6][i] * f, acc[qt][7][i] * f};
+    }
+  }
+}
+
+template <int RT, class Launch>
+hipError_t run(Args a, const kvplan::Plan& p, Launch launch, hipStream_t s) {
+  // launches of as many tiles as a grid's 32-bit thread count takes
+  for (int64_t tile = 0; tile < p.tiles; tile += p.tiles_per_launch) {
+    const int64_t n = std::min(p.tiles_per_launch, p.tiles - tile) * a.c.kv_heads;
+    a.tile0 = tile;
+    launch(a, (unsigned)(n * p.splits));
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (p.splits > 1) {
+      hipLaunchKernelGGL((kv_attn_join_kernel<RT>), dim3((unsigned)(n * RT / 4)), dim3(256), 0, s, a);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+  }
+  return hipSuccess;
 }
 
 }  // namespace
 
 hipError_t launch_kv_attn(const View& c, const float* q, int64_t ldq, float* out, int64_t ldo,
-                          int heads, float scale, int causal, hipStream_t s) {
-  hipLaunchKernelGGL(kv_attn_simple_kernel, dim3((unsigned)c.T, (unsigned)heads), dim3(64), 0, s, c,
-                     q, ldq, out, ldo, heads, scale * 1.44269504088896341f, causal);
-  return hipGetLastError();
+                          int heads, float scale, int causal, const kvplan::Plan& p,
+                          void* scratch, hipStream_t s) {
+  Args a{c, q, ldq, out, ldo, heads, heads / c.kv_heads, scale * 1.44269504088896341f, causal,
+         p.splits, 0, nullptr, nullptr};
+  if (p.splits > 1) {
+    a.part = static_cast<float*>(scratch);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + p.part_bytes);
+  }
+  if (p.rows == kFewRows)
+    return run<kFewRows>(a, p, [&](const Args& x, unsigned n) {
+      hipLaunchKernelGGL(kv_attn_few_kernel, dim3(n), dim3(64 * kFewWaves), 0, s, x);
+    }, s);
+  if (p.rows == 64)
+    return run<64>(a, p, [&](const Args& x, unsigned n) {
+      hipLaunchKernelGGL((kv_attn_chunk_kernel<4, 1>), dim3(n), dim3(256), 0, s, x);
+    }, s);
+  return run<256>(a, p, [&](const Args& x, unsigned n) {
+    hipLaunchKernelGGL((kv_attn_chunk_kernel<8, 2>), dim3(n), dim3(512), 0, s, x);
+  }, s);
 }
 
 }  // namespace sdq
