@@ -93,7 +93,7 @@ struct Workspace {
   size_t rinv_bytes = 0;
   char* grp = nullptr;  // sdq_qlinear_group's per-item scratch
   size_t grp_bytes = 0;
-  float* sdpa = nullptr;  // attention, paged or not: packed K and V, shares' partial outputs
+  float* sdpa = nullptr;  // attention (packed K and V, shares' partial outputs), 4-bit Linears
   size_t sdpa_bytes = 0;
   std::mutex sdpa_mu;  // held from its lookup to the last launch that uses it
 };
@@ -986,6 +986,22 @@ int kv_view(const sdq_kv_cache* c, const sdq_kv_batch* b, int64_t T, const std::
   if (!b->q_start || !b->lens || (b->max_pages > 0 && !b->table))
     return set_error(SDQ_ERR_INVALID, tag + ": null batch arrays");
   return SDQ_OK;
+}
+
+// The (device, stream) workspace's attention scratch, at least `bytes`, for a
+// call that holds `turn` until its last launch is queued: threads that share the
+// stream queue their calls one after the other, so that each call's scratch is
+// its own until the next begins.
+int shared_scratch(int dev, hipStream_t s, size_t bytes, float** out,
+                   std::unique_lock<std::mutex>* turn) {
+  std::unique_lock<std::mutex> lk(g_mu);
+  Workspace& ws = ws_of(dev, s);
+  lk.unlock();
+  *turn = std::unique_lock<std::mutex>(ws.sdpa_mu);
+  lk.lock();
+  const int rc = grow(s, reinterpret_cast<void**>(&ws.sdpa), &ws.sdpa_bytes, bytes);
+  if (rc == SDQ_OK) *out = ws.sdpa;
+  return rc;
 }
 
 int usable_device(int* dev) {
@@ -2347,7 +2363,13 @@ int sdq_q4linear(const sdq_weight4* w, const float* A, int64_t M, int64_t K,
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const W4View view{w->N, w->K, w->group, w->codes, w->scale, w->zero};
   const EpiArgs ea = make_epi(epi, K);
-  return timed("q4linear", s, [&] { return launch_w4(view, A, M, ea, Y, s); });
+  const W4Plan plan = plan_w4(view, M, g_dev[dev].cu_count);
+  float* scratch = nullptr;
+  std::unique_lock<std::mutex> turn;
+  if (plan.bytes > 0 &&
+      (rc = shared_scratch(dev, s, (size_t)plan.bytes, &scratch, &turn)))
+    return rc;
+  return timed("q4linear", s, [&] { return launch_w4(view, A, M, ea, Y, plan, scratch, s); });
 }
 
 // ---- the paged cache ----
@@ -2413,21 +2435,11 @@ int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* 
   const kvplan::Plan plan =
       kvplan::plan(T, view.nseq, heads / c->kv_heads, c->kv_heads,
                    view.max_pages << view.page_log2, g_dev[dev].cu_count);
-  // Threads that share the stream queue their calls' launches one after the
-  // other, so that each call's scratch is its own until the next begins.
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
-  if (plan.scratch_bytes > 0) {
-    std::unique_lock<std::mutex> lk(g_mu);
-    Workspace& ws = ws_of(dev, s);
-    lk.unlock();
-    turn = std::unique_lock<std::mutex>(ws.sdpa_mu);
-    lk.lock();
-    if ((rc = grow(s, reinterpret_cast<void**>(&ws.sdpa), &ws.sdpa_bytes,
-                   (size_t)plan.scratch_bytes)))
-      return rc;
-    scratch = ws.sdpa;
-  }
+  if (plan.scratch_bytes > 0 &&
+      (rc = shared_scratch(dev, s, (size_t)plan.scratch_bytes, &scratch, &turn)))
+    return rc;
   return timed("kv_attention", s, [&] {
     return launch_kv_attn(view, q, ldq, out, ldo, heads, scale, causal != 0, plan, scratch, s);
   });

@@ -249,8 +249,18 @@ struct W4View {
 hipError_t launch_w4_repack(const uint8_t* u, const float* scale, const uint8_t* zero, int64_t N,
                             int64_t K, int group, uint8_t* codes, float* scale_out,
                             int8_t* zero_out, hipStream_t s);
+// How a call of M rows runs, and its scratch.
+struct W4Plan {
+  bool few;      // one launch, digits in LDS, no scratch
+  int nb;        // blocks of 16 outputs a workgroup
+  int rt;        // blocks of 16 rows a workgroup (not few)
+  int splits;    // ranges of K in workgroups of their own
+  int64_t rows;  // rows whose digits are made at a time
+  int64_t power_at, sums_at, bad_at, part_at, bytes;  // scratch: digits first
+};
+W4Plan plan_w4(const W4View& w, int64_t M, int cu_count);
 hipError_t launch_w4(const W4View& w, const float* x, int64_t M, const EpiArgs& epi, float* y,
-                     hipStream_t s);
+                     const W4Plan& plan, void* scratch, hipStream_t s);
 // The paged cache (kv::View: sdq_kv.h).
 namespace kv {
 struct View;
