@@ -10,7 +10,7 @@
 // 2^-40 of the largest beneath them. The key's scale multiplies the finished
 // sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in [1/2, 1), E0 the exponent of
 // the sequence's first value: its exponent goes into the softmax,
-//   t_j = s_j + e_j,  X_j = 2^(t_j - m), m the running maximum of t,
+//   t_j = s_j + e_j,  X_j = 2^(t_j - m), m near the running maximum of t,
 //   out = 2^E0 sum_j X_j f_j code_j / sum_j X_j 2^-e_j,
 // one exponential a key as before, and the weights that are split into parts
 // are those that count: no value is lost beside another, however far apart the
@@ -41,7 +41,8 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kTop = 15;      // largest q of a tile below 2^kTop
-constexpr int kWeight = 13;   // weights X f enter as X f 2^kWeight
+constexpr int kSlack = 6;     // X stays below 2^kSlack
+constexpr int kWeight = 9;    // weights X f enter as X f 2^kWeight
 constexpr int kFar = 60;      // e_j is held to -kFar .. kFar
 
 struct Args {
@@ -66,9 +67,15 @@ struct Tile {
   int64_t r0;
   int64_t rows;   // of the sequence
   int64_t row0;   // the sequence's first row in q
-  int64_t len;    // keys
-  int64_t first;  // position of the sequence's first row
+  int len;        // keys, at most 2^30
+  int first;      // position of the sequence's first row
 };
+
+// A lane's value that is the same in the whole wave, as a scalar.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return ((int64_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v);
+}
 
 // The tile with number `tile` when every sequence is cut into tiles of RT rows:
 // a scan over the sequences, 64 at a time. The same in every wave.
@@ -91,12 +98,12 @@ __device__ __forceinline__ Tile find_tile(const View& c, int group, int64_t tile
     const uint64_t past = __ballot(base + upto > tile);
     if (past) {
       const int at = __builtin_ctzll(past);
-      t.s = __builtin_amdgcn_readfirstlane(s0 + at);
-      t.r0 = (tile - base - __shfl(upto - count, at)) * RT;
-      t.rows = __shfl(rows, at);
+      t.s = uniform(s0 + at);
+      t.r0 = uniform((tile - base - __shfl(upto - count, at)) * RT);
+      t.rows = uniform(__shfl(rows, at));
       t.row0 = kv::row_of(c, t.s);
-      t.len = kv::length_of(c, t.s);
-      t.first = t.len - t.rows / group;
+      t.len = (int)kv::length_of(c, t.s);
+      t.first = t.len - (int)(t.rows / group);
       return t;
     }
     base += __shfl(upto, 63);
@@ -104,12 +111,16 @@ __device__ __forceinline__ Tile find_tile(const View& c, int group, int64_t tile
   return t;
 }
 
-// Keys that the rows [r, r + n) of a tile see at most (0: none).
-__device__ __forceinline__ int64_t keys_of(const Tile& t, int64_t r, int n, int group, int causal) {
+// Keys that row r sees (0: it has no position, or is none).
+__device__ __forceinline__ int keys_of(const Tile& t, int64_t r, int group, int causal) {
   if (r >= t.rows) return 0;
-  const int64_t last = (r + n < t.rows ? r + n : t.rows) - 1;
-  const int64_t p = t.first + last / group;
+  const int p = t.first + (int)(r / group);
   return p < 0 ? 0 : causal ? (p + 1 < t.len ? p + 1 : t.len) : t.len;
+}
+// And the rows [r, r + n) at most: the last one.
+__device__ __forceinline__ int keys_of_rows(const Tile& t, int64_t r, int n, int group,
+                                            int causal) {
+  return keys_of(t, (r + n < t.rows ? r + n : t.rows) - 1, group, causal);
 }
 
 // Eight codes (two dwords) as fp16: 0x6400 | u is 1024 + u, with u = code + 128.
@@ -132,21 +143,34 @@ __device__ __forceinline__ v2h pair_of(uint32_t a, uint32_t b) {
   return less1152(__builtin_amdgcn_perm(b, a, sel) | 0x64006400u);
 }
 
-__device__ __forceinline__ float xor_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+// Over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a query, by swaps of lane rows.
+template <class F>
+__device__ __forceinline__ float quad(float v, F f) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ float xor_sum(float v) {
-  v = v + __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+__device__ __forceinline__ float quad_max(float v) {
+  return quad(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  return quad(v, [](float a, float b) { return a + b; });
 }
 
-// fp32 to two fp16 parts.
+// fp32 to two fp16 parts, both truncated (two conversions at a time): the high
+// part's remainder is exact, so the pair is off by less than 2^-21.
 __device__ __forceinline__ void parts8(const float x[8], v8h& hi, v8h& lo) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    hi[i] = (_Float16)x[i];
-    lo[i] = (_Float16)(x[i] - (float)hi[i]);
+  for (int i = 0; i < 8; i += 2) {
+    const v2h h = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]));
+    const v2h r = __builtin_bit_cast(
+        v2h, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.f, x[i]),
+                                        __builtin_fmaf((float)h[1], -1.f, x[i + 1])));
+    hi[i] = h[0];
+    hi[i + 1] = h[1];
+    lo[i] = r[0];
+    lo[i + 1] = r[1];
   }
 }
 
@@ -213,45 +237,56 @@ __device__ __forceinline__ int first_exp(const View& c, const Tile& t, int h) {
   return v != 0.f ? __builtin_amdgcn_frexp_expf(v) : 0;
 }
 
-// One query's softmax state in a lane: the maximum is the same in the query's
-// four lanes, the denominator is the lane's own share.
+// One query's softmax state in a lane: the reference m (the maximum of t, or up
+// to kSlack below it; -inf: no key yet) is the same in the query's four lanes,
+// the denominator is the lane's own share.
 struct State {
   float m, l;
 };
 
-// A 32-key block's scores of one query tile (tiles kt, elements i: key 16 kt +
-// 4 g + i) to the two parts of its weights. seen(kt, i): the row sees that key.
-// Returns the factor that the sums so far shrink by.
+// A 32-key block's logits of one query tile, in place of its scores (tiles kt,
+// elements i: key 16 kt + 4 g + i), and their largest. seen(kt, i): the row sees
+// that key.
 template <bool MASK, class Seen>
-__device__ __forceinline__ float soft_step(const v4f s[2], const KeyTerms k[2][4], State& st,
-                                           Seen seen, v8h& hi, v8h& lo) {
-  float t[8];
+__device__ __forceinline__ float logits(v4f s[2], const v4f c[2], const v4f e[2], Seen seen) {
   float mx = -INFINITY;
 #pragma unroll
   for (int kt = 0; kt < 2; kt++)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      float v = __builtin_fmaf(s[kt][i], k[kt][i].c, k[kt][i].e);
+      float v = __builtin_fmaf(s[kt][i], c[kt][i], e[kt][i]);
       if (MASK && !seen(kt, i)) v = -INFINITY;
-      t[4 * kt + i] = v;
+      s[kt][i] = v;
       mx = fmaxf(mx, v);
     }
-  mx = fmaxf(st.m, xor_max(mx));
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  const float shrink = __builtin_amdgcn_exp2f(st.m - ref);
-  st.m = mx;
-  float l = st.l * shrink;
+  return quad_max(mx);
+}
+// Logits to the two parts of the weights.
+template <bool MASK, class Seen>
+__device__ __forceinline__ void weights(const v4f t[2], const v4f w[2], const v4f f[2], State& st,
+                                        Seen seen, v8h& hi, v8h& lo) {
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
   float p[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    const float x = __builtin_amdgcn_exp2f(t[j] - ref);
-    l = __builtin_fmaf(x, k[j >> 2][j & 3].w, l);
-    p[j] = x * k[j >> 2][j & 3].f;
+    const float x = __builtin_amdgcn_exp2f(t[j >> 2][j & 3] - ref);
+    st.l = __builtin_fmaf(x, w[j >> 2][j & 3], st.l);
+    p[j] = x * f[j >> 2][j & 3];
     if (MASK && !seen(j >> 2, j & 3)) p[j] = 0.f;  // its scale may be NaN
   }
-  st.l = l;
   parts8(p, hi, lo);
-  return shrink;
+}
+// The reference rises only when a block's largest logit passes it by more than
+// kSlack (the weights then stay below 2^kSlack, inside fp16 with kWeight):
+// rarely, and then for the whole wave.
+__device__ __forceinline__ bool rises(const State& st, float mx) { return mx > st.m + kSlack; }
+__device__ __forceinline__ void raise(State& st, float mx, v4f acc[8]) {
+  const float m = fmaxf(st.m, mx);
+  const float shrink = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
+  st.m = m;
+  st.l *= shrink;
+#pragma unroll
+  for (int e = 0; e < 8; e++) acc[e] = acc[e] * shrink;
 }
 
 // ---- few rows: a tile of 16, the workgroup's waves share out the keys ----
@@ -260,7 +295,7 @@ constexpr int kFewRows = kvplan::kFewRows;
 constexpr int kFewWaves = kvplan::kFewWaves;
 constexpr int kFewStride = kHd + 4;  // LDS row of a merged sum (bank spread)
 
-__global__ void __launch_bounds__(64 * kFewWaves) kv_attn_few_kernel(Args a) {
+__global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) {
   const View& c = a.c;
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63, r16 = l & 15, g = l >> 4;
   const int z = (int)(blockIdx.x % a.splits);
@@ -286,93 +321,109 @@ __global__ void __launch_bounds__(64 * kFewWaves) kv_attn_few_kernel(Args a) {
   const float qk = __builtin_ldexpf(a.scale2, -qe);
   const int e0 = first_exp(c, t, h);
 
-  const int64_t keys = keys_of(t, t.r0, kFewRows, a.group, a.causal);
-  const int64_t blocks = (keys + 31) / 32;
-  const int64_t b0 = blocks * z / a.splits, b1 = blocks * (z + 1) / a.splits;
+  const int keys = keys_of_rows(t, t.r0, kFewRows, a.group, a.causal);
+  const int blocks = (keys + 31) / 32;
+  const int b0 = (int)((int64_t)blocks * z / a.splits);
+  const int b1 = (int)((int64_t)blocks * (z + 1) / a.splits);
   // what this lane's row sees, and what every row of the tile does
-  const int64_t pos = t.first + (t.r0 + r16) / a.group;
-  const int64_t mine = t.r0 + r16 >= t.rows || pos < 0 ? 0
-                       : a.causal                      ? (pos + 1 < t.len ? pos + 1 : t.len)
-                                                       : t.len;
-  int64_t all = mine;
-  if (t.r0 + r16 >= t.rows) all = keys;
-#pragma unroll
-  for (int o = 8; o; o >>= 1) {
-    const int64_t u = __shfl_xor(all, o);
-    all = u < all ? u : all;
-  }
+  const int mine = keys_of(t, t.r0 + r16, a.group, a.causal);
+  const int all = keys_of(t, t.r0, a.group, a.causal);  // the first row
 
   State st{-INFINITY, 0.f};
   v4f acc[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) acc[e] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  const int32_t* table = c.table + t.s * c.max_pages;
-  for (int64_t b = b0 + w; b < b1; b += kFewWaves) {
-    uint4 kr[2][2];
-    uint2 vr[2][4];
+  // A block's codes and scales, loaded one block ahead, its pages another one.
+  struct Raw {
+    uint4 k[2][2];
+    uint2 v[2][4];
     float4 ks[2], vs[2];
     bool there[2];
+  };
+  const int32_t* table = c.table + t.s * c.max_pages;
+  auto page_at = [&](int b, int kt) {
+    const int p = b * 32 + 16 * kt;
+    return b < b1 && p < keys ? table[p >> c.page_log2] : -1;
+  };
+  auto load = [&](int b, const int pages[2], Raw& r) {
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
-      const int64_t p = b * 32 + 16 * kt;
-      int64_t page = p < keys ? table[p >> c.page_log2] : -1;
-      there[kt] = page >= 0 && page < c.pages;
-      if (!there[kt]) page = 0;
-      const int64_t at =
-          ((page * c.kv_heads + h) << c.page_log2) + (p & ((1 << c.page_log2) - 1));
+      const int p = b * 32 + 16 * kt;
+      r.there[kt] = pages[kt] >= 0 && pages[kt] < c.pages;
+      const int64_t at = (((r.there[kt] ? pages[kt] : 0) * (int64_t)c.kv_heads + h)
+                          << c.page_log2) + (p & ((1 << c.page_log2) - 1));
       const int8_t* kp = c.k + (at + r16) * kHd + 16 * g;
-      kr[kt][0] = *reinterpret_cast<const uint4*>(kp);
-      kr[kt][1] = *reinterpret_cast<const uint4*>(kp + 64);
+      r.k[kt][0] = *reinterpret_cast<const uint4*>(kp);
+      r.k[kt][1] = *reinterpret_cast<const uint4*>(kp + 64);
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        vr[kt][i] = *reinterpret_cast<const uint2*>(c.v + (at + 4 * g + i) * kHd + 8 * r16);
-      ks[kt] = *reinterpret_cast<const float4*>(c.ks + at + 4 * g);
-      vs[kt] = *reinterpret_cast<const float4*>(c.vs + at + 4 * g);
+        r.v[kt][i] = *reinterpret_cast<const uint2*>(c.v + (at + 4 * g + i) * kHd + 8 * r16);
+      r.ks[kt] = *reinterpret_cast<const float4*>(c.ks + at + 4 * g);
+      r.vs[kt] = *reinterpret_cast<const float4*>(c.vs + at + 4 * g);
     }
-    v4f s[2];
-    KeyTerms kk[2][4];
+  };
+  Raw cur;
+  int pages[2];
+  if (b0 + w < b1) {
+    pages[0] = page_at(b0 + w, 0), pages[1] = page_at(b0 + w, 1);
+    load(b0 + w, pages, cur);
+    pages[0] = page_at(b0 + w + kFewWaves, 0), pages[1] = page_at(b0 + w + kFewWaves, 1);
+  }
+  for (int b = b0 + w; b < b1; b += kFewWaves) {
+    Raw nxt;
+    if (b + kFewWaves < b1) {
+      load(b + kFewWaves, pages, nxt);
+      pages[0] = page_at(b + 2 * kFewWaves, 0), pages[1] = page_at(b + 2 * kFewWaves, 1);
+    }
+    v4f s[2], kc[2], ke[2], kw[2], kf[2];
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
       s[kt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kb = 0; kb < 4; kb++) {
-        const uint4 r = kr[kt][kb >> 1];
+        const uint4 r = cur.k[kt][kb >> 1];
         const v8h ka = kb & 1 ? codes8(r.z, r.w) : codes8(r.x, r.y);
         s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[kb], s[kt], 0, 0, 0);
         s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[kb], s[kt], 0, 0, 0);
       }
-      const float ksv[4] = {ks[kt].x, ks[kt].y, ks[kt].z, ks[kt].w};
-      const float vsv[4] = {vs[kt].x, vs[kt].y, vs[kt].z, vs[kt].w};
+      const float ksv[4] = {cur.ks[kt].x, cur.ks[kt].y, cur.ks[kt].z, cur.ks[kt].w};
+      const float vsv[4] = {cur.vs[kt].x, cur.vs[kt].y, cur.vs[kt].z, cur.vs[kt].w};
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        kk[kt][i] = key_terms(ksv[i], vsv[i],
-                              there[kt] && b * 32 + 16 * kt + 4 * g + i < t.len, qk, e0);
+      for (int i = 0; i < 4; i++) {
+        const KeyTerms k = key_terms(ksv[i], vsv[i],
+                                     cur.there[kt] && b * 32 + 16 * kt + 4 * g + i < t.len, qk, e0);
+        kc[kt][i] = k.c, ke[kt][i] = k.e, kw[kt][i] = k.w, kf[kt][i] = k.f;
+      }
     }
     v8h ph, pl;
-    float shrink;
-    if (b * 32 + 32 <= all && there[0] && there[1]) {
-      shrink = soft_step<false>(s, kk, st, [](int, int) { return true; }, ph, pl);
+    auto softmax = [&](auto mask, auto seen) {
+      constexpr bool kMask = decltype(mask)::value;
+      const float mx = logits<kMask>(s, kc, ke, seen);
+      if (__any(rises(st, mx))) raise(st, mx, acc);
+      weights<kMask>(s, kw, kf, st, seen, ph, pl);
+    };
+    if (b * 32 + 32 <= all && cur.there[0] && cur.there[1]) {
+      softmax(std::false_type{}, [](int, int) { return true; });
     } else {
-      const int64_t k0 = b * 32 + 4 * g;
-      shrink = soft_step<true>(
-          s, kk, st,
-          [&](int kt, int i) { return there[kt] && k0 + 16 * kt + i < mine; }, ph, pl);
+      const int k0 = b * 32 + 4 * g;
+      softmax(std::true_type{}, [&](int kt, int i) {
+        return cur.there[kt] && k0 + 16 * kt + i < mine;
+      });
     }
     uint32_t va[8], vb[8];  // dims 0-3 and 4-7 of the lane's eight, keys in slot order
 #pragma unroll
     for (int kt = 0; kt < 2; kt++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        va[4 * kt + i] = vr[kt][i].x ^ 0x80808080u;
-        vb[4 * kt + i] = vr[kt][i].y ^ 0x80808080u;
+        va[4 * kt + i] = cur.v[kt][i].x ^ 0x80808080u;
+        vb[4 * kt + i] = cur.v[kt][i].y ^ 0x80808080u;
       }
     auto tile_e = [&](auto I, const uint32_t (&v)[8], v4f& o) {
       constexpr int i = decltype(I)::value;
       const v2h p0 = pair_of<i>(v[0], v[1]), p1 = pair_of<i>(v[2], v[3]);
       const v2h p2 = pair_of<i>(v[4], v[5]), p3 = pair_of<i>(v[6], v[7]);
       const v8h vv{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
-      o = o * shrink;
       o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o, 0, 0, 0);
       o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph, o, 0, 0, 0);
     };
@@ -384,12 +435,13 @@ __global__ void __launch_bounds__(64 * kFewWaves) kv_attn_few_kernel(Args a) {
     tile_e(std::integral_constant<int, 1>{}, vb, acc[5]);
     tile_e(std::integral_constant<int, 2>{}, vb, acc[6]);
     tile_e(std::integral_constant<int, 3>{}, vb, acc[7]);
+    cur = nxt;
   }
 
   // Join the waves: common maximum, then sums.
   __shared__ float2 ml[kFewWaves][kFewRows];
   __shared__ __attribute__((aligned(16))) float sums[kFewWaves][kFewRows][kFewStride];
-  st.l = xor_sum(st.l);
+  st.l = quad_sum(st.l);
   if (g == 0) ml[w][r16] = float2{st.m, st.l};
 #pragma unroll
   for (int i = 0; i < 4; i++) {  // dims 32 g + 8 i + e
@@ -442,18 +494,22 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
   const int row = (int)(i % RT), h = (int)(th % a.c.kv_heads);
   const Tile t = find_tile<RT>(a.c, a.group, a.tile0 + th / a.c.kv_heads);
   if (t.s < 0 || t.r0 + row >= t.rows) return;
+  // lane z holds share z's maximum and denominator (splits <= 64)
   const int64_t at = th * a.splits * RT + row;
-  float m = -INFINITY;
-  for (int z = 0; z < a.splits; z++) m = fmaxf(m, a.part_ml[at + (int64_t)z * RT].x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float den = 0.f, o0 = 0.f, o1 = 0.f;
+  const float2 ml = l < a.splits ? a.part_ml[at + (int64_t)l * RT] : float2{-INFINITY, 0.f};
+  float m = ml.x;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float own = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
+  float den = ml.y * own, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
+#pragma unroll 8
   for (int z = 0; z < a.splits; z++) {
-    const float2 ml = a.part_ml[at + (int64_t)z * RT];
     const float2 v = reinterpret_cast<const float2*>(a.part + (at + (int64_t)z * RT) * kHd)[l];
-    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-    den = __builtin_fmaf(ml.y, f, den);
-    o0 = __builtin_fmaf(v.x, f, o0);
-    o1 = __builtin_fmaf(v.y, f, o1);
+    const float w = __shfl(own, z);
+    o0 = __builtin_fmaf(v.x, w, o0);
+    o1 = __builtin_fmaf(v.y, w, o1);
   }
   const float f =
       den == 0.f ? 0.f : __builtin_ldexpf(1.f, first_exp(a.c, t, h) - kWeight) / den;
@@ -494,7 +550,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   if (t.s < 0) return;
 
   v8h qh[QT][4], ql[QT][4];
-  int64_t mine[QT];
+  int mine[QT];
   float qk;
   int e0;
   {
@@ -505,8 +561,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
       const int64_t r = t.r0 + (w * QT + qt) * 16 + r16;
       load_q(a, t, h, r, g, x[qt]);
       qm = fmaxf(qm, amax_finite(x[qt]));
-      const int64_t pos = t.first + r / a.group;
-      mine[qt] = r >= t.rows || pos < 0 ? 0 : a.causal ? (pos + 1 < t.len ? pos + 1 : t.len) : t.len;
+      mine[qt] = keys_of(t, r, a.group, a.causal);
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) qm = fmaxf(qm, __shfl_xor(qm, o));
@@ -526,27 +581,14 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     qk = __builtin_ldexpf(a.scale2, -qe);
     e0 = first_exp(c, t, h);
   }
-  const int64_t keys = keys_of(t, t.r0, kRows, a.group, a.causal);
-  const int64_t blocks = (keys + KB - 1) / KB;
-  const int64_t b0 = blocks * z / a.splits, b1 = blocks * (z + 1) / a.splits;
-  // keys that the wave's rows see at most, and all of them see
-  int64_t most = 0, all = keys;
-#pragma unroll
-  for (int qt = 0; qt < QT; qt++) {
-    most = mine[qt] > most ? mine[qt] : most;
-    if (t.r0 + (w * QT + qt) * 16 + r16 < t.rows) all = mine[qt] < all ? mine[qt] : all;
-  }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const int64_t u = __shfl_xor(most, o), v = __shfl_xor(all, o);
-    most = u > most ? u : most;
-    all = v < all ? v : all;
-  }
-  // uniform over the wave, so that the branches on them are scalar
-  const int64_t wmost = ((int64_t)__builtin_amdgcn_readfirstlane((int)(most >> 32)) << 32) |
-                        (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
-  const int64_t wall = ((int64_t)__builtin_amdgcn_readfirstlane((int)(all >> 32)) << 32) |
-                       (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
+  const int keys = keys_of_rows(t, t.r0, kRows, a.group, a.causal);
+  const int blocks = (keys + KB - 1) / KB;
+  const int b0 = (int)((int64_t)blocks * z / a.splits);
+  const int b1 = (int)((int64_t)blocks * (z + 1) / a.splits);
+  // keys that the wave's rows see at most, and all of them see (the first row)
+  const int64_t wr = t.r0 + w * QT * 16;
+  const int wmost = wr < t.rows ? keys_of_rows(t, wr, QT * 16, a.group, a.causal) : 0;
+  const int wall = keys_of(t, wr, a.group, a.causal);
 
   State st[QT];
   v4f acc[QT][8];
@@ -566,13 +608,13 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   uint32_t vr[4];
   float ksr = 0.f, vsr = 0.f;
   bool ok = false;
-  auto place = [&](int64_t p, bool& there) -> int64_t {
+  auto place = [&](int p, bool& there) -> int64_t {
     int64_t page = p < keys ? table[p >> c.page_log2] : -1;
     there = page >= 0 && page < c.pages;
     return (((there ? page : 0) * c.kv_heads + h) << c.page_log2) +
            (p & ((1 << c.page_log2) - 1));
   };
-  auto fetch = [&](int64_t b) {
+  auto fetch = [&](int b) {
     bool there;
     int64_t at = place(b * KB + k_key, there);
     kr = *reinterpret_cast<const uint4*>(c.k + at * kHd + 16 * k_j);
@@ -616,10 +658,10 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
       d.f[tid] = k.f;
     }
   };
-  auto compute = [&](const Blk& d, int64_t b) {
+  auto compute = [&](const Blk& d, int b) {
 #pragma unroll
     for (int sub = 0; sub < Blk::kSubs; sub++) {
-      const int64_t k0 = b * KB + 32 * sub;
+      const int k0 = b * KB + 32 * sub;
       if (k0 >= wmost) break;
       v4f s[QT][2];
 #pragma unroll
@@ -636,39 +678,50 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
           }
         }
       }
-      KeyTerms kk[2][4];
-#pragma unroll
-      for (int kt = 0; kt < 2; kt++) {
-        const int at = 32 * sub + 16 * kt + 4 * g;
-        const v4f vc = *reinterpret_cast<const v4f*>(d.c + at);
-        const v4f ve = *reinterpret_cast<const v4f*>(d.e + at);
-        const v4f vw = *reinterpret_cast<const v4f*>(d.w + at);
-        const v4f vf = *reinterpret_cast<const v4f*>(d.f + at);
-#pragma unroll
-        for (int i = 0; i < 4; i++) kk[kt][i] = KeyTerms{vc[i], ve[i], vw[i], vf[i]};
-      }
+      const int at = 32 * sub + 4 * g;
+      auto terms = [&](const float* p, v4f x[2]) {
+        x[0] = *reinterpret_cast<const v4f*>(p + at);
+        x[1] = *reinterpret_cast<const v4f*>(p + at + 16);
+      };
       v8h ph[QT], pl[QT];
-      float shrink[QT];
+      auto softmax = [&](auto mask, auto seen) {
+        constexpr bool kMask = decltype(mask)::value;
+        v4f x[2], y[2];
+        terms(d.c, x);
+        terms(d.e, y);
+        float mx[QT];
+        bool up = false;
 #pragma unroll
-      for (int qt = 0; qt < QT; qt++) {
-        if (k0 + 32 <= wall) {
-          shrink[qt] = soft_step<false>(s[qt], kk, st[qt], [](int, int) { return true; }, ph[qt],
-                                        pl[qt]);
-        } else {
-          const int64_t kg = k0 + 4 * g, end = mine[qt];
-          shrink[qt] = soft_step<true>(
-              s[qt], kk, st[qt], [&](int kt, int i) { return kg + 16 * kt + i < end; }, ph[qt],
-              pl[qt]);
+        for (int qt = 0; qt < QT; qt++) {
+          mx[qt] = logits<kMask>(s[qt], x, y, [&](int kt, int i) { return seen(qt, kt, i); });
+          up |= rises(st[qt], mx[qt]);
         }
+        if (__any(up)) {
+#pragma unroll
+          for (int qt = 0; qt < QT; qt++) raise(st[qt], mx[qt], acc[qt]);
+        }
+        terms(d.w, x);
+        terms(d.f, y);
+#pragma unroll
+        for (int qt = 0; qt < QT; qt++)
+          weights<kMask>(s[qt], x, y, st[qt], [&](int kt, int i) { return seen(qt, kt, i); },
+                         ph[qt], pl[qt]);
+      };
+      if (k0 + 32 <= wall) {
+        softmax(std::false_type{}, [](int, int, int) { return true; });
+      } else {
+        const int kg = k0 + 4 * g;
+        softmax(std::true_type{},
+                [&](int qt, int kt, int i) { return kg + 16 * kt + i < mine[qt]; });
       }
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const v8h va = *reinterpret_cast<const v8h*>(d.v[sub][e] + l * 16);
 #pragma unroll
         for (int qt = 0; qt < QT; qt++) {
-          v4f o = acc[qt][e] * shrink[qt];
+          v4f& o = acc[qt][e];
           o = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[qt], o, 0, 0, 0);
-          acc[qt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[qt], o, 0, 0, 0);
+          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[qt], o, 0, 0, 0);
         }
       }
     }
@@ -679,7 +732,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     stage(buf[b0 & 1]);
     if (b0 + 1 < b1) fetch(b0 + 1);
     __syncthreads();
-    for (int64_t b = b0; b < b1; b++) {
+    for (int b = b0; b < b1; b++) {
       if (b + 1 < b1) stage(buf[(b + 1) & 1]);
       if (b + 2 < b1) fetch(b + 2);
       compute(buf[b & 1], b);
@@ -692,7 +745,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     const int row = (w * QT + qt) * 16 + r16;
     const int64_t r = t.r0 + row;
     if (r >= t.rows) continue;
-    const float den = xor_sum(st[qt].l);
+    const float den = quad_sum(st[qt].l);
     float f = 1.f;
     float* dst;
     if (a.splits == 1) {

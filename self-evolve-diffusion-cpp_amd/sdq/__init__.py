@@ -188,13 +188,39 @@ def device_info() -> dict:
                 arch=info.arch.decode())
 
 
+_torch = None
+
+
+def _get_torch():
+    """torch, imported when the first device tensor is met."""
+    global _torch, _raw_stream
+    if _torch is None:
+        import torch
+        _DTYPES.update({k: getattr(torch, v) for k, v in _DT.items()})
+        _torch, _raw_stream = torch, _find_raw_stream()
+    return _torch
+
+
 def _stream(stream):
     if stream is None:
-        import torch
-        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        torch = _get_torch()
+        if _raw_stream is not None:  # the same handle without a Stream object
+            return _raw_stream(torch.cuda.current_device())
+        return torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
-        return ctypes.c_void_p(stream)
-    return ctypes.c_void_p(stream.cuda_stream)
+        return stream
+    return stream.cuda_stream
+
+
+def _find_raw_stream():
+    try:
+        from torch._C import _cuda_getCurrentRawStream
+        return _cuda_getCurrentRawStream
+    except ImportError:  # no torch, or one without it
+        return None
+
+
+_raw_stream = None
 
 
 def _ptr(t):
@@ -210,6 +236,7 @@ def _bad(msg):
 
 
 _DT = {"f32": "float32", "i32": "int32", "i8": "int8", "u8": "uint8"}
+_DTYPES = {}  # the same as torch dtypes, filled by _get_torch
 
 
 class _Args:
@@ -220,6 +247,8 @@ class _Args:
     SdqError (ERR_INVALID) here. Calling the object checks one argument's
     type, element type, shape and layout and returns its address; done()
     then checks that every argument lives on the current GPU."""
+
+    __slots__ = ("_seen",)
 
     def __init__(self):
         self._seen = []
@@ -232,34 +261,38 @@ class _Args:
             if optional:
                 return None
             raise _bad(f"{name}: required")
-        import torch
-
+        torch = _torch or _get_torch()
         if not isinstance(t, torch.Tensor):
             raise _bad(f"{name}: expected a torch device tensor, got {type(t).__name__}")
-        want = getattr(torch, _DT[dt])
-        if t.dtype != want:
-            raise _bad(f"{name}: dtype {t.dtype}, expected {want}")
+        if t.dtype is not _DTYPES[dt]:
+            raise _bad(f"{name}: dtype {t.dtype}, expected {_DTYPES[dt]}")
         if shape is not None:
-            if t.dim() != len(shape) or any(w is not None and int(d) != int(w)
-                                            for d, w in zip(t.shape, shape)):
+            have = t.shape
+            bad = len(have) != len(shape)
+            if not bad:
+                for d, w in zip(have, shape):
+                    if w is not None and d != w:
+                        bad = True
+            if bad:
                 want_s = tuple("*" if w is None else int(w) for w in shape)
-                raise _bad(f"{name}: shape {tuple(t.shape)}, expected {want_s}")
+                raise _bad(f"{name}: shape {tuple(have)}, expected {want_s}")
         if contig:
             if not t.is_contiguous():
                 raise _bad(f"{name}: must be contiguous")
         elif t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
             raise _bad(f"{name}: must be 2-D with contiguous rows")
         self._seen.append((name, t))
-        return ctypes.c_void_p(t.data_ptr())
+        return t.data_ptr()
 
     def done(self):
-        import torch
-
+        torch = _torch or _get_torch()
+        cur = None
         for name, t in self._seen:
             if not t.is_cuda:
                 raise _bad(f"{name}: must be on the GPU (got device {t.device})")
-            cur = torch.cuda.current_device()
-            if t.device.index is not None and t.device.index != cur:
+            if cur is None:
+                cur = torch.cuda.current_device()
+            if t.get_device() != cur:
                 raise _bad(f"{name}: on {t.device}, current device is cuda:{cur}")
 
 
@@ -839,18 +872,35 @@ def q4linear(w: Weight4, A, out, kind="none", bias=None, gate=None, resid=None, 
     return out
 
 
-class KvCache:
+class _KvTensors:
+    """Device tensors behind a struct of the paged cache, checked once: their
+    addresses are the struct's for the object's life, so they cannot be replaced."""
+
+    def __init__(self, tensors):
+        self._tensors = tensors
+        one = next(iter(tensors.items()))
+        for name, t in tensors.items():
+            if t.device != one[1].device:
+                raise _bad(f"{name}: on {t.device}, {one[0]} on {one[1].device}")
+        self._one = one
+
+
+class KvCache(_KvTensors):
     """A pool of pages of int8 keys and values (sdq_kv_cache): device tensors k, v
     int8 [pages, kv_heads, page_size, 128] and their scales ks, vs float32
     [pages, kv_heads, page_size], all contiguous."""
 
     def __init__(self, k, ks, v, vs):
-        if k.dim() != 4 or k.shape[3] != 128:
-            raise _bad(f"k: shape {tuple(k.shape)}, expected (pages, kv_heads, page_size, 128)")
-        self.pages, self.kv_heads, self.page_size = (int(n) for n in k.shape[:3])
+        c = _Args()
+        pk = c(k, "cache.k", "i8", (None, None, None, 128))
+        shape = tuple(int(n) for n in k.shape[:3])
+        self.pages, self.kv_heads, self.page_size = shape
         if self.page_size not in (1 << i for i in range(4, 16)):
             raise _bad(f"page_size: {self.page_size}, expected a power of two from 16 to 32768")
-        self.k, self.ks, self.v, self.vs = k, ks, v, vs
+        self._view = KvCacheView(pk, c(ks, "cache.ks", "f32", shape),
+                                 c(v, "cache.v", "i8", shape + (128,)),
+                                 c(vs, "cache.vs", "f32", shape), *shape[::2], shape[1])
+        super().__init__({"cache.k": k, "cache.ks": ks, "cache.v": v, "cache.vs": vs})
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, device="cuda"):
@@ -863,46 +913,47 @@ class KvCache:
                    torch.zeros(shape + (128,), dtype=torch.int8, device=device),
                    torch.zeros(shape, device=device))
 
-    def _view(self, c):
-        shape = (self.pages, self.kv_heads, self.page_size)
-        return KvCacheView(c(self.k, "cache.k", "i8", shape + (128,)).value,
-                           c(self.ks, "cache.ks", "f32", shape).value,
-                           c(self.v, "cache.v", "i8", shape + (128,)).value,
-                           c(self.vs, "cache.vs", "f32", shape).value,
-                           self.pages, self.page_size, self.kv_heads)
+    k = property(lambda self: self._tensors["cache.k"])
+    ks = property(lambda self: self._tensors["cache.ks"])
+    v = property(lambda self: self._tensors["cache.v"])
+    vs = property(lambda self: self._tensors["cache.vs"])
 
 
-class KvBatch:
+class KvBatch(_KvTensors):
     """A batch of ragged sequences over a KvCache (sdq_kv_batch): int32 device
     tensors q_start [nseq + 1] (rows of a call's tensors), lens [nseq] (tokens the
-    cache holds, new ones counted) and table [nseq, max_pages] (page ids)."""
+    cache holds, new ones counted) and table [nseq, max_pages] (page ids). Their
+    contents may change between calls, the tensors not."""
 
     def __init__(self, q_start, lens, table):
-        self.q_start, self.lens, self.table = q_start, lens, table
+        c = _Args()
+        pt = c(table, "table", "i32", (None, None))
+        nseq, most = (int(n) for n in table.shape)
+        self._view = KvBatchView(c(q_start, "q_start", "i32", (nseq + 1,)),
+                                 c(lens, "lens", "i32", (nseq,)), pt, nseq, most)
+        super().__init__({"q_start": q_start, "lens": lens, "table": table})
 
-    def _view(self, c):
-        pt = c(self.table, "table", "i32", (None, None))
-        nseq, most = (int(n) for n in self.table.shape)
-        return KvBatchView(c(self.q_start, "q_start", "i32", (nseq + 1,)).value,
-                           c(self.lens, "lens", "i32", (nseq,)).value, pt.value, nseq, most)
+    q_start = property(lambda self: self._tensors["q_start"])
+    lens = property(lambda self: self._tensors["lens"])
+    table = property(lambda self: self._tensors["table"])
 
 
 def _kv_args(cache, batch, rows, heads):
-    """The checked views of a paged call, and the addresses of its row tensors
-    ((name, tensor) pairs of heads * 128 columns, rows may be strided)."""
+    """The views of a paged call, and the addresses and row strides of its row
+    tensors ((name, tensor) pairs of heads * 128 columns, rows may be strided)."""
     if not isinstance(cache, KvCache) or not isinstance(batch, KvBatch):
         raise _bad("expected a KvCache and a KvBatch")
     c = _Args()
-    vc, vb = cache._view(c), batch._view(c)
     T = None
     ptrs = []
     for name, t in rows:
         p = c(t, name, "f32", (T, heads * 128), contig=False)
         T = t.shape[0]
-        ptrs += [p, _ld(t)]
+        ptrs += (p, _ld(t))
+    c._seen += (cache._one, batch._one)
     c.done()
     load_library()
-    return vc, vb, ptrs, T
+    return cache._view, batch._view, ptrs, T
 
 
 def kv_write(cache: KvCache, batch: KvBatch, k, v, stream=None):

@@ -181,9 +181,12 @@ def test_binding_tensors():
     _raises("v: shape", sdq.kv_write, cache, batch, kv, f(3, 128))
     _raises("k: shape", sdq.kv_read, cache, batch, f(4, 127), kv)
     _raises("q: shape", sdq.kv_attention, cache, batch, kv, kv, 2)
-    _raises("q_start: shape", sdq.kv_attention, cache, sdq.KvBatch(i32(3), i32(1), i32(1, 3)), kv,
-            kv, 1)
-    _raises("lens: dtype", sdq.kv_attention, cache, sdq.KvBatch(i32(2), f(1), i32(1, 3)), kv, kv, 1)
+    _raises("q_start: shape", sdq.KvBatch, i32(3), i32(1), i32(1, 3))
+    _raises("lens: dtype", sdq.KvBatch, i32(2), f(1), i32(1, 3))
+    _raises("expected a KvCache and a KvBatch", sdq.kv_attention, cache, None, kv, kv, 1)
+    with pytest.raises(AttributeError):
+        batch.lens = i32(1)
     _raises("KvCache", sdq.kv_attention, None, batch, kv, kv, 1)
-    _raises("cache.ks: shape", sdq.kv_write, sdq.KvCache(cache.k, f(2, 1, 15), cache.v, cache.vs),
-            batch, kv, kv)
+    _raises("cache.ks: shape", sdq.KvCache, cache.k, f(2, 1, 15), cache.v, cache.vs)
+    _raises("cache.v: must be contiguous", sdq.KvCache, cache.k, cache.ks,
+            torch.zeros(2, 1, 128, 16, dtype=torch.int8).transpose(2, 3), cache.vs)
