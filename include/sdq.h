@@ -438,9 +438,10 @@ int sdq_weight4_free(sdq_weight4* w);
 int sdq_weight4_dims(const sdq_weight4* w, int64_t* N, int64_t* K, int* group);
 /* A [M,K] and Y [M,N] device pointers, row-major, contiguous; epilogues as
  * sdq_qlinear except SDQ_EPI_ACC, which has no meaning here. Activations are
- * not quantized: each row's values enter as 24-bit integers with a power of two
- * per group, exact int32 sums per group, fp32 sums over the groups (errors of
- * a few 1e-7 of the row's norm times the weight's). A row that holds a NaN or an infinity
+ * not quantized: up to five rows enter as 24-bit integers with a power of two per
+ * group, whose sums with the codes are exact, more rows as two fp16 parts (22
+ * bits); sums over the groups are fp32 either way (errors of a few 1e-7 of the
+ * row's norm times the weight's). A row that holds a NaN or an infinity
  * gives NaN. Built for few rows: 1 to 32 read the weight once, more run in
  * blocks of 32. Y must not overlap A (resid may be Y). Stream-ordered; scratch
  * from the stream's workspace as sdq_qlinear (none for the fewest rows). */

@@ -52,7 +52,7 @@ struct sdq_weight4 {
   int group;
   uint8_t* codes;
   float* scale;
-  int8_t* zero;  // nullptr: 8 everywhere
+  uint8_t* zero;  // nullptr: 8 everywhere
 };
 
 namespace sdq {

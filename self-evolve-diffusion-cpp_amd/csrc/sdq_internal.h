@@ -243,20 +243,20 @@ struct W4View {
   int64_t N, K;
   int group;
   const uint8_t* codes;  // ceil(N/16) * ceil(K/128) * 1024 bytes
-  const float* scale;    // [ceil(N/16)][ceil(K/128) * 128 / group][16]
-  const int8_t* zero;    // the same, zero - 8; nullptr: 0
+  const float* scale;    // [ceil(N/16)][ceil(K/128)][128 / group][16]
+  const uint8_t* zero;   // [ceil(N/16)][ceil(K/128)][16][128 / group]; nullptr: 8
 };
 hipError_t launch_w4_repack(const uint8_t* u, const float* scale, const uint8_t* zero, int64_t N,
                             int64_t K, int group, uint8_t* codes, float* scale_out,
-                            int8_t* zero_out, hipStream_t s);
+                            uint8_t* zero_out, hipStream_t s);
 // How a call of M rows runs, and its scratch.
 struct W4Plan {
-  bool few;      // one launch, digits in LDS, no scratch
+  bool few;      // one launch, the rows split in LDS, no scratch
   int nb;        // blocks of 16 outputs a workgroup
   int rt;        // blocks of 16 rows a workgroup (not few)
   int splits;    // ranges of K in workgroups of their own
-  int64_t rows;  // rows whose digits are made at a time
-  int64_t power_at, sums_at, bad_at, part_at, bytes;  // scratch: digits first
+  int64_t rows;  // rows at a time (not few)
+  int64_t power_at, part_at, bytes;  // scratch: the rows' parts, powers, the ranges' sums
 };
 W4Plan plan_w4(const W4View& w, int64_t M, int cu_count);
 hipError_t launch_w4(const W4View& w, const float* x, int64_t M, const EpiArgs& epi, float* y,

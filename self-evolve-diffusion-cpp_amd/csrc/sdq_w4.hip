@@ -3,15 +3,25 @@
 //
 //   Y[m, n] = epilogue( sum_g scale[n, g] sum_{k in g} (u[n, k] - zero[n, g]) x[m, k] )
 //
+// What bounds it: the weight read, half a byte a value; the matrix cores multiply
+// the codes as they are, so that unpacking them and joining the groups' sums (fp32,
+// one scale each) is what the vector units do. Two forms, by the row count:
+//
+// Up to five rows: x as three signed bytes a value, exact int8 MFMAs of the codes,
+// all bytes of all rows in one tile of 16 columns. Three operations unpack eight
+// codes (fp16 ones take nine: 1 x 4096 -> 18432 14.0 us with those, 11.5 so).
+//
+// More rows: x as two fp16 parts, u - zero as exact fp16. Rows fill the tile's
+// columns, both parts add into one sum and a group costs one fma an output (as
+// bytes: eight to join three sums, the powers and the zero points).
+//
 // Layout: blocks of 16 outputs, cut along K into units of 128 values: 1024
-// bytes, lane l's 16 bytes at l * 16 belong to output l % 16 and lane group
-// g = l / 16. A byte holds two codes u - 8 in two's complement, so that
-// masking a half leaves 16 times the signed code in a byte. Group sizes 64 and
-// 128: byte b's low half is k = 16 g + b, its high half k = 64 + 16 g + b.
-// Group size 32: the low halves of bytes 0-7 and 8-15 are k = 8 g + b % 8 of the
-// unit's first and second 32, the high halves those of its third and fourth.
-// scale [block][group][16] f32, zero - 8 [block][group][16] int8. Rows and
-// values past N and K are zero codes with scale 0.
+// bytes, lane l's 16 bytes at l * 16 belong to output l % 16. Dword st holds values
+// k = 32 st + 8 (l / 16) + 0..7 of the unit, value 2 t in nibble t and 2 t + 1 in
+// nibble t + 4: a mask leaves two codes in the low mantissa bits of a pair of fp16
+// (1024 + u, or 1024 + 16 u four bits higher), or four codes as bytes.
+// scale [block][unit][group][16] f32; zero [block][unit][16][group] bytes. Rows
+// and values past N and K are codes 0 with zero 0 or scale 0.
 #include <algorithm>
 
 #include "sdq_device.h"
@@ -22,28 +32,33 @@
 namespace sdq {
 namespace {
 
-// k inside its unit of the nibble (byte b, half h) of lane group g.
-__host__ __device__ __forceinline__ int unit_k(int group, int b, int h, int g) {
-  return group == 32 ? 32 * ((b >> 3) + 2 * h) + 8 * g + (b & 7) : 64 * h + 16 * g + b;
-}
+using dev::v4f;
+using dev::v4i;
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 8;
+constexpr int64_t kFewMaxLds = 60 * 1024;
+constexpr int kNbTall = 4;  // blocks of outputs of a workgroup of 32 rows
+constexpr int kTop = 15;  // a row's largest value below 2^kTop
 
 // One wave a unit: gathers the lane's 32 codes from the row-major nibbles.
 __global__ void __launch_bounds__(256)
-w4_repack_kernel(const uint8_t* __restrict__ u, int64_t N, int64_t K, int group, int64_t units,
-                 int64_t total, uint8_t* __restrict__ out) {
+w4_repack_kernel(const uint8_t* __restrict__ u, int64_t N, int64_t K, int64_t units, int64_t total,
+                 uint8_t* __restrict__ out) {
   const int l = threadIdx.x & 63;
   const int64_t rb = (K + 1) / 2;
   for (int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); f < total;
        f += (int64_t)gridDim.x * 4) {
-    const int64_t n = f / units * 16 + (l & 15), k0 = f % units * 128;
+    const int64_t n = f / units * 16 + (l & 15), k0 = f % units * 128 + 8 * (l >> 4);
     uint32_t w[4] = {0, 0, 0, 0};
-    for (int b = 0; b < 16; b++)
-      for (int h = 0; h < 2; h++) {
-        const int64_t k = k0 + unit_k(group, b, h, l >> 4);
-        if (n < N && k < K) {
-          const uint32_t c = ((uint32_t)u[n * rb + k / 2] >> (4 * (k & 1))) & 15;
-          w[b >> 2] |= (c ^ 8) << (8 * (b & 3) + 4 * h);
-        }
+    for (int st = 0; st < 4; st++)
+      for (int i = 0; i < 8; i++) {
+        const int64_t k = k0 + 32 * st + i;
+        if (n < N && k < K)
+          w[st] |= (((uint32_t)u[n * rb + k / 2] >> (4 * (k & 1))) & 15)
+                   << (4 * ((i >> 1) + 4 * (i & 1)));
       }
     *reinterpret_cast<uint4*>(out + f * 1024 + l * 16) = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -51,14 +66,15 @@ w4_repack_kernel(const uint8_t* __restrict__ u, int64_t N, int64_t K, int group,
 
 __global__ void __launch_bounds__(256)
 w4_scales_kernel(const float* __restrict__ scale, const uint8_t* __restrict__ zero, int64_t N,
-                 int64_t G, int64_t Gp, int64_t total, float* __restrict__ scale_out,
-                 int8_t* __restrict__ zero_out) {
+                 int64_t G, int64_t Gp, int per, int64_t total, float* __restrict__ scale_out,
+                 uint8_t* __restrict__ zero_out) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {
     const int64_t n = i / (16 * Gp) * 16 + (i & 15), g = i / 16 % Gp;
     const bool ok = n < N && g < G;
     scale_out[i] = ok ? scale[n * G + g] : 0.f;
-    if (zero_out) zero_out[i] = ok ? (int8_t)((int)zero[n * G + g] - 8) : (int8_t)0;
+    if (zero_out) zero_out[((i / 16 - g % per) * 16) + (i & 15) * per + g % per] =
+        ok ? zero[n * G + g] & 15 : 0;
   }
 }
 
@@ -76,48 +92,11 @@ __device__ __forceinline__ void store_one(const EpiArgs& e, float* y, int64_t m,
   y[i] = v;
 }
 
-typedef int v2i __attribute__((ext_vector_type(2)));
-using dev::v4i;
+// ---- activations ----
 
-// ---- activations as three signed bytes a value ----
-//
-// A group's values become X = rint(x 2^p), p the largest power with |X| <=
-// 8355711 = 127 (2^16 + 2^8 + 1), and X = d0 2^16 + d1 2^8 + d2 with signed
-// bytes d: the bytes of X + 0x808080 with their top bits flipped. Their
-// products with the codes are int8 MFMAs, exact over a group, and need no
-// unpacking of the weight beyond a mask: the codes stand in the bytes' upper
-// halves, 16 times their value.
-
-// Power of a group whose largest magnitude is mx (finite).
-__device__ __forceinline__ int group_power(float mx) {
-  if (!(mx > 0.f)) return 0;
-  const int p = 23 - __builtin_amdgcn_frexp_expf(mx);
-  return __builtin_ldexpf(mx, p) > 8355711.f ? p - 1 : p;
-}
-__device__ __forceinline__ uint32_t biased(float x, int p) {
-  return (uint32_t)((int)__builtin_rintf(__builtin_ldexpf(x, p)) + 0x808080);
-}
-// Digit D (0 the highest) of eight biased values as two dwords.
-template <int D>
-__device__ __forceinline__ v2i digits8(const uint32_t y[8]) {
-  constexpr uint32_t b = 2 - D;
-  constexpr uint32_t lo = 0x0c0c0000u | b | ((b + 4) << 8), hi = (lo << 16) | 0x0c0cu;
-  auto four = [&](int i) {
-    const uint32_t v = __builtin_amdgcn_perm(y[i + 1], y[i], lo) |
-                       __builtin_amdgcn_perm(y[i + 3], y[i + 2], hi);
-    return (int)(v ^ 0x80808080u);
-  };
-  return v2i{four(0), four(4)};
-}
-__device__ __forceinline__ int sum8(v2i d) {
-  return __builtin_amdgcn_sdot4(d[0], 0x01010101,
-                                __builtin_amdgcn_sdot4(d[1], 0x01010101, 0, false), false);
-}
-
-// Eight consecutive values of a row (zeros past K), and their largest finite
-// magnitude; bad: one was not finite (it enters as 0, its row ends as NaN).
-__device__ __forceinline__ float load8(const float* row, int64_t k, int64_t K, bool vec,
-                                       float v[8], bool& bad) {
+// Eight consecutive values of a row, zeros past K.
+__device__ __forceinline__ void load8(const float* row, int64_t k, int64_t K, bool vec,
+                                      float v[8]) {
   if (vec && k + 8 <= K) {
     const float4 a = *reinterpret_cast<const float4*>(row + k);
     const float4 b = *reinterpret_cast<const float4*>(row + k + 4);
@@ -127,104 +106,127 @@ __device__ __forceinline__ float load8(const float* row, int64_t k, int64_t K, b
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = k + i < K ? row[k + i] : 0.f;
   }
-  float mx = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const bool fine = fabsf(v[i]) <= 3.402823466e38f;
-    bad |= !fine;
-    v[i] = fine ? v[i] : 0.f;
-    mx = fmaxf(mx, fabsf(v[i]));
-  }
-  return mx;
 }
 
-// The group's power and digits of eight values; the threads of a group are
-// GROUP / 8 consecutive lanes. Returns the power; ds[d]: the digits; with SUM,
-// sums[d]: the group's digit sums.
-template <int GROUP, bool SUM>
-__device__ __forceinline__ int digitize(const float v[8], float mx, v2i ds[3], int sums[3]) {
-#pragma unroll
-  for (int o = 1; o < GROUP / 8; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-  const int p = group_power(mx);
-  uint32_t y[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) y[i] = biased(v[i], p);
-  ds[0] = digits8<0>(y);
-  ds[1] = digits8<1>(y);
-  ds[2] = digits8<2>(y);
-  if constexpr (SUM) {
-#pragma unroll
-    for (int d = 0; d < 3; d++) {
-      sums[d] = sum8(ds[d]);
-#pragma unroll
-      for (int o = 1; o < GROUP / 8; o <<= 1) sums[d] += __shfl_xor(sums[d], o);
-    }
-  }
-  return p;
+// ---- weights ----
+
+// What a group's zero point takes off: 1024 + z and 64 + z as pairs of fp16.
+struct ZeroPair {
+  v2h a, b;
+};
+__device__ __forceinline__ ZeroPair zero_pair(uint32_t zz) {  // z in both halves
+  return {__builtin_bit_cast(v2h, 0x64006400u + zz),
+          __builtin_bit_cast(v2h, 0x54005400u + (zz << 4))};
+}
+// A dword's eight codes as an MFMA operand.
+__device__ __forceinline__ v8h operand(uint32_t w, const ZeroPair& z) {
+  const v2h sixteenth{(_Float16)0.0625f, (_Float16)0.0625f};
+  auto low = [&](uint32_t x) {
+    return __builtin_bit_cast(v2h, (x & 0x000f000fu) | 0x64006400u) - z.a;
+  };
+  auto high = [&](uint32_t x) {
+    return __builtin_elementwise_fma(__builtin_bit_cast(v2h, (x & 0x00f000f0u) | 0x64006400u),
+                                     sixteenth, -z.b);
+  };
+  const v2h a = low(w), b = high(w), c = low(w >> 8), d = high(w >> 8);
+  return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// One 64-value step of a weight's unit as an MFMA operand: the low halves of
-// the lane's bytes (H = 0) or the high ones.
-template <int H>
-__device__ __forceinline__ v4i half_of(const uint4& q) {
-  if constexpr (H == 0)
-    return v4i{(int)((q.x << 4) & 0xf0f0f0f0u), (int)((q.y << 4) & 0xf0f0f0f0u),
-               (int)((q.z << 4) & 0xf0f0f0f0u), (int)((q.w << 4) & 0xf0f0f0f0u)};
-  else
-    return v4i{(int)(q.x & 0xf0f0f0f0u), (int)(q.y & 0xf0f0f0f0u), (int)(q.z & 0xf0f0f0f0u),
-               (int)(q.w & 0xf0f0f0f0u)};
-}
-__device__ __forceinline__ long as_long(int a, int b) {
-  return (long)(((uint64_t)(uint32_t)b << 32) | (uint32_t)a);
-}
-
-// A unit's codes with their scales and zero points (lane group g: outputs
-// 4 g .. 4 g + 3 of the block).
-template <int GROUP, bool ZERO>
+// A unit of a block as it is loaded: the codes, the zero points of the lane's
+// output, and the unit's scales spread over the lanes (one each at most): 16
+// lanes share every scale, and they get it through LDS.
 struct Unit {
-  static constexpr int kPer = 128 / GROUP;
   uint4 q;
-  float4 s[kPer];
-  uint32_t z[kPer];
+  uint32_t z;
+  float s;
 };
 template <int GROUP, bool ZERO>
-__device__ __forceinline__ void load_unit(const W4View& w, int64_t unit, int l,
-                                          Unit<GROUP, ZERO>& u) {
+__device__ __forceinline__ void load_unit(const W4View& w, int64_t unit, int l, Unit& u) {
+  constexpr int per = 128 / GROUP;
   u.q = *reinterpret_cast<const uint4*>(w.codes + unit * 1024 + l * 16);
-#pragma unroll
-  for (int i = 0; i < Unit<GROUP, ZERO>::kPer; i++) {
-    const int64_t at = (unit * Unit<GROUP, ZERO>::kPer + i) * 16 + 4 * (l >> 4);
-    u.s[i] = *reinterpret_cast<const float4*>(w.scale + at);
-    if constexpr (ZERO) u.z[i] = *reinterpret_cast<const uint32_t*>(w.zero + at);
+  if (per == 4 || l < per * 16) u.s = w.scale[unit * per * 16 + l];
+  if constexpr (ZERO) {
+    const uint8_t* z = w.zero + unit * per * 16 + (l & 15) * per;
+    if constexpr (per == 4)
+      u.z = *reinterpret_cast<const uint32_t*>(z);
+    else if constexpr (per == 2)
+      u.z = *reinterpret_cast<const uint16_t*>(z);
+    else
+      u.z = *z;
   }
 }
-// Start of a group's sum: -16 (zero - 8) times the digit sum, so that the sum
-// ends as 16 sum (u - zero) d.
-template <bool ZERO>
-__device__ __forceinline__ v4i start_of(uint32_t z, int digit_sum) {
-  if constexpr (!ZERO) return v4i{0, 0, 0, 0};
-  const int s = -16 * digit_sum;
-  return v4i{__mul24((int8_t)z, s), __mul24((int8_t)(z >> 8), s), __mul24((int8_t)(z >> 16), s),
-             __mul24((int8_t)(z >> 24), s)};
+template <int GROUP, bool ZERO>
+__device__ __forceinline__ ZeroPair zeros_of(const Unit& u, int group) {
+  // byte `group` of the word, to the low byte of either half
+  return zero_pair(ZERO ? __builtin_amdgcn_perm(0u, u.z, 0x0c000c00u + 0x00010001u * group)
+                        : 0x00080008u);
+}
+
+// A wave's LDS words for the scales of NB units.
+template <int GROUP, int NB>
+struct ScaleLds {
+  __attribute__((aligned(16))) float s[NB][128 / GROUP * 16];
+};
+template <int GROUP, int NB>
+__device__ __forceinline__ void put_scales(ScaleLds<GROUP, NB>& o, const Unit (&u)[NB], int l) {
+  __builtin_amdgcn_wave_barrier();  // the wave's own words: its LDS accesses stay in order
+#pragma unroll
+  for (int j = 0; j < NB; j++)
+    if (GROUP == 32 || l < 128 / GROUP * 16) o.s[j][l] = u[j].s;
+  __builtin_amdgcn_wave_barrier();
 }
 
 // ---- fewest rows (3 M <= 15 columns of one MFMA tile): one launch ----
 //
-// A workgroup of eight waves makes the digits of all of A in LDS (its first
-// weight units already on their way), then its waves take every eighth unit of
-// NB blocks of 16 outputs. Bound by the weight read; the tile's spare columns
-// cost nothing.
+// A group's values become X = rint(x 2^p), p the largest power with |X| <=
+// 8355711 = 127 (2^16 + 2^8 + 1), and X = d0 2^16 + d1 2^8 + d2 with signed
+// bytes d: the bytes of X + 0x808080 with their top bits flipped. Their sums
+// with the codes are exact over a group.
+//
+// A workgroup of eight waves makes the bytes of all of A in LDS (its first weight
+// units already on their way), then its waves take every eighth unit of NB blocks
+// of 16 outputs. The tile's spare columns cost nothing.
 
-constexpr int kWaves = 8;
-constexpr int64_t kFewMaxLds = 60 * 1024;
+// Power of a group whose largest magnitude is mx (finite).
+__device__ __forceinline__ int group_power(float mx) {
+  if (!(mx > 0.f)) return 0;
+  const int p = 23 - __builtin_amdgcn_frexp_expf(mx);
+  return __builtin_ldexpf(mx, p) > 8355711.f ? p - 1 : p;
+}
+// Digit D (0 the highest) of eight biased values as two dwords, in the order in
+// which a weight dword's low and high halves hold them.
+template <int D>
+__device__ __forceinline__ v2i digits8(const uint32_t y[8]) {
+  constexpr uint32_t b = 2 - D;
+  constexpr uint32_t lo = 0x0c0c0000u | b | ((b + 4) << 8), hi = (lo << 16) | 0x0c0cu;
+  auto four = [&](int i) {  // values i, i + 4, i + 1, i + 5
+    const uint32_t v = __builtin_amdgcn_perm(y[i + 4], y[i], lo) |
+                       __builtin_amdgcn_perm(y[i + 5], y[i + 1], hi);
+    return (int)(v ^ 0x80808080u);
+  };
+  return v2i{four(0), four(2)};
+}
+__device__ __forceinline__ int sum8(v2i d) {
+  return __builtin_amdgcn_sdot4(d[0], 0x01010101,
+                                __builtin_amdgcn_sdot4(d[1], 0x01010101, 0, false), false);
+}
+__device__ __forceinline__ int low_half(uint32_t w) { return (int)(w & 0x0f0f0f0fu); }
+__device__ __forceinline__ int high_half(uint32_t w) { return (int)((w >> 4) & 0x0f0f0f0fu); }
+__device__ __forceinline__ long as_long(int a, int b) {
+  return (long)(((uint64_t)(uint32_t)b << 32) | (uint32_t)a);
+}
+
+constexpr int kFewMaxRows = 5;
 
 struct FewLds {  // offsets of the dynamic LDS, for the host too
-  int64_t digits, power, sums, bytes;
-  __host__ __device__ FewLds(int64_t units, int per, int M, bool zero) {
-    digits = 0;
-    power = units * 128 * 3 * M;
+  int64_t power, sums, scales, bytes;
+  __host__ __device__ FewLds(int64_t units, int per, int M, int nb) {
+    power = units * 128 * 3 * M;  // [64-value step][column][lane group][16 bytes] before it
     sums = power + units * per * M * 4;
-    bytes = sums + (zero ? units * per * 3 * M * 4 : 0);
+    scales = (sums + units * per * 3 * M * 4 + 15) & ~(int64_t)15;
+    bytes = scales + (int64_t)kWaves * nb * per * 16 * 4;
+    const int64_t red = (int64_t)kWaves * nb * 256 * 4;  // the waves' sums, at the end
+    bytes = bytes > red ? bytes : red;
   }
 };
 
@@ -233,101 +235,138 @@ __global__ void __launch_bounds__(64 * kWaves)
 w4_few_kernel(W4View wt, const float* __restrict__ x, int M, int vec, EpiArgs epi,
               float* __restrict__ y) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ int bad_row[5];
-  using U = Unit<GROUP, ZERO>;
-  constexpr int per = U::kPer;
+  __shared__ int bad_row[kFewMaxRows];
+  constexpr int per = 128 / GROUP;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 4;
   const int64_t units = (wt.K + 127) / 128, nblk = (wt.N + 15) / 16;
   const int64_t nb0 = (int64_t)blockIdx.x * NB;
-  const FewLds at(units, per, M, ZERO);
+  const FewLds at(units, per, M, NB);
   const int C = 3 * M;
   int* power = reinterpret_cast<int*>(lds + at.power);
   int* sums = reinterpret_cast<int*>(lds + at.sums);
 
-  U cur[NB];
-  auto load = [&](int64_t u, U (&o)[NB]) {
+  // The zero points here are those of the lane's four outputs of the sum.
+  Unit cur[NB];
+  uint32_t zcur[NB][per] = {};
+  auto load = [&](int64_t u, Unit (&o)[NB], uint32_t (&z)[NB][per]) {
 #pragma unroll
-    for (int j = 0; j < NB; j++)  // past the last block: any block, not stored
-      load_unit(wt, (nb0 + j < nblk ? nb0 + j : nblk - 1) * units + u, l, o[j]);
+    for (int j = 0; j < NB; j++) {  // past the last block: any block, not stored
+      const int64_t unit = (nb0 + j < nblk ? nb0 + j : nblk - 1) * units + u;
+      load_unit<GROUP, false>(wt, unit, l, o[j]);
+      if constexpr (ZERO) {
+#pragma unroll
+        for (int i = 0; i < per; i++)
+          z[j][i] = reinterpret_cast<const uint32_t*>(wt.zero + (unit * 16 + 4 * g) * per)[i];
+      }
+    }
   };
-  if (w < units) load(w, cur);
+  if (w < units) load(w, cur, zcur);
 
-  if (tid < 5) bad_row[tid] = 0;
+  if (tid < kFewMaxRows) bad_row[tid] = 0;
   __syncthreads();
   for (int m = 0; m < M; m++) {
-    const float* row = x + m * wt.K;
     for (int64_t k = tid * 8; k < units * 128; k += 64 * kWaves * 8) {
       float v[8];
-      bool bad = false;
-      const float mx = load8(row, k, wt.K, vec != 0, v, bad);
-      if (bad) bad_row[m] = 1;
-      v2i ds[3];
-      int sm[3];
-      const int p = digitize<GROUP, ZERO>(v, mx, ds, sm);
+      load8(x + m * wt.K, k, wt.K, vec != 0, v);
+      float mx = 0.f;
+      bool bad = false;  // not finite: enters as 0, its row ends as NaN
 #pragma unroll
-      for (int d = 0; d < 3; d++)
-        *reinterpret_cast<v2i*>(lds + ((k >> 6) * C + d * M + m) * 64 + (k & 63)) = ds[d];
+      for (int i = 0; i < 8; i++) {
+        const bool fine = fabsf(v[i]) <= 3.402823466e38f;
+        bad |= !fine;
+        v[i] = fine ? v[i] : 0.f;
+        mx = fmaxf(mx, fabsf(v[i]));
+      }
+      if (bad) bad_row[m] = 1;
+#pragma unroll
+      for (int o = 1; o < GROUP / 8; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+      const int p = group_power(mx);
+      uint32_t b[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        b[i] = (uint32_t)((int)__builtin_rintf(__builtin_ldexpf(v[i], p)) + 0x808080);
+      const v2i ds[3] = {digits8<0>(b), digits8<1>(b), digits8<2>(b)};
+      int sm[3];
+#pragma unroll
+      for (int d = 0; d < 3; d++) {
+        // lane group (k / 8) % 4 of its step: the dwords of 32 values side by side
+        int* o = reinterpret_cast<int*>(
+            lds + (((k >> 6) * C + d * M + m) * 4 + ((k >> 3) & 3)) * 16 + ((k >> 5) & 1) * 4);
+        o[0] = ds[d][0];
+        o[2] = ds[d][1];
+        sm[d] = sum8(ds[d]);
+#pragma unroll
+        for (int i = 1; i < GROUP / 8; i <<= 1) sm[d] += __shfl_xor(sm[d], i);
+      }
       if ((k & (GROUP - 1)) == 0) {
         const int64_t grp = k / GROUP;
         power[grp * M + m] = p;
-        if constexpr (ZERO) {
 #pragma unroll
-          for (int d = 0; d < 3; d++) sums[grp * C + d * M + m] = sm[d];
-        }
+        for (int d = 0; d < 3; d++) sums[grp * C + d * M + m] = sm[d];
       }
     }
   }
   __syncthreads();
 
+  auto& sl = *reinterpret_cast<ScaleLds<GROUP, NB>*>(lds + at.scales +
+                                                     w * (int64_t)sizeof(ScaleLds<GROUP, NB>));
   const int col = (l & 15) < C ? l & 15 : C - 1, m = col % M;
-  const int place = 12 - 8 * (col / M);  // the digit's 2^16, 2^8, 1 and the codes' 1/16
+  const int place = 16 - 8 * (col / M);  // the digit's 2^16, 2^8, 1
   float f[NB][4] = {};
   for (int64_t u = w; u < units; u += kWaves) {
-    U nxt[NB];
-    if (u + kWaves < units) load(u + kWaves, nxt);
-    const char* b = lds + (2 * u * C + col) * 64;
-    int pw[per], sm[per] = {};
+    Unit nxt[NB];
+    uint32_t znxt[NB][per] = {};
+    if (u + kWaves < units) load(u + kWaves, nxt, znxt);
+    put_scales<GROUP, NB>(sl, cur, l);
+    const char* b = lds + ((2 * u * C + col) * 4 + g) * 16;
+    const v4i d0 = *reinterpret_cast<const v4i*>(b);
+    const v4i d1 = *reinterpret_cast<const v4i*>(b + C * 64);
 #pragma unroll
-    for (int i = 0; i < per; i++) {
-      pw[i] = place - power[(u * per + i) * M + m];
-      if constexpr (ZERO) sm[i] = sums[(u * per + i) * C + col];
-    }
-    v4i acc[NB][per];
-    if constexpr (GROUP == 32) {
-#pragma unroll
-      for (int st = 0; st < 4; st++) {  // 32 values each
-        const v2i d = *reinterpret_cast<const v2i*>(b + (st >> 1) * C * 64 + (st & 1) * 32 + 8 * g);
-#pragma unroll
-        for (int j = 0; j < NB; j++) {
-          const v4i a = st < 2 ? half_of<0>(cur[j].q) : half_of<1>(cur[j].q);
-          acc[j][st] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-              st & 1 ? as_long(a[2], a[3]) : as_long(a[0], a[1]), as_long(d[0], d[1]),
-              start_of<ZERO>(cur[j].z[st], sm[st]), 0, 0, 0);
-        }
-      }
-    } else {
-      const v4i d0 = *reinterpret_cast<const v4i*>(b + 16 * g);
-      const v4i d1 = *reinterpret_cast<const v4i*>(b + C * 64 + 16 * g);
-#pragma unroll
-      for (int j = 0; j < NB; j++) {
-        acc[j][0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-            half_of<0>(cur[j].q), d0, start_of<ZERO>(cur[j].z[0], sm[0]), 0, 0, 0);
-        acc[j][per - 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-            half_of<1>(cur[j].q), d1,
-            per == 1 ? acc[j][0] : start_of<ZERO>(cur[j].z[per - 1], sm[per - 1]), 0, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NB; j++)
-#pragma unroll
-      for (int i = 0; i < per; i++) {
-        const float s[4] = {cur[j].s[i].x, cur[j].s[i].y, cur[j].s[i].z, cur[j].s[i].w};
+    for (int j = 0; j < NB; j++) {
+      const uint32_t q[4] = {cur[j].q.x, cur[j].q.y, cur[j].q.z, cur[j].q.w};
+      // a group's sum starts at -z times its digit sum
+      auto start = [&](int i) {
+        const int s = -sums[(u * per + i) * C + col];
+        if constexpr (!ZERO) return v4i{8 * s, 8 * s, 8 * s, 8 * s};
+        auto z = [&](int e) {
+          const int b = e * per + i;
+          return __mul24((int)((zcur[j][b / 4] >> (8 * (b & 3))) & 255u), s);
+        };
+        return v4i{z(0), z(1), z(2), z(3)};
+      };
+      auto join = [&](const v4i& a, int i) {
+        const int p = place - power[(u * per + i) * M + m];
+        const v4f s = *reinterpret_cast<const v4f*>(&sl.s[j][i * 16 + 4 * g]);
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          f[j][e] = __builtin_fmaf(__builtin_ldexpf((float)acc[j][i][e], pw[i]), s[e], f[j][e]);
-      }
+          f[j][e] = __builtin_fmaf(__builtin_ldexpf((float)a[e], p), s[e], f[j][e]);
+      };
+      if constexpr (GROUP == 32) {
 #pragma unroll
-    for (int j = 0; j < NB; j++) cur[j] = nxt[j];
+        for (int st = 0; st < 4; st++) {  // 32 values each
+          const v4i d = st < 2 ? d0 : d1;
+          join(__builtin_amdgcn_mfma_i32_16x16x32_i8(
+                   as_long(low_half(q[st]), high_half(q[st])),
+                   as_long(d[st & 1], d[2 + (st & 1)]), start(st), 0, 0, 0),
+               st);
+        }
+      } else {
+        const v4i a0{low_half(q[0]), low_half(q[1]), high_half(q[0]), high_half(q[1])};
+        const v4i a1{low_half(q[2]), low_half(q[3]), high_half(q[2]), high_half(q[3])};
+        v4i acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, d0, start(0), 0, 0, 0);
+        if constexpr (per == 2) {
+          join(acc, 0);
+          acc = start(1);
+        }
+        join(__builtin_amdgcn_mfma_i32_16x16x64_i8(a1, d1, acc, 0, 0, 0), per - 1);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; j++) {
+      cur[j] = nxt[j];
+#pragma unroll
+      for (int i = 0; i < per; i++) zcur[j][i] = znxt[j][i];
+    }
   }
 
   // Join the waves and the digits, the lowest first.
@@ -339,163 +378,178 @@ w4_few_kernel(W4View wt, const float* __restrict__ x, int M, int vec, EpiArgs ep
     for (int e = 0; e < 4; e++) red[((w * NB + j) * 16 + 4 * g + e) * 16 + (l & 15)] = f[j][e];
   __syncthreads();
   for (int i = tid; i < NB * 16 * M; i += 64 * kWaves) {
-    const int n = i % (NB * 16), mm = i / (NB * 16);
+    const int n = i % (NB * 16), r = i / (NB * 16);
     float v = 0.f;
 #pragma unroll
     for (int d = 2; d >= 0; d--) {
       float t = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWaves; k++) t += red[(k * NB * 16 + n) * 16 + d * M + mm];
+      for (int k = 0; k < kWaves; k++) t += red[(k * NB * 16 + n) * 16 + d * M + r];
       v += t;
     }
-    if (bad_row[mm]) v = __builtin_nanf("");
-    if (nb0 * 16 + n < wt.N) store_one(epi, y, mm, nb0 * 16 + n, wt.N, v);
+    if (bad_row[r]) v = __builtin_nanf("");
+    if (nb0 * 16 + n < wt.N) store_one(epi, y, r, nb0 * 16 + n, wt.N, v);
   }
 }
 
-// ---- more rows: digits made once by a kernel of their own ----
+// ---- more rows ----
 //
-// digits [16-row block][64-value step][digit][row][64 bytes], power [block][group][row],
-// digit sums [block][group][digit][row], bad [row]. One workgroup a row (rows past M: zeros).
+// A first kernel scales each row by a power of two that puts its largest value into
+// [2^14, 2^15) and splits it into fp16 parts, x = hi + lo to 22 bits of every value down
+// to 2^-18 of the largest and an absolute 2^-40 of it below.
+//
+// A workgroup takes NB blocks of 16 outputs and RT blocks of 16 rows, its eight waves
+// every eighth unit of K, their codes one unit ahead, the parts from the L2 a step
+// ahead: with few outputs a workgroup that traffic (128 bytes a value and 32 rows)
+// is the bound, about 10 TB/s, with many the parallelism. (32 x 14336 -> 5120, the
+// product alone: 32 outputs a workgroup 31 us, 64 and K in three ranges 20 us. The
+// waves over outputs instead, 256 of them, and the parts of a range of K in LDS:
+// 28-45 us, filling the LDS and the join of many ranges took what the traffic had;
+// the rows split in that kernel too: no faster.)
+//
+// parts [rows / 16 RT][unit][32-value step][row block][part][lane group][row][16 bytes],
+// power [row].
 
-struct Digits {
-  int8_t* d;
+struct Rows {
+  char* parts;
   int* power;
-  int* sums;
-  int* bad;
 };
 
-template <int GROUP, bool ZERO>
-__global__ void __launch_bounds__(256)
-w4_digits_kernel(const float* __restrict__ x, int64_t M, int64_t K, int vec, Digits o) {
+// One workgroup a row; rows past M are zeros. The first 16384 values stay in
+// registers between the row's maximum and its parts.
+template <int RT>
+__global__ void __launch_bounds__(1024)
+w4_parts_kernel(const float* __restrict__ x, int64_t M, int64_t K, int vec, Rows o) {
+  __shared__ float maxima[16];
   const int64_t r = blockIdx.x, units = (K + 127) / 128;
-  const int64_t rb = r >> 4, groups = units * (128 / GROUP);
-  const int r16 = (int)(r & 15);
-  __shared__ int any;
-  if (threadIdx.x == 0) any = 0;
-  __syncthreads();
+  const int64_t k1 = r < M ? K : 0, k0 = threadIdx.x * 8;
   const float* row = x + (r < M ? r : 0) * K;
-  for (int64_t k = threadIdx.x * 8; k < units * 128; k += 2048) {
-    float v[8];
-    bool bad = false;
-    const float mx = load8(row, r < M ? k : K, K, vec != 0, v, bad);
-    if (bad) any = 1;
-    v2i ds[3];
-    int sm[3];
-    const int p = digitize<GROUP, ZERO>(v, mx, ds, sm);
+  // the largest finite one: what is not makes its own row NaN by itself
+  float mx = 0.f;
+  auto see = [&](const float t[8]) {
 #pragma unroll
-    for (int d = 0; d < 3; d++)
-      *reinterpret_cast<v2i*>(o.d + (((rb * 2 * units + (k >> 6)) * 3 + d) * 16 + r16) * 64 +
-                              (k & 63)) = ds[d];
-    if ((k & (GROUP - 1)) == 0) {
-      const int64_t at = rb * groups + k / GROUP;
-      o.power[at * 16 + r16] = p;
-      if constexpr (ZERO) {
-#pragma unroll
-        for (int d = 0; d < 3; d++) o.sums[(at * 3 + d) * 16 + r16] = sm[d];
-      }
+    for (int e = 0; e < 8; e++) {
+      const float a = fabsf(t[e]);
+      mx = a <= 3.402823466e38f ? fmaxf(mx, a) : mx;
     }
+  };
+  float v[2][8];
+  load8(row, k0, k1, vec != 0, v[0]);
+  load8(row, k0 + 8192, k1, vec != 0, v[1]);
+  see(v[0]);
+  see(v[1]);
+  for (int64_t k = k0 + 16384; k < k1; k += 8192) {
+    float t[8];
+    load8(row, k, k1, vec != 0, t);
+    see(t);
   }
+#pragma unroll
+  for (int i = 32; i; i >>= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
+  if ((threadIdx.x & 63) == 0) maxima[threadIdx.x >> 6] = mx;
   __syncthreads();
-  if (threadIdx.x == 0) o.bad[r] = any;
+#pragma unroll
+  for (int i = 0; i < 16; i++) mx = fmaxf(mx, maxima[i]);
+  const int p = mx > 0.f ? kTop - __builtin_amdgcn_frexp_expf(mx) : 0;
+  if (threadIdx.x == 0) o.power[r] = p;
+  char* to = o.parts + r / (16 * RT) * units * 8192 * RT + (r / 16 % RT) * 2048 + (r & 15) * 16;
+  auto put = [&](int64_t k, const float t[8]) {
+    if (k >= units * 128) return;
+    v8h hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float f = __builtin_ldexpf(t[e], p);
+      hi[e] = (_Float16)f;
+      lo[e] = (_Float16)(f - (float)hi[e]);
+    }
+    char* d = to + (k >> 5) * 2048 * RT + ((k >> 3) & 3) * 256;
+    *reinterpret_cast<v8h*>(d) = hi;
+    *reinterpret_cast<v8h*>(d + 1024) = lo;
+  };
+  put(k0, v[0]);
+  put(k0 + 8192, v[1]);
+  for (int64_t k = k0 + 16384; k < units * 128; k += 8192) {
+    float t[8];
+    load8(row, k, k1, vec != 0, t);
+    put(k, t);
+  }
 }
 
-// RT blocks of 16 rows against NB blocks of 16 outputs, units [units z / S,
-// units (z+1) / S) shared out over eight waves. Columns of an MFMA are the 16
-// rows of one digit, so that a lane holds the three digits' sums of its
-// output and row and joins them at once: d1 2^8 + d2 in int32 (below 2^30), then
-// one fma, the power, the scale.
 template <int GROUP, bool ZERO, int RT, int NB>
-__global__ void __launch_bounds__(64 * kWaves)
-w4_batch_kernel(W4View wt, Digits dg, int64_t M, int splits, EpiArgs epi, float* __restrict__ y,
+__global__ void __launch_bounds__(64 * kWaves, 2)
+w4_batch_kernel(W4View wt, Rows rows, int64_t M, int splits, EpiArgs epi, float* __restrict__ y,
                 float* __restrict__ part) {
-  using U = Unit<GROUP, ZERO>;
-  constexpr int per = U::kPer;
-  constexpr int kRowsP = 16 * RT + 1;  // LDS row of the joined sums
-  __shared__ float red[kWaves][NB * 16][kRowsP];
+  constexpr int kOut = NB * 16, kRowsT = 16 * RT;
+  __shared__ union {
+    float red[kWaves][kRowsT][kOut + 4];
+    ScaleLds<GROUP, NB> s[kWaves];
+  } lds;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 4, r16 = l & 15;
   const int64_t units = (wt.K + 127) / 128, nblk = (wt.N + 15) / 16;
   const int64_t ntiles = (nblk + NB - 1) / NB;
   const int z = (int)(blockIdx.x % splits);
   const int64_t nb0 = blockIdx.x / splits % ntiles * NB;
-  const int64_t rb0 = blockIdx.x / splits / ntiles * RT;
-  const int64_t u0 = units * z / splits, u1 = units * (z + 1) / splits;
+  const int64_t row0 = blockIdx.x / splits / ntiles * kRowsT;
+  const int u0 = (int)(units * z / splits), u1 = (int)(units * (z + 1) / splits);
 
   float f[NB][RT][4] = {};
-  U cur[NB];
-  auto load = [&](int64_t u, U (&o)[NB]) {
+  Unit cur[NB];
+  auto load = [&](int u, Unit (&o)[NB]) {
 #pragma unroll
-    for (int j = 0; j < NB; j++)
-      load_unit(wt, (nb0 + j < nblk ? nb0 + j : nblk - 1) * units + u, l, o[j]);
+    for (int j = 0; j < NB; j++)  // past the last block: any block, not stored
+      load_unit<GROUP, ZERO>(wt, (nb0 + j < nblk ? nb0 + j : nblk - 1) * units + u, l, o[j]);
   };
-  if (u0 + w < u1) load(u0 + w, cur);
-  for (int64_t u = u0 + w; u < u1; u += kWaves) {
-    U nxt[NB];
-    if (u + kWaves < u1) load(u + kWaves, nxt);
-    int pw[RT][per], sm[RT][per][3] = {};
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-      for (int i = 0; i < per; i++) {
-        const int64_t at = (rb0 + rt) * units * per + u * per + i;
-        pw[rt][i] = -4 - dg.power[at * 16 + r16];
-        if constexpr (ZERO) {
-#pragma unroll
-          for (int d = 0; d < 3; d++) sm[rt][i][d] = dg.sums[(at * 3 + d) * 16 + r16];
-        }
-      }
-    auto join = [&](const v4i a[3], int j, int rt, int i) {
-      const float s[4] = {cur[j].s[i].x, cur[j].s[i].y, cur[j].s[i].z, cur[j].s[i].w};
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float c = __builtin_fmaf((float)a[0][e], 65536.f, (float)((a[1][e] << 8) + a[2][e]));
-        f[j][rt][e] = __builtin_fmaf(__builtin_ldexpf(c, pw[rt][i]), s[e], f[j][rt][e]);
-      }
-    };
+  struct Step {
+    v8h hi[RT], lo[RT];
+  };
+  const char* parts = rows.parts + row0 / 16 * units * 8192 + l * 16;
+  auto load_step = [&](int u, int st, Step& x) {
+    const char* b = parts + (u * 4 + st) * (int64_t)(2048 * RT);
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-      const int8_t* b = dg.d + ((rb0 + rt) * 2 * units + 2 * u) * 3072 + r16 * 64;
-      if constexpr (GROUP == 32) {
+      x.hi[rt] = *reinterpret_cast<const v8h*>(b + rt * 2048);
+      x.lo[rt] = *reinterpret_cast<const v8h*>(b + rt * 2048 + 1024);
+    }
+  };
+  Step x[2];
+  if (u0 + w < u1) {
+    load(u0 + w, cur);
+    load_step(u0 + w, 0, x[0]);
+  }
+  for (int u = u0 + w; u < u1; u += kWaves) {
+    // The last unit loads itself again: a branch here, between the matrix
+    // instructions and what reads their results, could make the compiler miss the
+    // wait between the two (tests/test_mfma_hazards.py).
+    const int un = u + kWaves < u1 ? u + kWaves : u;
+    Unit nxt[NB];
+    load(un, nxt);
+    put_scales<GROUP, NB>(lds.s[w], cur, l);
+    v4f acc[NB][RT];
 #pragma unroll
-        for (int st = 0; st < 4; st++) {
-          v2i d[3];
+    for (int st = 0; st < 4; st++) {
+      constexpr int steps = GROUP / 32;  // of a group
+      const int i = st / steps;
+      load_step(st < 3 ? u : un, (st + 1) & 3, x[(st + 1) & 1]);
+      const Step& now = x[st & 1];
 #pragma unroll
-          for (int i = 0; i < 3; i++)
-            d[i] = *reinterpret_cast<const v2i*>(b + (st >> 1) * 3072 + i * 1024 + (st & 1) * 32 +
-                                                 8 * g);
+      for (int j = 0; j < NB; j++) {
+        const uint32_t q[4] = {cur[j].q.x, cur[j].q.y, cur[j].q.z, cur[j].q.w};
+        const v8h a = operand(q[st], zeros_of<GROUP, ZERO>(cur[j], i));
 #pragma unroll
-          for (int j = 0; j < NB; j++) {
-            const v4i q = st < 2 ? half_of<0>(cur[j].q) : half_of<1>(cur[j].q);
-            v4i acc[3];
-#pragma unroll
-            for (int i = 0; i < 3; i++)
-              acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-                  st & 1 ? as_long(q[2], q[3]) : as_long(q[0], q[1]), as_long(d[i][0], d[i][1]),
-                  start_of<ZERO>(cur[j].z[st], sm[rt][st][i]), 0, 0, 0);
-            join(acc, j, rt, st);
-          }
+        for (int rt = 0; rt < RT; rt++) {
+          if (st % steps == 0) acc[j][rt] = v4f{0.f, 0.f, 0.f, 0.f};
+          acc[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, now.lo[rt], acc[j][rt], 0, 0, 0);
+          acc[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, now.hi[rt], acc[j][rt], 0, 0, 0);
         }
-      } else {
-        v4i d[2][3];
-#pragma unroll
-        for (int st = 0; st < 2; st++)
-#pragma unroll
-          for (int i = 0; i < 3; i++)
-            d[st][i] = *reinterpret_cast<const v4i*>(b + st * 3072 + i * 1024 + 16 * g);
+      }
+      if (st % steps == steps - 1) {
 #pragma unroll
         for (int j = 0; j < NB; j++) {
-          v4i acc[3];
+          const v4f s = *reinterpret_cast<const v4f*>(&lds.s[w].s[j][i * 16 + 4 * g]);
 #pragma unroll
-          for (int i = 0; i < 3; i++)
-            acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                half_of<0>(cur[j].q), d[0][i], start_of<ZERO>(cur[j].z[0], sm[rt][0][i]), 0, 0, 0);
-          if constexpr (per == 2) join(acc, j, rt, 0);
+          for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-          for (int i = 0; i < 3; i++)
-            acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                half_of<1>(cur[j].q), d[1][i],
-                per == 1 ? acc[i] : start_of<ZERO>(cur[j].z[per - 1], sm[rt][per - 1][i]), 0, 0, 0);
-          join(acc, j, rt, per - 1);
+            for (int e = 0; e < 4; e++)
+              f[j][rt][e] = __builtin_fmaf(acc[j][rt][e], s[e], f[j][rt][e]);
         }
       }
     }
@@ -503,39 +557,40 @@ w4_batch_kernel(W4View wt, Digits dg, int64_t M, int splits, EpiArgs epi, float*
     for (int j = 0; j < NB; j++) cur[j] = nxt[j];
   }
 
-#pragma unroll
-  for (int j = 0; j < NB; j++)
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) red[w][j * 16 + 4 * g + e][rt * 16 + r16] = f[j][rt][e];
   __syncthreads();
-  for (int i = tid; i < NB * 16 * RT * 16; i += 64 * kWaves) {
-    const int n = i % (NB * 16), r = i / (NB * 16);
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+      *reinterpret_cast<v4f*>(&lds.red[w][rt * 16 + r16][j * 16 + 4 * g]) =
+          v4f{f[j][rt][0], f[j][rt][1], f[j][rt][2], f[j][rt][3]};
+  __syncthreads();
+  // kOut divides the step: a thread keeps its output column
+  const int c = tid % kOut;
+  const int64_t n = nb0 * 16 + c;
+  if (n >= wt.N) return;
+#pragma unroll 1
+  for (int r = tid / kOut; r < kRowsT && row0 + r < M; r += 64 * kWaves / kOut) {
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < kWaves; k++) v += red[k][n][r];
-    const int64_t row = rb0 * 16 + r, at = nb0 * 16 + n;
-    if (row >= M || at >= wt.N) continue;
-    if (splits > 1) {
-      part[((int64_t)z * M + row) * wt.N + at] = v;
-    } else {
-      if (dg.bad[row]) v = __builtin_nanf("");
-      store_one(epi, y, row, at, wt.N, v);
-    }
+    for (int k = 0; k < kWaves; k++) v += lds.red[k][r][c];
+    if (splits > 1)
+      part[((int64_t)z * M + row0 + r) * wt.N + n] = v;
+    else
+      store_one(epi, y, row0 + r, n, wt.N, __builtin_ldexpf(v, -rows.power[row0 + r]));
   }
 }
 
 __global__ void __launch_bounds__(256)
-w4_join_kernel(const float* __restrict__ part, const int* __restrict__ bad, int64_t M, int64_t N,
+w4_join_kernel(const float* __restrict__ part, const int* __restrict__ power, int64_t M, int64_t N,
                int splits, EpiArgs epi, float* __restrict__ y) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * N;
        i += (int64_t)gridDim.x * 256) {
     float v = 0.f;
+#pragma unroll 8
     for (int z = 0; z < splits; z++) v += part[z * M * N + i];
     const int64_t m = i / N;
-    if (bad[m]) v = __builtin_nanf("");
-    store_one(epi, y, m, i - m * N, N, v);
+    store_one(epi, y, m, i - m * N, N, __builtin_ldexpf(v, -power[m]));
   }
 }
 
@@ -545,45 +600,40 @@ hipError_t launch_form(const W4View& w, const float* x, int64_t M, EpiArgs epi, 
   const int vec = w.K % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   const int64_t units = ceil_div(w.K, 128), nblk = ceil_div(w.N, 16);
   if (p.few) {
-    const FewLds lds(units, 128 / GROUP, (int)M, ZERO);
-    const int64_t bytes = std::max<int64_t>(lds.bytes, kWaves * p.nb * 256 * 4);
+    const unsigned bytes = (unsigned)FewLds(units, 128 / GROUP, (int)M, p.nb).bytes;
     const dim3 grid((unsigned)ceil_div(nblk, p.nb)), block(64 * kWaves);
     if (p.nb == 1)
-      hipLaunchKernelGGL((w4_few_kernel<GROUP, ZERO, 1>), grid, block, (unsigned)bytes, s, w, x,
-                         (int)M, vec, epi, y);
+      hipLaunchKernelGGL((w4_few_kernel<GROUP, ZERO, 1>), grid, block, bytes, s, w, x, (int)M, vec,
+                         epi, y);
     else
-      hipLaunchKernelGGL((w4_few_kernel<GROUP, ZERO, 2>), grid, block, (unsigned)bytes, s, w, x,
-                         (int)M, vec, epi, y);
+      hipLaunchKernelGGL((w4_few_kernel<GROUP, ZERO, 2>), grid, block, bytes, s, w, x, (int)M, vec,
+                         epi, y);
     return hipGetLastError();
   }
-  const Digits dg{reinterpret_cast<int8_t*>(scratch), reinterpret_cast<int*>(scratch + p.power_at),
-                  reinterpret_cast<int*>(scratch + p.sums_at),
-                  reinterpret_cast<int*>(scratch + p.bad_at)};
+  const Rows rows{scratch, reinterpret_cast<int*>(scratch + p.power_at)};
   float* part = reinterpret_cast<float*>(scratch + p.part_at);
   for (int64_t r = 0; r < M; r += p.rows) {  // p.rows rows at a time
     const int64_t n = std::min(p.rows, M - r);
-    const int64_t blocks = ceil_div(n, 16 * p.rt);
-    hipLaunchKernelGGL((w4_digits_kernel<GROUP, ZERO>), dim3((unsigned)(blocks * 16 * p.rt)),
-                       dim3(256), 0, s, x + r * w.K, n, w.K, vec, dg);
+    const dim3 all((unsigned)round_up(n, 16 * p.rt));
+    if (p.rt == 1)
+      hipLaunchKernelGGL((w4_parts_kernel<1>), all, dim3(1024), 0, s, x + r * w.K, n, w.K, vec, rows);
+    else
+      hipLaunchKernelGGL((w4_parts_kernel<2>), all, dim3(1024), 0, s, x + r * w.K, n, w.K, vec, rows);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     EpiArgs ep = epi;
     if (ep.resid) ep.resid += r * w.N;
-    const dim3 grid((unsigned)(blocks * ceil_div(nblk, p.nb) * p.splits)), block(64 * kWaves);
+    const dim3 grid((unsigned)(ceil_div(n, 16 * p.rt) * ceil_div(nblk, p.nb) * p.splits));
 #define SDQ_W4B(RT, NB)                                                                         \
-  hipLaunchKernelGGL((w4_batch_kernel<GROUP, ZERO, RT, NB>), grid, block, 0, s, w, dg, n,       \
-                     p.splits, ep, y + r * w.N, part)
-    if (p.rt == 1) {
-      if (p.nb == 2) SDQ_W4B(1, 2); else SDQ_W4B(1, 4);
-    } else {
-      if (p.nb == 2) SDQ_W4B(2, 2); else SDQ_W4B(2, 4);
-    }
+  hipLaunchKernelGGL((w4_batch_kernel<GROUP, ZERO, RT, NB>), grid, dim3(64 * kWaves), 0, s, w,  \
+                     rows, n, p.splits, ep, y + r * w.N, part)
+    if (p.rt == 1) SDQ_W4B(1, 2); else SDQ_W4B(2, kNbTall);
 #undef SDQ_W4B
     e = hipGetLastError();
     if (e == hipSuccess && p.splits > 1) {
       hipLaunchKernelGGL(w4_join_kernel,
                          dim3((unsigned)std::min<int64_t>(ceil_div(n * w.N, 256), 1 << 16)),
-                         dim3(256), 0, s, part, dg.bad, n, w.N, p.splits, ep, y + r * w.N);
+                         dim3(256), 0, s, part, rows.power, n, w.N, p.splits, ep, y + r * w.N);
       e = hipGetLastError();
     }
     if (e != hipSuccess) return e;
@@ -595,52 +645,51 @@ hipError_t launch_form(const W4View& w, const float* x, int64_t M, EpiArgs epi, 
 
 hipError_t launch_w4_repack(const uint8_t* u, const float* scale, const uint8_t* zero, int64_t N,
                             int64_t K, int group, uint8_t* codes, float* scale_out,
-                            int8_t* zero_out, hipStream_t s) {
+                            uint8_t* zero_out, hipStream_t s) {
   const int64_t nb = ceil_div(N, 16), units = ceil_div(K, 128), total = nb * units;
   constexpr int64_t kMaxBlocks = 1 << 22;  // a grid's threads are a 32-bit number
   hipLaunchKernelGGL(w4_repack_kernel,
-                     dim3((unsigned)std::min(ceil_div(total, 4), kMaxBlocks)), dim3(256), 0, s, u, N, K,
-                     group, units, total, codes);
+                     dim3((unsigned)std::min(ceil_div(total, 4), kMaxBlocks)), dim3(256), 0, s, u, N,
+                     K, units, total, codes);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t Gp = units * (128 / group), n = nb * Gp * 16;
-  hipLaunchKernelGGL(w4_scales_kernel, dim3((unsigned)std::min(ceil_div(n, 256), kMaxBlocks)), dim3(256), 0, s, scale,
-                     zero, N, ceil_div(K, group), Gp, n, scale_out, zero_out);
+  const int per = 128 / group;
+  const int64_t Gp = units * per, n = nb * Gp * 16;
+  hipLaunchKernelGGL(w4_scales_kernel, dim3((unsigned)std::min(ceil_div(n, 256), kMaxBlocks)),
+                     dim3(256), 0, s, scale, zero, N, ceil_div(K, group), Gp, per, n, scale_out,
+                     zero_out);
   return hipGetLastError();
 }
 
 W4Plan plan_w4(const W4View& w, int64_t M, int cu_count) {
   W4Plan p{};
   const int64_t units = ceil_div(w.K, 128), nblk = ceil_div(w.N, 16);
-  const int per = 128 / w.group;
   p.splits = 1;
-  p.few = M <= 5 && FewLds(units, per, (int)M, w.zero != nullptr).bytes <= kFewMaxLds;
-  if (p.few) {
-    p.nb = nblk >= 4 * cu_count ? 2 : 1;
-    return p;
-  }
+  p.nb = nblk >= 4 * cu_count ? 2 : 1;
+  p.few = M <= kFewMaxRows && FewLds(units, 128 / w.group, (int)M, p.nb).bytes <= kFewMaxLds;
+  if (p.few) return p;
   p.rt = M > 16 ? 2 : 1;
-  const int64_t high = 16 * p.rt;
-  // digits of at most about 256 MiB at a time
-  p.rows = std::max<int64_t>(1, std::min<int64_t>(ceil_div(M, high),
-                                                  (int64_t(1) << 28) / (units * 384 * high))) * high;
-  const int64_t blocks = ceil_div(std::min(M, p.rows), high);
-  p.nb = nblk * blocks >= 2 * cu_count ? 4 : 2;
-  const int64_t groups = ceil_div(nblk, p.nb) * blocks;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cu_count / std::max<int64_t>(groups, 1) + 1,
-                                                          units / (2 * kWaves), 8}));
-  // a grid's threads are a 32-bit number
-  while (p.rows > high && ceil_div(p.rows, high) * ceil_div(nblk, p.nb) * p.splits > (1 << 22))
-    p.rows -= high;
+  p.nb = p.rt == 2 ? kNbTall : 2;
+  // Ranges of K while all workgroups run at once (two fit a CU of the short form, one
+  // of the tall one) and every wave keeps two units.
+  const int64_t rows = ceil_div(M, 16 * p.rt);
+  p.splits = (int)std::max<int64_t>(
+      1, std::min<int64_t>({(p.rt == 2 ? 1 : 2) * cu_count / (ceil_div(nblk, p.nb) * rows),
+                            units / (2 * kWaves), 16}));
+  // rows at a time: at most 2^22 workgroups (a grid's threads are a 32-bit number)
+  // and 256 MiB of parts, or of partial sums
+  const int64_t high = 16 * p.rt, tiles = ceil_div(nblk, p.nb) * p.splits;
+  int64_t most = std::min((int64_t(1) << 22) / std::max(tiles, high),
+                          (int64_t(1) << 28) / (units * 512 * high));
+  if (p.splits > 1) most = std::min(most, (int64_t(1) << 28) / (p.splits * high * w.N * 4));
+  p.rows = std::min(rows, std::max<int64_t>(1, most)) * high;
   auto put = [&](int64_t bytes) {
     const int64_t at = p.bytes;
     p.bytes += round_up(bytes, 256);
     return at;
   };
-  put(p.rows * units * 384);
-  p.power_at = put(p.rows * units * per * 4);
-  p.sums_at = put(w.zero ? p.rows * units * per * 12 : 0);
-  p.bad_at = put(p.rows * 4);
+  put(p.rows * units * 512);
+  p.power_at = put(p.rows * 4);
   p.part_at = put(p.splits > 1 ? p.splits * std::min(M, p.rows) * w.N * 4 : 0);
   return p;
 }

@@ -1,11 +1,15 @@
 """sdq_q4linear (4-bit weights with group scales and zero points) against the
 product in 64 bits.
 
-Tolerance, from the kernel's arithmetic (sdq.h): every x enters its group as a
-multiple of 2^(E - 22), 2^E <= max|x| of the group, so it is off by at most
-2^-23 of that maximum; sums inside a group are exact; a group's sum takes three
-roundings (conversion, power-of-two and group scale), the sum over G groups and the
-joining of parts at most G + 40 more, each 2^-24 of the sum of magnitudes."""
+Tolerance, from the kernels' arithmetic, the larger of their two forms'. As bytes
+(up to five rows): every x enters its group as a multiple of 2^(E - 22), 2^E <=
+max|x| of the group, so it is off by at most 2^-23 of that maximum; sums inside a
+group are exact. As fp16 parts, scaled so that the largest value of a row's range
+lies in [2^14, 2^15): two roundings by at most 2^-11 of what they round, 2^-22 of
+every value, or half of fp16's smallest step, 2^-25, which is 2^-39 of the largest;
+a group's sum is 2 * group / 32 MFMAs of 32 exact products, of which each is
+counted with 8 roundings to fp32 of 2^-24. Both: three roundings a group and at
+most G + 40 over the G groups, where waves, parts and ranges join."""
 import numpy as np
 import pytest
 
@@ -36,15 +40,17 @@ def expected(x, u, scale, zero, group):
     c, s = weights64(u, scale, zero, K, group)
     x = x.astype(np.float64)
     G = -(-K // group)
-    y, size, off = 0.0, 0.0, 0.0
+    y, size, coarse = 0.0, 0.0, 0.0
     for g in range(G):
         k = slice(g * group, min(K, (g + 1) * group))
         part = x[:, k] @ (c[:, k] * s[:, k]).T
         y = y + part
         size = size + np.abs(part)
-        off = off + np.abs(x[:, k]).max(1)[:, None] * np.abs(c[:, k] * s[:, k]).sum(1)[None]
-    tol = 2.0**-23 * off + (G + 43) * 2.0**-24 * size
-    return y, tol
+        coarse = coarse + np.abs(x[:, k]).max(1)[:, None] * np.abs(c[:, k] * s[:, k]).sum(1)[None]
+    products = np.abs(x) @ np.abs(c * s).T
+    parts = ((2.0**-22 + 2 * group / 32 * 8 * 2.0**-24) * products
+             + 2.0**-39 * np.abs(x).max(1)[:, None] * np.abs(c * s).sum(1)[None])
+    return y, np.maximum(parts, 2.0**-23 * coarse) + (G + 43) * 2.0**-24 * size
 
 
 def gelu(y):
