@@ -201,11 +201,13 @@ def _get_torch():
     return _torch
 
 
-def _stream(stream):
+def _stream(stream, device=None):
+    """The handle of a torch stream, an int or None (torch's current stream on
+    `device`, the current one by default)."""
     if stream is None:
-        torch = _get_torch()
+        torch = _torch or _get_torch()
         if _raw_stream is not None:  # the same handle without a Stream object
-            return _raw_stream(torch.cuda.current_device())
+            return _raw_stream(torch.cuda.current_device() if device is None else device)
         return torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
         return stream
@@ -261,39 +263,37 @@ class _Args:
             if optional:
                 return None
             raise _bad(f"{name}: required")
-        torch = _torch or _get_torch()
-        if not isinstance(t, torch.Tensor):
+        if not isinstance(t, (_torch or _get_torch()).Tensor):
             raise _bad(f"{name}: expected a torch device tensor, got {type(t).__name__}")
         if t.dtype is not _DTYPES[dt]:
             raise _bad(f"{name}: dtype {t.dtype}, expected {_DTYPES[dt]}")
-        if shape is not None:
+        if shape is not None and t.shape != shape:
             have = t.shape
-            bad = len(have) != len(shape)
-            if not bad:
-                for d, w in zip(have, shape):
-                    if w is not None and d != w:
-                        bad = True
-            if bad:
+            if len(have) != len(shape) or any(w is not None and d != w
+                                              for d, w in zip(have, shape)):
                 want_s = tuple("*" if w is None else int(w) for w in shape)
                 raise _bad(f"{name}: shape {tuple(have)}, expected {want_s}")
         if contig:
             if not t.is_contiguous():
                 raise _bad(f"{name}: must be contiguous")
-        elif t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        elif t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
             raise _bad(f"{name}: must be 2-D with contiguous rows")
         self._seen.append((name, t))
         return t.data_ptr()
 
     def done(self):
-        torch = _torch or _get_torch()
-        cur = None
+        """The current device, on which every tensor is."""
+        cur = -2
         for name, t in self._seen:
-            if not t.is_cuda:
-                raise _bad(f"{name}: must be on the GPU (got device {t.device})")
-            if cur is None:
-                cur = torch.cuda.current_device()
-            if t.get_device() != cur:
-                raise _bad(f"{name}: on {t.device}, current device is cuda:{cur}")
+            dev = t.get_device()
+            if dev != cur:
+                if not t.is_cuda:
+                    raise _bad(f"{name}: must be on the GPU (got device {t.device})")
+                if cur == -2:
+                    cur = _torch.cuda.current_device()
+                if dev != cur:
+                    raise _bad(f"{name}: on {t.device}, current device is cuda:{cur}")
+        return cur
 
 
 def _ld(t):
@@ -752,8 +752,8 @@ def dequant(aq, asc, y, stream=None):
     M, K = aq.shape
     ps, py = c(asc, "as", "f32", (M,)), c(y, "y", "f32", (M, K))
     load_library()
-    c.done()
-    _check(_lib.sdq_dequant(pq, ps, M, K, py, _stream(stream)))
+    dev = c.done()
+    _check(_lib.sdq_dequant(pq, ps, M, K, py, _stream(stream, dev)))
     return y
 
 
@@ -767,8 +767,9 @@ def qlinear_codes(w: Weight, aq, asc, out, kind="none", bias=None, gate=None, re
     M = aq.shape[0]
     ps = c(asc, "as", "f32", (M,))
     e = _epilogue_args(c, kind, M, w.N, out, bias, gate, resid, gate_fma)
-    c.done()
-    _check(_lib.sdq_qlinear_codes(h, pq, ps, M, w.K, ctypes.byref(e), _ptr(out), _stream(stream)))
+    dev = c.done()
+    _check(_lib.sdq_qlinear_codes(h, pq, ps, M, w.K, ctypes.byref(e), out.data_ptr(),
+                                  _stream(stream, dev)))
     return out
 
 
@@ -784,10 +785,11 @@ def rmsnorm_quant(x, aq, asc, w=None, delta=None, sum_out=None, eps=1e-6, stream
     pw = c(w, "w", "f32", (K,), optional=True)
     pq, ps = c(aq, "aq", "i8", (M, K)), c(asc, "as", "f32", (M,))
     load_library()
-    c.done()
-    ld = lambda t: 0 if t is None else _ld(t)  # noqa: E731
-    _check(_lib.sdq_rmsnorm_quant(px, _ld(x), pd, ld(delta), M, K, pw, eps, ph, ld(sum_out), pq, ps,
-                                  _stream(stream)))
+    dev = c.done()
+    ldd = 0 if delta is None else _ld(delta)
+    lds = 0 if sum_out is None else _ld(sum_out)
+    _check(_lib.sdq_rmsnorm_quant(px, _ld(x), pd, ldd, M, K, pw, eps, ph, lds, pq, ps,
+                                  _stream(stream, dev)))
     return aq, asc
 
 
@@ -867,8 +869,9 @@ def q4linear(w: Weight4, A, out, kind="none", bias=None, gate=None, resid=None, 
     pa = c(A, "A", "f32", (None, w.K))
     M = A.shape[0]
     e = _epilogue_args(c, kind, M, w.N, out, bias, gate, resid, gate_fma)
-    c.done()
-    _check(_lib.sdq_q4linear(w.h, pa, M, w.K, ctypes.byref(e), _ptr(out), _stream(stream)))
+    dev = c.done()
+    _check(_lib.sdq_q4linear(w.h, pa, M, w.K, ctypes.byref(e), out.data_ptr(),
+                             _stream(stream, dev)))
     return out
 
 
@@ -900,6 +903,7 @@ class KvCache(_KvTensors):
         self._view = KvCacheView(pk, c(ks, "cache.ks", "f32", shape),
                                  c(v, "cache.v", "i8", shape + (128,)),
                                  c(vs, "cache.vs", "f32", shape), *shape[::2], shape[1])
+        self._ref = ctypes.byref(self._view)
         super().__init__({"cache.k": k, "cache.ks": ks, "cache.v": v, "cache.vs": vs})
 
     @classmethod
@@ -931,6 +935,7 @@ class KvBatch(_KvTensors):
         nseq, most = (int(n) for n in table.shape)
         self._view = KvBatchView(c(q_start, "q_start", "i32", (nseq + 1,)),
                                  c(lens, "lens", "i32", (nseq,)), pt, nseq, most)
+        self._ref = ctypes.byref(self._view)
         super().__init__({"q_start": q_start, "lens": lens, "table": table})
 
     q_start = property(lambda self: self._tensors["q_start"])
@@ -951,22 +956,22 @@ def _kv_args(cache, batch, rows, heads):
         T = t.shape[0]
         ptrs += (p, _ld(t))
     c._seen += (cache._one, batch._one)
-    c.done()
+    dev = c.done()
     load_library()
-    return cache._view, batch._view, ptrs, T
+    return cache._ref, batch._ref, ptrs, T, dev
 
 
 def kv_write(cache: KvCache, batch: KvBatch, k, v, stream=None):
     """Quantizes the rows of k and v [T, kv_heads*128] into the last places of
     their sequences (sdq_kv_write); rows may be strided."""
-    vc, vb, p, T = _kv_args(cache, batch, (("k", k), ("v", v)), cache.kv_heads)
-    _check(_lib.sdq_kv_write(ctypes.byref(vc), ctypes.byref(vb), *p, T, _stream(stream)))
+    vc, vb, p, T, dev = _kv_args(cache, batch, (("k", k), ("v", v)), cache.kv_heads)
+    _check(_lib.sdq_kv_write(vc, vb, *p, T, _stream(stream, dev)))
 
 
 def kv_read(cache: KvCache, batch: KvBatch, k, v, stream=None):
     """Reads the same places back into k and v (sdq_kv_read)."""
-    vc, vb, p, T = _kv_args(cache, batch, (("k", k), ("v", v)), cache.kv_heads)
-    _check(_lib.sdq_kv_read(ctypes.byref(vc), ctypes.byref(vb), *p, T, _stream(stream)))
+    vc, vb, p, T, dev = _kv_args(cache, batch, (("k", k), ("v", v)), cache.kv_heads)
+    _check(_lib.sdq_kv_read(vc, vb, *p, T, _stream(stream, dev)))
     return k, v
 
 
@@ -975,10 +980,10 @@ def kv_attention(cache: KvCache, batch: KvBatch, q, out, heads, causal=True, sca
     """out = attention of the batch's new tokens over the cache
     (sdq_kv_attention): q and out [T, heads*128], rows may be strided; scale
     defaults to 1/sqrt(128). Rows of no sequence are left as they are."""
-    vc, vb, p, T = _kv_args(cache, batch, (("q", q), ("out", out)), int(heads))
+    vc, vb, p, T, dev = _kv_args(cache, batch, (("q", q), ("out", out)), int(heads))
     scale = 128 ** -0.5 if scale is None else float(scale)
-    _check(_lib.sdq_kv_attention(ctypes.byref(vc), ctypes.byref(vb), *p, T, int(heads), scale,
-                                 1 if causal else 0, _stream(stream)))
+    _check(_lib.sdq_kv_attention(vc, vb, *p, T, int(heads), scale, 1 if causal else 0,
+                                 _stream(stream, dev)))
     return out
 
 
