@@ -158,6 +158,17 @@ __device__ __forceinline__ float quad_sum(float v) {
   return quad(v, [](float a, float b) { return a + b; });
 }
 
+// x - hi of either half of a pair of fp16, exact, in one operation.
+__device__ __forceinline__ float less_low(v2h hi, float x) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(hi), "v"(x));
+  return r;
+}
+__device__ __forceinline__ float less_high(v2h hi, float x) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(hi), "v"(x));
+  return r;
+}
 // fp32 to two fp16 parts, both truncated (two conversions at a time): the high
 // part's remainder is exact, so the pair is off by less than 2^-21.
 __device__ __forceinline__ void parts8(const float x[8], v8h& hi, v8h& lo) {
@@ -165,8 +176,7 @@ __device__ __forceinline__ void parts8(const float x[8], v8h& hi, v8h& lo) {
   for (int i = 0; i < 8; i += 2) {
     const v2h h = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]));
     const v2h r = __builtin_bit_cast(
-        v2h, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.f, x[i]),
-                                        __builtin_fmaf((float)h[1], -1.f, x[i + 1])));
+        v2h, __builtin_amdgcn_cvt_pkrtz(less_low(h, x[i]), less_high(h, x[i + 1])));
     hi[i] = h[0];
     hi[i + 1] = h[1];
     lo[i] = r[0];
@@ -297,7 +307,7 @@ constexpr int kFewStride = kHd + 4;  // LDS row of a merged sum (bank spread)
 
 __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) {
   const View& c = a.c;
-  const int w = threadIdx.x >> 6, l = threadIdx.x & 63, r16 = l & 15, g = l >> 4;
+  const int w = uniform((int)threadIdx.x >> 6), l = threadIdx.x & 63, r16 = l & 15, g = l >> 4;
   const int z = (int)(blockIdx.x % a.splits);
   const int64_t th = blockIdx.x / a.splits;
   const int h = (int)(th % c.kv_heads);
@@ -523,7 +533,16 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 //
 // A block of 8 NW keys is loaded as codes, two blocks ahead, turned to fp16 once
 // by the whole workgroup in the order of the MFMA operands and read by every
-// wave from LDS (two buffers, one barrier a block).
+// wave from LDS (two buffers, one barrier a block). The first half of the waves
+// turns its part before the block's products and the second half after them, so
+// that the two waves of a SIMD meet less often in the same kind of work (768
+// tokens x 28048 keys x 24 heads 605 -> 580 us, twice 4099 x 16411 2560 -> 2410;
+// wave priorities around the products make no difference to either).
+//
+// Bound: 4 MFMA products a score and value (two parts each); 580 us are 76% of the
+// rate that a large fp16 matrix product reaches on this card. Turns taken phase by
+// phase (a barrier after each score, softmax and product phase, the waves of a SIMD
+// one phase apart) do not fit the registers: 1560 us.
 
 template <int NW>
 struct Block {
@@ -732,10 +751,17 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     stage(buf[b0 & 1]);
     if (b0 + 1 < b1) fetch(b0 + 1);
     __syncthreads();
+    const bool first = threadIdx.x < 32 * NW;
     for (int b = b0; b < b1; b++) {
-      if (b + 1 < b1) stage(buf[(b + 1) & 1]);
-      if (b + 2 < b1) fetch(b + 2);
+      if (first) {
+        if (b + 1 < b1) stage(buf[(b + 1) & 1]);
+        if (b + 2 < b1) fetch(b + 2);
+      }
       compute(buf[b & 1], b);
+      if (!first) {
+        if (b + 1 < b1) stage(buf[(b + 1) & 1]);
+        if (b + 2 < b1) fetch(b + 2);
+      }
       __syncthreads();
     }
   }
