@@ -494,16 +494,23 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
     *reinterpret_cast<v4f*>(dst + d) = v4f{o[d], o[d + 1], o[d + 2], o[d + 3]};
 }
 
-// ---- joining the shares of cut keys: one wave a row ----
+// ---- joining the shares of cut keys: W waves a row ----
+//
+// A wave reads up to 8 shares of a row at a time, and its latency is that of its rounds
+// and of finding its tile: more than 8 shares are divided over a row's W = 4 waves (64
+// shares of 32 rows: 20 us with one, 6.6 with four). Few shares of many rows are bound by
+// their bytes (7 of 18432 rows 17 us, 4.9 TB/s; four rows to a wave the same).
 
-template <int RT>
+constexpr int kJoin = 8;  // shares that a wave reads at a time
+
+template <int RT, int W>
 __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
-  const int l = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int l = threadIdx.x & 63, w = uniform((int)threadIdx.x >> 6);
+  const int64_t i = (int64_t)blockIdx.x * (4 / W) + w / W;
   const int64_t th = i / RT;
   const int row = (int)(i % RT), h = (int)(th % a.c.kv_heads);
   const Tile t = find_tile<RT>(a.c, a.group, a.tile0 + th / a.c.kv_heads);
-  if (t.s < 0 || t.r0 + row >= t.rows) return;
+  if (t.s < 0 || t.r0 + row >= t.rows) return;  // with W = 4 for the whole workgroup
   // lane z holds share z's maximum and denominator (splits <= 64)
   const int64_t at = th * a.splits * RT + row;
   const float2 ml = l < a.splits ? a.part_ml[at + (int64_t)l * RT] : float2{-INFINITY, 0.f};
@@ -511,15 +518,34 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   const float own = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
-  float den = ml.y * own, o0 = 0.f, o1 = 0.f;
+  float den = ml.y * own;
 #pragma unroll
   for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
-#pragma unroll 8
-  for (int z = 0; z < a.splits; z++) {
-    const float2 v = reinterpret_cast<const float2*>(a.part + (at + (int64_t)z * RT) * kHd)[l];
-    const float w = __shfl(own, z);
-    o0 = __builtin_fmaf(v.x, w, o0);
-    o1 = __builtin_fmaf(v.y, w, o1);
+  float o0 = 0.f, o1 = 0.f;
+  for (int z0 = kJoin * (w % W); z0 < a.splits; z0 += kJoin * W) {
+    float2 v[kJoin];
+#pragma unroll
+    for (int k = 0; k < kJoin; k++)
+      if (z0 + k < a.splits)
+        v[k] = reinterpret_cast<const float2*>(a.part + (at + (int64_t)(z0 + k) * RT) * kHd)[l];
+#pragma unroll
+    for (int k = 0; k < kJoin; k++)
+      if (z0 + k < a.splits) {
+        const float f = __shfl(own, z0 + k);
+        o0 = __builtin_fmaf(v[k].x, f, o0);
+        o1 = __builtin_fmaf(v[k].y, f, o1);
+      }
+  }
+  if (W > 1) {
+    __shared__ float2 sums[W][64];
+    sums[w][l] = float2{o0, o1};
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int k = 1; k < W; k++) {
+      o0 += sums[k][l].x;
+      o1 += sums[k][l].y;
+    }
   }
   const float f =
       den == 0.f ? 0.f : __builtin_ldexpf(1.f, first_exp(a.c, t, h) - kWeight) / den;
@@ -804,7 +830,10 @@ hipError_t run(Args a, const kvplan::Plan& p, Launch launch, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (p.splits > 1) {
-      hipLaunchKernelGGL((kv_attn_join_kernel<RT>), dim3((unsigned)(n * RT / 4)), dim3(256), 0, s, a);
+      if (p.splits > kJoin)
+        hipLaunchKernelGGL((kv_attn_join_kernel<RT, 4>), dim3((unsigned)(n * RT)), dim3(256), 0, s, a);
+      else
+        hipLaunchKernelGGL((kv_attn_join_kernel<RT, 1>), dim3((unsigned)(n * RT / 4)), dim3(256), 0, s, a);
       e = hipGetLastError();
       if (e != hipSuccess) return e;
     }

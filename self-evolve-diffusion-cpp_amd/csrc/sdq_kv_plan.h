@@ -34,8 +34,10 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   // sum of ceil(rows_s / height) over the sequences that have any
   p.tiles = (rows + std::min<int64_t>(nseq, T) * (p.rows - 1)) / p.rows;
   const int64_t groups = p.tiles * kv_heads;  // workgroups without a cut
-  // Enough workgroups for every CU: a few-row one is four waves that wait for
-  // memory (three to a CU), a chunk's fills half a CU.
+  // Enough workgroups for every CU. A few-row one is four waves that wait for memory, and
+  // two fit a CU at once: three to a CU (8 sequences x 24 heads x 4099 keys: two 52 us,
+  // three 42, four 45, six 47). A chunk's of 256 rows takes a CU's registers, and the
+  // second round evens out what the first leaves idle.
   const int64_t want = (p.rows == kFewRows ? 3 : p.rows == 64 ? 4 : 2) * (int64_t)cu_count;
   const int64_t least = p.rows == kFewRows ? 256 : 512;  // keys of a share
   int64_t s = std::min<int64_t>(want / std::max<int64_t>(groups, 1), most / least);
@@ -43,8 +45,8 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   const int64_t per = (int64_t)kv_heads * p.rows * (128 + 2) * 4;  // bytes a tile and share
   while (s > 1 && p.tiles * per * s > kMaxScratch) s--;
   p.splits = (int)s;
-  // a launch's threads (the join has 64 a row) stay under 2^31
-  const int64_t threads = (int64_t)kv_heads * std::max<int64_t>(512 * s, 64 * p.rows);
+  // a launch's threads (the join has up to 256 a row) stay under 2^31
+  const int64_t threads = (int64_t)kv_heads * std::max<int64_t>(512 * s, 256 * p.rows);
   p.tiles_per_launch = std::max<int64_t>(1, ((int64_t(1) << 31) - 1) / threads);
   if (s > 1) p.tiles_per_launch = std::max(p.tiles_per_launch, p.tiles);
   if (s > 1) {
