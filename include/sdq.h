@@ -442,8 +442,8 @@ int sdq_weight4_dims(const sdq_weight4* w, int64_t* N, int64_t* K, int* group);
  * group, whose sums with the codes are exact, more rows as two fp16 parts (22
  * bits); sums over the groups are fp32 either way (errors of a few 1e-7 of the
  * row's norm times the weight's). A row that holds a NaN or an infinity
- * gives NaN. Built for few rows: 1 to 32 read the weight once, more run in
- * blocks of 32. Y must not overlap A (resid may be Y). Stream-ordered; scratch
+ * gives NaN, and no row's result depends on the others' contents. Built for few rows: 1
+ * to 32 read the weight once, more run in blocks of 32. Y must not overlap A (resid may be Y). Stream-ordered; scratch
  * from the stream's workspace as sdq_qlinear (none for the fewest rows). */
 int sdq_q4linear(const sdq_weight4* w, const float* A, int64_t M, int64_t K,
                  const sdq_epilogue* epi, float* Y, void* stream);
@@ -496,13 +496,15 @@ int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t 
  *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / (heads/kv_heads)]) v[j, ...]
  * over j < lens[s], and j <= p where causal != 0. q and out [T, heads*128] with
  * row strides (16-byte aligned rows), heads a multiple of kv_heads; out must not
- * overlap q. Rows that see no key get 0. The cached codes enter exactly, q and the
- * softmax weights as two fp16 parts each (22 bits), fp32 sums and statistics:
- * errors of about 1e-6 of the values' scale, whatever the scales of keys and
- * values between 2^-60 and 2^60. Few rows cut the keys into shares joined by a second kernel, their
- * scratch from the stream's workspace: a capture needs one call of the same shape
- * before it (SDQ_ERR_INVALID otherwise, the capture stays usable).
- * Results do not depend on the other sequences' contents, nor on timing. */
+ * overlap q (column blocks of one array are fine). Rows that see no key get 0. The
+ * cached codes enter exactly, q and the softmax weights as two fp16 parts each (off by
+ * less than 2^-21), fp32 sums and statistics: errors of about 1e-6 of the values' scale.
+ * Scales of values may lie up to 2^60 on either side of the first one of the sequence and
+ * head (of 2^-16, where that one is smaller); rows that see a larger one are NaN. Up to 32
+ * rows a sequence, and chunks too few for the machine, cut the keys into shares joined
+ * by a second kernel, their scratch from the stream's workspace: a capture needs one call
+ * of the same shape before it (SDQ_ERR_INVALID otherwise, the capture stays usable).
+ * A row's result depends on no other row's contents, nor on timing. */
 int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
                      float* out, int64_t ldo, int64_t T, int heads, float scale, int causal,
                      void* stream);

@@ -4,17 +4,19 @@
 // s_j = scale log2(e) q . k_j:   out = sum_j 2^s_j v_j / sum_j 2^s_j.
 //
 // Numbers. A cached value is code * scale; the codes are exact in fp16, so each
-// fp32 product costs two fp16 MFMA products: q = (hi + lo) 2^-r, r one power of
-// two for a tile of rows that puts its largest element into [2^14, 2^15), and
-// the softmax weight = hi + lo below. hi + lo hold 22 bits, and an absolute
-// 2^-40 of the largest beneath them. The key's scale multiplies the finished
+// fp32 product costs two fp16 MFMA products: q = (hi + lo) 2^-r, r a power of two
+// for each row that puts its largest element into [2^14, 2^15), and the softmax
+// weight = hi + lo below. Both parts are truncated: hi + lo is off by less than
+// 2^-21 of the value, or an absolute 2^-39 of the row's largest. The key's scale multiplies the finished
 // sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in [1/2, 1), E0 the exponent of
-// the sequence's first value: its exponent goes into the softmax,
+// the sequence's first value, at least -16: its exponent goes into the softmax,
 //   t_j = s_j + e_j,  X_j = 2^(t_j - m), m near the running maximum of t,
 //   out = 2^E0 sum_j X_j f_j code_j / sum_j X_j 2^-e_j,
 // one exponential a key as before, and the weights that are split into parts
 // are those that count: no value is lost beside another, however far apart the
-// scales of heavy and light keys are (e_j is held to -60 .. 60).
+// scales of heavy and light keys are. e_j is held to -60 .. 60 (2^-e_j and X_j have to
+// be floats together); a value under that counts with fewer bits, one over it makes
+// its rows NaN.
 //
 // Scores are computed transposed, S^T = K Q^T (16x16x32): a lane then holds one
 // query's scores for keys 4 g + 0..3 (g = lane / 16) of two 16-key tiles, which
@@ -40,10 +42,11 @@ using dev::v4f;
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-constexpr int kTop = 15;      // largest q of a tile below 2^kTop
+constexpr int kTop = 15;      // largest q of a row below 2^kTop
 constexpr int kSlack = 6;     // X stays below 2^kSlack
 constexpr int kWeight = 9;    // weights X f enter as X f 2^kWeight
 constexpr int kFar = 60;      // e_j is held to -kFar .. kFar
+constexpr int kLeast = -16;   // of E0
 
 struct Args {
   View c;
@@ -216,8 +219,9 @@ __device__ __forceinline__ float amax_finite(const float x[4][8]) {
     }
   return m;
 }
-// Exponent that scales a tile's largest |q| below 2^kTop; within what a float's
-// power of two can hold.
+// Exponent that scales a row's largest |q| below 2^kTop; within what a float's power
+// of two can hold. Each row has its own: one of the same tile that holds something
+// huge takes no bits from it.
 __device__ __forceinline__ int q_exp(float m) {
   const int e = m > 0.f ? kTop - __builtin_amdgcn_frexp_expf(m) : 0;
   return e > 100 ? 100 : e;
@@ -230,21 +234,25 @@ struct KeyTerms {
   float c, e, w, f;
 };
 __device__ __forceinline__ KeyTerms key_terms(float ks, float vs, bool ok, float qk, int e0) {
+  const float top = __builtin_ldexpf(1.f, kFar + e0);  // inf: every finite scale fits
   KeyTerms k;
   int e = vs != 0.f ? __builtin_amdgcn_frexp_expf(vs) - e0 : 0;
   e = e < -kFar ? -kFar : e > kFar ? kFar : e;
   k.c = ok ? ks * qk : 0.f;
   k.e = ok ? (float)e : 0.f;
   k.w = ok ? __builtin_ldexpf(1.f, -e) : 0.f;
-  k.f = ok ? __builtin_ldexpf(vs, kWeight - e - e0) : 0.f;
+  // past kFar the weights would not fit fp16, and the conversion would cut them off
+  k.f = !ok ? 0.f : fabsf(vs) >= top ? __builtin_nanf("") : __builtin_ldexpf(vs, kWeight - e - e0);
   return k;
 }
-// E0: the exponent of the sequence's first value scale.
+// E0: the exponent of the sequence's first value scale; from kLeast on, so that a
+// first value of next to nothing leaves those after it their range.
 __device__ __forceinline__ int first_exp(const View& c, const Tile& t, int h) {
   if (t.len <= 0) return 0;
   const int64_t at = kv::place_of(c, t.s, 0, h);
   const float v = at >= 0 ? c.vs[at] : 0.f;
-  return v != 0.f ? __builtin_amdgcn_frexp_expf(v) : 0;
+  const int e = v != 0.f ? __builtin_amdgcn_frexp_expf(v) : 0;
+  return e < kLeast ? kLeast : e;
 }
 
 // One query's softmax state in a lane: the reference m (the maximum of t, or up
@@ -288,10 +296,11 @@ __device__ __forceinline__ void weights(const v4f t[2], const v4f w[2], const v4
 }
 // The reference rises only when a block's largest logit passes it by more than
 // kSlack (the weights then stay below 2^kSlack, inside fp16 with kWeight):
-// rarely, and then for the whole wave.
+// rarely. The branch is the wave's, the rise each row's own, so that no row's bits
+// depend on its neighbours.
 __device__ __forceinline__ bool rises(const State& st, float mx) { return mx > st.m + kSlack; }
 __device__ __forceinline__ void raise(State& st, float mx, v4f acc[8]) {
-  const float m = fmaxf(st.m, mx);
+  const float m = rises(st, mx) ? mx : st.m;
   const float shrink = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
   st.m = m;
   st.l *= shrink;
@@ -317,10 +326,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 
   float x[4][8];
   load_q(a, t, h, t.r0 + r16, g, x);
-  float qm = amax_finite(x);
-#pragma unroll
-  for (int o = 32; o; o >>= 1) qm = fmaxf(qm, __shfl_xor(qm, o));
-  const int qe = q_exp(qm);
+  const int qe = q_exp(quad_max(amax_finite(x)));
   v8h qh[4], ql[4];
 #pragma unroll
   for (int kb = 0; kb < 4; kb++) {
@@ -563,9 +569,10 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 // turns its part before the block's products and the second half after them, so
 // that the two waves of a SIMD meet less often in the same kind of work (768
 // tokens x 28048 keys x 24 heads 605 -> 580 us, twice 4099 x 16411 2560 -> 2410;
-// wave priorities around the products make no difference to either).
+// wave priorities around the products make no difference to either). A power of two for
+// each query row, one more product a score, costs 2.5% and keeps rows independent.
 //
-// Bound: 4 MFMA products a score and value (two parts each); 580 us are 76% of the
+// Bound: 4 MFMA products a score and value (two parts each); 590 us are 76% of the
 // rate that a large fp16 matrix product reaches on this card. Turns taken phase by
 // phase (a barrier after each score, softmax and product phase, the waves of a SIMD
 // one phase apart) do not fit the registers: 1560 us.
@@ -585,7 +592,6 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   using Blk = Block<NW>;
   constexpr int KB = Blk::kKeys;
   __shared__ Blk buf[2];
-  __shared__ float wave_max[NW];
   const View& c = a.c;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, r16 = l & 15, g = l >> 4;
   const int z = (int)(blockIdx.x % a.splits);
@@ -596,36 +602,23 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
 
   v8h qh[QT][4], ql[QT][4];
   int mine[QT];
-  float qk;
-  int e0;
-  {
-    float x[QT][4][8];
-    float qm = 0.f;
+  float qk[QT];
 #pragma unroll
-    for (int qt = 0; qt < QT; qt++) {
-      const int64_t r = t.r0 + (w * QT + qt) * 16 + r16;
-      load_q(a, t, h, r, g, x[qt]);
-      qm = fmaxf(qm, amax_finite(x[qt]));
-      mine[qt] = keys_of(t, r, a.group, a.causal);
+  for (int qt = 0; qt < QT; qt++) {
+    const int64_t r = t.r0 + (w * QT + qt) * 16 + r16;
+    float x[4][8];
+    load_q(a, t, h, r, g, x);
+    mine[qt] = keys_of(t, r, a.group, a.causal);
+    const int qe = q_exp(quad_max(amax_finite(x)));
+#pragma unroll
+    for (int kb = 0; kb < 4; kb++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[kb][i] = __builtin_ldexpf(x[kb][i], qe);
+      parts8(x[kb], qh[qt][kb], ql[qt][kb]);
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) qm = fmaxf(qm, __shfl_xor(qm, o));
-    if (l == 0) wave_max[w] = qm;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NW; i++) qm = fmaxf(qm, wave_max[i]);
-    const int qe = q_exp(qm);
-#pragma unroll
-    for (int qt = 0; qt < QT; qt++)
-#pragma unroll
-      for (int kb = 0; kb < 4; kb++) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[qt][kb][i] = __builtin_ldexpf(x[qt][kb][i], qe);
-        parts8(x[qt][kb], qh[qt][kb], ql[qt][kb]);
-      }
-    qk = __builtin_ldexpf(a.scale2, -qe);
-    e0 = first_exp(c, t, h);
+    qk[qt] = __builtin_ldexpf(a.scale2, -qe);
   }
+  const int e0 = first_exp(c, t, h);
   const int keys = keys_of_rows(t, t.r0, kRows, a.group, a.causal);
   const int blocks = (keys + KB - 1) / KB;
   const int b0 = (int)((int64_t)blocks * z / a.splits);
@@ -696,7 +689,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     put(std::integral_constant<int, 2>{});
     put(std::integral_constant<int, 3>{});
     if (tid < KB) {
-      const KeyTerms k = key_terms(ksr, vsr, ok, qk, e0);
+      const KeyTerms k = key_terms(ksr, vsr, ok, 1.f, e0);
       d.c[tid] = ok ? k.c : 0.f;
       d.e[tid] = ok ? k.e : -INFINITY;  // no key: its logit is -inf in every row
       d.w[tid] = k.w;
@@ -738,6 +731,8 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
         bool up = false;
 #pragma unroll
         for (int qt = 0; qt < QT; qt++) {
+          s[qt][0] = s[qt][0] * qk[qt];
+          s[qt][1] = s[qt][1] * qk[qt];
           mx[qt] = logits<kMask>(s[qt], x, y, [&](int kt, int i) { return seen(qt, kt, i); });
           up |= rises(st[qt], mx[qt]);
         }

@@ -3,8 +3,8 @@
 cache holds.
 
 Attention's tolerance, per row, from its arithmetic: a logit (in units of log2)
-is off by the q parts' 2^-22 and 136 fp32 roundings of the sum of |q k| products,
-plus two roundings of itself and of the running maximum; a weight by its logit's
+is off by the q parts and the fp32 roundings of the sum of |q k| products (128 and 8 more
+beyond them; the parts' 2^-21 are eight of those), plus two roundings of itself and of the running maximum; a weight by its logit's
 error times ln 2, exp2's 2^-22 and the parts' 2^-21; the sums over n keys by
 (n / 8 + 64) 2^-24. Numerator and denominator each, so twice that, of max |v|."""
 import numpy as np
@@ -299,6 +299,48 @@ def test_nan_stays_where_it_is(sdq_dev, new):
     assert np.isnan(got[new:]).all() and np.isfinite(clean).all()
 
 
+@pytest.mark.parametrize("new", [1, 100])
+def test_a_huge_row_takes_nothing_from_others(sdq_dev, new):
+    """A head of a token holds 1e30: the rows beside it, of its own tile among
+    them, keep every bit."""
+    c = Case(sdq_dev, [new], [new + 300], 1, 32, seed=12)
+    q = c.rng.standard_normal((c.T, 3 * HD)).astype(F)
+    first = c.check(3, True, q=q)
+    big = q.copy()
+    big[-1, HD:2 * HD] = F(1e30)
+    out = c.torch.zeros((c.T, 3 * HD), device=sdq_dev)
+    c.sdq.kv_attention(c.cache, c.batch, c.t(big), out, 3, causal=True)
+    got = out.cpu().numpy()
+    keep = np.ones(first.shape, bool)
+    keep[-1, HD:2 * HD] = False
+    assert_bitexact(got[keep], first[keep], "the other rows")
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_range_of_value_scales(sdq_dev, new):
+    """A first value of next to nothing leaves the others their precision; scales
+    2^60 past the first one's are refused the only way a kernel can: NaN in the rows
+    that see them, and in those alone."""
+    c = Case(sdq_dev, [new], [new + 100], 1, 16, seed=13)
+    at = lambda p: (c.table[0, p // 16], 0, p % 16)  # noqa: E731
+    for tiny in (2.0**-40, 2.0**-90, 2.0**-130):
+        c.vs[at(0)] = F(tiny)
+        c.up()
+        q = c.rng.standard_normal((c.T, 2 * HD)).astype(F)
+        got = c.check(2, True, q=q)
+    c.vs[at(0)] = F(0.75)  # its exponent is 0
+    c.vs[at(new + 90)] = F(2.0**59 * 1.99)
+    c.up()
+    c.check(2, True, q=q)
+    c.vs[at(new + 90)] = F(2.0**60)
+    c.up()
+    out = c.torch.zeros((c.T, 2 * HD), device=sdq_dev)
+    c.sdq.kv_attention(c.cache, c.batch, c.t(q), out, 2, causal=True)
+    got = out.cpu().numpy()
+    sees = 100 + np.arange(new) >= new + 90
+    assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
+
+
 def test_shared_pages_and_independence(sdq_dev):
     """Two sequences that share their first pages; a batch's rows do not depend on
     who else is in it, bit for bit where the call's sizes are the same."""
@@ -388,6 +430,89 @@ def test_captured_and_two_streams(sdq_dev, new):
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o, again)
+
+
+def test_growth_under_capture_is_refused(sdq_dev):
+    """A call whose scratch the stream does not have yet raises under capture and leaves the
+    capture usable; after one eager call it captures. (torch hands out pooled streams:
+    the first one that other tests have not grown is taken.)"""
+    import torch
+
+    c = Case(sdq_dev, [250], [40000], 8, 64, seed=14)
+    q = torch.randn((250, 8 * HD), device=sdq_dev)
+    out, want = torch.zeros_like(q), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    for _ in range(64):
+        side = torch.cuda.Stream()
+        g = torch.cuda.CUDAGraph()
+        try:
+            with torch.cuda.graph(g, stream=side):
+                c.sdq.kv_attention(c.cache, c.batch, q, out, 8)
+        except c.sdq.SdqError as e:
+            assert "captures a graph" in str(e)
+            break
+    else:
+        pytest.fail("every stream has the scratch")
+    del g
+    with torch.cuda.stream(side):
+        c.sdq.kv_attention(c.cache, c.batch, q, want, 8)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        c.sdq.kv_attention(c.cache, c.batch, q, out, 8)
+    for _ in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_threads_on_one_stream(sdq_dev):
+    """Four threads on one stream, the calls' scratch the same memory: attention with its keys
+    cut, 4-bit Linears, and the packed attention: each result equals the call alone."""
+    import threading
+
+    import torch
+
+    import sdq
+    import test_gpu_q4linear as q4
+
+    cases = [Case(sdq_dev, [1, 1], [9000, 70], 2, 64, seed=15),
+             Case(sdq_dev, [200], [9000], 2, 32, seed=16)]
+    qs = [torch.randn((c.T, 4 * HD), device=sdq_dev) for c in cases]
+    u, scale, zero = q4.make(512, 4096, 64, True, 3)
+    w = sdq.Weight4.from_host(u, scale, zero, group=64)
+    x = torch.randn((20, 4096), device=sdq_dev)
+    kv = torch.randn((1500, 2 * 384), device=sdq_dev)
+    calls = [(lambda o, s, i=i: sdq.kv_attention(cases[i].cache, cases[i].batch, qs[i], o, 4, stream=s),
+              qs[i].shape) for i in range(2)]
+    calls.append((lambda o, s: sdq.q4linear(w, x, o, stream=s), (20, 512)))
+    calls.append((lambda o, s: sdq.sdpa(kv, kv, kv, o, 3, qcol=0, kcol=0, vcol=384, stream=s),
+                  (1500, 384)))
+    own = torch.cuda.Stream()
+    outs = [[torch.zeros(shape, device=sdq_dev) for _ in range(9)] for _, shape in calls]
+    torch.cuda.synchronize()
+    go = threading.Barrier(len(calls))
+
+    def run(i):
+        sdq.init(0)
+        go.wait()
+        for o in outs[i][1:]:
+            calls[i][0](o, own)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i, (call, _) in enumerate(calls):
+        call(outs[i][0], own)
+        own.synchronize()
+        assert outs[i][0].abs().sum() > 0
+        for o in outs[i][1:]:
+            assert torch.equal(o, outs[i][0]), i
 
 
 # ---- a serving step out of all of them ----
