@@ -399,10 +399,12 @@ w4_few_kernel(W4View wt, const float* __restrict__ x, int M, int vec, EpiArgs ep
 // to 2^-18 of the largest and an absolute 2^-40 of it below.
 //
 // A workgroup takes NB blocks of 16 outputs and RT blocks of 16 rows, its eight waves
-// every eighth unit of K, their codes one unit ahead, the parts from the L2 a step
-// ahead: with few outputs a workgroup that traffic (128 bytes a value and 32 rows)
-// is the bound, about 10 TB/s, with many the parallelism. (32 x 14336 -> 5120, the
-// product alone: 32 outputs a workgroup 31 us, 64 and K in three ranges 20 us. The
+// every eighth unit of K, their codes and the parts one unit ahead. With few outputs a
+// workgroup the parts' traffic (128 bytes a value and 32 rows) is the bound, with
+// many the parallelism: a wave has about five units, and each waits for memory. (32 x
+// 14336 -> 5120, the product alone: 32 outputs a workgroup 31 us, 64 and K in three
+// ranges 20, the parts a unit instead of a step ahead 19; codes two units ahead, or two
+// or four waves over the outputs of one unit: 20-22. The
 // waves over outputs instead, 256 of them, and the parts of a range of K in LDS:
 // 28-45 us, filling the LDS and the join of many ranges took what the traffic had;
 // the rows split in that kernel too: no faster.)
@@ -510,10 +512,11 @@ w4_batch_kernel(W4View wt, Rows rows, int64_t M, int splits, EpiArgs epi, float*
       x.lo[rt] = *reinterpret_cast<const v8h*>(b + rt * 2048 + 1024);
     }
   };
-  Step x[2];
+  Step x[4];
   if (u0 + w < u1) {
     load(u0 + w, cur);
-    load_step(u0 + w, 0, x[0]);
+#pragma unroll
+    for (int st = 0; st < 4; st++) load_step(u0 + w, st, x[st]);
   }
   for (int u = u0 + w; u < u1; u += kWaves) {
     // The last unit loads itself again: a branch here, between the matrix
@@ -528,8 +531,7 @@ w4_batch_kernel(W4View wt, Rows rows, int64_t M, int splits, EpiArgs epi, float*
     for (int st = 0; st < 4; st++) {
       constexpr int steps = GROUP / 32;  // of a group
       const int i = st / steps;
-      load_step(st < 3 ? u : un, (st + 1) & 3, x[(st + 1) & 1]);
-      const Step& now = x[st & 1];
+      const Step& now = x[st];
 #pragma unroll
       for (int j = 0; j < NB; j++) {
         const uint32_t q[4] = {cur[j].q.x, cur[j].q.y, cur[j].q.z, cur[j].q.w};
@@ -541,6 +543,7 @@ w4_batch_kernel(W4View wt, Rows rows, int64_t M, int splits, EpiArgs epi, float*
           acc[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, now.hi[rt], acc[j][rt], 0, 0, 0);
         }
       }
+      load_step(un, st, x[st]);
       if (st % steps == steps - 1) {
 #pragma unroll
         for (int j = 0; j < NB; j++) {
