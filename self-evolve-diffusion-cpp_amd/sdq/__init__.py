@@ -193,10 +193,11 @@ _torch = None
 
 def _get_torch():
     """torch, imported when the first device tensor is met."""
-    global _torch, _raw_stream
+    global _torch, _raw_stream, _Tensor, _f32
     if _torch is None:
         import torch
         _DTYPES.update({k: getattr(torch, v) for k, v in _DT.items()})
+        _Tensor, _f32 = torch.Tensor, torch.float32
         _torch, _raw_stream = torch, _find_raw_stream()
     return _torch
 
@@ -223,6 +224,7 @@ def _find_raw_stream():
 
 
 _raw_stream = None
+_Tensor, _f32 = (), None  # torch's, filled by _get_torch
 
 
 def _ptr(t):
@@ -250,10 +252,11 @@ class _Args:
     type, element type, shape and layout and returns its address; done()
     then checks that every argument lives on the current GPU."""
 
-    __slots__ = ("_seen",)
+    __slots__ = ("_seen", "_dev")
 
     def __init__(self):
-        self._seen = []
+        self._seen = []   # the first tensor of each run on one device
+        self._dev = None
 
     def __call__(self, t, name, dt="f32", shape=None, contig=True, optional=False):
         """shape: the exact shape (None entries are free); contig=False accepts
@@ -263,14 +266,18 @@ class _Args:
             if optional:
                 return None
             raise _bad(f"{name}: required")
-        if not isinstance(t, (_torch or _get_torch()).Tensor):
+        if not isinstance(t, _Tensor or _get_torch().Tensor):
             raise _bad(f"{name}: expected a torch device tensor, got {type(t).__name__}")
         if t.dtype is not _DTYPES[dt]:
             raise _bad(f"{name}: dtype {t.dtype}, expected {_DTYPES[dt]}")
         if shape is not None and t.shape != shape:
             have = t.shape
-            if len(have) != len(shape) or any(w is not None and d != w
-                                              for d, w in zip(have, shape)):
+            ok = len(have) == len(shape)
+            if ok:
+                for d, w in zip(have, shape):
+                    if d != w and w is not None:
+                        ok = False
+            if not ok:
                 want_s = tuple("*" if w is None else int(w) for w in shape)
                 raise _bad(f"{name}: shape {tuple(have)}, expected {want_s}")
         if contig:
@@ -278,8 +285,26 @@ class _Args:
                 raise _bad(f"{name}: must be contiguous")
         elif t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
             raise _bad(f"{name}: must be 2-D with contiguous rows")
-        self._seen.append((name, t))
+        dev = t.get_device()
+        if dev != self._dev:
+            self._dev = dev
+            self._seen.append((name, t))
         return t.data_ptr()
+
+    def rows(self, t, name, M, K):
+        """A float32 tensor [M, K] (M None: any) whose rows may be strided: its
+        address and row stride. The same checks in fewer steps."""
+        if isinstance(t, _Tensor) and t.dtype is _f32:
+            shape = t.shape
+            if len(shape) == 2 and shape[1] == K and (M is None or shape[0] == M):
+                ld, one = t.stride()
+                if one == 1 or K <= 1:
+                    dev = t.get_device()
+                    if dev != self._dev:
+                        self._dev = dev
+                        self._seen.append((name, t))
+                    return t.data_ptr(), ld if shape[0] > 1 else K
+        return self(t, name, "f32", (M, K), contig=False), _ld(t)  # says what is wrong
 
     def done(self):
         """The current device, on which every tensor is."""
@@ -751,9 +776,8 @@ def dequant(aq, asc, y, stream=None):
     pq = c(aq, "aq", "i8", (None, None))
     M, K = aq.shape
     ps, py = c(asc, "as", "f32", (M,)), c(y, "y", "f32", (M, K))
-    load_library()
     dev = c.done()
-    _check(_lib.sdq_dequant(pq, ps, M, K, py, _stream(stream, dev)))
+    _check((_lib or load_library()).sdq_dequant(pq, ps, M, K, py, _stream(stream, dev)))
     return y
 
 
@@ -780,16 +804,13 @@ def rmsnorm_quant(x, aq, asc, w=None, delta=None, sum_out=None, eps=1e-6, stream
     c = _Args()
     px = c(x, "x", "f32", (None, None), contig=False)
     M, K = x.shape
-    pd = c(delta, "delta", "f32", (M, K), contig=False, optional=True)
-    ph = c(sum_out, "sum_out", "f32", (M, K), contig=False, optional=True)
-    pw = c(w, "w", "f32", (K,), optional=True)
+    pd, ldd = (None, 0) if delta is None else c.rows(delta, "delta", M, K)
+    ph, lds = (None, 0) if sum_out is None else c.rows(sum_out, "sum_out", M, K)
+    pw = None if w is None else c(w, "w", "f32", (K,))
     pq, ps = c(aq, "aq", "i8", (M, K)), c(asc, "as", "f32", (M,))
-    load_library()
     dev = c.done()
-    ldd = 0 if delta is None else _ld(delta)
-    lds = 0 if sum_out is None else _ld(sum_out)
-    _check(_lib.sdq_rmsnorm_quant(px, _ld(x), pd, ldd, M, K, pw, eps, ph, lds, pq, ps,
-                                  _stream(stream, dev)))
+    _check((_lib or load_library()).sdq_rmsnorm_quant(px, _ld(x), pd, ldd, M, K, pw, eps, ph, lds,
+                                                      pq, ps, _stream(stream, dev)))
     return aq, asc
 
 
@@ -886,6 +907,7 @@ class _KvTensors:
             if t.device != one[1].device:
                 raise _bad(f"{name}: on {t.device}, {one[0]} on {one[1].device}")
         self._one = one
+        self._dev = one[1].get_device()
 
 
 class KvCache(_KvTensors):
@@ -949,16 +971,17 @@ def _kv_args(cache, batch, rows, heads):
     if not isinstance(cache, KvCache) or not isinstance(batch, KvBatch):
         raise _bad("expected a KvCache and a KvBatch")
     c = _Args()
-    T = None
-    ptrs = []
-    for name, t in rows:
-        p = c(t, name, "f32", (T, heads * 128), contig=False)
-        T = t.shape[0]
-        ptrs += (p, _ld(t))
-    c._seen += (cache._one, batch._one)
+    (a, x), (b, y) = rows
+    C = heads * 128
+    px, ldx = c.rows(x, a, None, C)
+    T = x.shape[0]
+    py, ldy = c.rows(y, b, T, C)
+    if cache._dev != c._dev or batch._dev != c._dev:
+        c._seen += (cache._one, batch._one)
     dev = c.done()
-    load_library()
-    return cache._ref, batch._ref, ptrs, T, dev
+    if _lib is None:
+        load_library()
+    return cache._ref, batch._ref, (px, ldx, py, ldy), T, dev
 
 
 def kv_write(cache: KvCache, batch: KvBatch, k, v, stream=None):
