@@ -7,8 +7,8 @@
 // fp32 product costs two fp16 MFMA products: q = (hi + lo) 2^-r, r a power of two
 // for each row that puts its largest element into [2^14, 2^15), and the softmax
 // weight = hi + lo below. Both parts are truncated: hi + lo is off by less than
-// 2^-21 of the value, or an absolute 2^-39 of the row's largest. The key's scale multiplies the finished
-// sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in [1/2, 1), E0 the exponent of
+// 2^-21 of the value, or an absolute 2^-39 of the row's largest. The key's scale
+// multiplies the finished sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in [1/2, 1), E0 the exponent of
 // the sequence's first value, at least -16: its exponent goes into the softmax,
 //   t_j = s_j + e_j,  X_j = 2^(t_j - m), m near the running maximum of t,
 //   out = 2^E0 sum_j X_j f_j code_j / sum_j X_j 2^-e_j,
@@ -126,6 +126,10 @@ __device__ __forceinline__ int keys_of_rows(const Tile& t, int64_t r, int n, int
   return keys_of(t, (r + n < t.rows ? r + n : t.rows) - 1, group, causal);
 }
 
+__device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
 // Eight codes (two dwords) as fp16: 0x6400 | u is 1024 + u, with u = code + 128.
 __device__ __forceinline__ v2h less1152(uint32_t x) {
   return __builtin_bit_cast(v2h, x) + v2h{(_Float16)-1152.f, (_Float16)-1152.f};
@@ -169,7 +173,9 @@ __device__ __forceinline__ float less_low(v2h hi, float x) {
 }
 __device__ __forceinline__ float less_high(v2h hi, float x) {
   float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(hi), "v"(x));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+      : "=v"(r)
+      : "v"(hi), "v"(x));
   return r;
 }
 // fp32 to two fp16 parts, both truncated (two conversions at a time): the high
@@ -400,8 +406,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
       for (int kb = 0; kb < 4; kb++) {
         const uint4 r = cur.k[kt][kb >> 1];
         const v8h ka = kb & 1 ? codes8(r.z, r.w) : codes8(r.x, r.y);
-        s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[kb], s[kt], 0, 0, 0);
-        s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[kb], s[kt], 0, 0, 0);
+        s[kt] = mma(ka, ql[kb], s[kt]);
+        s[kt] = mma(ka, qh[kb], s[kt]);
       }
       const float ksv[4] = {cur.ks[kt].x, cur.ks[kt].y, cur.ks[kt].z, cur.ks[kt].w};
       const float vsv[4] = {cur.vs[kt].x, cur.vs[kt].y, cur.vs[kt].z, cur.vs[kt].w};
@@ -440,8 +446,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
       const v2h p0 = pair_of<i>(v[0], v[1]), p1 = pair_of<i>(v[2], v[3]);
       const v2h p2 = pair_of<i>(v[4], v[5]), p3 = pair_of<i>(v[6], v[7]);
       const v8h vv{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
-      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o, 0, 0, 0);
-      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph, o, 0, 0, 0);
+      o = mma(vv, pl, o);
+      o = mma(vv, ph, o);
     };
     tile_e(std::integral_constant<int, 0>{}, va, acc[0]);
     tile_e(std::integral_constant<int, 1>{}, va, acc[1]);
@@ -571,11 +577,16 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 // tokens x 28048 keys x 24 heads 605 -> 580 us, twice 4099 x 16411 2560 -> 2410;
 // wave priorities around the products make no difference to either). A power of two for
 // each query row, one more product a score, costs 2.5% and keeps rows independent.
+// The operands of the next eight MFMAs are read from LDS before the eight at hand are
+// issued, in an order that the compiler is held to (it reads each pair just before its
+// use: 611 -> 576 and 2500 -> 2390 us).
 //
-// Bound: 4 MFMA products a score and value (two parts each); 590 us are 76% of the
-// rate that a large fp16 matrix product reaches on this card. Turns taken phase by
-// phase (a barrier after each score, softmax and product phase, the waves of a SIMD
-// one phase apart) do not fit the registers: 1560 us.
+// Bound: 4 MFMA products a score and value (two parts each), beside which the rest does
+// not disappear: without the softmax 135 us less, without turning keys 100, without the
+// LDS reads of operands 100. Not faster: turns taken phase by phase (a barrier after
+// each phase, the waves of a SIMD one phase apart), which does not fit the registers
+// (1560 us); one sub-block's softmax between the next one's scores, with the queries' low
+// parts in LDS to make room (640); four waves of 64 rows (2100, no room either).
 
 template <int NW>
 struct Block {
@@ -646,26 +657,32 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   uint32_t vr[4];
   float ksr = 0.f, vsr = 0.f;
   bool ok = false;
-  auto place = [&](int p, bool& there) -> int64_t {
-    int64_t page = p < keys ? table[p >> c.page_log2] : -1;
-    there = page >= 0 && page < c.pages;
-    return (((there ? page : 0) * c.kv_heads + h) << c.page_log2) +
+  // Pages are looked up one block before the codes.
+  auto page_of = [&](int p) { return p < keys ? table[p >> c.page_log2] : -1; };
+  auto place = [&](int page, int p) -> int64_t {  // a page that is none: the first, masked
+    return (((page >= 0 && page < c.pages ? page : 0) * (int64_t)c.kv_heads + h) << c.page_log2) +
            (p & ((1 << c.page_log2) - 1));
   };
+  int k_page = -1, v_page = -1, one_page = -1;
+  auto look = [&](int b) {
+    k_page = page_of(b * KB + k_key);
+    v_page = page_of(b * KB + v_row);
+    if (tid < KB) one_page = page_of(b * KB + tid);
+  };
   auto fetch = [&](int b) {
-    bool there;
-    int64_t at = place(b * KB + k_key, there);
+    int64_t at = place(k_page, b * KB + k_key);
     kr = *reinterpret_cast<const uint4*>(c.k + at * kHd + 16 * k_j);
-    at = place(b * KB + v_row, there);
+    at = place(v_page, b * KB + v_row);
 #pragma unroll
     for (int i = 0; i < 4; i++)
       vr[i] = *reinterpret_cast<const uint32_t*>(c.v + (at + i) * kHd + v_d);
     if (tid < KB) {
-      at = place(b * KB + tid, there);
+      at = place(one_page, b * KB + tid);
       ksr = c.ks[at];
       vsr = c.vs[at];
-      ok = there && b * KB + tid < t.len;
+      ok = one_page >= 0 && one_page < c.pages && b * KB + tid < t.len;
     }
+    look(b + 1);
   };
   auto stage = [&](Blk& d) {
     const int kt = tid >> 7;  // 16-key tile of the block
@@ -696,25 +713,44 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
       d.f[tid] = k.f;
     }
   };
+  // MFMA operands of K (both key tiles of step kb) and V (dim tiles 2 p, 2 p + 1).
+  auto load_k = [&](const Blk& d, int sub, int kb, v8h (&o)[2]) {
+#pragma unroll
+    for (int kt = 0; kt < 2; kt++) o[kt] = *reinterpret_cast<const v8h*>(d.k[sub][kt][kb] + l * 16);
+  };
+  auto load_v = [&](const Blk& d, int sub, int p, v8h (&o)[2]) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) o[j] = *reinterpret_cast<const v8h*>(d.v[sub][2 * p + j] + l * 16);
+  };
   auto compute = [&](const Blk& d, int b) {
+    v8h op[2][2];
+    load_k(d, 0, 0, op[0]);
 #pragma unroll
     for (int sub = 0; sub < Blk::kSubs; sub++) {
       const int k0 = b * KB + 32 * sub;
       if (k0 >= wmost) break;
       v4f s[QT][2];
 #pragma unroll
-      for (int kt = 0; kt < 2; kt++) {
+      for (int qt = 0; qt < QT; qt++) s[qt][0] = s[qt][1] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int qt = 0; qt < QT; qt++) s[qt][kt] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int kb = 0; kb < 4; kb++) {
+        if (kb < 3)
+          load_k(d, sub, kb + 1, op[(kb + 1) & 1]);
+        else
+          load_v(d, sub, 0, op[0]);
+        __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead of the products
+        const v8h(&ka)[2] = op[kb & 1];
 #pragma unroll
-        for (int kb = 0; kb < 4; kb++) {
-          const v8h ka = *reinterpret_cast<const v8h*>(d.k[sub][kt][kb] + l * 16);
+        for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-          for (int qt = 0; qt < QT; qt++) {
-            s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[qt][kb], s[qt][kt], 0, 0, 0);
-            s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[qt][kb], s[qt][kt], 0, 0, 0);
-          }
-        }
+          for (int qt = 0; qt < QT; qt++)
+            s[qt][kt] = mma(ka[kt], ql[qt][kb], s[qt][kt]);
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+          for (int qt = 0; qt < QT; qt++)
+            s[qt][kt] = mma(ka[kt], qh[qt][kb], s[qt][kt]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       const int at = 32 * sub + 4 * g;
       auto terms = [&](const float* p, v4f x[2]) {
@@ -755,19 +791,34 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
                 [&](int qt, int kt, int i) { return kg + 16 * kt + i < mine[qt]; });
       }
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const v8h va = *reinterpret_cast<const v8h*>(d.v[sub][e] + l * 16);
+      for (int p = 0; p < 4; p++) {
+        if (p < 3)
+          load_v(d, sub, p + 1, op[(p + 1) & 1]);
+        else if (sub + 1 < Blk::kSubs)
+          load_k(d, sub + 1, 0, op[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        const v8h(&va)[2] = op[p & 1];
 #pragma unroll
-        for (int qt = 0; qt < QT; qt++) {
-          v4f& o = acc[qt][e];
-          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[qt], o, 0, 0, 0);
-          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[qt], o, 0, 0, 0);
-        }
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int qt = 0; qt < QT; qt++) {
+            v4f& o = acc[qt][2 * p + j];
+            o = mma(va[j], pl[qt], o);
+          }
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int qt = 0; qt < QT; qt++) {
+            v4f& o = acc[qt][2 * p + j];
+            o = mma(va[j], ph[qt], o);
+          }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
 
   if (b0 < b1) {
+    look(b0);
     fetch(b0);
     stage(buf[b0 & 1]);
     if (b0 + 1 < b1) fetch(b0 + 1);
@@ -826,9 +877,11 @@ hipError_t run(Args a, const kvplan::Plan& p, Launch launch, hipStream_t s) {
     if (e != hipSuccess) return e;
     if (p.splits > 1) {
       if (p.splits > kJoin)
-        hipLaunchKernelGGL((kv_attn_join_kernel<RT, 4>), dim3((unsigned)(n * RT)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((kv_attn_join_kernel<RT, 4>), dim3((unsigned)(n * RT)), dim3(256), 0, s,
+                           a);
       else
-        hipLaunchKernelGGL((kv_attn_join_kernel<RT, 1>), dim3((unsigned)(n * RT / 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((kv_attn_join_kernel<RT, 1>), dim3((unsigned)(n * RT / 4)), dim3(256), 0,
+                           s, a);
       e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
