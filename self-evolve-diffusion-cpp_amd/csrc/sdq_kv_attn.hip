@@ -579,7 +579,8 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 // each query row, one more product a score, costs 2.5% and keeps rows independent.
 // The operands of the next eight MFMAs are read from LDS before the eight at hand are
 // issued, in an order that the compiler is held to (it reads each pair just before its
-// use: 611 -> 576 and 2500 -> 2390 us).
+// use: 611 -> 576 and 2500 -> 2390 us). A wave's part of a block lies in one page, so its
+// place is scalar arithmetic (a place a thread: 574 and 2363 us, now 548 and 2279).
 //
 // Bound: 4 MFMA products a score and value (two parts each), beside which the rest does
 // not disappear: without the softmax 135 us less, without turning keys 100, without the
@@ -648,11 +649,13 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     for (int e = 0; e < 8; e++) acc[qt][e] = v4f{0.f, 0.f, 0.f, 0.f};
   }
 
-  // The thread's part of a block: 16 dims of a key, 4 dims of four values' rows,
-  // one key's scales (the first KB threads).
+  // The thread's part of a block: 16 dims of key (tid % 16) and 4 dims of four values'
+  // rows, both of its wave's tile of 16 keys, which lies in one page; one key's scales
+  // (the first KB threads).
   const int32_t* table = c.table + t.s * c.max_pages;
-  const int k_key = 16 * (tid >> 7) + (tid & 15), k_j = (tid >> 4) & 7;   // dims 16 k_j ..
-  const int v_row = 4 * (tid >> 5), v_d = 4 * (tid & 31);                 // keys, dims
+  const int k_j = (tid >> 4) & 7;                          // dims 16 k_j ..
+  const int v_row = 4 * (tid >> 5), v_d = 4 * (tid & 31);  // keys of the block, dims
+  const int wave_tile = uniform(v_row & ~15);
   uint4 kr;
   uint32_t vr[4];
   float ksr = 0.f, vsr = 0.f;
@@ -663,21 +666,20 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     return (((page >= 0 && page < c.pages ? page : 0) * (int64_t)c.kv_heads + h) << c.page_log2) +
            (p & ((1 << c.page_log2) - 1));
   };
-  int k_page = -1, v_page = -1, one_page = -1;
+  int wave_page = -1, one_page = -1;
   auto look = [&](int b) {
-    k_page = page_of(b * KB + k_key);
-    v_page = page_of(b * KB + v_row);
+    wave_page = page_of(b * KB + wave_tile);
     if (tid < KB) one_page = page_of(b * KB + tid);
   };
   auto fetch = [&](int b) {
-    int64_t at = place(k_page, b * KB + k_key);
-    kr = *reinterpret_cast<const uint4*>(c.k + at * kHd + 16 * k_j);
-    at = place(v_page, b * KB + v_row);
+    const int64_t tile = place(uniform(wave_page), b * KB + wave_tile) * kHd;
+    kr = *reinterpret_cast<const uint4*>(c.k + tile + (uint32_t)((tid & 15) * kHd + 16 * k_j));
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      vr[i] = *reinterpret_cast<const uint32_t*>(c.v + (at + i) * kHd + v_d);
+      vr[i] = *reinterpret_cast<const uint32_t*>(
+          c.v + tile + (uint32_t)(((v_row & 15) + i) * kHd + v_d));
     if (tid < KB) {
-      at = place(one_page, b * KB + tid);
+      const int64_t at = place(one_page, b * KB + tid);
       ksr = c.ks[at];
       vsr = c.vs[at];
       ok = one_page >= 0 && one_page < c.pages && b * KB + tid < t.len;
