@@ -99,11 +99,26 @@ struct Workspace {
 };
 std::map<std::pair<int, hipStream_t>, Workspace> g_ws;
 
+// A thread's use of its hipStreamPerThread. The runtime drops that stream with the
+// thread, and a device synchronization after that does not wait for what it still held;
+// the next thread at this address would meet it in the workspace. So the thread waits
+// for its own work as it ends (made after the runtime's own thread state, so gone before).
+struct ThreadStream {
+  uint64_t devices = 0;
+  ~ThreadStream() {
+    for (int d = 0; d < kMaxDev; d++)
+      if (devices >> d & 1 && hipSetDevice(d) == hipSuccess)
+        (void)hipStreamSynchronize(hipStreamPerThread);
+  }
+};
+
 // The workspace of (device, stream), under g_mu. hipStreamPerThread is another
 // stream in every thread: the thread's own address stands for it.
 Workspace& ws_of(int dev, hipStream_t s) {
-  thread_local char self;
-  return g_ws[{dev, s == hipStreamPerThread ? reinterpret_cast<hipStream_t>(&self) : s}];
+  if (s != hipStreamPerThread) return g_ws[{dev, s}];
+  thread_local ThreadStream self;
+  self.devices |= uint64_t(1) << dev;
+  return g_ws[{dev, reinterpret_cast<hipStream_t>(&self)}];
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
