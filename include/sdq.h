@@ -443,8 +443,9 @@ int sdq_weight4_dims(const sdq_weight4* w, int64_t* N, int64_t* K, int* group);
  * bits); sums over the groups are fp32 either way (errors of a few 1e-7 of the
  * row's norm times the weight's). A row that holds a NaN or an infinity
  * gives NaN, and no row's result depends on the others' contents. Built for few rows: 1
- * to 32 read the weight once, more run in blocks of 32. Y must not overlap A (resid may be Y). Stream-ordered; scratch
- * from the stream's workspace as sdq_qlinear (none for the fewest rows). */
+ * to 32 read the weight once, more run in blocks of 32. Y must not overlap A (resid
+ * may be Y). Stream-ordered; scratch from the stream's workspace as sdq_qlinear (none
+ * for the fewest rows). */
 int sdq_q4linear(const sdq_weight4* w, const float* A, int64_t M, int64_t K,
                  const sdq_epilogue* epi, float* Y, void* stream);
 

@@ -8,8 +8,9 @@
 // for each row that puts its largest element into [2^14, 2^15), and the softmax
 // weight = hi + lo below. Both parts are truncated: hi + lo is off by less than
 // 2^-21 of the value, or an absolute 2^-39 of the row's largest. The key's scale
-// multiplies the finished sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in [1/2, 1), E0 the exponent of
-// the sequence's first value, at least -16: its exponent goes into the softmax,
+// multiplies the finished sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in
+// [1/2, 1), E0 the exponent of the sequence's first value, at least -16: its exponent
+// goes into the softmax,
 //   t_j = s_j + e_j,  X_j = 2^(t_j - m), m near the running maximum of t,
 //   out = 2^E0 sum_j X_j f_j code_j / sum_j X_j 2^-e_j,
 // one exponential a key as before, and the weights that are split into parts
@@ -315,6 +316,13 @@ __device__ __forceinline__ void raise(State& st, float mx, v4f acc[8]) {
 }
 
 // ---- few rows: a tile of 16, the workgroup's waves share out the keys ----
+//
+// Bound by the cache's bytes, 264 a key and cached head, each read once by the wave
+// that uses it, straight into the MFMA operands' lanes, a block of 32 keys ahead: 1
+// token x 262145 keys, 8 cached heads, 107 us, 5.2 TB/s, the rate of a large copy.
+// 8 tokens of ragged sequences up to 4099 keys, 24 heads: 35 us, 3.3 TB/s; there a wave
+// has eight blocks at most, and finding its tile, the first loads and an uneven
+// last round take what is missing.
 
 constexpr int kFewRows = kvplan::kFewRows;
 constexpr int kFewWaves = kvplan::kFewWaves;
@@ -582,12 +590,14 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 // use: 611 -> 576 and 2500 -> 2390 us). A wave's part of a block lies in one page, so its
 // place is scalar arithmetic (a place a thread: 574 and 2363 us, now 548 and 2279).
 //
-// Bound: 4 MFMA products a score and value (two parts each), beside which the rest does
-// not disappear: without the softmax 135 us less, without turning keys 100, without the
-// LDS reads of operands 100. Not faster: turns taken phase by phase (a barrier after
-// each phase, the waves of a SIMD one phase apart), which does not fit the registers
-// (1560 us); one sub-block's softmax between the next one's scores, with the queries' low
-// parts in LDS to make room (640); four waves of 64 rows (2100, no room either).
+// Bound: 4 MFMA products a score and value (two parts each), busy 47% of the cycles:
+// 92% of the rate of a large library product for the first of these, 93% for the
+// second. What stands beside them does not disappear; at 611 us the first took 135 less
+// without the softmax, 100 without turning keys, 100 without reading operands. Not
+// faster: turns taken phase by phase (a barrier after each phase, the waves of a SIMD
+// one phase apart), which does not fit the registers (1560 us); one sub-block's softmax
+// between the next one's scores, with the queries' low parts in LDS to make room (640);
+// four waves of 64 rows (2100, no room either).
 
 template <int NW>
 struct Block {

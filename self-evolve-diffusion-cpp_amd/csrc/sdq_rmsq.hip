@@ -10,9 +10,11 @@
 // for memory either way) and rounded once. From y on the steps are those of
 // the plain quantizer (sdq_quant.hip), in fp32.
 //
-// Bound by HBM: 8 bytes read and 5 written per value. A row is read once and
-// stays in the registers of its threads (T of them, NV groups of four values
-// each) over the two reductions; rows past the register form are read again.
+// Bound by HBM: with a residual and its sum 8 bytes read and 5 written per value. A
+// row is read once and stays in the registers of its threads (T of them, NV groups of
+// four values each) over the two reductions; rows past the register form are read
+// again. 27280 x 5120: 358 us, 5.07 TB/s, the rate of a large copy (the codes' way
+// back 116 us, 6.0 TB/s); 509 x 4096 10.4 us and one row 4.1 us, which is latency.
 #include <algorithm>
 
 #include "sdq_device.h"

@@ -3,9 +3,9 @@
 cache holds.
 
 Attention's tolerance, per row, from its arithmetic: a logit (in units of log2)
-is off by the q parts and the fp32 roundings of the sum of |q k| products (128 and 8 more
-beyond them; the parts' 2^-21 are eight of those), plus two roundings of itself and of the running maximum; a weight by its logit's
-error times ln 2, exp2's 2^-22 and the parts' 2^-21; the sums over n keys by
+is off by the q parts and the fp32 roundings of the sum of |q k| products (128, and 8
+more that stand for the parts' 2^-21), plus two roundings of itself and of the running
+maximum; a weight by its logit's error times ln 2, exp2's 2^-22 and the parts' 2^-21; the sums over n keys by
 (n / 8 + 64) 2^-24. Numerator and denominator each, so twice that, of max |v|."""
 import numpy as np
 import pytest
@@ -513,6 +513,35 @@ def test_threads_on_one_stream(sdq_dev):
         assert outs[i][0].abs().sum() > 0
         for o in outs[i][1:]:
             assert torch.equal(o, outs[i][0]), i
+
+
+def test_a_thread_that_ends_waits_for_its_stream(sdq_dev):
+    """Calls queued on a thread's own stream are done when the thread is: nothing can wait
+    for them afterwards, and the next thread's calls may use the same scratch."""
+    import threading
+
+    import torch
+
+    import sdq
+
+    cases = [Case(sdq_dev, [1, 1], [20000, 9000], 2, 64, seed=17 + i) for i in range(2)]
+    qs = [torch.randn((c.T, 4 * HD), device=sdq_dev) for c in cases]
+    want = [sdq.kv_attention(c.cache, c.batch, q, torch.zeros_like(q), 4) for c, q in zip(cases, qs)]
+    outs = [[torch.zeros_like(q) for _ in range(40)] for q in qs]
+    torch.cuda.synchronize()
+
+    def run(i):
+        sdq.init(0)
+        for o in outs[i]:
+            sdq.kv_attention(cases[i].cache, cases[i].batch, qs[i], o, 4, stream=2)
+
+    for i in range(2):
+        t = threading.Thread(target=run, args=(i,))
+        t.start()
+        t.join()
+    for w, os_ in zip(want, outs):
+        for o in os_:
+            assert torch.equal(o, w)
 
 
 # ---- a serving step out of all of them ----
