@@ -81,37 +81,33 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   return ((int64_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v);
 }
 
-// The tile with number `tile` when every sequence is cut into tiles of RT rows:
-// a scan over the sequences, 64 at a time. The same in every wave.
+// Tile number `tile`. Sequence s, whose rows start at row a and end before row b of all
+// (row: a token's head of the group), has the numbers from a / RT + s to b / RT + s, at
+// least as many as it has tiles of RT rows: a number without a tile is none. So the
+// sequence is found by search, 64 ways at a time, with no sum over those before it
+// (a scan over them took a fifth of a microsecond for each 64). The same in every wave.
 template <int RT>
 __device__ __forceinline__ Tile find_tile(const View& c, int group, int64_t tile) {
   const int l = threadIdx.x & 63;
   Tile t{-1, 0, 0, 0, 0, 0};
-  int64_t base = 0;
-  for (int s0 = 0; s0 < c.nseq; s0 += 64) {
-    const int s = s0 + l;
-    const int64_t n = s < c.nseq ? kv::row_of(c, s + 1) - kv::row_of(c, s) : 0;
-    const int64_t rows = n > 0 ? n * group : 0;
-    const int64_t count = (rows + RT - 1) / RT;
-    int64_t upto = count;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t u = __shfl_up(upto, o);
-      upto += l >= o ? u : 0;
-    }
-    const uint64_t past = __ballot(base + upto > tile);
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      t.s = uniform(s0 + at);
-      t.r0 = uniform((tile - base - __shfl(upto - count, at)) * RT);
-      t.rows = uniform(__shfl(rows, at));
-      t.row0 = kv::row_of(c, t.s);
-      t.len = (int)kv::length_of(c, t.s);
-      t.first = t.len - (int)(t.rows / group);
-      return t;
-    }
-    base += __shfl(upto, 63);
-  }
+  auto first = [&](int s) { return kv::row_of(c, s) * group / RT + s; };
+  int lo = 0, n = c.nseq, step;
+  do {
+    step = (n + 63) / 64;
+    const uint64_t upto = __ballot((int64_t)l * step < n && first(min(lo + l * step, c.nseq)) <= tile);
+    if (!upto) return t;
+    const int k = 63 - __builtin_clzll(upto);
+    lo += k * step;
+    n = min(step, n - k * step);
+  } while (step > 1);
+  lo = uniform(lo);
+  t.row0 = kv::row_of(c, lo);
+  const int64_t tokens = kv::row_of(c, lo + 1) - t.row0;
+  t.r0 = (tile - first(lo)) * RT;
+  t.rows = tokens > 0 ? tokens * group : 0;
+  t.len = (int)kv::length_of(c, lo);
+  t.first = t.len - (int)(tokens > 0 ? tokens : 0);
+  if (t.r0 < t.rows) t.s = lo;
   return t;
 }
 

@@ -16,7 +16,7 @@ constexpr int kMaxSplits = 64;
 struct Plan {
   int rows;                  // of a tile: 16 (few rows), 64 or 256 (chunks)
   int splits;                // shares that the keys are cut into
-  int64_t tiles;             // at most this many, over all sequences
+  int64_t tiles;             // numbers of tiles, over all sequences
   int64_t tiles_per_launch;
   int64_t part_bytes;        // partial sums; maxima and denominators follow
   int64_t scratch_bytes;     // 0: none
@@ -31,9 +31,11 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   // right for any lengths.
   const int64_t mean = (rows + nseq - 1) / nseq;
   p.rows = mean <= 32 ? kFewRows : mean <= 128 ? 64 : 256;
-  // sum of ceil(rows_s / height) over the sequences that have any
-  p.tiles = (rows + std::min<int64_t>(nseq, T) * (p.rows - 1)) / p.rows;
-  const int64_t groups = p.tiles * kv_heads;  // workgroups without a cut
+  // Numbers of tiles: rows / height and one a sequence (csrc/sdq_kv_attn.hip); those that
+  // hold one are at most the sum of ceil(rows_s / height) over the sequences that have any.
+  p.tiles = rows / p.rows + nseq;
+  const int64_t groups =  // workgroups without a cut
+      (rows + std::min<int64_t>(nseq, T) * (p.rows - 1)) / p.rows * kv_heads;
   // Enough workgroups for every CU. A few-row one is four waves that wait for memory, and
   // two fit a CU at once: three to a CU (8 sequences x 24 heads x 4099 keys: two 52 us,
   // three 42, four 45, six 47). A chunk's of 256 rows takes a CU's registers, and the

@@ -30,12 +30,16 @@ int main() {
     const kp::Plan p = kp::plan(T, nseq, group, kvh, most, 256);
     REQUIRE(p.rows == 16 || p.rows == 64 || p.rows == 256);
     REQUIRE(p.splits >= 1 && p.splits <= kp::kMaxSplits);
-    // the most tiles that T rows in nseq sequences can make: one row in all but one
-    const int64_t filled = std::min<int64_t>(nseq, T);
-    const int64_t ones = (group + p.rows - 1) / p.rows;  // tiles of a sequence of one token
-    const int64_t rest = (T - (filled - 1)) * group;
-    const int64_t tiles = (filled - 1) * ones + (rest + p.rows - 1) / p.rows;
-    REQUIRE(tiles <= p.tiles);
+    // ragged sequences: each has as many numbers as tiles, the last one within the plan's
+    int64_t at = 0;
+    const int seqs = std::min(nseq, 40);
+    for (int s = 0; s < seqs; s++) {
+      const int64_t end = s == nseq - 1 || rng() % 8 == 0 ? T : at + (int64_t)(rng() % (T - at + 1));
+      const int64_t first = at * group / p.rows + s, next = end * group / p.rows + s + 1;
+      REQUIRE(next - first >= ((end - at) * group + p.rows - 1) / p.rows);
+      REQUIRE(next <= p.tiles);
+      at = end;
+    }
     REQUIRE(p.tiles_per_launch >= 1);
     const int64_t n = std::min(p.tiles, p.tiles_per_launch) * kvh;
     const int64_t block = p.rows == 16 ? 64 * kp::kFewWaves : p.rows == 64 ? 256 : 512;

@@ -299,6 +299,17 @@ def test_nan_stays_where_it_is(sdq_dev, new):
     assert np.isnan(got[new:]).all() and np.isfinite(clean).all()
 
 
+@pytest.mark.parametrize("nseq,most", [(63, 3), (64, 2), (65, 40), (200, 9), (4100, 2)])
+def test_many_sequences(sdq_dev, nseq, most):
+    """Ragged batches around the search's widths, empty sequences among them, rows
+    before the first and behind the last."""
+    rng = np.random.default_rng(nseq)
+    new = rng.integers(0, most + 1, nseq)
+    lens = new + rng.integers(0, 30, nseq)
+    c = Case(sdq_dev, new, lens, 1, 16, seed=18, first=3, behind=2)
+    c.check(3, True)
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_a_huge_row_takes_nothing_from_others(sdq_dev, new):
     """A head of a token holds 1e30: the rows beside it, of its own tile among
