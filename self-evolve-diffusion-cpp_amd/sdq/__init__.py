@@ -193,12 +193,13 @@ _torch = None
 
 def _get_torch():
     """torch, imported when the first device tensor is met."""
-    global _torch, _raw_stream, _Tensor, _f32
+    global _torch, _raw_stream, _current_device, _Tensor, _f32
     if _torch is None:
         import torch
         _DTYPES.update({k: getattr(torch, v) for k, v in _DT.items()})
         _Tensor, _f32 = torch.Tensor, torch.float32
         _torch, _raw_stream = torch, _find_raw_stream()
+        _current_device = _find_current_device(torch)
     return _torch
 
 
@@ -223,7 +224,16 @@ def _find_raw_stream():
         return None
 
 
+def _find_current_device(torch):
+    try:  # without the check that the GPU is initialized: asked once a tensor is on it
+        from torch._C import _cuda_getDevice
+        return _cuda_getDevice
+    except ImportError:
+        return torch.cuda.current_device
+
+
 _raw_stream = None
+_current_device = None
 _Tensor, _f32 = (), None  # torch's, filled by _get_torch
 
 
@@ -315,7 +325,7 @@ class _Args:
                 if not t.is_cuda:
                     raise _bad(f"{name}: must be on the GPU (got device {t.device})")
                 if cur == -2:
-                    cur = _torch.cuda.current_device()
+                    cur = _current_device()
                 if dev != cur:
                     raise _bad(f"{name}: on {t.device}, current device is cuda:{cur}")
         return cur
