@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 // place is scalar arithmetic (a place a thread: 574 and 2363 us, now 548 and 2279).
 //
 // Bound: 4 MFMA products a score and value (two parts each), busy 47% of the cycles:
-// 92% of the rate of a large library product for the first of these, 93% for the
+// 91% of the rate of a large library product for the first of these, 93% for the
 // second. What stands beside them does not disappear; at 611 us the first took 135 less
 // without the softmax, 100 without turning keys, 100 without reading operands. Not
 // faster: turns taken phase by phase (a barrier after each phase, the waves of a SIMD
