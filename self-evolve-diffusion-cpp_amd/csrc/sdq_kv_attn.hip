@@ -15,9 +15,10 @@
 //   out = 2^E0 sum_j X_j f_j code_j / sum_j X_j 2^-e_j,
 // one exponential a key as before, and the weights that are split into parts
 // are those that count: no value is lost beside another, however far apart the
-// scales of heavy and light keys are. e_j is held to -60 .. 60 (2^-e_j and X_j have to
-// be floats together); a value under that counts with fewer bits, one over it makes
-// its rows NaN.
+// scales of heavy and light keys are. e_j is held to -60 .. 60 (2^-e_j and the sums have to
+// be floats); a value under that counts with fewer bits, one over it makes its rows NaN.
+// X_j can lie under the smallest float where X_j 2^-e_j, at most 2^(60 + 60) larger, is
+// still most of the denominator: such terms are formed apart (add_faint, times_exp2).
 //
 // Scores are computed transposed, S^T = K Q^T (16x16x32): a lane then holds one
 // query's scores for keys 4 g + 0..3 (g = lane / 16) of two 16-key tiles, which
@@ -48,6 +49,9 @@ constexpr int kSlack = 6;     // X stays below 2^kSlack
 constexpr int kWeight = 9;    // weights X f enter as X f 2^kWeight
 constexpr int kFar = 60;      // e_j is held to -kFar .. kFar
 constexpr int kLeast = -16;   // of E0
+// A key with e >= kNear whose X is under 2^-126 is less than 2^(-126 - kNear) of a
+// denominator that holds at least 2^-kFar: 2^30 of them less than 2^-26 of it.
+constexpr float kNear = -10.f;
 
 struct Args {
   View c;
@@ -297,6 +301,24 @@ __device__ __forceinline__ void weights(const v4f t[2], const v4f w[2], const v4
   }
   parts8(p, hi, lo);
 }
+// a 2^d, also where 2^d alone is under the smallest float (exp2 gives 0 there).
+__device__ __forceinline__ float times_exp2(float a, float d) {
+  const float h = __builtin_amdgcn_exp2f(0.5f * d);
+  return a * h * h;
+}
+// The denominator's terms 2^(t - m - e) of keys whose X is under the smallest float (what
+// is 2^-1000 is nothing, masked keys among it); their X is 0 from here on. Called
+// where a block has a key with e < kNear.
+__device__ __forceinline__ void add_faint(v4f t[2], const v4f e[2], State& st) {
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float x = t[j >> 2][j & 3] - ref;
+    const bool faint = x < -126.f && x > -1000.f;
+    st.l += __builtin_amdgcn_exp2f(faint ? x - e[j >> 2][j & 3] : -INFINITY);
+    t[j >> 2][j & 3] = faint ? -INFINITY : t[j >> 2][j & 3];
+  }
+}
 // The reference rises only when a block's largest logit passes it by more than
 // kSlack (the weights then stay below 2^kSlack, inside fp16 with kWeight):
 // rarely. The branch is the wave's, the rise each row's own, so that no row's bits
@@ -304,9 +326,10 @@ __device__ __forceinline__ void weights(const v4f t[2], const v4f w[2], const v4
 __device__ __forceinline__ bool rises(const State& st, float mx) { return mx > st.m + kSlack; }
 __device__ __forceinline__ void raise(State& st, float mx, v4f acc[8]) {
   const float m = rises(st, mx) ? mx : st.m;
-  const float shrink = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
+  const float d = m == -INFINITY ? 0.f : st.m - m;
+  const float shrink = __builtin_amdgcn_exp2f(d);
   st.m = m;
-  st.l *= shrink;
+  st.l = times_exp2(st.l, d);
 #pragma unroll
   for (int e = 0; e < 8; e++) acc[e] = acc[e] * shrink;
 }
@@ -423,10 +446,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
       }
     }
     v8h ph, pl;
+    float least = ke[0][0];
+#pragma unroll
+    for (int j = 1; j < 8; j++) least = fminf(least, ke[j >> 2][j & 3]);
     auto softmax = [&](auto mask, auto seen) {
       constexpr bool kMask = decltype(mask)::value;
       const float mx = logits<kMask>(s, kc, ke, seen);
       if (__any(rises(st, mx))) raise(st, mx, acc);
+      if (__any(least < kNear)) add_faint(s, ke, st);
       weights<kMask>(s, kw, kf, st, seen, ph, pl);
     };
     if (b * 32 + 32 <= all && cur.there[0] && cur.there[1]) {
@@ -488,7 +515,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 #pragma unroll
   for (int i = 0; i < kFewWaves; i++) {
     const float f = __builtin_amdgcn_exp2f(ml[i][row].x - ref);
-    den = __builtin_fmaf(ml[i][row].y, f, den);
+    den += times_exp2(ml[i][row].y, ml[i][row].x - ref);
 #pragma unroll
     for (int d = 0; d < kPer; d++) o[d] = __builtin_fmaf(sums[i][row][d0 + d], f, o[d]);
   }
@@ -533,8 +560,9 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
   float m = ml.x;
 #pragma unroll
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  const float own = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
-  float den = ml.y * own;
+  const float d = ml.x - (m == -INFINITY ? 0.f : m);
+  const float own = __builtin_amdgcn_exp2f(d);
+  float den = times_exp2(ml.y, d);
 #pragma unroll
   for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
   float o0 = 0.f, o1 = 0.f;
@@ -602,6 +630,7 @@ struct Block {
   __attribute__((aligned(16))) char k[kSubs][2][4][1024];  // [sub][kt][kb][lane 16 B]
   __attribute__((aligned(16))) char v[kSubs][8][1024];     // [sub][e][lane 16 B]
   __attribute__((aligned(16))) float c[kKeys], e[kKeys], w[kKeys], f[kKeys];
+  int far;  // a key has e < kNear
 };
 
 template <int NW, int QT>
@@ -719,6 +748,8 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
       d.e[tid] = ok ? k.e : -INFINITY;  // no key: its logit is -inf in every row
       d.w[tid] = k.w;
       d.f[tid] = k.f;
+      const int far = __any(ok && k.e < kNear);  // the first wave holds all keys
+      if (tid == 0) d.far = far;
     }
   };
   // MFMA operands of K (both key tiles of step kb) and V (dim tiles 2 p, 2 p + 1).
@@ -733,6 +764,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   auto compute = [&](const Blk& d, int b) {
     v8h op[2][2];
     load_k(d, 0, 0, op[0]);
+    const int far = uniform(d.far);
 #pragma unroll
     for (int sub = 0; sub < Blk::kSubs; sub++) {
       const int k0 = b * KB + 32 * sub;
@@ -783,6 +815,11 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
         if (__any(up)) {
 #pragma unroll
           for (int qt = 0; qt < QT; qt++) raise(st[qt], mx[qt], acc[qt]);
+        }
+        if (far) {
+          terms(d.e, y);
+#pragma unroll
+          for (int qt = 0; qt < QT; qt++) add_faint(s[qt], y, st[qt]);
         }
         terms(d.w, x);
         terms(d.f, y);

@@ -352,6 +352,40 @@ def test_range_of_value_scales(sdq_dev, new):
     assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
 
 
+@pytest.mark.parametrize("new,L", [(1, 200), (1, 1500), (1, 4200), (100, 200), (100, 4200),
+                                   (300, 700), (300, 4200)])
+@pytest.mark.parametrize("where", ["early", "late"])
+def test_both_ends_of_the_value_scales(sdq_dev, new, L, where):
+    """One value of scale nearly 2^60 times the first, all others of nearly 2^-60 of it, and
+    eight octaves less weight: its logit and exponent put the others' weights under the
+    smallest float, and they still own most of the denominator. The large value before and
+    behind them, in the same wave's keys and in other shares.
+
+    A small key's exponent is a difference of numbers up to 2^8: three roundings of at most
+    2^-17, 2^-16 of its weight; the same relative to the result, beside check()'s terms."""
+    c = Case(sdq_dev, [new], [L], 1, 64, seed=21)
+    at = lambda p: (c.table[0, p // 64], 0, p % 64)  # noqa: E731
+    big = 3 if where == "early" else L - new - 1
+    keys = np.arange(1, L)
+    c.vs[at(keys)] = F(0.75 * 2.0**-60)
+    c.vs[at(0)], c.vs[at(big)] = F(0.75), F(2.0**59 * 1.9)
+    c.ks[at(np.arange(L))] = F(0.01)
+    c.k[at(np.arange(L))] = c.rng.integers(-3, 4, (L, HD))
+    for p in range(L):
+        c.k[c.table[0, p // 64], 0, p % 64, 0] = 100 if p == big else 0
+    c.v[at(0)] = 0
+    c.up()
+    q = np.zeros((c.T, HD), F)
+    q[:, 0] = 8 * np.log(2) * HD**0.5
+    out = c.torch.zeros((c.T, HD), device=sdq_dev)
+    for causal in (True, False):
+        c.sdq.kv_attention(c.cache, c.batch, c.t(q), out, 1, causal=causal)
+        want, tol = c.attend(q, 1, HD**-0.5, causal)
+        got = out.cpu().numpy()
+        bad = ~(np.abs(got - want) <= tol + 2.0**-16 * 2 * np.abs(want))
+        assert not bad.any(), (causal, np.argwhere(bad)[:3], got[bad][:3], want[bad][:3])
+
+
 def test_shared_pages_and_independence(sdq_dev):
     """Two sequences that share their first pages; a batch's rows do not depend on
     who else is in it, bit for bit where the call's sizes are the same."""
