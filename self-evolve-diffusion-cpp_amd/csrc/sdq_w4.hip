@@ -181,7 +181,9 @@ __device__ __forceinline__ void put_scales(ScaleLds<GROUP, NB>& o, const Unit (&
 // A group's values become X = rint(x 2^p), p the largest power with |X| <=
 // 8355711 = 127 (2^16 + 2^8 + 1), and X = d0 2^16 + d1 2^8 + d2 with signed
 // bytes d: the bytes of X + 0x808080 with their top bits flipped. Their sums
-// with the codes are exact over a group.
+// with the codes are exact over a group. A sum in its row's own units, before the
+// weight's scale, passes fp32's range for values from 2^117 on: a row that holds one
+// of 2^64 or more is summed in units 2^32 larger, and the result shifted back.
 //
 // A workgroup of eight waves makes the bytes of all of A in LDS (its first weight
 // units already on their way), then its waves take every eighth unit of NB blocks
@@ -217,6 +219,8 @@ __device__ __forceinline__ long as_long(int a, int b) {
 }
 
 constexpr int kFewMaxRows = 5;
+constexpr float kHuge = 0x1p64f;
+constexpr int kHugeShift = 32;  // values under 2^128, their sums with 128 codes under 2^139
 
 struct FewLds {  // offsets of the dynamic LDS, for the host too
   int64_t power, sums, scales, bytes;
@@ -235,7 +239,7 @@ __global__ void __launch_bounds__(64 * kWaves)
 w4_few_kernel(W4View wt, const float* __restrict__ x, int M, int vec, EpiArgs epi,
               float* __restrict__ y) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ int bad_row[kFewMaxRows];
+  __shared__ int bad_row[kFewMaxRows], shift_row[kFewMaxRows];
   constexpr int per = 128 / GROUP;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 4;
   const int64_t units = (wt.K + 127) / 128, nblk = (wt.N + 15) / 16;
@@ -262,7 +266,7 @@ w4_few_kernel(W4View wt, const float* __restrict__ x, int M, int vec, EpiArgs ep
   };
   if (w < units) load(w, cur, zcur);
 
-  if (tid < kFewMaxRows) bad_row[tid] = 0;
+  if (tid < kFewMaxRows) bad_row[tid] = shift_row[tid] = 0;
   __syncthreads();
   for (int m = 0; m < M; m++) {
     for (int64_t k = tid * 8; k < units * 128; k += 64 * kWaves * 8) {
@@ -278,6 +282,7 @@ w4_few_kernel(W4View wt, const float* __restrict__ x, int M, int vec, EpiArgs ep
         mx = fmaxf(mx, fabsf(v[i]));
       }
       if (bad) bad_row[m] = 1;
+      if (mx >= kHuge) shift_row[m] = kHugeShift;
 #pragma unroll
       for (int o = 1; o < GROUP / 8; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
       const int p = group_power(mx);
@@ -311,7 +316,7 @@ w4_few_kernel(W4View wt, const float* __restrict__ x, int M, int vec, EpiArgs ep
   auto& sl = *reinterpret_cast<ScaleLds<GROUP, NB>*>(lds + at.scales +
                                                      w * (int64_t)sizeof(ScaleLds<GROUP, NB>));
   const int col = (l & 15) < C ? l & 15 : C - 1, m = col % M;
-  const int place = 16 - 8 * (col / M);  // the digit's 2^16, 2^8, 1
+  const int place = 16 - 8 * (col / M) - shift_row[m];  // the digit's 2^16, 2^8, 1
   float f[NB][4] = {};
   for (int64_t u = w; u < units; u += kWaves) {
     Unit nxt[NB];
@@ -387,6 +392,7 @@ w4_few_kernel(W4View wt, const float* __restrict__ x, int M, int vec, EpiArgs ep
       for (int k = 0; k < kWaves; k++) t += red[(k * NB * 16 + n) * 16 + d * M + r];
       v += t;
     }
+    v = __builtin_ldexpf(v, shift_row[r]);
     if (bad_row[r]) v = __builtin_nanf("");
     if (nb0 * 16 + n < wt.N) store_one(epi, y, r, nb0 * 16 + n, wt.N, v);
   }

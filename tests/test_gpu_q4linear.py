@@ -156,6 +156,32 @@ def test_special_values(sdq_dev, M):
             assert (np.abs(got[:M - 1] - want) <= tol).all()
 
 
+@pytest.mark.parametrize("M", [1, 3, 5, 6, 17, 32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_rows_near_the_largest_float(sdq_dev, M, group):
+    """Values up to fp32's largest whose results are finite: dense rows of one sign, where a
+    group's sum with the codes alone passes fp32's range, rows of both signs, and one such value
+    beside ordinary ones."""
+    N, K = 70, 1024
+    u, scale, zero = make(N, K, group, True, 31)
+    rng = np.random.default_rng(32)
+    top = float(np.finfo(F).max)
+    for size, sc in ((1e36, 1e-3), (top, 2e-6), (top, 1e-30)):
+        one = np.full((M, K), size)
+        two = size * rng.uniform(-1, 1, (M, K))
+        few = rng.standard_normal((M, K))
+        few[:, 300] = size
+        for x in (one, two, few):
+            x = x.astype(F)
+            s = (scale * (sc / 0.02)).astype(F)
+            codes = np.where(u & 1, u | 0x77, u)  # more of one sign
+            want, tol = expected(x, codes, s, zero, group)
+            assert (np.abs(want) < top / 4).all()
+            got = call(sdq_dev, codes, s, zero, group, x)
+            bad = ~(np.abs(got - want) <= tol + 64 * 2.0**-149)
+            assert not bad.any(), (size, sc, np.argwhere(bad)[:3], got[bad][:3], want[bad][:3])
+
+
 def test_in_place_residual_and_two_streams(sdq_dev):
     """resid is Y; two calls of different sizes at once on two streams."""
     import torch
