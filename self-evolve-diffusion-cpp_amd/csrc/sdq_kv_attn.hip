@@ -807,9 +807,9 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
         bool up = false;
 #pragma unroll
         for (int qt = 0; qt < QT; qt++) {
-          s[qt][0] = s[qt][0] * qk[qt];
-          s[qt][1] = s[qt][1] * qk[qt];
-          mx[qt] = logits<kMask>(s[qt], x, y, [&](int kt, int i) { return seen(qt, kt, i); });
+          // the key's scale first: the score alone may pass fp32's range
+          const v4f cq[2] = {x[0] * qk[qt], x[1] * qk[qt]};
+          mx[qt] = logits<kMask>(s[qt], cq, y, [&](int kt, int i) { return seen(qt, kt, i); });
           up |= rises(st[qt], mx[qt]);
         }
         if (__any(up)) {

@@ -327,6 +327,26 @@ def test_a_huge_row_takes_nothing_from_others(sdq_dev, new):
     assert_bitexact(got[keep], first[keep], "the other rows")
 
 
+@pytest.mark.parametrize("new", [1, 20, 100, 300])
+@pytest.mark.parametrize("size", [1e30, 3e35, 1e36])
+def test_large_queries(sdq_dev, new, size):
+    """Queries whose products with the codes alone pass fp32's range, with the key's scale they do
+    not: one key's logit is far above all others, and its value is the result (its code times its
+    scale: the weight's parts and three roundings)."""
+    L = new + 200
+    c = Case(sdq_dev, [new], [L], 1, 32, seed=22)
+    sign = np.where(np.arange(HD) % 3, 1, -1)
+    c.k[c.table[0, 1], 0, 7] = 127 * sign  # token 39
+    c.ks[c.table[0, 1], 0, 7] = F(0.018)
+    c.up()
+    q = np.repeat((size * sign).astype(F)[None], new, 0)
+    q = np.concatenate([q, q * F(0.5)], 1)
+    out = c.torch.zeros((new, 2 * HD), device=sdq_dev)
+    c.sdq.kv_attention(c.cache, c.batch, c.t(q), out, 2, causal=True)
+    want = np.tile(c.values(0, 0)[1][39], 2)[None]
+    assert (np.abs(out.cpu().numpy() - want) <= 2.0**-20 * np.abs(want)).all()
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_range_of_value_scales(sdq_dev, new):
     """A first value of next to nothing leaves the others their precision; scales
