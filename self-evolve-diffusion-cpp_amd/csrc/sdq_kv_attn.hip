@@ -764,7 +764,6 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   auto compute = [&](const Blk& d, int b) {
     v8h op[2][2];
     load_k(d, 0, 0, op[0]);
-    const int far = uniform(d.far);
 #pragma unroll
     for (int sub = 0; sub < Blk::kSubs; sub++) {
       const int k0 = b * KB + 32 * sub;
@@ -805,6 +804,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
         terms(d.e, y);
         float mx[QT];
         bool up = false;
+        const int far = d.far;
 #pragma unroll
         for (int qt = 0; qt < QT; qt++) {
           // the key's scale first: the score alone may pass fp32's range
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
 #pragma unroll
           for (int qt = 0; qt < QT; qt++) raise(st[qt], mx[qt], acc[qt]);
         }
-        if (far) {
+        if (uniform(far)) {
           terms(d.e, y);
 #pragma unroll
           for (int qt = 0; qt < QT; qt++) add_faint(s[qt], y, st[qt]);
