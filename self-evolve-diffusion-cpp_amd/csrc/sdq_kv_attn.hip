@@ -6,9 +6,12 @@
 // Numbers. A cached value is code * scale; the codes are exact in fp16, so each
 // fp32 product costs two fp16 MFMA products: q = (hi + lo) 2^-r, r a power of two
 // for each row that puts its largest element into [2^14, 2^15), and the softmax
-// weight = hi + lo below. Both parts are truncated: hi + lo is off by less than
-// 2^-21 of the value, or an absolute 2^-39 of the row's largest. The key's scale
-// multiplies the finished sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in
+// weight = hi + lo below. Both parts are rounded: hi + lo is off by at most 2^-22
+// of the value, or half of fp16's smallest step, an absolute 2^-39 of the row's largest
+// element and 2^-34 of its largest weight. (Truncated parts lost up to 1.4e-4 where 2^17 equal
+// light keys stand beside a heavy one, of values of 2.5; now 1.7e-5. A reference that
+// rises by 2^2 instead of 2^6, the weights 2^4 further from the smallest step: 0.9e-5, and
+// 2% slower for 768 tokens.) The key's scale multiplies the finished sum. The value's scale is v_j = f_j 2^(e_j + E0), f_j in
 // [1/2, 1), E0 the exponent of the sequence's first value, at least -16: its exponent
 // goes into the softmax,
 //   t_j = s_j + e_j,  X_j = 2^(t_j - m), m near the running maximum of t,
@@ -46,7 +49,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kTop = 15;      // largest q of a row below 2^kTop
 constexpr int kSlack = 6;     // X stays below 2^kSlack
-constexpr int kWeight = 9;    // weights X f enter as X f 2^kWeight
+constexpr int kWeight = 9;    // weights X f enter as X f 2^kWeight, below 2^15
 constexpr int kFar = 60;      // e_j is held to -kFar .. kFar
 constexpr int kLeast = -16;   // of E0
 // A key with e >= kNear whose X is under 2^-126 is less than 2^(-126 - kNear) of a
@@ -179,14 +182,17 @@ __device__ __forceinline__ float less_high(v2h hi, float x) {
       : "v"(hi), "v"(x));
   return r;
 }
-// fp32 to two fp16 parts, both truncated (two conversions at a time): the high
-// part's remainder is exact, so the pair is off by less than 2^-21.
+// fp32 to two fp16 parts, both rounded (two conversions at a time): the high
+// part's remainder is exact, so the pair is off by at most 2^-22.
+__device__ __forceinline__ v2h rounded(float a, float b) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  return __builtin_convertvector((v2f{a, b}), v2h);
+}
 __device__ __forceinline__ void parts8(const float x[8], v8h& hi, v8h& lo) {
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const v2h h = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]));
-    const v2h r = __builtin_bit_cast(
-        v2h, __builtin_amdgcn_cvt_pkrtz(less_low(h, x[i]), less_high(h, x[i + 1])));
+    const v2h h = rounded(x[i], x[i + 1]);
+    const v2h r = rounded(less_low(h, x[i]), less_high(h, x[i + 1]));
     hi[i] = h[0];
     hi[i + 1] = h[1];
     lo[i] = r[0];
@@ -291,14 +297,15 @@ template <bool MASK, class Seen>
 __device__ __forceinline__ void weights(const v4f t[2], const v4f w[2], const v4f f[2], State& st,
                                         Seen seen, v8h& hi, v8h& lo) {
   const float ref = st.m == -INFINITY ? 0.f : st.m;
-  float p[8];
+  float p[8], l = 0.f;  // the block's share first: an eighth of the roundings of a long sum
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     const float x = __builtin_amdgcn_exp2f(t[j >> 2][j & 3] - ref);
-    st.l = __builtin_fmaf(x, w[j >> 2][j & 3], st.l);
+    l = __builtin_fmaf(x, w[j >> 2][j & 3], l);
     p[j] = x * f[j >> 2][j & 3];
     if (MASK && !seen(j >> 2, j & 3)) p[j] = 0.f;  // its scale may be NaN
   }
+  st.l += l;
   parts8(p, hi, lo);
 }
 // a 2^d, also where 2^d alone is under the smallest float (exp2 gives 0 there).
@@ -311,13 +318,15 @@ __device__ __forceinline__ float times_exp2(float a, float d) {
 // where a block has a key with e < kNear.
 __device__ __forceinline__ void add_faint(v4f t[2], const v4f e[2], State& st) {
   const float ref = st.m == -INFINITY ? 0.f : st.m;
+  float l = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     const float x = t[j >> 2][j & 3] - ref;
     const bool faint = x < -126.f && x > -1000.f;
-    st.l += __builtin_amdgcn_exp2f(faint ? x - e[j >> 2][j & 3] : -INFINITY);
+    l += __builtin_amdgcn_exp2f(faint ? x - e[j >> 2][j & 3] : -INFINITY);
     t[j >> 2][j & 3] = faint ? -INFINITY : t[j >> 2][j & 3];
   }
+  st.l += l;
 }
 // The reference rises only when a block's largest logit passes it by more than
 // kSlack (the weights then stay below 2^kSlack, inside fp16 with kWeight):

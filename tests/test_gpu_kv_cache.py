@@ -406,6 +406,44 @@ def test_both_ends_of_the_value_scales(sdq_dev, new, L, where):
         assert not bad.any(), (causal, np.argwhere(bad)[:3], got[bad][:3], want[bad][:3])
 
 
+@pytest.mark.parametrize("nseq,new", [(800, 1), (1100, 100), (1, 1 << 17)])
+def test_many_light_keys(sdq_dev, nseq, new):
+    """2^17 keys of equal weight, 22 octaves under that of the first, whose value is zero, seen
+    by so many rows that their keys are not cut: each light weight is rounded to the parts'
+    smallest step, all of them the same way, and the sum keeps them.
+
+    Of max |v|: the weights' second part is off by at most 2^-25 where the largest weight is 2^9
+    (2^-34 a key, 2^-17 of all), the parts otherwise and the query's by 2^-21 of a share of 2^-5; the
+    logits' roundings 2^-19 of it. A lane adds up the denominator of a block of 32 keys at a time, and
+    every addition of an equal share to a sum near 1 can be off the same way by 2^-24: n / 32 of
+    them, 2^-12 of the denominator, of which the result is a share of 2^-5."""
+    n = 1 << 17
+    L = n + 1
+    c = Case(sdq_dev, [1], [L], 1, 1024, seed=23)
+    p = np.arange(L)
+    at = c.table[0, p // 1024], 0, p % 1024
+    c.vs[at] = F(0.0199)
+    c.ks[at] = F(0.01)
+    k = np.zeros((L, HD), np.int8)
+    k[0, 0] = 100
+    v = np.full((L, HD), 127, np.int8)
+    v[0] = 0
+    c.k[at], c.v[at] = k, v
+    c.table = np.repeat(c.table, nseq, 0)  # shared pages
+    c.lens, c.start, c.T = [L] * nseq, new * np.arange(nseq + 1, dtype=np.int32), nseq * new
+    c.up()
+    tol = (2.0**-17 + 2.0**-5 * (2.0**-21 + 2.0**-19 + 2.0**-12)) * 127 * 0.0199
+    out = c.torch.zeros((c.T, HD), device=sdq_dev)
+    for octaves in (22.0, 22.17, 22.31, 22.5, 22.63, 22.9):
+        q = c.torch.zeros((c.T, HD), device=sdq_dev)
+        q[:, 0] = octaves * np.log(2) * HD**0.5
+        c.sdq.kv_attention(c.cache, c.batch, q, out, 1, causal=False)
+        w = np.exp2(-float(q[0, 0]) * 100 * float(F(0.01)) * HD**-0.5 / np.log(2))
+        want = n * w / (1 + n * w) * 127 * float(F(0.0199))
+        err = (out.double() - want).abs().max().item()
+        assert err <= tol, (octaves, err / tol)
+
+
 def test_shared_pages_and_independence(sdq_dev):
     """Two sequences that share their first pages; a batch's rows do not depend on
     who else is in it, bit for bit where the call's sizes are the same."""
