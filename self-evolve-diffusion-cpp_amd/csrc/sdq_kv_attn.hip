@@ -221,16 +221,25 @@ __device__ __forceinline__ void load_q(const Args& a, const Tile& t, int h, int6
       x[kb][4 * j + 3] = v.w;
     }
 }
-__device__ __forceinline__ float amax_finite(const float x[4][8]) {
-  float m = 0.f;
+// The largest magnitude of a row's slice. NaN and infinities become zeros, and the row (of
+// four lanes) is `bad`: its denominator is NaN once it has seen a key, and 0 before.
+__device__ __forceinline__ float clean(float x[4][8], bool& bad) {
+  float m = 0.f, b = 0.f;
 #pragma unroll
   for (int kb = 0; kb < 4; kb++)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float v = fabsf(x[kb][i]);
-      m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
+      const bool fine = fabsf(x[kb][i]) <= 3.402823466e38f;
+      x[kb][i] = fine ? x[kb][i] : 0.f;
+      b = fine ? b : 1.f;
+      m = fmaxf(m, fabsf(x[kb][i]));
     }
-  return m;
+  bad = quad_max(b) != 0.f;
+  return quad_max(m);
+}
+__device__ __forceinline__ float den_of(float l, bool bad) {
+  const float den = quad_sum(l);
+  return bad && den != 0.f ? __builtin_nanf("") : den;
 }
 // Exponent that scales a row's largest |q| below 2^kTop; within what a float's power
 // of two can hold. Each row has its own: one of the same tile that holds something
@@ -368,7 +377,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 
   float x[4][8];
   load_q(a, t, h, t.r0 + r16, g, x);
-  const int qe = q_exp(quad_max(amax_finite(x)));
+  bool bad;
+  const int qe = q_exp(clean(x, bad));
   v8h qh[4], ql[4];
 #pragma unroll
   for (int kb = 0; kb < 4; kb++) {
@@ -503,8 +513,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
   // Join the waves: common maximum, then sums.
   __shared__ float2 ml[kFewWaves][kFewRows];
   __shared__ __attribute__((aligned(16))) float sums[kFewWaves][kFewRows][kFewStride];
-  st.l = quad_sum(st.l);
-  if (g == 0) ml[w][r16] = float2{st.m, st.l};
+  const float own = den_of(st.l, bad);
+  if (g == 0) ml[w][r16] = float2{st.m, own};
 #pragma unroll
   for (int i = 0; i < 4; i++) {  // dims 32 g + 8 i + e
     float* o = &sums[w][r16][32 * g + 8 * i];
@@ -659,13 +669,14 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   v8h qh[QT][4], ql[QT][4];
   int mine[QT];
   float qk[QT];
+  bool bad[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; qt++) {
     const int64_t r = t.r0 + (w * QT + qt) * 16 + r16;
     float x[4][8];
     load_q(a, t, h, r, g, x);
     mine[qt] = keys_of(t, r, a.group, a.causal);
-    const int qe = q_exp(quad_max(amax_finite(x)));
+    const int qe = q_exp(clean(x, bad[qt]));
 #pragma unroll
     for (int kb = 0; kb < 4; kb++) {
 #pragma unroll
@@ -897,7 +908,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     const int row = (w * QT + qt) * 16 + r16;
     const int64_t r = t.r0 + row;
     if (r >= t.rows) continue;
-    const float den = quad_sum(st[qt].l);
+    const float den = den_of(st[qt].l, bad[qt]);
     float f = 1.f;
     float* dst;
     if (a.splits == 1) {

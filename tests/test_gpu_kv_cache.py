@@ -299,6 +299,32 @@ def test_nan_stays_where_it_is(sdq_dev, new):
     assert np.isnan(got[new:]).all() and np.isfinite(clean).all()
 
 
+@pytest.mark.parametrize("new", [1, 40, 100, 300])
+def test_nan_queries_that_see_no_key(sdq_dev, new):
+    """Rows of padding, whatever they hold, whose sequence has no page or no keys are 0."""
+    c = Case(sdq_dev, [new, new, new], [new + 40, new + 90, 0], 1, 16, seed=24)
+    c.table[0] = -1
+    c.up()
+    q = c.rng.standard_normal((c.T, 2 * HD)).astype(F)
+    want = c.check(2, True, q=q)
+    for bad in (np.nan, np.inf):
+        q[:new] = bad
+        q[2 * new:, 5] = bad
+        for causal in (True, False):
+            out = c.torch.full((c.T, 2 * HD), 4.0, device=sdq_dev)
+            c.sdq.kv_attention(c.cache, c.batch, c.t(q), out, 2, causal=causal)
+            got = out.cpu().numpy()
+            assert (got[:new] == 0).all() and (got[2 * new:] == 0).all()
+            if causal:
+                assert_bitexact(got[new:2 * new], want[new:2 * new], "the other sequence")
+    # the first half of the pages is missing: rows that see none of the others
+    c.table[1, :c.lens[1] // 32] = -1
+    c.up()
+    q = c.rng.standard_normal((c.T, 2 * HD)).astype(F)
+    c.check(2, True, q=q)
+    c.check(2, False, q=q)
+
+
 @pytest.mark.parametrize("nseq,most", [(63, 3), (64, 2), (65, 40), (200, 9), (4100, 2)])
 def test_many_sequences(sdq_dev, nseq, most):
     """Ragged batches around the search's widths, empty sequences among them, rows
