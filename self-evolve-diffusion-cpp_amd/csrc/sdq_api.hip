@@ -111,14 +111,25 @@ struct ThreadStream {
         (void)hipStreamSynchronize(hipStreamPerThread);
   }
 };
+ThreadStream& thread_stream() {
+  thread_local ThreadStream self;
+  return self;
+}
+
+// An entry point's stream argument; all of them take it through here, also those that use
+// no workspace.
+hipStream_t stream_of(void* stream) {
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  int dev = -1;
+  if (s == hipStreamPerThread && hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < kMaxDev)
+    thread_stream().devices |= uint64_t(1) << dev;
+  return s;
+}
 
 // The workspace of (device, stream), under g_mu. hipStreamPerThread is another
 // stream in every thread: the thread's own address stands for it.
 Workspace& ws_of(int dev, hipStream_t s) {
-  if (s != hipStreamPerThread) return g_ws[{dev, s}];
-  thread_local ThreadStream self;
-  self.devices |= uint64_t(1) << dev;
-  return g_ws[{dev, reinterpret_cast<hipStream_t>(&self)}];
+  return g_ws[{dev, s == hipStreamPerThread ? reinterpret_cast<hipStream_t>(&thread_stream()) : s}];
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -668,7 +679,7 @@ int sdq_weight_upload(const int8_t* q, const float* scale, int64_t N, int64_t K,
   int rc = current_device(&dev);
   if (rc) return rc;
   if ((rc = ensure_device(dev))) return rc;
-  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipStream_t s = stream_of(stream);
   sdq_weight* w = nullptr;
   if ((rc = alloc_weight(dev, N, K, &w))) return rc;
   // Stage the .sdcpp blob as it is on disk (int8 rows, then the scales,
@@ -1173,7 +1184,7 @@ int sdq_weight_upload_batch(const sdq_weight_src* src, int n, void* stream, sdq_
     }
     return SDQ_OK;
   };
-  return upload_ring(dev, Ns, Ks, fill, static_cast<hipStream_t>(stream), out);
+  return upload_ring(dev, Ns, Ks, fill, stream_of(stream), out);
 }
 
 int sdq_weight_upload_file(const char* path, const sdq_weight_fsrc* src, int n, void* stream,
@@ -1242,7 +1253,7 @@ int sdq_weight_upload_file(const char* path, const sdq_weight_fsrc* src, int n, 
         return set_error(SDQ_ERR_FORMAT, std::string("short read from ") + path);
       return SDQ_OK;
     };
-    rc = upload_ring(dev, Ns, Ks, fill, static_cast<hipStream_t>(stream), out);
+    rc = upload_ring(dev, Ns, Ks, fill, stream_of(stream), out);
   }
   ::close(fd);
   return rc;
@@ -1259,7 +1270,7 @@ int sdq_weight_upload_device(const int8_t* q_dev, const float* scale_dev, int64_
   int rc = current_device(&dev);
   if (rc) return rc;
   if ((rc = ensure_device(dev))) return rc;
-  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipStream_t s = stream_of(stream);
   sdq_weight* w = nullptr;
   if ((rc = alloc_weight(dev, N, K, &w))) return rc;
   hipError_t e = launch_repack_weight(q_dev, scale_dev, N, K, w->Np, w->KFp, w->frags, w->scale, s);
@@ -1309,14 +1320,14 @@ int sdq_weight_export_host(const sdq_weight* w, int8_t* q, float* scale) {
 
 int sdq_qlinear(const sdq_weight* w, const float* A, int64_t M, int64_t K, const sdq_epilogue* epi,
                 void* Y, void* stream) {
-  return qlinear_device(w, A, M, K, epi, Y, static_cast<hipStream_t>(stream));
+  return qlinear_device(w, A, M, K, epi, Y, stream_of(stream));
 }
 
 
 int sdq_qlinear_group(const sdq_group_item* items, int n, void* stream) {
   if (n < 0 || n > SDQ_MAX_GROUP) return set_error(SDQ_ERR_INVALID, "group: n must be 0..16");
   if (n > 0 && !items) return set_error(SDQ_ERR_INVALID, "group: null items");
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   int dev = -1;
   int rc = current_device(&dev);
   if (rc) return rc;
@@ -1490,7 +1501,7 @@ int sdq_qlinear_stack(const sdq_group_item* items, int n, int ngroup, const sdq_
   if (n < 0 || n > SDQ_MAX_GROUP) return set_error(SDQ_ERR_INVALID, "stack: n must be 0..16");
   if (ngroup < 0 || ngroup > n) return set_error(SDQ_ERR_INVALID, "stack: need 0 <= ngroup <= n");
   if (n > 0 && !items) return set_error(SDQ_ERR_INVALID, "stack: null items");
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   int dev = -1;
   int rc = current_device(&dev);
   if (rc) return rc;
@@ -1834,7 +1845,7 @@ int sdq_ffn(const sdq_weight* fc1, const float* b1, const sdq_weight* fc2, const
             const float* h, int64_t M, const float* gate, int gate_fma, float* hid, float* x,
             void* stream) {
   return ffn_device(fc1, b1, fc2, b2, h, M, gate, gate_fma, hid, x,
-                    static_cast<hipStream_t>(stream), nullptr);
+                    stream_of(stream), nullptr);
 }
 
 int sdq_ffn_lnmod(const sdq_weight* fc1, const float* b1, const sdq_weight* fc2, const float* b2,
@@ -1843,7 +1854,7 @@ int sdq_ffn_lnmod(const sdq_weight* fc1, const float* b1, const sdq_weight* fc2,
   if (!shift || !scale) return set_error(SDQ_ERR_INVALID, "ffn: null shift or scale");
   const LnMod lm{shift, scale, eps};
   return ffn_device(fc1, b1, fc2, b2, x, M, gate, gate_fma, hid, x,
-                    static_cast<hipStream_t>(stream), &lm);
+                    stream_of(stream), &lm);
 }
 
 int sdq_qlinear_lnmod(const sdq_weight* w, const float* x, int64_t M, int64_t K,
@@ -1851,7 +1862,7 @@ int sdq_qlinear_lnmod(const sdq_weight* w, const float* x, int64_t M, int64_t K,
                       const sdq_epilogue* epi, void* Y, void* stream) {
   if (!shift || !scale) return set_error(SDQ_ERR_INVALID, "null shift or scale");
   const LnMod lm{shift, scale, eps};
-  return qlinear_device(w, x, M, K, epi, Y, static_cast<hipStream_t>(stream), nullptr, nullptr,
+  return qlinear_device(w, x, M, K, epi, Y, stream_of(stream), nullptr, nullptr,
                         &lm);
 }
 
@@ -1882,7 +1893,7 @@ int sdq_rmsnorm_rope_batch(const sdq_rms_seg* segs, int nseg, int64_t C, int hea
   int rc = current_device(&dev);
   if (rc) return rc;
   if ((rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   float* inv = nullptr;
   if (rows_w > 0 && !rms_rows_fits(g, n, C, heads) &&
       (rc = ws_floats(dev, s, &Workspace::rinv, &Workspace::rinv_bytes, (size_t)rows_w * 4, &inv)))
@@ -1925,7 +1936,7 @@ int sdq_layernorm(const float* x, int64_t M, int64_t K, const float* w, const fl
   int rc = current_device(&dev);
   if (rc) return rc;
   if ((rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   const bool rows = ln_rows_fits(x, M, K, w, b, y);
   float2* st = nullptr;
   if (!rows) {
@@ -1959,7 +1970,7 @@ int sdq_add(float* x, const float* y, int64_t n, void* stream) {
   if (n < 0) return set_error(SDQ_ERR_INVALID, "negative n");
   if (n == 0) return SDQ_OK;
   if (!x || !y) return set_error(SDQ_ERR_INVALID, "add: null pointer");
-  hipError_t e = launch_add(x, y, n, static_cast<hipStream_t>(stream));
+  hipError_t e = launch_add(x, y, n, stream_of(stream));
   return e == hipSuccess ? SDQ_OK : hip_error(e, "add launch");
 }
 
@@ -1972,7 +1983,7 @@ int sdq_linear_f32(const float* x, int64_t M, int64_t K, const float* w, int64_t
   int rc = current_device(&dev);
   if (rc) return rc;
   if ((rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   hipEvent_t p0 = t_prof ? prof_mark(s) : nullptr;
   const hipError_t e = launch_linear_f32(x, M, K, w, N, bias, y, g_dev[dev].cu_count, s);
   if (e != hipSuccess) {
@@ -2017,7 +2028,7 @@ int sdq_sdpa_batched(const float* q, int64_t ldq, const float* k, int64_t ldk, c
   int rc = current_device(&dev);
   if (rc) return rc;
   if ((rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   const int cu_count = g_dev[dev].cu_count;
   // The packed form when its scratch can be had (at most
   // sdpa::kMaxScratch bytes), else the form without scratch: an attention call is
@@ -2063,7 +2074,7 @@ int sdq_sdpa_batched(const float* q, int64_t ldq, const float* k, int64_t ldk, c
 }
 
 int sdq_qgemm(const sdq_weight* w, const float* A, int64_t M, int64_t K, float* Y, void* stream) {
-  return qlinear_device(w, A, M, K, nullptr, Y, static_cast<hipStream_t>(stream));
+  return qlinear_device(w, A, M, K, nullptr, Y, stream_of(stream));
 }
 
 int sdq_qlinear_host(const sdq_weight* w, const float* A, int64_t M, int64_t K,
@@ -2187,7 +2198,7 @@ int sdq_act_quant(const float* A, int64_t M, int64_t K, int8_t* aq, float* as, v
   int rc = current_device(&dev);
   if (rc) return rc;
   if ((rc = ensure_device(dev))) return rc;
-  hipError_t e = launch_act_quant_rowmajor(A, M, K, aq, as, static_cast<hipStream_t>(stream));
+  hipError_t e = launch_act_quant_rowmajor(A, M, K, aq, as, stream_of(stream));
   if (e != hipSuccess) return hip_error(e, "act_quant launch");
   return SDQ_OK;
 }
@@ -2204,7 +2215,7 @@ int sdq_dequant(const int8_t* aq, const float* as, int64_t M, int64_t K, float* 
   int dev = -1;
   int rc = current_device(&dev);
   if (rc || (rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   return timed("dequant", s, [&] { return launch_dequant(aq, as, M, K, y, s); });
 }
 
@@ -2217,7 +2228,7 @@ int sdq_qlinear_codes(const sdq_weight* w, const int8_t* aq, const float* as, in
       return set_error(SDQ_ERR_INVALID, "qlinear_codes: Y overlaps an input");
   }
   const Codes codes{aq, as};
-  return qlinear_device(w, nullptr, M, K, epi, Y, static_cast<hipStream_t>(stream), nullptr,
+  return qlinear_device(w, nullptr, M, K, epi, Y, stream_of(stream), nullptr,
                         nullptr, nullptr, nullptr, &codes);
 }
 
@@ -2252,7 +2263,7 @@ int sdq_rmsnorm_quant(const float* x, int64_t ldx, const float* d, int64_t ldd, 
   int dev = -1;
   int rc = current_device(&dev);
   if (rc || (rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   return timed("rmsnorm_quant", s, [&] {
     return launch_rmsnorm_quant(x, ldx, d, ldd, M, K, w, eps, sum, ldsum, aq, as,
                                 g_dev[dev].cu_count, s);
@@ -2269,7 +2280,7 @@ int sdq_weight4_upload_device(const uint8_t* u, const float* scale, const uint8_
   if (rc) return rc;
   int dev = -1;
   if ((rc = current_device(&dev)) || (rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   if (capturing(s))
     return set_error(SDQ_ERR_INVALID, "a weight cannot be uploaded while the stream captures a graph");
   sdq_weight4* w = new (std::nothrow) sdq_weight4{dev, N, K, group, nullptr, nullptr, nullptr};
@@ -2304,7 +2315,7 @@ int sdq_weight4_upload(const uint8_t* u, const float* scale, const uint8_t* zero
   if (rc) return rc;
   int dev = -1;
   if ((rc = current_device(&dev)) || (rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   if (capturing(s))
     return set_error(SDQ_ERR_INVALID, "a weight cannot be uploaded while the stream captures a graph");
   const size_t nu = (size_t)N * (size_t)((K + 1) / 2), ng = (size_t)(N * ceil_div(K, group));
@@ -2375,7 +2386,7 @@ int sdq_q4linear(const sdq_weight4* w, const float* A, int64_t M, int64_t K,
       bytes_overlap(Y, ny, epi ? epi->bias : nullptr, (size_t)w->N * 4))
     return set_error(SDQ_ERR_INVALID, "q4linear: Y overlaps an input (resid may be Y as a whole)");
   if ((rc = ensure_device(dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   const W4View view{w->N, w->K, w->group, w->codes, w->scale, w->zero};
   const EpiArgs ea = make_epi(epi, K);
   const W4Plan plan = plan_w4(view, M, g_dev[dev].cu_count);
@@ -2399,7 +2410,7 @@ int sdq_kv_write(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* k, i
     return rc;
   int dev = -1;
   if ((rc = usable_device(&dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   return timed("kv_write", s, [&] { return launch_kv_write(view, k, ldk, v, ldv, s); });
 }
 
@@ -2419,7 +2430,7 @@ int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t 
   }
   int dev = -1;
   if ((rc = usable_device(&dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   return timed("kv_read", s, [&] { return launch_kv_read(view, k, ldk, v, ldv, s); });
 }
 
@@ -2446,7 +2457,7 @@ int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* 
   }
   int dev = -1;
   if ((rc = usable_device(&dev))) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const hipStream_t s = stream_of(stream);
   const kvplan::Plan plan =
       kvplan::plan(T, view.nseq, heads / c->kv_heads, c->kv_heads,
                    view.max_pages << view.page_log2, g_dev[dev].cu_count);
@@ -2488,13 +2499,13 @@ int sdq_memcpy(void* dst, const void* src, size_t bytes, int kind, void* stream)
     case SDQ_D2D: k = hipMemcpyDeviceToDevice; break;
     default: return set_error(SDQ_ERR_INVALID, "bad copy kind");
   }
-  hipError_t e = hipMemcpyAsync(dst, src, bytes, k, static_cast<hipStream_t>(stream));
+  hipError_t e = hipMemcpyAsync(dst, src, bytes, k, stream_of(stream));
   if (e != hipSuccess) return hip_error(e, "hipMemcpyAsync");
   return SDQ_OK;
 }
 
 int sdq_stream_sync(void* stream) {
-  hipError_t e = hipStreamSynchronize(static_cast<hipStream_t>(stream));
+  hipError_t e = hipStreamSynchronize(stream_of(stream));
   if (e != hipSuccess) return hip_error(e, "hipStreamSynchronize");
   return SDQ_OK;
 }
@@ -2518,8 +2529,8 @@ int sdq_stream_wait(void* waiter, void* signaler) {
       return hip_error(e, "hipEventCreateWithFlags");
     }
   }
-  e = hipEventRecord(ev, static_cast<hipStream_t>(signaler));
-  if (e == hipSuccess) e = hipStreamWaitEvent(static_cast<hipStream_t>(waiter), ev, 0);
+  e = hipEventRecord(ev, stream_of(signaler));
+  if (e == hipSuccess) e = hipStreamWaitEvent(stream_of(waiter), ev, 0);
   if (e != hipSuccess) return hip_error(e, "stream wait");
   return SDQ_OK;
 }
@@ -2542,7 +2553,7 @@ int sdq_qlinear_noalloc(const sdq_weight* w, const float* A, int64_t M, int64_t 
     why = g_dev[w->device].scratch_err;
   }
   if (!p) return set_error(SDQ_ERR_HIP, "sdq_qlinear_noalloc: scratch unavailable (" + why + ")");
-  return qlinear_device(w, A, M, K, epi, Y, static_cast<hipStream_t>(stream), nullptr, nullptr,
+  return qlinear_device(w, A, M, K, epi, Y, stream_of(stream), nullptr, nullptr,
                         nullptr, p);
 }
 

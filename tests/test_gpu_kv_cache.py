@@ -673,6 +673,70 @@ def test_a_thread_that_ends_waits_for_its_stream(sdq_dev):
             assert torch.equal(o, w)
 
 
+@pytest.mark.parametrize("what", ["write", "read", "attention", "norm", "dequant", "linear"])
+def test_a_thread_that_ends_waits_for_calls_without_scratch(sdq_dev, what):
+    """The same for calls that ask the stream's workspace for nothing: what a thread queued is
+    there when it has ended."""
+    import threading
+
+    import torch
+
+    import sdq
+    import test_gpu_q4linear as q4
+
+    n = 20000
+    c = Case(sdq_dev, [n], [n], 2, 64, seed=25)
+    x, y = (torch.randn((n, 256), device=sdq_dev) for _ in range(2))
+    u, scale, _ = q4.make(8192, 4096, 128, False, 3)
+    w = sdq.Weight4.from_host(u, scale, group=128)
+    one = torch.randn((1, 4096), device=sdq_dev)
+    codes = torch.empty((n, 256), dtype=torch.int8, device=sdq_dev)
+    scales = torch.empty(n, device=sdq_dev)
+    sdq.act_quant(x, codes, scales)
+    fresh = lambda *like: [torch.zeros_like(t) for t in like]  # noqa: E731
+    pool = lambda: sdq.KvCache(*fresh(c.cache.k, c.cache.ks, c.cache.v, c.cache.vs))  # noqa: E731
+    few = Case(sdq_dev, [1] * 400, [200] * 400, 2, 64, seed=26)  # too few keys to be cut
+    q = torch.randn((400, 512), device=sdq_dev)
+
+    def make():  # outputs, and the call that fills them
+        if what == "write":
+            p = pool()
+            return [p.k, p.ks, p.v, p.vs], lambda s: sdq.kv_write(p, c.batch, x, y, stream=s)
+        if what == "read":
+            o = fresh(x, y)
+            return o, lambda s: sdq.kv_read(c.cache, c.batch, *o, stream=s)
+        if what == "attention":
+            o = fresh(q)
+            return o, lambda s: sdq.kv_attention(few.cache, few.batch, q, o[0], 4, stream=s)
+        if what == "norm":
+            o = fresh(codes, scales, x)
+            return o, lambda s: sdq.rmsnorm_quant(x, *o[:2], delta=y, sum_out=o[2], stream=s)
+        if what == "dequant":
+            o = fresh(x)
+            return o, lambda s: sdq.dequant(codes, scales, o[0], stream=s)
+        o = [torch.zeros((1, 8192), device=sdq_dev)]
+        return o, lambda s: sdq.q4linear(w, one, o[0], stream=s)
+
+    want, call = make()
+    call(None)
+    assert all(t.float().abs().sum() > 0 for t in want)
+    made = [make() for _ in range(24)]
+    torch.cuda.synchronize()
+
+    def run():
+        sdq.init(0)
+        for _ in range(5):
+            for _, call in made:
+                call(2)  # hipStreamPerThread
+
+    t = threading.Thread(target=run)
+    t.start()
+    t.join()
+    for got, _ in made:
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 # ---- a serving step out of all of them ----
 
 def test_serving_step(sdq_dev, oracle):

@@ -3,6 +3,7 @@ ABI's own checks, the binding's checks of tensors, and the layout of the structs
 that cross between them."""
 import ctypes
 import os
+import re
 import shutil
 import subprocess
 
@@ -11,7 +12,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import sdq  # noqa: E402
-from conftest import ROOT  # noqa: E402
+from conftest import PKG, ROOT  # noqa: E402
 
 P = 0x10000  # an address that is never read: the checks come first
 
@@ -190,3 +191,19 @@ def test_binding_tensors():
     _raises("cache.ks: shape", sdq.KvCache, cache.k, f(2, 1, 15), cache.v, cache.vs)
     _raises("cache.v: must be contiguous", sdq.KvCache, cache.k, cache.ks,
             torch.zeros(2, 1, 128, 16, dtype=torch.int8).transpose(2, 3), cache.vs)
+
+
+def test_every_stream_argument_is_known_to_its_thread():
+    """A thread waits as it ends for what it queued on its hipStreamPerThread: each entry point's
+    stream passes stream_of, which notes the thread, or goes to an entry point that does so."""
+    with open(os.path.join(PKG, "csrc", "sdq_api.hip")) as f:
+        text = f.read()
+    with open(os.path.join(ROOT, "include", "sdq.h")) as f:
+        header = f.read()
+    names = [m.group(1) for m in re.finditer(r"^int (sdq_\w+)\(([^;{]*)\);", header, re.M)
+             if re.search(r"void ?\* ?(stream|waiter)", m.group(2))]
+    assert len(names) >= 30 and "sdq_kv_write" in names and "sdq_stream_wait" in names
+    for name in names:
+        body = re.search(r"^int %s\([^{;]*\) \{\n(.*?)^\}" % name, text, re.M | re.S).group(1)
+        assert "stream_of(" in body or re.search(r"\bsdq_\w+\([^;]*\bstream\b", body), name
+    assert text.count("static_cast<hipStream_t>") == 1  # stream_of's own
