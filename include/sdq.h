@@ -454,7 +454,8 @@ int sdq_q4linear(const sdq_weight4* w, const float* A, int64_t M, int64_t K,
  * denoising steps, the frames already made for a chunk of new ones. Device
  * memory of the caller, a pool of pages of page_size tokens:
  *   k, v   [pages, kv_heads, page_size, 128] int8 codes, 16-byte aligned
- *   ks, vs [pages, kv_heads, page_size] f32, the scale of each token and head
+ *   ks, vs [pages, kv_heads, page_size] f32, the scale of each token and head,
+ *          with a float's alignment
  * A value is code * scale; the codes of 128 values are sdq_act_quant's.
  * page_size: a power of two from 16 to 32768; head_dim 128. */
 typedef struct sdq_kv_cache {

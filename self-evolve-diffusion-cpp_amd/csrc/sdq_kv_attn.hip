@@ -47,6 +47,9 @@ using dev::v4f;
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
+// Four scales as they lie in the cache, whose scales need no more than a float's alignment.
+typedef v4f v4f_any __attribute__((aligned(4)));
+
 constexpr int kTop = 15;      // largest q of a row below 2^kTop
 constexpr int kSlack = 6;     // X stays below 2^kSlack
 constexpr int kWeight = 9;    // weights X f enter as X f 2^kWeight, below 2^15
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
   struct Raw {
     uint4 k[2][2];
     uint2 v[2][4];
-    float4 ks[2], vs[2];
+    v4f ks[2], vs[2];
     bool there[2];
   };
   const int32_t* table = c.table + t.s * c.max_pages;
@@ -427,8 +430,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 #pragma unroll
       for (int i = 0; i < 4; i++)
         r.v[kt][i] = *reinterpret_cast<const uint2*>(c.v + (at + 4 * g + i) * kHd + 8 * r16);
-      r.ks[kt] = *reinterpret_cast<const float4*>(c.ks + at + 4 * g);
-      r.vs[kt] = *reinterpret_cast<const float4*>(c.vs + at + 4 * g);
+      r.ks[kt] = *reinterpret_cast<const v4f_any*>(c.ks + at + 4 * g);
+      r.vs[kt] = *reinterpret_cast<const v4f_any*>(c.vs + at + 4 * g);
     }
   };
   Raw cur;
@@ -455,11 +458,9 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
         s[kt] = mma(ka, ql[kb], s[kt]);
         s[kt] = mma(ka, qh[kb], s[kt]);
       }
-      const float ksv[4] = {cur.ks[kt].x, cur.ks[kt].y, cur.ks[kt].z, cur.ks[kt].w};
-      const float vsv[4] = {cur.vs[kt].x, cur.vs[kt].y, cur.vs[kt].z, cur.vs[kt].w};
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const KeyTerms k = key_terms(ksv[i], vsv[i],
+        const KeyTerms k = key_terms(cur.ks[kt][i], cur.vs[kt][i],
                                      cur.there[kt] && b * 32 + 16 * kt + 4 * g + i < t.len, qk, e0);
         kc[kt][i] = k.c, ke[kt][i] = k.e, kw[kt][i] = k.w, kf[kt][i] = k.f;
       }

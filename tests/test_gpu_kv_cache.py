@@ -237,6 +237,28 @@ def test_scale_and_strides(sdq_dev, new):
     assert_bitexact(got[:, 256:768], q, "q")
 
 
+@pytest.mark.parametrize("new", [1, 20, 100])
+def test_scales_at_any_float(sdq_dev, new):
+    """Scales that begin one, two or three floats past a 16-byte boundary: the same bits."""
+    c = Case(sdq_dev, [new, new], [new + 300, new + 77], 2, 32, seed=27)
+    q = c.rng.standard_normal((c.T, 512)).astype(F)
+    first = c.check(4, True, q=q)
+    for off in (1, 2, 3):
+        moved = []
+        for t in (c.cache.ks, c.cache.vs):
+            wide = c.torch.zeros(t.numel() + 4, device=sdq_dev)
+            moved.append(wide[off:off + t.numel()].view(t.shape))
+            moved[-1].copy_(t)
+            assert moved[-1].data_ptr() % 16 == 4 * off
+        c.cache = c.sdq.KvCache(c.cache.k, moved[0], c.cache.v, moved[1])
+        assert_bitexact(c.check(4, True, q=q), first, f"offset {off}")
+        c.sdq.kv_write(c.cache, c.batch, c.t(q[:, :256]), c.t(q[:, 256:]))
+        k, v = (c.torch.zeros((c.T, 256), device=sdq_dev) for _ in range(2))
+        c.sdq.kv_read(c.cache, c.batch, k, v)
+        assert (k - c.t(q[:, :256])).abs().max() < 0.05
+        c.up()
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_sharp_and_far_apart(sdq_dev, new):
     """Logits of hundreds; scales of keys and values far apart, weights the other
