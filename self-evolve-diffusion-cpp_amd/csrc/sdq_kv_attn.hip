@@ -87,9 +87,6 @@ struct Tile {
 
 // A lane's value that is the same in the whole wave, as a scalar.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  return ((int64_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v);
-}
 
 // Tile number `tile`. Sequence s, whose rows start at row a and end before row b of all
 // (row: a token's head of the group), has the numbers from a / RT + s to b / RT + s, at
