@@ -406,8 +406,8 @@ int sdq_qlinear_codes(const sdq_weight* w, const int8_t* aq, const float* as, in
  * For the Linears that read a normalized copy of a residual stream (pre-norm
  * layers with RMS norms: a text encoder's; sdq_qlinear_lnmod is the DiT's
  * layernorm form). x, d and sum have row strides ldx, ldd, ldsum (floats, >= K);
- * sum (nullable) receives h and may be x or d itself; no other output may
- * overlap anything. aq [M,K] and as [M] contiguous; w [K]. A row of NaN or
+ * sum (nullable) receives h and may be x or d itself, or a column block beside
+ * them in one array; no other output may overlap anything. aq [M,K] and as [M] contiguous; w [K]. A row of NaN or
  * infinities follows the same steps (NaN codes are -127). eps >= 0.
  * Stream-ordered, no scratch: it can be captured without a call before. No
  * counterpart in the reference's DiT; its text encoder normalizes this way

@@ -951,6 +951,17 @@ bool bytes_overlap(const void* a, size_t na, const void* b, size_t nb) {
   return a && b && na && nb && x < y + nb && y < x + na;
 }
 
+// Whether two arrays of M rows of C floats, lda and ldb apart, share an element. Column blocks of
+// one array do not, though their spans overlap.
+bool rows_overlap(const float* a, int64_t lda, const float* b, int64_t ldb, int64_t M, int64_t C) {
+  if (!a || !b ||
+      !bytes_overlap(a, (size_t)((M - 1) * lda + C) * 4, b, (size_t)((M - 1) * ldb + C) * 4))
+    return false;
+  if (M == 1 || lda != ldb) return true;
+  const int64_t by = (a < b ? b - a : a - b) % lda;
+  return by < C || by > lda - C;
+}
+
 // One timed launch: a record of its own between sdq_profile_begin / _end.
 template <class F>
 int timed(const char* name, hipStream_t s, F launch) {
@@ -2250,8 +2261,8 @@ int sdq_rmsnorm_quant(const float* x, int64_t ldx, const float* d, int64_t ldd, 
   const size_t nx = span(ldx), nd = d ? span(ldd) : 0, ns = sum ? span(ldsum) : 0;
   const size_t nq = (size_t)M * (size_t)K, na = (size_t)M * 4, nw = (size_t)K * 4;
   const bool bad_sum =
-      sum && ((bytes_overlap(sum, ns, x, nx) && !(sum == x && ldsum == ldx)) ||
-              (bytes_overlap(sum, ns, d, nd) && !(sum == d && ldsum == ldd)) ||
+      sum && ((rows_overlap(sum, ldsum, x, ldx, M, K) && !(sum == x && (ldsum == ldx || M == 1))) ||
+              (rows_overlap(sum, ldsum, d, ldd, M, K) && !(sum == d && (ldsum == ldd || M == 1))) ||
               bytes_overlap(sum, ns, w, nw));
   auto bad_out = [&](const void* p, size_t n) {
     return bytes_overlap(p, n, x, nx) || bytes_overlap(p, n, d, nd) ||
@@ -2422,12 +2433,7 @@ int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t 
   const int64_t C = (int64_t)c->kv_heads * kv::kHd;
   if ((rc = kv_rows("kv_read", "k", k, ldk, C)) || (rc = kv_rows("kv_read", "v", v, ldv, C)))
     return rc;
-  // k and v may be column blocks of one array: rows apart or side by side
-  if (bytes_overlap(k, (size_t)((T - 1) * ldk + C) * 4, v, (size_t)((T - 1) * ldv + C) * 4)) {
-    const int64_t by = k < v ? v - k : k - v;
-    if (ldk != ldv || by % ldk < C || by % ldk > ldk - C)
-      return set_error(SDQ_ERR_INVALID, "kv_read: k and v overlap");
-  }
+  if (rows_overlap(k, ldk, v, ldv, T, C)) return set_error(SDQ_ERR_INVALID, "kv_read: k and v overlap");
   int dev = -1;
   if ((rc = usable_device(&dev))) return rc;
   const hipStream_t s = stream_of(stream);
@@ -2450,11 +2456,8 @@ int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* 
   if ((rc = kv_rows("kv_attention", "q", q, ldq, C)) ||
       (rc = kv_rows("kv_attention", "out", out, ldo, C)))
     return rc;
-  if (bytes_overlap(out, (size_t)((T - 1) * ldo + C) * 4, q, (size_t)((T - 1) * ldq + C) * 4)) {
-    const int64_t by = q < out ? out - q : q - out;
-    if (ldq != ldo || by % ldq < C || by % ldq > ldq - C)
-      return set_error(SDQ_ERR_INVALID, "kv_attention: out overlaps q");
-  }
+  if (rows_overlap(out, ldo, q, ldq, T, C))
+    return set_error(SDQ_ERR_INVALID, "kv_attention: out overlaps q");
   int dev = -1;
   if ((rc = usable_device(&dev))) return rc;
   const hipStream_t s = stream_of(stream);

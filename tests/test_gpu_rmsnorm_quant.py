@@ -99,6 +99,31 @@ def test_strides_aliases_and_alignment(sdq_dev, K, sum_out, pad, offset):
         assert (tx.as_strided((4, pad), (K + pad, 1), tx.storage_offset() + K) == 7).all()
 
 
+@pytest.mark.parametrize("M,K", [(1, 300), (5, 300), (7, 4096), (600, 1024)])
+def test_column_blocks_of_one_array(sdq_dev, M, K):
+    """x, delta and sum side by side in one array, in any order, and what stands beside them."""
+    import torch
+
+    import sdq
+
+    x, d = rows(M, K, 41), rows(M, K, 42)
+    w = np.ones(K, F)
+    h, q, s = oracle_norm(x, d, w, 1e-6)
+    for order in ((0, 1, 2), (2, 1, 0), (1, 2, 0)):
+        wide = torch.full((M, 3 * K + 4), 7.0, device=sdq_dev)
+        tx, td, th = (wide[:, i * K:(i + 1) * K] for i in order)
+        tx.copy_(torch.from_numpy(x)), td.copy_(torch.from_numpy(d))
+        aq = torch.empty((M, K), dtype=torch.int8, device=sdq_dev)
+        asc = torch.empty(M, device=sdq_dev)
+        sdq.rmsnorm_quant(tx, aq, asc, w=torch.from_numpy(w).to(sdq_dev), delta=td, sum_out=th)
+        assert_bitexact(th.cpu().numpy(), h, "sum")
+        assert_bitexact(aq.cpu().numpy(), q, "codes")
+        assert_bitexact(asc.cpu().numpy(), s, "scales")
+        assert_bitexact(tx.cpu().numpy(), x, "x")
+        assert_bitexact(td.cpu().numpy(), d, "delta")
+        assert (wide[:, 3 * K:] == 7).all()
+
+
 @pytest.mark.parametrize("K", [64, 1000, 4096, 17000])
 def test_special_rows(sdq_dev, K):
     """Zero, constant, tiny, huge, infinite and NaN rows; eps 0."""

@@ -207,3 +207,12 @@ def test_every_stream_argument_is_known_to_its_thread():
         body = re.search(r"^int %s\([^{;]*\) \{\n(.*?)^\}" % name, text, re.M | re.S).group(1)
         assert "stream_of(" in body or re.search(r"\bsdq_\w+\([^;]*\bstream\b", body), name
     assert text.count("static_cast<hipStream_t>") == 1  # stream_of's own
+
+
+def test_column_blocks_that_share_a_column():
+    """A sum beside x in one array may not reach into its columns, nor have another stride."""
+    for s in (P + 63 * 4, P + 129 * 4, P + (192 + 63) * 4):
+        _refused("overlaps", "sdq_rmsnorm_quant", *_norm(x=P, ldx=192, s=s, lds=192))
+        _refused("overlaps", "sdq_rmsnorm_quant", *_norm(d=P << 10, ldd=192, s=s - P + (P << 10),
+                                                         lds=192))
+    _refused("overlaps", "sdq_rmsnorm_quant", *_norm(x=P, ldx=192, s=P + 64 * 4, lds=193))
