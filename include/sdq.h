@@ -423,7 +423,8 @@ int sdq_rmsnorm_quant(const float* x, int64_t ldx, const float* d, int64_t ldd, 
  *   Y = epilogue(A . W^T (+ bias))
  * u: 4-bit codes, two to a byte, the even k in the low half; row n starts at byte
  * n * ceil(K/2). group 32, 64 or 128, G = ceil(K / group) groups a row. scale
- * [N,G] f32; zero [N,G] bytes 0..15, or NULL: 8 everywhere. The handle owns a
+ * [N,G] f32, up to 2^100 in magnitude (a group's sum with a larger one may pass fp32's
+ * range before its result does); zero [N,G] bytes 0..15, or NULL: 8 everywhere. The handle owns a
  * copy in the kernels' layout; the sources may be freed after the call.
  * N at most 2^20, K at most 2^22, both at least 1.
  * No counterpart in the reference (its packs hold int8). */

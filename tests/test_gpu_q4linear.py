@@ -182,6 +182,21 @@ def test_rows_near_the_largest_float(sdq_dev, M, group):
             assert not bad.any(), (size, sc, np.argwhere(bad)[:3], got[bad][:3], want[bad][:3])
 
 
+@pytest.mark.parametrize("M", [1, 5, 6, 32])
+@pytest.mark.parametrize("group", [32, 128])
+def test_range_of_weight_scales(sdq_dev, M, group):
+    """Weight scales up to 2^100 of either sign, and as small, with values the other way round."""
+    N, K = 70, 640
+    u, scale, zero = make(N, K, group, True, 33)
+    rng = np.random.default_rng(34)
+    for e in (-120, -60, 60, 99):
+        s = (scale / F(0.02) * F(2.0)**e * rng.choice([-1, 1], scale.shape)).astype(F)
+        x = (rng.standard_normal((M, K)) * 2.0**-e).astype(F)
+        want, tol = expected(x, u, s, zero, group)
+        got = call(sdq_dev, u, s, zero, group, x)
+        assert (np.abs(got - want) <= tol).all(), e
+
+
 def test_in_place_residual_and_two_streams(sdq_dev):
     """resid is Y; two calls of different sizes at once on two streams."""
     import torch
