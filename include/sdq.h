@@ -500,8 +500,11 @@ int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t 
  * over j < lens[s], and j <= p where causal != 0. q and out [T, heads*128] with
  * row strides (16-byte aligned rows), heads a multiple of kv_heads; out must not
  * overlap q (column blocks of one array are fine). Rows that see no key get 0. The
- * cached codes enter exactly, q and the softmax weights as two fp16 parts each (off by
- * less than 2^-21), fp32 sums and statistics: errors of about 1e-6 of the values' scale.
+ * cached codes enter exactly, q and the softmax weights as two rounded fp16 parts each (off
+ * by at most 2^-22, or 2^-39 of the row's largest element, 2^-34 of its largest weight), fp32
+ * sums and statistics: errors of about 1e-6 of the values' scale, and of up to 1.5e-5 where 2^17
+ * keys of the same weight and value round all the same way. A row that holds a NaN or an
+ * infinity is NaN where it sees a key.
  * Scales of values may lie up to 2^60 on either side of the first one of the sequence and
  * head (of 2^-16, where that one is smaller); rows that see a larger one are NaN. Up to 32
  * rows a sequence, and chunks too few for the machine, cut the keys into shares joined

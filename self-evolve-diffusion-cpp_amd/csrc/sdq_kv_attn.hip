@@ -356,10 +356,11 @@ __device__ __forceinline__ void raise(State& st, float mx, v4f acc[8]) {
 //
 // Bound by the cache's bytes, 264 a key and cached head, each read once by the wave
 // that uses it, straight into the MFMA operands' lanes, a block of 32 keys ahead: 1
-// token x 262145 keys, 8 cached heads, 107 us, 5.2 TB/s, the rate of a large copy.
-// 8 tokens of ragged sequences up to 4099 keys, 24 heads: 35 us, 3.3 TB/s; there a wave
-// has eight blocks at most, and finding its tile, the first loads and an uneven
-// last round take what is missing.
+// token x 262145 keys, 8 cached heads, 111 us, 5.0 TB/s, the rate of a large copy.
+// 8 tokens of ragged sequences up to 4099 keys, 24 heads: 34 us, 3.4 TB/s; there a wave
+// has eight blocks at most, and every sequence has the same number of shares: the longest
+// has shares of 1025 keys, where the mean is 652. Two tiles read their keys twice (8
+// sequences of up to 24 rows 45 us).
 
 constexpr int kFewRows = kvplan::kFewRows;
 constexpr int kFewWaves = kvplan::kFewWaves;
@@ -629,11 +630,14 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 // The operands of the next eight MFMAs are read from LDS before the eight at hand are
 // issued, in an order that the compiler is held to (it reads each pair just before its
 // use: 611 -> 576 and 2500 -> 2390 us). A wave's part of a block lies in one page, so its
-// place is scalar arithmetic (a place a thread: 574 and 2363 us, now 548 and 2279).
+// place is scalar arithmetic (a place a thread: 574 and 2363 us, then 548 and 2279 with the
+// join). The flag of far value scales is read where the keys' terms are (at the block's start
+// it waited for LDS: 1% and 1.5%).
 //
-// Bound: 4 MFMA products a score and value (two parts each), busy 47% of the cycles:
-// 91% of the rate of a large library product for the first of these, 93% for the
-// second. What stands beside them does not disappear; at 611 us the first took 135 less
+// Bound: 4 MFMA products a score and value (two parts each), busy 46% of the cycles:
+// 91% of the rate of a large library product for the first of these, 92% for the
+// second. Tiles of 64 rows: 8 sequences of up to 100 tokens over up to 4099 keys, 24 heads,
+// 90 us. What stands beside them does not disappear; at 611 us the first took 135 less
 // without the softmax, 100 without turning keys, 100 without reading operands. Not
 // faster: turns taken phase by phase (a barrier after each phase, the waves of a SIMD
 // one phase apart), which does not fit the registers (1560 us); one sub-block's softmax

@@ -14,7 +14,9 @@
 // row is read once and stays in the registers of its threads (T of them, NV groups of
 // four values each) over the two reductions; rows past the register form are read
 // again. 27280 x 5120: 358 us, 5.07 TB/s, the rate of a large copy (the codes' way
-// back 116 us, 6.0 TB/s); 509 x 4096 10.4 us and one row 4.1 us, which is latency.
+// back 116 us, 6.0 TB/s); 509 x 4096 10.2 us, 2.6 TB/s (a load a thread and array, and the
+// weight's behind the first reduction), and one row 4.1 us, which is latency. Rows past
+// the register form: 1000 x 20000 104 us, 2.5 TB/s of what it has to move.
 #include <algorithm>
 
 #include "sdq_device.h"

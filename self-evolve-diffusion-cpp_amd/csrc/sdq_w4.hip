@@ -187,7 +187,8 @@ __device__ __forceinline__ void put_scales(ScaleLds<GROUP, NB>& o, const Unit (&
 //
 // A workgroup of eight waves makes the bytes of all of A in LDS (its first weight
 // units already on their way), then its waves take every eighth unit of NB blocks
-// of 16 outputs. The tile's spare columns cost nothing.
+// of 16 outputs. The tile's spare columns cost nothing. (1 x 4096 -> 18432 11.3 us, 3.6
+// TB/s: 576 workgroups on 256 CUs, so that some have three and most two.)
 
 // Power of a group whose largest magnitude is mx (finite).
 __device__ __forceinline__ int group_power(float mx) {
