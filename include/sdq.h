@@ -515,6 +515,68 @@ int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* 
                      float* out, int64_t ldo, int64_t T, int heads, float scale, int causal,
                      void* stream);
 
+/* Attention of any rows over cached tokens of another length (an encoder's states: a text
+ * context over all denoising steps, the other branch's tokens): rows [q_start[s],
+ * q_start[s+1]) see all lens[s] tokens of sequence s, however many rows there are;
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / (heads/kv_heads)]) v[j, ...].
+ * Rows of a sequence without tokens get 0. Everything else as sdq_kv_attention.
+ * Cached counterpart of sdq_sdpa_batched, whose sequences have one length
+ * (src/model/ovi_dit.cpp:241, 249). */
+int sdq_kv_cross_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
+                           float* out, int64_t ldo, int64_t T, int heads, float scale,
+                           void* stream);
+/* Beginnings that sequences of a batch share (several continuations of one prompt or clip):
+ * part g holds lens[g] tokens, token p in row p % page_size of page table[g * max_pages +
+ * p / page_size], and is the beginning of sequences s_start[g] .. s_start[g+1] - 1 (s_start
+ * must not fall; sequences before s_start[0] and from s_start[n] on have none). Device
+ * arrays, read when the call runs on the stream; bounds as in sdq_kv_batch. */
+typedef struct sdq_kv_shared {
+  const int32_t* s_start; /* [n + 1] */
+  const int32_t* lens;    /* [n] */
+  const int32_t* table;   /* [n, max_pages] */
+  int n;                  /* 0 .. 65535 */
+  int64_t max_pages;      /* max_pages * page_size at most 2^30 */
+} sdq_kv_shared;
+/* sdq_kv_attention of sequences that begin with a shared part: b's lens and table are a
+ * sequence's own tokens behind it (as sdq_kv_write fills them). A row sees its shared part
+ * whole and of its own tokens what sdq_kv_attention shows it, in one softmax; a row without
+ * a position among its own tokens sees nothing and gets 0. A part's keys are read once for
+ * all of its sequences' rows together. The range of value scales counts from the shared
+ * part's first token (the sequence's own where that part is empty). Scratch from the
+ * stream's workspace in every call, 1040 bytes and up for a row and head (of as many heads
+ * at a time as 512 MiB take): a capture needs one call of the same shape before it. */
+int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, const sdq_kv_batch* b,
+                            const float* q, int64_t ldq, float* out, int64_t ldo, int64_t T,
+                            int heads, float scale, int causal, void* stream);
+/* sdq_kv_attention (the same out) that keeps count of what each cached token was given: for
+ * every token j and cached head of a sequence with rows in this call, with p_ij the softmax
+ * weight of row i and query head h,
+ *   sum = sum over rows i that see j, and query heads h of the cached head, of p_ij
+ *   weights[place of j] = sum                       for the sequence's last tokens, those of
+ *                                                   the call's rows (whose places are new)
+ *   weights[place of j] = weights[place of j] + sum for the tokens before them
+ * weights: device memory of the caller, [pages, kv_heads, page_size] f32 as the cache's
+ * scales, with a float's alignment. fp32 sums in the order of rows; the same bits every time.
+ * Rows that hold a NaN or an infinity add nothing. No two of the call's sequences may have a
+ * page in common (their sums would be lost in part). Scratch from the stream's workspace in
+ * every call. */
+int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights,
+                             const float* q, int64_t ldq, float* out, int64_t ldo, int64_t T,
+                             int heads, float scale, int causal, void* stream);
+/* Thins sequences out to at most `keep` tokens, each cached head its own choice: of the tokens
+ * that have a page, the first `first` and the last `last` positions stay, and of the others
+ * those with the largest weights (of equal ones the lower position; NaN after all numbers)
+ * until there are `keep`. They go, in the order of their positions, to places 0, 1, .. of
+ * other pages (to_table [nseq, to_max_pages], to_max_pages * page_size >= keep), codes,
+ * scales and weights; to_lens [nseq] and kept [nseq, kv_heads, keep] receive how many there
+ * are and their positions (-1 behind the last). Of b, lens and table are read. The pages left
+ * are as they were; what goes to a page id outside the pool is lost. A page of to_table may
+ * be in no sequence's table and in to_table once only. first + last <= keep; no output may
+ * overlap another array (to_lens is not b's lens). Stream-ordered, no scratch. */
+int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, int64_t first,
+                 int64_t last, int64_t keep, const int32_t* to_table, int64_t to_max_pages,
+                 int32_t* to_lens, int32_t* kept, void* stream);
+
 /* ---- device memory, for host code that reaches HIP only through this ABI */
 #define SDQ_H2D 0
 #define SDQ_D2H 1

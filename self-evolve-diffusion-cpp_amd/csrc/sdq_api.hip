@@ -1056,6 +1056,39 @@ int kv_rows(const std::string& tag, const char* name, const float* p, int64_t ld
   return SDQ_OK;
 }
 
+// Scales of a cache's keys (or values).
+size_t kv_scales(const kv::View& v) { return ((size_t)v.pages * v.kv_heads) << v.page_log2; }
+
+// A checked call of one of the paged attentions (view.T == 0: nothing to do).
+struct KvCall {
+  kv::View view;
+  KvRows rows;
+  int dev;
+};
+int kv_call(const sdq_kv_cache* c, const sdq_kv_batch* b, const KvRows& r, int64_t T,
+            const std::string& tag, KvCall* out) {
+  out->rows = r;
+  out->dev = -1;
+  int rc = kv_view(c, b, T, tag, &out->view);
+  if (rc) return rc;
+  if (r.heads < 1 || r.heads > 65535 || r.heads % c->kv_heads)
+    return set_error(SDQ_ERR_INVALID,
+                     tag + ": heads must be a multiple of the cache's kv_heads, at most 65535");
+  if (!(r.scale >= -3.4e38f && r.scale <= 3.4e38f))
+    return set_error(SDQ_ERR_INVALID, tag + ": scale must be finite");
+  if (out->view.T == 0) return SDQ_OK;
+  const int64_t C = (int64_t)r.heads * kv::kHd;
+  if ((rc = kv_rows(tag, "q", r.q, r.ldq, C)) || (rc = kv_rows(tag, "out", r.out, r.ldo, C)))
+    return rc;
+  if (rows_overlap(r.out, r.ldo, r.q, r.ldq, T, C))
+    return set_error(SDQ_ERR_INVALID, tag + ": out overlaps q");
+  return SDQ_OK;
+}
+kvplan::Plan plan_of(const KvCall& k) {
+  return kvplan::plan(k.view.T, k.view.nseq, k.rows.heads / k.view.kv_heads, k.view.kv_heads,
+                      k.view.max_pages << k.view.page_log2, g_dev[k.dev].cu_count);
+}
+
 // Host -> device through the first two slots' pinned buffers, on the first
 // one's stream. A buffer is refilled only
 // after the DMA that read it finished.
@@ -2443,35 +2476,142 @@ int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t 
 int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
                      float* out, int64_t ldo, int64_t T, int heads, float scale, int causal,
                      void* stream) {
-  kv::View view;
-  int rc = kv_view(c, b, T, "kv_attention", &view);
-  if (rc) return rc;
-  if (heads < 1 || heads > 65535 || heads % c->kv_heads)
-    return set_error(SDQ_ERR_INVALID,
-                     "kv_attention: heads must be a multiple of the cache's kv_heads, at most 65535");
-  if (!(scale >= -3.4e38f && scale <= 3.4e38f))
-    return set_error(SDQ_ERR_INVALID, "kv_attention: scale must be finite");
-  if (view.T == 0) return SDQ_OK;
-  const int64_t C = (int64_t)heads * kv::kHd;
-  if ((rc = kv_rows("kv_attention", "q", q, ldq, C)) ||
-      (rc = kv_rows("kv_attention", "out", out, ldo, C)))
-    return rc;
-  if (rows_overlap(out, ldo, q, ldq, T, C))
-    return set_error(SDQ_ERR_INVALID, "kv_attention: out overlaps q");
-  int dev = -1;
-  if ((rc = usable_device(&dev))) return rc;
+  KvCall call;
+  int rc = kv_call(c, b, {q, ldq, out, ldo, heads, scale, causal != 0}, T, "kv_attention", &call);
+  if (rc || call.view.T == 0) return rc;
+  if ((rc = usable_device(&call.dev))) return rc;
   const hipStream_t s = stream_of(stream);
-  const kvplan::Plan plan =
-      kvplan::plan(T, view.nseq, heads / c->kv_heads, c->kv_heads,
-                   view.max_pages << view.page_log2, g_dev[dev].cu_count);
+  const kvplan::Plan plan = plan_of(call);
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
   if (plan.scratch_bytes > 0 &&
-      (rc = shared_scratch(dev, s, (size_t)plan.scratch_bytes, &scratch, &turn)))
+      (rc = shared_scratch(call.dev, s, (size_t)plan.scratch_bytes, &scratch, &turn)))
     return rc;
-  return timed("kv_attention", s, [&] {
-    return launch_kv_attn(view, q, ldq, out, ldo, heads, scale, causal != 0, plan, scratch, s);
+  return timed("kv_attention", s,
+               [&] { return launch_kv_attn(call.view, call.rows, plan, scratch, s); });
+}
+
+int sdq_kv_cross_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
+                           float* out, int64_t ldo, int64_t T, int heads, float scale,
+                           void* stream) {
+  KvCall call;
+  int rc = kv_call(c, b, {q, ldq, out, ldo, heads, scale, 0}, T, "kv_cross_attention", &call);
+  if (rc || call.view.T == 0) return rc;
+  if ((rc = usable_device(&call.dev))) return rc;
+  const hipStream_t s = stream_of(stream);
+  const kvplan::Plan plan = plan_of(call);
+  float* scratch = nullptr;
+  std::unique_lock<std::mutex> turn;
+  if (plan.scratch_bytes > 0 &&
+      (rc = shared_scratch(call.dev, s, (size_t)plan.scratch_bytes, &scratch, &turn)))
+    return rc;
+  return timed("kv_cross_attention", s,
+               [&] { return launch_kv_cross(call.view, call.rows, plan, scratch, s); });
+}
+
+int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, const sdq_kv_batch* b,
+                            const float* q, int64_t ldq, float* out, int64_t ldo, int64_t T,
+                            int heads, float scale, int causal, void* stream) {
+  const std::string tag = "kv_attention_shared";
+  if (!shared) return set_error(SDQ_ERR_INVALID, tag + ": null shared parts");
+  KvCall call;
+  int rc = kv_call(c, b, {q, ldq, out, ldo, heads, scale, causal != 0}, T, tag, &call);
+  if (rc) return rc;
+  if (shared->n < 0 || shared->n > 65535)
+    return set_error(SDQ_ERR_INVALID, tag + ": n must be 0 .. 65535 shared parts");
+  if (shared->max_pages < 0 || shared->max_pages > kMaxRows / c->page_size)
+    return set_error(SDQ_ERR_INVALID, tag + ": the shared max_pages * page_size must be 0 .. 2^30");
+  if (call.view.T == 0) return SDQ_OK;
+  if (shared->n > 0 && (!shared->s_start || !shared->lens || (shared->max_pages > 0 && !shared->table)))
+    return set_error(SDQ_ERR_INVALID, tag + ": null arrays of the shared parts");
+  if (shared->n == 0)
+    return sdq_kv_attention(c, b, q, ldq, out, ldo, T, heads, scale, causal, stream);
+  const kv::Shared parts{shared->s_start, shared->lens, shared->table, shared->n,
+                         c->pages > 0 ? shared->max_pages : 0, call.view.nseq};
+  if ((rc = usable_device(&call.dev))) return rc;
+  const hipStream_t s = stream_of(stream);
+  const kvplan::SharedPlan plan = kvplan::shared_plan(
+      T, call.view.nseq, parts.n, heads / c->kv_heads, c->kv_heads,
+      call.view.max_pages << call.view.page_log2, parts.max_pages << call.view.page_log2,
+      g_dev[call.dev].cu_count);
+  float* scratch = nullptr;
+  std::unique_lock<std::mutex> turn;
+  if ((rc = shared_scratch(call.dev, s, (size_t)plan.scratch_bytes, &scratch, &turn))) return rc;
+  return timed("kv_attention_shared", s, [&] {
+    return launch_kv_shared(call.view, parts, call.rows, plan, scratch, s);
   });
+}
+
+int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights,
+                             const float* q, int64_t ldq, float* out, int64_t ldo, int64_t T,
+                             int heads, float scale, int causal, void* stream) {
+  const std::string tag = "kv_attention_weights";
+  KvCall call;
+  int rc = kv_call(c, b, {q, ldq, out, ldo, heads, scale, causal != 0}, T, tag, &call);
+  if (rc || call.view.T == 0) return rc;
+  if (c->pages > 0 && !weights) return set_error(SDQ_ERR_INVALID, tag + ": null weights");
+  const size_t nw = kv_scales(call.view) * 4;
+  if (bytes_overlap(weights, nw, out, (size_t)((T - 1) * ldo + (int64_t)heads * kv::kHd) * 4) ||
+      bytes_overlap(weights, nw, q, (size_t)((T - 1) * ldq + (int64_t)heads * kv::kHd) * 4) ||
+      bytes_overlap(weights, nw, c->ks, nw))
+    return set_error(SDQ_ERR_INVALID, tag + ": weights overlaps another array");
+  if ((rc = usable_device(&call.dev))) return rc;
+  const hipStream_t s = stream_of(stream);
+  const kvplan::Plan plan = plan_of(call);
+  // the shares' sums, then two numbers a row and head
+  const size_t stats_at = (size_t)round_up(plan.scratch_bytes, 16);
+  float* scratch = nullptr;
+  std::unique_lock<std::mutex> turn;
+  if ((rc = shared_scratch(call.dev, s, stats_at + (size_t)T * heads * sizeof(float2), &scratch,
+                           &turn)))
+    return rc;
+  float2* stats = reinterpret_cast<float2*>(reinterpret_cast<char*>(scratch) + stats_at);
+  rc = timed("kv_attention_weights", s, [&] {
+    return launch_kv_counted(call.view, call.rows, plan, scratch, stats, s);
+  });
+  if (rc) return rc;
+  return timed("kv_weights", s, [&] {
+    return launch_kv_weights(call.view, call.rows, stats, weights, g_dev[call.dev].cu_count, s);
+  });
+}
+
+int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, int64_t first,
+                 int64_t last, int64_t keep, const int32_t* to_table, int64_t to_max_pages,
+                 int32_t* to_lens, int32_t* kept, void* stream) {
+  const std::string tag = "kv_evict";
+  if (!c || !b) return set_error(SDQ_ERR_INVALID, tag + ": null cache or batch");
+  sdq_kv_batch lens = *b;
+  lens.q_start = b->lens;  // not read
+  kv::View view;
+  int rc = kv_view(c, &lens, 1, tag, &view);
+  if (rc) return rc;
+  if (first < 0 || last < 0 || keep < 1 || keep > kMaxRows || first > keep || last > keep - first)
+    return set_error(SDQ_ERR_INVALID,
+                     tag + ": keep must be 1 .. 2^30, first and last not negative and at most keep together");
+  if (to_max_pages < 0 || to_max_pages > kMaxRows / c->page_size ||
+      keep > to_max_pages * c->page_size)
+    return set_error(SDQ_ERR_INVALID,
+                     tag + ": to_max_pages * page_size must be keep .. 2^30");
+  if (b->nseq == 0) return SDQ_OK;
+  if ((int64_t)b->nseq * c->kv_heads * keep > (int64_t(1) << 33))
+    return set_error(SDQ_ERR_INVALID, tag + ": nseq * kv_heads * keep must be at most 2^33");
+  if ((c->pages > 0 && !weights) || !to_table || !to_lens || !kept)
+    return set_error(SDQ_ERR_INVALID, tag + ": null pointer");
+  const size_t nw = kv_scales(view) * 4, nl = (size_t)b->nseq * 4;
+  const size_t nk = (size_t)b->nseq * c->kv_heads * keep * 4;
+  const size_t nt = (size_t)b->nseq * b->max_pages * 4, nto = (size_t)b->nseq * to_max_pages * 4;
+  auto meets = [&](const void* p, size_t n) {  // an output on an input
+    return bytes_overlap(p, n, b->lens, nl) || bytes_overlap(p, n, b->table, nt) ||
+           bytes_overlap(p, n, to_table, nto) || bytes_overlap(p, n, weights, nw);
+  };
+  if (meets(to_lens, nl) || meets(kept, nk) || bytes_overlap(to_lens, nl, kept, nk) ||
+      bytes_overlap(weights, nw, c->ks, nw) || bytes_overlap(weights, nw, c->vs, nw))
+    return set_error(SDQ_ERR_INVALID, tag + ": an output overlaps another array");
+  int dev = -1;
+  if ((rc = usable_device(&dev))) return rc;
+  const hipStream_t s = stream_of(stream);
+  const kv::Kept k{first, last, keep, to_table, to_max_pages, to_lens, kept};
+  return timed("kv_evict", s, [&] { return launch_kv_evict(view, weights, k, s); });
 }
 
 int sdq_device_alloc(size_t bytes, void** out) {

@@ -264,18 +264,41 @@ hipError_t launch_w4(const W4View& w, const float* x, int64_t M, const EpiArgs& 
 // The paged cache (kv::View: sdq_kv.h).
 namespace kv {
 struct View;
+struct Shared;
+struct Kept;
 }
 namespace kvplan {
 struct Plan;
+struct SharedPlan;
 }
 hipError_t launch_kv_write(const kv::View& c, const float* k, int64_t ldk, const float* v,
                            int64_t ldv, hipStream_t s);
 hipError_t launch_kv_read(const kv::View& c, float* k, int64_t ldk, float* v, int64_t ldv,
                           hipStream_t s);
+// Query rows of a paged attention and where its output goes.
+struct KvRows {
+  const float* q;
+  int64_t ldq;
+  float* out;
+  int64_t ldo;
+  int heads;
+  float scale;
+  int causal;
+};
 // plan: kvplan::plan's for this call; scratch: its scratch_bytes.
-hipError_t launch_kv_attn(const kv::View& c, const float* q, int64_t ldq, float* out, int64_t ldo,
-                          int heads, float scale, int causal, const kvplan::Plan& plan,
+hipError_t launch_kv_attn(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
                           void* scratch, hipStream_t s);
+hipError_t launch_kv_cross(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
+                           void* scratch, hipStream_t s);
+hipError_t launch_kv_shared(const kv::View& c, const kv::Shared& pre, const KvRows& r,
+                            const kvplan::SharedPlan& plan, void* scratch, hipStream_t s);
+// launch_kv_attn that keeps each row's maximum and reciprocal denominator, and the sums of
+// the weights by key that go by them: w as the cache's scales.
+hipError_t launch_kv_counted(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
+                             void* scratch, float2* stats, hipStream_t s);
+hipError_t launch_kv_weights(const kv::View& c, const KvRows& r, const float2* stats, float* w,
+                             int cu_count, hipStream_t s);
+hipError_t launch_kv_evict(const kv::View& c, float* w, const kv::Kept& k, hipStream_t s);
 
 // GEMM tile configurations.
 enum GemmCfg : int {

@@ -25,6 +25,30 @@ struct View {
   int64_t T;
 };
 
+// Token runs that several sequences of a batch share (include/sdq.h): part g is the
+// beginning of sequences s_start[g] .. s_start[g + 1] - 1.
+struct Shared {
+  const int32_t* s_start;
+  const int32_t* lens;
+  const int32_t* table;
+  int n;
+  int64_t max_pages;
+  int nseq;  // of the batch
+  __device__ __forceinline__ int seq_of(int g) const {
+    const int s = s_start[g];
+    return s < 0 ? 0 : s > nseq ? nseq : s;
+  }
+};
+
+// Where an eviction's kept tokens go (include/sdq.h).
+struct Kept {
+  int64_t first, last, keep;
+  const int32_t* table;
+  int64_t max_pages;
+  int32_t* lens;
+  int32_t* kept;
+};
+
 // Row range of sequence s inside the call's T rows, and its length inside the
 // table, whatever the arrays hold.
 __device__ __forceinline__ int64_t row_of(const View& c, int s) {

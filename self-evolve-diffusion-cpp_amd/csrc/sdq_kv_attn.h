@@ -1,0 +1,393 @@
+// Device code that the paged attention's kernels share: tiles of query rows, the two
+// fp16 parts of an fp32 number, keys' terms and one query's softmax state. The numbers
+// that stand here are derived at the head of sdq_kv_attn.hip.
+#pragma once
+
+#include "sdq_device.h"
+#include "sdq_kv.h"
+
+#pragma clang fp contract(off)
+
+namespace sdq {
+namespace kvattn {
+
+using kv::kHd;
+using kv::View;
+using dev::v4f;
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// Four scales as they lie in the cache, whose scales need no more than a float's alignment.
+typedef v4f v4f_any __attribute__((aligned(4)));
+
+constexpr int kTop = 15;      // largest q of a row below 2^kTop
+constexpr int kSlack = 6;     // X stays below 2^kSlack
+constexpr int kWeight = 9;    // weights X f enter as X f 2^kWeight, below 2^15
+constexpr int kFar = 60;      // e_j is held to -kFar .. kFar
+constexpr int kLeast = -16;   // of E0
+// A key with e >= kNear whose X is under 2^-126 is less than 2^(-126 - kNear) of a
+// denominator that holds at least 2^-kFar: 2^30 of them less than 2^-26 of it.
+constexpr float kNear = -10.f;
+
+// What the rows of a launch see, and where their sums go.
+struct Own {  // a sequence's last tokens, its own keys
+  static constexpr bool kFree = false, kGroups = false, kByRow = false, kStats = false;
+};
+struct Cross : Own {  // any rows, all keys of their sequence
+  static constexpr bool kFree = true;
+};
+struct Counted : Own {  // each row's maximum and denominator are kept
+  static constexpr bool kStats = true;
+};
+struct Prefix : Cross {  // the rows of a run of sequences, the keys that those share
+  static constexpr bool kGroups = true, kByRow = true;
+};
+struct Rest : Own {  // own keys behind shared ones
+  static constexpr bool kByRow = true;
+};
+
+struct Args {
+  View c;
+  const float* q;
+  int64_t ldq;
+  float* out;
+  int64_t ldo;
+  int heads, group;  // query heads, query heads per cached head
+  float scale2;      // scale * log2(e)
+  int causal;
+  int splits;
+  int64_t tile0;     // first tile of this launch
+  float* part;       // [tile][kv head][split][row][128], unscaled sums
+  float2* part_ml;   // the same without dims: maximum, denominator
+  // kStats: [row][head] maximum and reciprocal denominator (infinity and 0: adds nothing)
+  float2* stats;
+  // kByRow: cached heads h0 .. h0 + nh - 1 of this launch, shares z0 .. of `shares`; the
+  // sums are [row][head of those][share][128]
+  int h0, nh, z0, shares;
+  kv::Shared pre;  // Prefix: c has its lens, table, max_pages and number of parts
+};
+
+// A tile of rows: rows [r0, r0 + RT) of sequence s, row r = token r / group,
+// query head r % group of the tile's cached head.
+struct Tile {
+  int s;          // -1: none
+  int64_t r0;
+  int64_t rows;   // of the sequence
+  int64_t row0;   // the sequence's first row in q
+  int len;        // keys, at most 2^30
+  int first;      // position of the sequence's first row
+};
+
+// A lane's value that is the same in the whole wave, as a scalar.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The last of indexes 0 .. n - 1 whose f, which does not fall, is at most v; -1: none. By a
+// search 64 ways at a time; f(n) may be asked for. The same in every wave.
+template <class F>
+__device__ __forceinline__ int last_upto(int most, F f, int64_t v) {
+  const int l = threadIdx.x & 63;
+  int lo = 0, n = most, step;
+  do {
+    step = (n + 63) / 64;
+    const uint64_t upto = __ballot((int64_t)l * step < n && f(min(lo + l * step, most)) <= v);
+    if (!upto) return -1;
+    const int k = 63 - __builtin_clzll(upto);
+    lo += k * step;
+    n = min(step, n - k * step);
+  } while (step > 1);
+  return uniform(lo);
+}
+
+// Tile number `tile`. Sequence s, whose rows start at row a and end before row b of all
+// (row: a token's head of the group), has the numbers from a / RT + s to b / RT + s, at
+// least as many as it has tiles of RT rows: a number without a tile is none. So the
+// sequence is found by search, with no sum over those before it
+// (a scan over them took a fifth of a microsecond for each 64). The same in every wave.
+template <class K, int RT>
+__device__ __forceinline__ Tile find_tile(const Args& a, int64_t tile) {
+  const View& c = a.c;
+  const int group = a.group;
+  Tile t{-1, 0, 0, 0, 0, 0};
+  auto row_of = [&](int s) { return kv::row_of(c, K::kGroups ? a.pre.seq_of(s) : s); };
+  auto first = [&](int s) { return row_of(s) * group / RT + s; };
+  const int lo = last_upto(c.nseq, first, tile);
+  if (lo < 0) return t;
+  t.row0 = row_of(lo);
+  const int64_t tokens = row_of(lo + 1) - t.row0;
+  t.r0 = (tile - first(lo)) * RT;
+  t.rows = tokens > 0 ? tokens * group : 0;
+  t.len = (int)kv::length_of(c, lo);
+  t.first = K::kFree ? 0 : t.len - (int)(tokens > 0 ? tokens : 0);
+  if (t.r0 < t.rows) t.s = lo;
+  return t;
+}
+
+// The sequence of row t, -1: none.
+__device__ __forceinline__ int seq_at(const View& c, int64_t t) {
+  const int s = last_upto(c.nseq, [&](int i) { return kv::row_of(c, i); }, t);
+  return s >= 0 && t < kv::row_of(c, s + 1) ? s : -1;
+}
+
+// Keys that row r sees (0: it has no position, or is none).
+__device__ __forceinline__ int keys_of(const Tile& t, int64_t r, int group, int causal) {
+  if (r >= t.rows) return 0;
+  const int p = t.first + (int)(r / group);
+  return p < 0 ? 0 : causal ? (p + 1 < t.len ? p + 1 : t.len) : t.len;
+}
+// And the rows [r, r + n) at most: the last one.
+__device__ __forceinline__ int keys_of_rows(const Tile& t, int64_t r, int n, int group,
+                                            int causal) {
+  return keys_of(t, (r + n < t.rows ? r + n : t.rows) - 1, group, causal);
+}
+
+__device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Eight codes (two dwords) as fp16: 0x6400 | u is 1024 + u, with u = code + 128.
+__device__ __forceinline__ v2h less1152(uint32_t x) {
+  return __builtin_bit_cast(v2h, x) + v2h{(_Float16)-1152.f, (_Float16)-1152.f};
+}
+__device__ __forceinline__ v8h codes8(uint32_t a, uint32_t b) {
+  a ^= 0x80808080u;
+  b ^= 0x80808080u;
+  const v2h x = less1152(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u));
+  const v2h y = less1152(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u));
+  const v2h z = less1152(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u));
+  const v2h w = less1152(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u));
+  return v8h{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
+}
+// Byte I of two dwords (codes xor 0x80) as a pair of fp16.
+template <int I>
+__device__ __forceinline__ v2h pair_of(uint32_t a, uint32_t b) {
+  constexpr uint32_t sel = 0x0c000c00u | (uint32_t)I | ((uint32_t)(I + 4) << 16);
+  return less1152(__builtin_amdgcn_perm(b, a, sel) | 0x64006400u);
+}
+
+// Over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a query, by swaps of lane rows.
+template <class F>
+__device__ __forceinline__ float quad(float v, F f) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float quad_max(float v) {
+  return quad(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  return quad(v, [](float a, float b) { return a + b; });
+}
+
+// x - hi of either half of a pair of fp16, exact, in one operation.
+__device__ __forceinline__ float less_low(v2h hi, float x) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(hi), "v"(x));
+  return r;
+}
+__device__ __forceinline__ float less_high(v2h hi, float x) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+      : "=v"(r)
+      : "v"(hi), "v"(x));
+  return r;
+}
+// fp32 to two fp16 parts, both rounded (two conversions at a time): the high
+// part's remainder is exact, so the pair is off by at most 2^-22.
+__device__ __forceinline__ v2h rounded(float a, float b) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  return __builtin_convertvector((v2f{a, b}), v2h);
+}
+__device__ __forceinline__ void parts8(const float x[8], v8h& hi, v8h& lo) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const v2h h = rounded(x[i], x[i + 1]);
+    const v2h r = rounded(less_low(h, x[i]), less_high(h, x[i + 1]));
+    hi[i] = h[0];
+    hi[i + 1] = h[1];
+    lo[i] = r[0];
+    lo[i + 1] = r[1];
+  }
+}
+
+// The lane's slice of a query row (head of a token), zeros where it is none.
+__device__ __forceinline__ void load_q(const Args& a, const Tile& t, int h, int64_t r, int g,
+                                       float x[4][8]) {
+  const bool ok = r < t.rows;
+  const int64_t rr = ok ? r : 0;
+  const int64_t tok = rr / a.group;
+  const float* p =
+      a.q + (t.row0 + tok) * a.ldq + (int64_t)(h * a.group + (int)(rr - tok * a.group)) * kHd;
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const float4 v =
+          ok ? *reinterpret_cast<const float4*>(p + 64 * (kb >> 1) + 16 * g + 8 * (kb & 1) + 4 * j)
+             : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[kb][4 * j] = v.x;
+      x[kb][4 * j + 1] = v.y;
+      x[kb][4 * j + 2] = v.z;
+      x[kb][4 * j + 3] = v.w;
+    }
+}
+// The largest magnitude of a row's slice. NaN and infinities become zeros, and the row (of
+// four lanes) is `bad`: its denominator is NaN once it has seen a key, and 0 before.
+__device__ __forceinline__ float clean(float x[4][8], bool& bad) {
+  float m = 0.f, b = 0.f;
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const bool fine = fabsf(x[kb][i]) <= 3.402823466e38f;
+      x[kb][i] = fine ? x[kb][i] : 0.f;
+      b = fine ? b : 1.f;
+      m = fmaxf(m, fabsf(x[kb][i]));
+    }
+  bad = quad_max(b) != 0.f;
+  return quad_max(m);
+}
+__device__ __forceinline__ float den_of(float l, bool bad) {
+  const float den = quad_sum(l);
+  return bad && den != 0.f ? __builtin_nanf("") : den;
+}
+// Exponent that scales a row's largest |q| below 2^kTop; within what a float's power
+// of two can hold. Each row has its own: one of the same tile that holds something
+// huge takes no bits from it.
+__device__ __forceinline__ int q_exp(float m) {
+  const int e = m > 0.f ? kTop - __builtin_amdgcn_frexp_expf(m) : 0;
+  return e > 100 ? 100 : e;
+}
+
+// What a key contributes: c (score to log2 units), e, 2^-e and f 2^kWeight. One
+// that is not there (masked, no page) gives zeros, so that whatever its memory
+// holds stays out.
+struct KeyTerms {
+  float c, e, w, f;
+};
+__device__ __forceinline__ KeyTerms key_terms(float ks, float vs, bool ok, float qk, int e0) {
+  const float top = __builtin_ldexpf(1.f, kFar + e0);  // inf: every finite scale fits
+  KeyTerms k;
+  int e = vs != 0.f ? __builtin_amdgcn_frexp_expf(vs) - e0 : 0;
+  e = e < -kFar ? -kFar : e > kFar ? kFar : e;
+  k.c = ok ? ks * qk : 0.f;
+  k.e = ok ? (float)e : 0.f;
+  k.w = ok ? __builtin_ldexpf(1.f, -e) : 0.f;
+  // past kFar the weights would not fit fp16, and the conversion would cut them off
+  k.f = !ok ? 0.f : fabsf(vs) >= top ? __builtin_nanf("") : __builtin_ldexpf(vs, kWeight - e - e0);
+  return k;
+}
+// E0: the exponent of the sequence's first value scale; from kLeast on, so that a
+// first value of next to nothing leaves those after it their range. pages: the
+// sequence's.
+__device__ __forceinline__ int first_exp(const View& c, const int32_t* pages, int64_t len, int h) {
+  if (len <= 0) return 0;
+  const int64_t page = pages[0];
+  const float v =
+      page >= 0 && page < c.pages ? c.vs[(page * c.kv_heads + h) << c.page_log2] : 0.f;
+  const int e = v != 0.f ? __builtin_amdgcn_frexp_expf(v) : 0;
+  return e < kLeast ? kLeast : e;
+}
+__device__ __forceinline__ int first_exp(const View& c, const Tile& t, int h) {
+  return first_exp(c, c.table + t.s * c.max_pages, t.len, h);
+}
+
+// The shared part that sequence s begins with, -1: none.
+__device__ __forceinline__ int part_of(const kv::Shared& p, int s) {
+  const int g = last_upto(p.n, [&](int i) { return (int64_t)p.seq_of(i); }, s);
+  return g >= 0 && s < p.seq_of(g + 1) ? g : -1;
+}
+__device__ __forceinline__ int64_t length_of(const View& c, const kv::Shared& p, int g) {
+  const int64_t n = p.lens[g], most = p.max_pages << c.page_log2;
+  return n < 0 ? 0 : n > most ? most : n;
+}
+// E0 of sequence s behind its part g of the shared ones: the first value of all, so that
+// both passes' sums have the same units.
+__device__ __forceinline__ int first_exp(const Args& a, int s, int g, int h) {
+  const int64_t n = g >= 0 ? length_of(a.c, a.pre, g) : 0;
+  return n > 0 ? first_exp(a.c, a.pre.table + g * a.pre.max_pages, n, h)
+               : first_exp(a.c, a.c.table + s * a.c.max_pages, kv::length_of(a.c, s), h);
+}
+
+// One query's softmax state in a lane: the reference m (the maximum of t, or up
+// to kSlack below it; -inf: no key yet) is the same in the query's four lanes,
+// the denominator is the lane's own share.
+struct State {
+  float m, l;
+};
+
+// A 32-key block's logits of one query tile, in place of its scores (tiles kt,
+// elements i: key 16 kt + 4 g + i), and their largest. seen(kt, i): the row sees
+// that key.
+template <bool MASK, class Seen>
+__device__ __forceinline__ float logits(v4f s[2], const v4f c[2], const v4f e[2], Seen seen) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float v = __builtin_fmaf(s[kt][i], c[kt][i], e[kt][i]);
+      if (MASK && !seen(kt, i)) v = -INFINITY;
+      s[kt][i] = v;
+      mx = fmaxf(mx, v);
+    }
+  return quad_max(mx);
+}
+// Logits to the two parts of the weights.
+template <bool MASK, class Seen>
+__device__ __forceinline__ void weights(const v4f t[2], const v4f w[2], const v4f f[2], State& st,
+                                        Seen seen, v8h& hi, v8h& lo) {
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+  float p[8], l = 0.f;  // the block's share first: an eighth of the roundings of a long sum
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float x = __builtin_amdgcn_exp2f(t[j >> 2][j & 3] - ref);
+    l = __builtin_fmaf(x, w[j >> 2][j & 3], l);
+    p[j] = x * f[j >> 2][j & 3];
+    if (MASK && !seen(j >> 2, j & 3)) p[j] = 0.f;  // its scale may be NaN
+  }
+  st.l += l;
+  parts8(p, hi, lo);
+}
+// a 2^d, also where 2^d alone is under the smallest float (exp2 gives 0 there).
+__device__ __forceinline__ float times_exp2(float a, float d) {
+  const float h = __builtin_amdgcn_exp2f(0.5f * d);
+  return a * h * h;
+}
+// The denominator's terms 2^(t - m - e) of keys whose X is under the smallest float (what
+// is 2^-1000 is nothing, masked keys among it); their X is 0 from here on. Called
+// where a block has a key with e < kNear.
+__device__ __forceinline__ void add_faint(v4f t[2], const v4f e[2], State& st) {
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+  float l = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float x = t[j >> 2][j & 3] - ref;
+    const bool faint = x < -126.f && x > -1000.f;
+    l += __builtin_amdgcn_exp2f(faint ? x - e[j >> 2][j & 3] : -INFINITY);
+    t[j >> 2][j & 3] = faint ? -INFINITY : t[j >> 2][j & 3];
+  }
+  st.l += l;
+}
+// The reference rises only when a block's largest logit passes it by more than
+// kSlack (the weights then stay below 2^kSlack, inside fp16 with kWeight):
+// rarely. The branch is the wave's, the rise each row's own, so that no row's bits
+// depend on its neighbours.
+__device__ __forceinline__ bool rises(const State& st, float mx) { return mx > st.m + kSlack; }
+__device__ __forceinline__ void raise(State& st, float mx, v4f acc[8]) {
+  const float m = rises(st, mx) ? mx : st.m;
+  const float d = m == -INFINITY ? 0.f : st.m - m;
+  const float shrink = __builtin_amdgcn_exp2f(d);
+  st.m = m;
+  st.l = times_exp2(st.l, d);
+#pragma unroll
+  for (int e = 0; e < 8; e++) acc[e] = acc[e] * shrink;
+}
+
+// A row's entry of Args::stats.
+__device__ __forceinline__ float2 stat_of(float m, float den) {
+  return den > 0.f ? float2{m, 1.f / den} : float2{INFINITY, 0.f};
+}
+
+}  // namespace kvattn
+}  // namespace sdq

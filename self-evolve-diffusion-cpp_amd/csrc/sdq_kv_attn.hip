@@ -32,8 +32,7 @@
 // bytes), so that lane group g ends with dims 32 g .. 32 g + 31 of its query.
 #include <algorithm>
 
-#include "sdq_device.h"
-#include "sdq_kv.h"
+#include "sdq_kv_attn.h"
 #include "sdq_kv_plan.h"
 
 #pragma clang fp contract(off)
@@ -41,315 +40,24 @@
 namespace sdq {
 namespace {
 
-using kv::kHd;
-using kv::View;
-using dev::v4f;
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+using namespace kvattn;
 
-// Four scales as they lie in the cache, whose scales need no more than a float's alignment.
-typedef v4f v4f_any __attribute__((aligned(4)));
-
-constexpr int kTop = 15;      // largest q of a row below 2^kTop
-constexpr int kSlack = 6;     // X stays below 2^kSlack
-constexpr int kWeight = 9;    // weights X f enter as X f 2^kWeight, below 2^15
-constexpr int kFar = 60;      // e_j is held to -kFar .. kFar
-constexpr int kLeast = -16;   // of E0
-// A key with e >= kNear whose X is under 2^-126 is less than 2^(-126 - kNear) of a
-// denominator that holds at least 2^-kFar: 2^30 of them less than 2^-26 of it.
-constexpr float kNear = -10.f;
-
-struct Args {
-  View c;
-  const float* q;
-  int64_t ldq;
-  float* out;
-  int64_t ldo;
-  int heads, group;  // query heads, query heads per cached head
-  float scale2;      // scale * log2(e)
-  int causal;
-  int splits;
-  int64_t tile0;     // first tile of this launch
-  float* part;       // [tile][kv head][split][row][128], unscaled sums
-  float2* part_ml;   // the same without dims: maximum, denominator
-};
-
-// A tile of rows: rows [r0, r0 + RT) of sequence s, row r = token r / group,
-// query head r % group of the tile's cached head.
-struct Tile {
-  int s;          // -1: none
-  int64_t r0;
-  int64_t rows;   // of the sequence
-  int64_t row0;   // the sequence's first row in q
-  int len;        // keys, at most 2^30
-  int first;      // position of the sequence's first row
-};
-
-// A lane's value that is the same in the whole wave, as a scalar.
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// Tile number `tile`. Sequence s, whose rows start at row a and end before row b of all
-// (row: a token's head of the group), has the numbers from a / RT + s to b / RT + s, at
-// least as many as it has tiles of RT rows: a number without a tile is none. So the
-// sequence is found by search, 64 ways at a time, with no sum over those before it
-// (a scan over them took a fifth of a microsecond for each 64). The same in every wave.
-template <int RT>
-__device__ __forceinline__ Tile find_tile(const View& c, int group, int64_t tile) {
-  const int l = threadIdx.x & 63;
-  Tile t{-1, 0, 0, 0, 0, 0};
-  auto first = [&](int s) { return kv::row_of(c, s) * group / RT + s; };
-  int lo = 0, n = c.nseq, step;
-  do {
-    step = (n + 63) / 64;
-    const uint64_t upto = __ballot((int64_t)l * step < n && first(min(lo + l * step, c.nseq)) <= tile);
-    if (!upto) return t;
-    const int k = 63 - __builtin_clzll(upto);
-    lo += k * step;
-    n = min(step, n - k * step);
-  } while (step > 1);
-  lo = uniform(lo);
-  t.row0 = kv::row_of(c, lo);
-  const int64_t tokens = kv::row_of(c, lo + 1) - t.row0;
-  t.r0 = (tile - first(lo)) * RT;
-  t.rows = tokens > 0 ? tokens * group : 0;
-  t.len = (int)kv::length_of(c, lo);
-  t.first = t.len - (int)(tokens > 0 ? tokens : 0);
-  if (t.r0 < t.rows) t.s = lo;
-  return t;
+template <class K>
+__device__ __forceinline__ int e0_of(const Args& a, const Tile& t, int h) {
+  if constexpr (std::is_same<K, Rest>::value)
+    return first_exp(a, t.s, part_of(a.pre, t.s), h);
+  else
+    return first_exp(a.c, t, h);
 }
 
-// Keys that row r sees (0: it has no position, or is none).
-__device__ __forceinline__ int keys_of(const Tile& t, int64_t r, int group, int causal) {
-  if (r >= t.rows) return 0;
-  const int p = t.first + (int)(r / group);
-  return p < 0 ? 0 : causal ? (p + 1 < t.len ? p + 1 : t.len) : t.len;
-}
-// And the rows [r, r + n) at most: the last one.
-__device__ __forceinline__ int keys_of_rows(const Tile& t, int64_t r, int n, int group,
-                                            int causal) {
-  return keys_of(t, (r + n < t.rows ? r + n : t.rows) - 1, group, causal);
-}
-
-__device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// Eight codes (two dwords) as fp16: 0x6400 | u is 1024 + u, with u = code + 128.
-__device__ __forceinline__ v2h less1152(uint32_t x) {
-  return __builtin_bit_cast(v2h, x) + v2h{(_Float16)-1152.f, (_Float16)-1152.f};
-}
-__device__ __forceinline__ v8h codes8(uint32_t a, uint32_t b) {
-  a ^= 0x80808080u;
-  b ^= 0x80808080u;
-  const v2h x = less1152(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u));
-  const v2h y = less1152(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u));
-  const v2h z = less1152(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u));
-  const v2h w = less1152(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u));
-  return v8h{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
-}
-// Byte I of two dwords (codes xor 0x80) as a pair of fp16.
-template <int I>
-__device__ __forceinline__ v2h pair_of(uint32_t a, uint32_t b) {
-  constexpr uint32_t sel = 0x0c000c00u | (uint32_t)I | ((uint32_t)(I + 4) << 16);
-  return less1152(__builtin_amdgcn_perm(b, a, sel) | 0x64006400u);
-}
-
-// Over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a query, by swaps of lane rows.
-template <class F>
-__device__ __forceinline__ float quad(float v, F f) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float quad_max(float v) {
-  return quad(v, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float quad_sum(float v) {
-  return quad(v, [](float a, float b) { return a + b; });
-}
-
-// x - hi of either half of a pair of fp16, exact, in one operation.
-__device__ __forceinline__ float less_low(v2h hi, float x) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(hi), "v"(x));
-  return r;
-}
-__device__ __forceinline__ float less_high(v2h hi, float x) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-      : "=v"(r)
-      : "v"(hi), "v"(x));
-  return r;
-}
-// fp32 to two fp16 parts, both rounded (two conversions at a time): the high
-// part's remainder is exact, so the pair is off by at most 2^-22.
-__device__ __forceinline__ v2h rounded(float a, float b) {
-  typedef float v2f __attribute__((ext_vector_type(2)));
-  return __builtin_convertvector((v2f{a, b}), v2h);
-}
-__device__ __forceinline__ void parts8(const float x[8], v8h& hi, v8h& lo) {
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const v2h h = rounded(x[i], x[i + 1]);
-    const v2h r = rounded(less_low(h, x[i]), less_high(h, x[i + 1]));
-    hi[i] = h[0];
-    hi[i + 1] = h[1];
-    lo[i] = r[0];
-    lo[i + 1] = r[1];
-  }
-}
-
-// The lane's slice of a query row (head of a token), zeros where it is none.
-__device__ __forceinline__ void load_q(const Args& a, const Tile& t, int h, int64_t r, int g,
-                                       float x[4][8]) {
-  const bool ok = r < t.rows;
-  const int64_t rr = ok ? r : 0;
-  const int64_t tok = rr / a.group;
-  const float* p =
-      a.q + (t.row0 + tok) * a.ldq + (int64_t)(h * a.group + (int)(rr - tok * a.group)) * kHd;
-#pragma unroll
-  for (int kb = 0; kb < 4; kb++)
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const float4 v =
-          ok ? *reinterpret_cast<const float4*>(p + 64 * (kb >> 1) + 16 * g + 8 * (kb & 1) + 4 * j)
-             : make_float4(0.f, 0.f, 0.f, 0.f);
-      x[kb][4 * j] = v.x;
-      x[kb][4 * j + 1] = v.y;
-      x[kb][4 * j + 2] = v.z;
-      x[kb][4 * j + 3] = v.w;
-    }
-}
-// The largest magnitude of a row's slice. NaN and infinities become zeros, and the row (of
-// four lanes) is `bad`: its denominator is NaN once it has seen a key, and 0 before.
-__device__ __forceinline__ float clean(float x[4][8], bool& bad) {
-  float m = 0.f, b = 0.f;
-#pragma unroll
-  for (int kb = 0; kb < 4; kb++)
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const bool fine = fabsf(x[kb][i]) <= 3.402823466e38f;
-      x[kb][i] = fine ? x[kb][i] : 0.f;
-      b = fine ? b : 1.f;
-      m = fmaxf(m, fabsf(x[kb][i]));
-    }
-  bad = quad_max(b) != 0.f;
-  return quad_max(m);
-}
-__device__ __forceinline__ float den_of(float l, bool bad) {
-  const float den = quad_sum(l);
-  return bad && den != 0.f ? __builtin_nanf("") : den;
-}
-// Exponent that scales a row's largest |q| below 2^kTop; within what a float's power
-// of two can hold. Each row has its own: one of the same tile that holds something
-// huge takes no bits from it.
-__device__ __forceinline__ int q_exp(float m) {
-  const int e = m > 0.f ? kTop - __builtin_amdgcn_frexp_expf(m) : 0;
-  return e > 100 ? 100 : e;
-}
-
-// What a key contributes: c (score to log2 units), e, 2^-e and f 2^kWeight. One
-// that is not there (masked, no page) gives zeros, so that whatever its memory
-// holds stays out.
-struct KeyTerms {
-  float c, e, w, f;
-};
-__device__ __forceinline__ KeyTerms key_terms(float ks, float vs, bool ok, float qk, int e0) {
-  const float top = __builtin_ldexpf(1.f, kFar + e0);  // inf: every finite scale fits
-  KeyTerms k;
-  int e = vs != 0.f ? __builtin_amdgcn_frexp_expf(vs) - e0 : 0;
-  e = e < -kFar ? -kFar : e > kFar ? kFar : e;
-  k.c = ok ? ks * qk : 0.f;
-  k.e = ok ? (float)e : 0.f;
-  k.w = ok ? __builtin_ldexpf(1.f, -e) : 0.f;
-  // past kFar the weights would not fit fp16, and the conversion would cut them off
-  k.f = !ok ? 0.f : fabsf(vs) >= top ? __builtin_nanf("") : __builtin_ldexpf(vs, kWeight - e - e0);
-  return k;
-}
-// E0: the exponent of the sequence's first value scale; from kLeast on, so that a
-// first value of next to nothing leaves those after it their range.
-__device__ __forceinline__ int first_exp(const View& c, const Tile& t, int h) {
-  if (t.len <= 0) return 0;
-  const int64_t at = kv::place_of(c, t.s, 0, h);
-  const float v = at >= 0 ? c.vs[at] : 0.f;
-  const int e = v != 0.f ? __builtin_amdgcn_frexp_expf(v) : 0;
-  return e < kLeast ? kLeast : e;
-}
-
-// One query's softmax state in a lane: the reference m (the maximum of t, or up
-// to kSlack below it; -inf: no key yet) is the same in the query's four lanes,
-// the denominator is the lane's own share.
-struct State {
-  float m, l;
-};
-
-// A 32-key block's logits of one query tile, in place of its scores (tiles kt,
-// elements i: key 16 kt + 4 g + i), and their largest. seen(kt, i): the row sees
-// that key.
-template <bool MASK, class Seen>
-__device__ __forceinline__ float logits(v4f s[2], const v4f c[2], const v4f e[2], Seen seen) {
-  float mx = -INFINITY;
-#pragma unroll
-  for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float v = __builtin_fmaf(s[kt][i], c[kt][i], e[kt][i]);
-      if (MASK && !seen(kt, i)) v = -INFINITY;
-      s[kt][i] = v;
-      mx = fmaxf(mx, v);
-    }
-  return quad_max(mx);
-}
-// Logits to the two parts of the weights.
-template <bool MASK, class Seen>
-__device__ __forceinline__ void weights(const v4f t[2], const v4f w[2], const v4f f[2], State& st,
-                                        Seen seen, v8h& hi, v8h& lo) {
-  const float ref = st.m == -INFINITY ? 0.f : st.m;
-  float p[8], l = 0.f;  // the block's share first: an eighth of the roundings of a long sum
-#pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const float x = __builtin_amdgcn_exp2f(t[j >> 2][j & 3] - ref);
-    l = __builtin_fmaf(x, w[j >> 2][j & 3], l);
-    p[j] = x * f[j >> 2][j & 3];
-    if (MASK && !seen(j >> 2, j & 3)) p[j] = 0.f;  // its scale may be NaN
-  }
-  st.l += l;
-  parts8(p, hi, lo);
-}
-// a 2^d, also where 2^d alone is under the smallest float (exp2 gives 0 there).
-__device__ __forceinline__ float times_exp2(float a, float d) {
-  const float h = __builtin_amdgcn_exp2f(0.5f * d);
-  return a * h * h;
-}
-// The denominator's terms 2^(t - m - e) of keys whose X is under the smallest float (what
-// is 2^-1000 is nothing, masked keys among it); their X is 0 from here on. Called
-// where a block has a key with e < kNear.
-__device__ __forceinline__ void add_faint(v4f t[2], const v4f e[2], State& st) {
-  const float ref = st.m == -INFINITY ? 0.f : st.m;
-  float l = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const float x = t[j >> 2][j & 3] - ref;
-    const bool faint = x < -126.f && x > -1000.f;
-    l += __builtin_amdgcn_exp2f(faint ? x - e[j >> 2][j & 3] : -INFINITY);
-    t[j >> 2][j & 3] = faint ? -INFINITY : t[j >> 2][j & 3];
-  }
-  st.l += l;
-}
-// The reference rises only when a block's largest logit passes it by more than
-// kSlack (the weights then stay below 2^kSlack, inside fp16 with kWeight):
-// rarely. The branch is the wave's, the rise each row's own, so that no row's bits
-// depend on its neighbours.
-__device__ __forceinline__ bool rises(const State& st, float mx) { return mx > st.m + kSlack; }
-__device__ __forceinline__ void raise(State& st, float mx, v4f acc[8]) {
-  const float m = rises(st, mx) ? mx : st.m;
-  const float d = m == -INFINITY ? 0.f : st.m - m;
-  const float shrink = __builtin_amdgcn_exp2f(d);
-  st.m = m;
-  st.l = times_exp2(st.l, d);
-#pragma unroll
-  for (int e = 0; e < 8; e++) acc[e] = acc[e] * shrink;
+// Where a share of a tile's row keeps its sums (th: the workgroup's tile and head).
+template <class K>
+__device__ __forceinline__ int64_t share_at(const Args& a, const Tile& t, int64_t th, int h, int z,
+                                            int rows, int row) {
+  if (!K::kByRow) return (th * a.splits + z) * rows + row;
+  const int64_t r = t.r0 + row, tok = r / a.group;
+  const int64_t at = (t.row0 + tok) * (a.nh * a.group) + (h - a.h0) * a.group + (r - tok * a.group);
+  return at * a.shares + a.z0 + z;
 }
 
 // ---- few rows: a tile of 16, the workgroup's waves share out the keys ----
@@ -366,14 +74,15 @@ constexpr int kFewRows = kvplan::kFewRows;
 constexpr int kFewWaves = kvplan::kFewWaves;
 constexpr int kFewStride = kHd + 4;  // LDS row of a merged sum (bank spread)
 
+template <class K>
 __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) {
   const View& c = a.c;
+  const int nh = K::kByRow ? a.nh : c.kv_heads;
   const int w = uniform((int)threadIdx.x >> 6), l = threadIdx.x & 63, r16 = l & 15, g = l >> 4;
   const int z = (int)(blockIdx.x % a.splits);
   const int64_t th = blockIdx.x / a.splits;
-  const int h = (int)(th % c.kv_heads);
-  const int64_t tile = a.tile0 + th / c.kv_heads;
-  const Tile t = find_tile<kFewRows>(c, a.group, tile);
+  const int h = (K::kByRow ? a.h0 : 0) + (int)(th % nh);
+  const Tile t = find_tile<K, kFewRows>(a, a.tile0 + th / nh);
   if (t.s < 0) return;
 
   float x[4][8];
@@ -388,7 +97,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
     parts8(x[kb], qh[kb], ql[kb]);
   }
   const float qk = __builtin_ldexpf(a.scale2, -qe);
-  const int e0 = first_exp(c, t, h);
+  const int e0 = e0_of<K>(a, t, h);
 
   const int keys = keys_of_rows(t, t.r0, kFewRows, a.group, a.causal);
   const int blocks = (keys + 31) / 32;
@@ -538,15 +247,16 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
     for (int d = 0; d < kPer; d++) o[d] = __builtin_fmaf(sums[i][row][d0 + d], f, o[d]);
   }
   float* dst;
-  if (a.splits == 1) {
+  if (!K::kByRow && a.splits == 1) {
     const float f = den == 0.f ? 0.f : __builtin_ldexpf(1.f, e0 - kWeight) / den;
 #pragma unroll
     for (int d = 0; d < kPer; d++) o[d] = o[d] * f;
     const int64_t tok = r / a.group;
-    dst = a.out + (t.row0 + tok) * a.ldo +
-          (int64_t)(h * a.group + (int)(r - tok * a.group)) * kHd + d0;
+    const int head = h * a.group + (int)(r - tok * a.group);
+    dst = a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd + d0;
+    if (K::kStats && d0 == 0) a.stats[(t.row0 + tok) * a.heads + head] = stat_of(m, den);
   } else {
-    const int64_t at = (th * a.splits + z) * kFewRows + row;
+    const int64_t at = share_at<K>(a, t, th, h, z, kFewRows, row);
     if (d0 == 0) a.part_ml[at] = float2{m, den};
     dst = a.part + at * kHd + d0;
   }
@@ -564,35 +274,31 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 
 constexpr int kJoin = 8;  // shares that a wave reads at a time
 
-template <int RT, int W>
-__global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
-  const int l = threadIdx.x & 63, w = uniform((int)threadIdx.x >> 6);
-  const int64_t i = (int64_t)blockIdx.x * (4 / W) + w / W;
-  const int64_t th = i / RT;
-  const int row = (int)(i % RT), h = (int)(th % a.c.kv_heads);
-  const Tile t = find_tile<RT>(a.c, a.group, a.tile0 + th / a.c.kv_heads);
-  if (t.s < 0 || t.r0 + row >= t.rows) return;  // with W = 4 for the whole workgroup
-  // lane z holds share z's maximum and denominator (splits <= 64)
-  const int64_t at = th * a.splits * RT + row;
-  const float2 ml = l < a.splits ? a.part_ml[at + (int64_t)l * RT] : float2{-INFINITY, 0.f};
-  float m = ml.x;
+// The sum of a row's shares, two dims a lane, at `at` + z * step of the shares z < n that
+// `ml` (lane z's) holds: to out, unnormalized sums times 2^-kWeight 2^E0 / denominator. W waves
+// a row; false: the wave has no part in what follows.
+template <int W>
+__device__ __forceinline__ bool join(const Args& a, float2 ml, int64_t at, int64_t step, int n, int w,
+                                     float& m, float& den, float& o0, float& o1) {
+  const int l = threadIdx.x & 63;
+  m = ml.x;
 #pragma unroll
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   const float d = ml.x - (m == -INFINITY ? 0.f : m);
   const float own = __builtin_amdgcn_exp2f(d);
-  float den = times_exp2(ml.y, d);
+  den = times_exp2(ml.y, d);
 #pragma unroll
   for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
-  float o0 = 0.f, o1 = 0.f;
-  for (int z0 = kJoin * (w % W); z0 < a.splits; z0 += kJoin * W) {
+  o0 = 0.f, o1 = 0.f;
+  for (int z0 = kJoin * (w % W); z0 < n; z0 += kJoin * W) {
     float2 v[kJoin];
 #pragma unroll
     for (int k = 0; k < kJoin; k++)
-      if (z0 + k < a.splits)
-        v[k] = reinterpret_cast<const float2*>(a.part + (at + (int64_t)(z0 + k) * RT) * kHd)[l];
+      if (z0 + k < n)
+        v[k] = reinterpret_cast<const float2*>(a.part + (at + (int64_t)(z0 + k) * step) * kHd)[l];
 #pragma unroll
     for (int k = 0; k < kJoin; k++)
-      if (z0 + k < a.splits) {
+      if (z0 + k < n) {
         const float f = __shfl(own, z0 + k);
         o0 = __builtin_fmaf(v[k].x, f, o0);
         o1 = __builtin_fmaf(v[k].y, f, o1);
@@ -602,19 +308,60 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
     __shared__ float2 sums[W][64];
     sums[w][l] = float2{o0, o1};
     __syncthreads();
-    if (w) return;
+    if (w) return false;
 #pragma unroll
     for (int k = 1; k < W; k++) {
       o0 += sums[k][l].x;
       o1 += sums[k][l].y;
     }
   }
+  return true;
+}
+
+template <class K, int RT, int W>
+__global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
+  const int l = threadIdx.x & 63, w = uniform((int)threadIdx.x >> 6);
+  const int64_t i = (int64_t)blockIdx.x * (4 / W) + w / W;
+  const int64_t th = i / RT;
+  const int row = (int)(i % RT), h = (int)(th % a.c.kv_heads);
+  const Tile t = find_tile<K, RT>(a, a.tile0 + th / a.c.kv_heads);
+  if (t.s < 0 || t.r0 + row >= t.rows) return;  // with W = 4 for the whole workgroup
+  // lane z holds share z's maximum and denominator (splits <= 64)
+  const int64_t at = th * a.splits * RT + row;
+  const float2 ml = l < a.splits ? a.part_ml[at + (int64_t)l * RT] : float2{-INFINITY, 0.f};
+  float m, den, o0, o1;
+  if (!join<W>(a, ml, at, RT, a.splits, w, m, den, o0, o1)) return;
   const float f =
       den == 0.f ? 0.f : __builtin_ldexpf(1.f, first_exp(a.c, t, h) - kWeight) / den;
   const int64_t r = t.r0 + row, tok = r / a.group;
-  float* dst = a.out + (t.row0 + tok) * a.ldo +
-               (int64_t)(h * a.group + (int)(r - tok * a.group)) * kHd;
-  reinterpret_cast<float2*>(dst)[l] = float2{o0 * f, o1 * f};
+  const int head = h * a.group + (int)(r - tok * a.group);
+  reinterpret_cast<float2*>(a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd)[l] =
+      float2{o0 * f, o1 * f};
+  if (K::kStats && l == 0) a.stats[(t.row0 + tok) * a.heads + head] = stat_of(m, den);
+}
+
+// The same for rows behind a shared part: shares z < z0 are its, the others the row's own.
+template <int W>
+__global__ void __launch_bounds__(256) kv_attn_join_rows_kernel(Args a, int64_t i0) {
+  const int l = threadIdx.x & 63, w = uniform((int)threadIdx.x >> 6);
+  const int64_t i = i0 + (int64_t)blockIdx.x * (4 / W) + w / W;
+  const int per = a.nh * a.group;
+  const int64_t t = i / per;
+  if (t >= a.c.T) return;
+  const int s = seq_at(a.c, t);
+  if (s < 0) return;
+  const int g = part_of(a.pre, s);
+  const int head = a.h0 * a.group + (int)(i - t * per);
+  // a sequence without a shared part has none of its shares, a row without a position none
+  const bool placed = kv::length_of(a.c, s) - kv::row_of(a.c, s + 1) + t >= 0;
+  const int z0 = g < 0 ? a.z0 : 0, n = placed ? a.shares - z0 : 0;
+  const int64_t at = i * a.shares + z0;
+  const float2 ml = l < n ? a.part_ml[at + l] : float2{-INFINITY, 0.f};
+  float m, den, o0, o1;
+  if (!join<W>(a, ml, at, 1, n, w, m, den, o0, o1)) return;
+  const float f = den == 0.f ? 0.f
+                             : __builtin_ldexpf(1.f, first_exp(a, s, g, head / a.group) - kWeight) / den;
+  reinterpret_cast<float2*>(a.out + t * a.ldo + (int64_t)head * kHd)[l] = float2{o0 * f, o1 * f};
 }
 
 // ---- chunks: NW waves of 16 QT rows over the same keys ----
@@ -654,18 +401,19 @@ struct Block {
   int far;  // a key has e < kNear
 };
 
-template <int NW, int QT>
+template <class K, int NW, int QT>
 __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   constexpr int kRows = 16 * QT * NW;
   using Blk = Block<NW>;
   constexpr int KB = Blk::kKeys;
   __shared__ Blk buf[2];
   const View& c = a.c;
+  const int nh = K::kByRow ? a.nh : c.kv_heads;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, r16 = l & 15, g = l >> 4;
   const int z = (int)(blockIdx.x % a.splits);
   const int64_t th = blockIdx.x / a.splits;
-  const int h = (int)(th % c.kv_heads);
-  const Tile t = find_tile<kRows>(c, a.group, a.tile0 + th / c.kv_heads);
+  const int h = (K::kByRow ? a.h0 : 0) + (int)(th % nh);
+  const Tile t = find_tile<K, kRows>(a, a.tile0 + th / nh);
   if (t.s < 0) return;
 
   v8h qh[QT][4], ql[QT][4];
@@ -687,7 +435,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     }
     qk[qt] = __builtin_ldexpf(a.scale2, -qe);
   }
-  const int e0 = first_exp(c, t, h);
+  const int e0 = e0_of<K>(a, t, h);
   const int keys = keys_of_rows(t, t.r0, kRows, a.group, a.causal);
   const int blocks = (keys + KB - 1) / KB;
   const int b0 = (int)((int64_t)blocks * z / a.splits);
@@ -913,13 +661,15 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     const float den = den_of(st[qt].l, bad[qt]);
     float f = 1.f;
     float* dst;
-    if (a.splits == 1) {
+    if (!K::kByRow && a.splits == 1) {
       f = den == 0.f ? 0.f : __builtin_ldexpf(1.f, e0 - kWeight) / den;
       const int64_t tok = r / a.group;
-      dst = a.out + (t.row0 + tok) * a.ldo +
-            (int64_t)(h * a.group + (int)(r - tok * a.group)) * kHd + 32 * g;
+      const int head = h * a.group + (int)(r - tok * a.group);
+      dst = a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd + 32 * g;
+      if (K::kStats && g == 0)
+        a.stats[(t.row0 + tok) * a.heads + head] = stat_of(st[qt].m, den);
     } else {
-      const int64_t at = (th * a.splits + z) * kRows + row;
+      const int64_t at = share_at<K>(a, t, th, h, z, kRows, row);
       if (g == 0) a.part_ml[at] = float2{st[qt].m, den};
       dst = a.part + at * kHd + 32 * g;
     }
@@ -933,51 +683,118 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   }
 }
 
-template <int RT, class Launch>
-hipError_t run(Args a, const kvplan::Plan& p, Launch launch, hipStream_t s) {
+// Workgroups for n tiles (from a.tile0 on) of nh heads.
+template <class K>
+hipError_t launch_tiles(const Args& a, const kvplan::Plan& p, int64_t n, int nh, hipStream_t s) {
+  const dim3 grid((unsigned)(n * nh * p.splits));
+  if (p.rows == kFewRows)
+    hipLaunchKernelGGL(kv_attn_few_kernel<K>, grid, dim3(64 * kFewWaves), 0, s, a);
+  else if (p.rows == 64)
+    hipLaunchKernelGGL((kv_attn_chunk_kernel<K, 4, 1>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((kv_attn_chunk_kernel<K, 8, 2>), grid, dim3(512), 0, s, a);
+  return hipGetLastError();
+}
+
+template <class K, int RT>
+hipError_t launch_join(const Args& a, int64_t n, hipStream_t s) {
+  if (a.splits > kJoin)
+    hipLaunchKernelGGL((kv_attn_join_kernel<K, RT, 4>), dim3((unsigned)(n * RT)), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((kv_attn_join_kernel<K, RT, 1>), dim3((unsigned)(n * RT / 4)), dim3(256), 0, s,
+                       a);
+  return hipGetLastError();
+}
+
+template <class K>
+hipError_t run(Args a, const kvplan::Plan& p, hipStream_t s) {
+  a.splits = p.splits;
   // launches of as many tiles as a grid's 32-bit thread count takes
   for (int64_t tile = 0; tile < p.tiles; tile += p.tiles_per_launch) {
-    const int64_t n = std::min(p.tiles_per_launch, p.tiles - tile) * a.c.kv_heads;
+    const int64_t n = std::min(p.tiles_per_launch, p.tiles - tile);
     a.tile0 = tile;
-    launch(a, (unsigned)(n * p.splits));
-    hipError_t e = hipGetLastError();
+    hipError_t e = launch_tiles<K>(a, p, n, a.c.kv_heads, s);
     if (e != hipSuccess) return e;
     if (p.splits > 1) {
-      if (p.splits > kJoin)
-        hipLaunchKernelGGL((kv_attn_join_kernel<RT, 4>), dim3((unsigned)(n * RT)), dim3(256), 0, s,
-                           a);
-      else
-        hipLaunchKernelGGL((kv_attn_join_kernel<RT, 1>), dim3((unsigned)(n * RT / 4)), dim3(256), 0,
-                           s, a);
-      e = hipGetLastError();
+      e = p.rows == kFewRows ? launch_join<K, kFewRows>(a, n * a.c.kv_heads, s)
+          : p.rows == 64     ? launch_join<K, 64>(a, n * a.c.kv_heads, s)
+                             : launch_join<K, 256>(a, n * a.c.kv_heads, s);
       if (e != hipSuccess) return e;
     }
   }
   return hipSuccess;
 }
 
+Args args_of(const View& c, const KvRows& r, void* scratch, int64_t part_bytes) {
+  Args a{};
+  a.c = c;
+  a.q = r.q, a.ldq = r.ldq, a.out = r.out, a.ldo = r.ldo;
+  a.heads = r.heads, a.group = r.heads / c.kv_heads;
+  a.scale2 = r.scale * 1.44269504088896341f;
+  a.causal = r.causal;
+  a.part = static_cast<float*>(scratch);
+  a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + part_bytes);
+  return a;
+}
+
 }  // namespace
 
-hipError_t launch_kv_attn(const View& c, const float* q, int64_t ldq, float* out, int64_t ldo,
-                          int heads, float scale, int causal, const kvplan::Plan& p,
-                          void* scratch, hipStream_t s) {
-  Args a{c, q, ldq, out, ldo, heads, heads / c.kv_heads, scale * 1.44269504088896341f, causal,
-         p.splits, 0, nullptr, nullptr};
-  if (p.splits > 1) {
-    a.part = static_cast<float*>(scratch);
-    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(scratch) + p.part_bytes);
+hipError_t launch_kv_attn(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
+                          hipStream_t s) {
+  return run<Own>(args_of(c, r, scratch, p.part_bytes), p, s);
+}
+
+hipError_t launch_kv_cross(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
+                           hipStream_t s) {
+  return run<Cross>(args_of(c, r, scratch, p.part_bytes), p, s);
+}
+
+hipError_t launch_kv_counted(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
+                             float2* stats, hipStream_t s) {
+  Args a = args_of(c, r, scratch, p.part_bytes);
+  a.stats = stats;
+  return run<Counted>(a, p, s);
+}
+
+hipError_t launch_kv_shared(const View& c, const kv::Shared& pre, const KvRows& r,
+                            const kvplan::SharedPlan& p, void* scratch, hipStream_t s) {
+  Args own = args_of(c, r, scratch, p.part_bytes);
+  own.pre = pre;
+  own.shares = p.pre.splits + p.own.splits;
+  Args shared = own;
+  own.z0 = p.pre.splits, own.splits = p.own.splits;
+  shared.z0 = 0, shared.splits = p.pre.splits, shared.causal = 0;
+  shared.c.lens = pre.lens, shared.c.table = pre.table;
+  shared.c.nseq = pre.n, shared.c.max_pages = pre.max_pages;
+  for (int h0 = 0; h0 < c.kv_heads; h0 += p.heads) {
+    own.h0 = shared.h0 = h0;
+    own.nh = shared.nh = std::min(p.heads, c.kv_heads - h0);
+    hipError_t e;
+    for (int64_t t = 0; t < p.pre.tiles; t += p.pre.tiles_per_launch) {
+      shared.tile0 = t;
+      if ((e = launch_tiles<Prefix>(shared, p.pre, std::min(p.pre.tiles_per_launch, p.pre.tiles - t),
+                                    own.nh, s)) != hipSuccess)
+        return e;
+    }
+    for (int64_t t = 0; t < p.own.tiles; t += p.own.tiles_per_launch) {
+      own.tile0 = t;
+      if ((e = launch_tiles<Rest>(own, p.own, std::min(p.own.tiles_per_launch, p.own.tiles - t),
+                                  own.nh, s)) != hipSuccess)
+        return e;
+    }
+    // rows a launch: a grid's threads are a 32-bit number
+    const int64_t rows = c.T * own.nh * own.group, most = int64_t(1) << 22;
+    for (int64_t i = 0; i < rows; i += most) {
+      const int64_t n = std::min(most, rows - i);
+      if (own.shares > kJoin)
+        hipLaunchKernelGGL((kv_attn_join_rows_kernel<4>), dim3((unsigned)n), dim3(256), 0, s, own, i);
+      else
+        hipLaunchKernelGGL((kv_attn_join_rows_kernel<1>), dim3((unsigned)ceil_div(n, 4)), dim3(256),
+                           0, s, own, i);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
   }
-  if (p.rows == kFewRows)
-    return run<kFewRows>(a, p, [&](const Args& x, unsigned n) {
-      hipLaunchKernelGGL(kv_attn_few_kernel, dim3(n), dim3(64 * kFewWaves), 0, s, x);
-    }, s);
-  if (p.rows == 64)
-    return run<64>(a, p, [&](const Args& x, unsigned n) {
-      hipLaunchKernelGGL((kv_attn_chunk_kernel<4, 1>), dim3(n), dim3(256), 0, s, x);
-    }, s);
-  return run<256>(a, p, [&](const Args& x, unsigned n) {
-    hipLaunchKernelGGL((kv_attn_chunk_kernel<8, 2>), dim3(n), dim3(512), 0, s, x);
-  }, s);
+  return hipSuccess;
 }
 
 }  // namespace sdq

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 
 namespace sdq {
 namespace kvplan {
@@ -58,6 +59,34 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
     p.part_bytes = p.tiles * kv_heads * s * p.rows * 128 * 4;
     p.scratch_bytes = p.part_bytes / 128 * 130;
   }
+  return p;
+}
+
+// Attention over shared parts and own keys: both as plan() cuts them, their shares' sums one
+// beside the other for every row, cached heads at a time that the scratch takes.
+struct SharedPlan {
+  Plan pre, own;
+  int heads;              // cached heads at a time
+  int64_t part_bytes;     // partial sums; maxima and denominators follow
+  int64_t scratch_bytes;
+};
+
+// n shared parts of up to most_pre tokens.
+inline SharedPlan shared_plan(int64_t T, int nseq, int n, int group, int kv_heads, int64_t most,
+                              int64_t most_pre, int cu_count) {
+  SharedPlan p{};
+  p.own = plan(T, nseq, group, kv_heads, most, cu_count);
+  p.pre = plan(T, n, group, kv_heads, most_pre, cu_count);
+  p.own.splits = std::min(p.own.splits, 16);  // a wave of the join has a share a lane
+  p.pre.splits = std::min(p.pre.splits, kMaxSplits - 16);
+  const int shares = p.own.splits + p.pre.splits;
+  const int64_t head = T * group * shares * (128 + 2) * 4;
+  p.heads = (int)std::max<int64_t>(1, std::min<int64_t>(kv_heads, kMaxScratch / std::max<int64_t>(head, 1)));
+  for (Plan* q : {&p.pre, &p.own})
+    q->tiles_per_launch = std::max<int64_t>(
+        1, ((int64_t(1) << 31) - 1) / ((int64_t)p.heads * q->splits * 512));
+  p.part_bytes = T * group * p.heads * shares * 128 * 4;
+  p.scratch_bytes = p.part_bytes / 128 * 130;
   return p;
 }
 

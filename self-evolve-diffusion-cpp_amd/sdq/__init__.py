@@ -72,6 +72,11 @@ class KvBatchView(ctypes.Structure):
                 ("max_pages", ctypes.c_int64)]
 
 
+class KvSharedView(ctypes.Structure):
+    _fields_ = [("s_start", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("n", ctypes.c_int), ("max_pages", ctypes.c_int64)]
+
+
 class KernelTime(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 48), ("launches", ctypes.c_int),
                 ("total_ms", ctypes.c_double)]
@@ -139,6 +144,20 @@ SIGNATURES = {
     "sdq_kv_attention": (ctypes.c_int, [ctypes.POINTER(KvCacheView), ctypes.POINTER(KvBatchView),
                                         _vp, _i64, _vp, _i64, _i64, ctypes.c_int, ctypes.c_float,
                                         ctypes.c_int, _vp]),
+    "sdq_kv_cross_attention": (ctypes.c_int, [ctypes.POINTER(KvCacheView),
+                                              ctypes.POINTER(KvBatchView), _vp, _i64, _vp, _i64,
+                                              _i64, ctypes.c_int, ctypes.c_float, _vp]),
+    "sdq_kv_attention_shared": (ctypes.c_int, [ctypes.POINTER(KvCacheView),
+                                               ctypes.POINTER(KvSharedView),
+                                               ctypes.POINTER(KvBatchView), _vp, _i64, _vp, _i64,
+                                               _i64, ctypes.c_int, ctypes.c_float, ctypes.c_int,
+                                               _vp]),
+    "sdq_kv_attention_weights": (ctypes.c_int, [ctypes.POINTER(KvCacheView),
+                                                ctypes.POINTER(KvBatchView), _vp, _vp, _i64, _vp,
+                                                _i64, _i64, ctypes.c_int, ctypes.c_float,
+                                                ctypes.c_int, _vp]),
+    "sdq_kv_evict": (ctypes.c_int, [ctypes.POINTER(KvCacheView), ctypes.POINTER(KvBatchView), _vp,
+                                    _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
     "sdq_device_alloc": (ctypes.c_int, [ctypes.c_size_t, ctypes.POINTER(_vp)]),
     "sdq_device_free": (ctypes.c_int, [_vp]),
     "sdq_memcpy": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, ctypes.c_int, _vp]),
@@ -975,12 +994,32 @@ class KvBatch(_KvTensors):
     table = property(lambda self: self._tensors["table"])
 
 
-def _kv_args(cache, batch, rows, heads):
+class KvShared(_KvTensors):
+    """Beginnings that sequences of a batch share (sdq_kv_shared): int32 device tensors
+    s_start [n + 1] (sequences of the batch), lens [n] (tokens) and table [n, max_pages]
+    (page ids). Their contents may change between calls, the tensors not."""
+
+    def __init__(self, s_start, lens, table):
+        c = _Args()
+        pt = c(table, "table", "i32", (None, None))
+        n, most = (int(n) for n in table.shape)
+        self._view = KvSharedView(c(s_start, "s_start", "i32", (n + 1,)),
+                                  c(lens, "lens", "i32", (n,)), pt, n, most)
+        self._ref = ctypes.byref(self._view)
+        super().__init__({"s_start": s_start, "lens": lens, "table": table})
+
+    s_start = property(lambda self: self._tensors["s_start"])
+    lens = property(lambda self: self._tensors["lens"])
+    table = property(lambda self: self._tensors["table"])
+
+
+def _kv_args(cache, batch, rows, heads, c=None):
     """The views of a paged call, and the addresses and row strides of its row
     tensors ((name, tensor) pairs of heads * 128 columns, rows may be strided)."""
     if not isinstance(cache, KvCache) or not isinstance(batch, KvBatch):
         raise _bad("expected a KvCache and a KvBatch")
-    c = _Args()
+    if c is None:
+        c = _Args()
     (a, x), (b, y) = rows
     C = heads * 128
     px, ldx = c.rows(x, a, None, C)
@@ -1018,6 +1057,73 @@ def kv_attention(cache: KvCache, batch: KvBatch, q, out, heads, causal=True, sca
     _check(_lib.sdq_kv_attention(vc, vb, *p, T, int(heads), scale, 1 if causal else 0,
                                  _stream(stream, dev)))
     return out
+
+
+def kv_cross_attention(cache: KvCache, batch: KvBatch, q, out, heads, scale=None, stream=None):
+    """out = attention of each sequence's rows over all of its cached tokens, whose
+    number is another (sdq_kv_cross_attention): q and out [T, heads*128], rows may be
+    strided; scale defaults to 1/sqrt(128). Rows of no sequence are left as they are."""
+    vc, vb, p, T, dev = _kv_args(cache, batch, (("q", q), ("out", out)), int(heads))
+    scale = 128 ** -0.5 if scale is None else float(scale)
+    _check(_lib.sdq_kv_cross_attention(vc, vb, *p, T, int(heads), scale, _stream(stream, dev)))
+    return out
+
+
+def kv_attention_shared(cache: KvCache, shared: KvShared, batch: KvBatch, q, out, heads,
+                        causal=True, scale=None, stream=None):
+    """kv_attention of sequences that begin with shared tokens, read once for all of them
+    (sdq_kv_attention_shared): batch has the tokens behind those."""
+    if not isinstance(shared, KvShared):
+        raise _bad("expected a KvShared")
+    c = _Args()
+    c._seen.append(shared._one)
+    vc, vb, p, T, dev = _kv_args(cache, batch, (("q", q), ("out", out)), int(heads), c)
+    scale = 128 ** -0.5 if scale is None else float(scale)
+    _check(_lib.sdq_kv_attention_shared(vc, shared._ref, vb, *p, T, int(heads), scale,
+                                        1 if causal else 0, _stream(stream, dev)))
+    return out
+
+
+def kv_attention_weights(cache: KvCache, batch: KvBatch, weights, q, out, heads, causal=True,
+                         scale=None, stream=None):
+    """kv_attention that adds the softmax weights which each cached token is given to
+    weights [pages, kv_heads, page_size] (sdq_kv_attention_weights)."""
+    c = _Args()
+    pw = c(weights, "weights", "f32", _kv_shape(cache))
+    vc, vb, p, T, dev = _kv_args(cache, batch, (("q", q), ("out", out)), int(heads), c)
+    scale = 128 ** -0.5 if scale is None else float(scale)
+    _check(_lib.sdq_kv_attention_weights(vc, vb, pw, *p, T, int(heads), scale, 1 if causal else 0,
+                                         _stream(stream, dev)))
+    return out
+
+
+def kv_evict(cache: KvCache, batch: KvBatch, weights, to_table, to_lens, kept, first=0, last=0,
+             stream=None):
+    """Copies the tokens worth keeping, by weights [pages, kv_heads, page_size], to the pages
+    of to_table [nseq, n] (sdq_kv_evict): at most kept.shape[2] of each sequence and head,
+    the first `first` and the last `last` among them. to_lens int32 [nseq] and kept int32
+    [nseq, kv_heads, keep] receive their numbers and positions."""
+    if not isinstance(batch, KvBatch):
+        raise _bad("expected a KvCache and a KvBatch")
+    c = _Args()
+    pw = c(weights, "weights", "f32", _kv_shape(cache))
+    nseq = batch.lens.shape[0]
+    pt = c(to_table, "to_table", "i32", (nseq, None))
+    pl = c(to_lens, "to_lens", "i32", (nseq,))
+    pk = c(kept, "kept", "i32", (nseq, cache.kv_heads, None))
+    c._seen += (cache._one, batch._one)
+    dev = c.done()
+    if _lib is None:
+        load_library()
+    _check(_lib.sdq_kv_evict(cache._ref, batch._ref, pw, int(first), int(last), kept.shape[2], pt,
+                             to_table.shape[1], pl, pk, _stream(stream, dev)))
+    return kept
+
+
+def _kv_shape(cache):
+    if not isinstance(cache, KvCache):
+        raise _bad("expected a KvCache and a KvBatch")
+    return cache.pages, cache.kv_heads, cache.page_size
 
 
 def qlinear_plan(w: Weight, M: int, kind="none") -> list:
