@@ -2558,20 +2558,39 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
   if ((rc = usable_device(&call.dev))) return rc;
   const hipStream_t s = stream_of(stream);
   const kvplan::Plan plan = plan_of(call);
-  // the shares' sums, then two numbers a row and head
-  const size_t stats_at = (size_t)round_up(plan.scratch_bytes, 16);
+  const int cus = g_dev[call.dev].cu_count;
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
-  if ((rc = shared_scratch(call.dev, s, stats_at + (size_t)T * heads * sizeof(float2), &scratch,
-                           &turn)))
-    return rc;
+  char* base;
+  // the shares' sums, two numbers a row and head, and few rows' logits
+  size_t stats_at = (size_t)round_up(plan.scratch_bytes, 16);
+  const size_t stats_bytes = (size_t)round_up(T * heads * (int64_t)sizeof(float2), 16);
+  const int64_t row = kv_logit_keys(call.view) * 4;
+  if (plan.rows == kvplan::kFewRows && row <= kvplan::kMaxScratch / (T * heads) &&
+      (int64_t)call.view.nseq * c->kv_heads <= 1 << 21) {
+    if ((rc = shared_scratch(call.dev, s, stats_at + stats_bytes + (size_t)(row * T * heads), &scratch,
+                             &turn)))
+      return rc;
+    base = reinterpret_cast<char*>(scratch) + stats_at;
+    return timed("kv_attention_weights", s, [&] {
+      return launch_kv_counted_few(call.view, call.rows, plan, scratch,
+                                   reinterpret_cast<float2*>(base),
+                                   reinterpret_cast<float*>(base + stats_bytes), weights, cus, s);
+    });
+  }
+  const KvWeightsPlan wplan =
+      plan_kv_weights(T, call.view.nseq, heads / c->kv_heads, c->kv_heads,
+                      call.view.max_pages << call.view.page_log2, cus);
+  // the shares' sums or, once they are joined, the ranges'
+  stats_at = (size_t)round_up(std::max(plan.scratch_bytes, wplan.scratch_bytes), 16);
+  if ((rc = shared_scratch(call.dev, s, stats_at + stats_bytes, &scratch, &turn))) return rc;
   float2* stats = reinterpret_cast<float2*>(reinterpret_cast<char*>(scratch) + stats_at);
   rc = timed("kv_attention_weights", s, [&] {
     return launch_kv_counted(call.view, call.rows, plan, scratch, stats, s);
   });
   if (rc) return rc;
   return timed("kv_weights", s, [&] {
-    return launch_kv_weights(call.view, call.rows, stats, weights, g_dev[call.dev].cu_count, s);
+    return launch_kv_weights(call.view, call.rows, stats, weights, wplan, scratch, s);
   });
 }
 
@@ -2611,7 +2630,14 @@ int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, i
   if ((rc = usable_device(&dev))) return rc;
   const hipStream_t s = stream_of(stream);
   const kv::Kept k{first, last, keep, to_table, to_max_pages, to_lens, kept};
-  return timed("kv_evict", s, [&] { return launch_kv_evict(view, weights, k, s); });
+  const KvEvictPlan plan =
+      plan_kv_evict(view.nseq, view.kv_heads, view.max_pages << view.page_log2);
+  float* scratch = nullptr;
+  std::unique_lock<std::mutex> turn;
+  if (plan.scratch_bytes > 0 &&
+      (rc = shared_scratch(dev, s, (size_t)plan.scratch_bytes, &scratch, &turn)))
+    return rc;
+  return timed("kv_evict", s, [&] { return launch_kv_evict(view, weights, k, plan, scratch, s); });
 }
 
 int sdq_device_alloc(size_t bytes, void** out) {

@@ -31,13 +31,17 @@ constexpr float kNear = -10.f;
 
 // What the rows of a launch see, and where their sums go.
 struct Own {  // a sequence's last tokens, its own keys
-  static constexpr bool kFree = false, kGroups = false, kByRow = false, kStats = false;
+  static constexpr bool kFree = false, kGroups = false, kByRow = false, kStats = false,
+                        kLogits = false;
 };
 struct Cross : Own {  // any rows, all keys of their sequence
   static constexpr bool kFree = true;
 };
 struct Counted : Own {  // each row's maximum and denominator are kept
   static constexpr bool kStats = true;
+};
+struct Logits : Counted {  // and the logits
+  static constexpr bool kLogits = true;
 };
 struct Prefix : Cross {  // the rows of a run of sequences, the keys that those share
   static constexpr bool kGroups = true, kByRow = true;
@@ -61,6 +65,9 @@ struct Args {
   float2* part_ml;   // the same without dims: maximum, denominator
   // kStats: [row][head] maximum and reciprocal denominator (infinity and 0: adds nothing)
   float2* stats;
+  // kLogits: [row][head][key], `keys` of them a row
+  float* logits;
+  int64_t keys;
   // kByRow: cached heads h0 .. h0 + nh - 1 of this launch, shares z0 .. of `shares`; the
   // sums are [row][head of those][share][128]
   int h0, nh, z0, shares;
@@ -80,6 +87,13 @@ struct Tile {
 
 // A lane's value that is the same in the whole wave, as a scalar.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Memory that no kernel of the launch writes, for loads through the scalar cache also where
+// the kernel stores elsewhere.
+template <class T>
+__device__ __forceinline__ const __attribute__((address_space(4))) T* scalar_ptr(const T* p) {
+  return (const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
 
 // The last of indexes 0 .. n - 1 whose f, which does not fall, is at most v; -1: none. By a
 // search 64 ways at a time; f(n) may be asked for. The same in every wave.
@@ -119,6 +133,16 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int64_t tile) {
   t.len = (int)kv::length_of(c, lo);
   t.first = K::kFree ? 0 : t.len - (int)(tokens > 0 ? tokens : 0);
   if (t.r0 < t.rows) t.s = lo;
+  return t;
+}
+
+// All rows of sequence s.
+__device__ __forceinline__ Tile rows_of(const Args& a, int s) {
+  Tile t{s, 0, 0, kv::row_of(a.c, s), 0, 0};
+  const int64_t tokens = kv::row_of(a.c, s + 1) - t.row0;
+  t.rows = tokens > 0 ? tokens * a.group : 0;
+  t.len = (int)kv::length_of(a.c, s);
+  t.first = t.len - (int)(tokens > 0 ? tokens : 0);
   return t;
 }
 

@@ -112,6 +112,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 #pragma unroll
   for (int e = 0; e < 8; e++) acc[e] = v4f{0.f, 0.f, 0.f, 0.f};
 
+  float* row_logits = nullptr;  // of the lane's keys 4 g .. of a tile
+  if (K::kLogits && t.r0 + r16 < t.rows) {
+    const int64_t tok = (t.r0 + r16) / a.group;
+    const int head = h * a.group + (int)(t.r0 + r16 - tok * a.group);
+    row_logits = a.logits + ((t.row0 + tok) * a.heads + head) * a.keys + 4 * g;
+  }
   // A block's codes and scales, loaded one block ahead, its pages another one.
   struct Raw {
     uint4 k[2][2];
@@ -119,16 +125,16 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
     v4f ks[2], vs[2];
     bool there[2];
   };
-  const int32_t* table = c.table + t.s * c.max_pages;
-  auto page_at = [&](int b, int kt) {
-    const int p = b * 32 + 16 * kt;
-    return b < b1 && p < keys ? table[p >> c.page_log2] : -1;
-  };
+  // Every load is made whether or not there is a block (of the first page then): behind a branch
+  // the compiler would wait for a block's loads in the round that issues them.
+  const auto* table = scalar_ptr(c.table + t.s * c.max_pages);
+  const int last = (keys - 1) >> c.page_log2;
+  auto page_at = [&](int b, int kt) { return table[min((b * 32 + 16 * kt) >> c.page_log2, last)]; };
   auto load = [&](int b, const int pages[2], Raw& r) {
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
       const int p = b * 32 + 16 * kt;
-      r.there[kt] = pages[kt] >= 0 && pages[kt] < c.pages;
+      r.there[kt] = b < b1 && p < keys && pages[kt] >= 0 && pages[kt] < c.pages;
       const int64_t at = (((r.there[kt] ? pages[kt] : 0) * (int64_t)c.kv_heads + h)
                           << c.page_log2) + (p & ((1 << c.page_log2) - 1));
       const int8_t* kp = c.k + (at + r16) * kHd + 16 * g;
@@ -141,19 +147,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
       r.vs[kt] = *reinterpret_cast<const v4f_any*>(c.vs + at + 4 * g);
     }
   };
-  Raw cur;
-  int pages[2];
-  if (b0 + w < b1) {
-    pages[0] = page_at(b0 + w, 0), pages[1] = page_at(b0 + w, 1);
-    load(b0 + w, pages, cur);
-    pages[0] = page_at(b0 + w + kFewWaves, 0), pages[1] = page_at(b0 + w + kFewWaves, 1);
-  }
-  for (int b = b0 + w; b < b1; b += kFewWaves) {
-    Raw nxt;
-    if (b + kFewWaves < b1) {
-      load(b + kFewWaves, pages, nxt);
-      pages[0] = page_at(b + 2 * kFewWaves, 0), pages[1] = page_at(b + 2 * kFewWaves, 1);
-    }
+  auto block = [&](int b, const Raw& cur) {
     v4f s[2], kc[2], ke[2], kw[2], kf[2];
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
@@ -179,6 +173,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
     auto softmax = [&](auto mask, auto seen) {
       constexpr bool kMask = decltype(mask)::value;
       const float mx = logits<kMask>(s, kc, ke, seen);
+      if (K::kLogits && row_logits) {
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+          *reinterpret_cast<v4f*>(row_logits + b * 32 + 16 * kt) = s[kt];
+      }
       if (__any(rises(st, mx))) raise(st, mx, acc);
       if (__any(least < kNear)) add_faint(s, ke, st);
       weights<kMask>(s, kw, kf, st, seen, ph, pl);
@@ -215,7 +214,26 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
     tile_e(std::integral_constant<int, 1>{}, vb, acc[5]);
     tile_e(std::integral_constant<int, 2>{}, vb, acc[6]);
     tile_e(std::integral_constant<int, 3>{}, vb, acc[7]);
-    cur = nxt;
+  };
+  // Two blocks in turn, each loaded while the other is at work (a copy from one to the other
+  // would wait for its loads).
+  Raw raw[2];
+  int pages[2];
+  auto look = [&](int b) { pages[0] = page_at(b, 0), pages[1] = page_at(b, 1); };
+  int b = b0 + w;
+  if (b < b1) {
+    look(b);
+    load(b, pages, raw[0]);
+    look(b + kFewWaves);
+  }
+  for (; b < b1; b += 2 * kFewWaves) {
+    load(b + kFewWaves, pages, raw[1]);
+    look(b + 2 * kFewWaves);
+    block(b, raw[0]);
+    if (b + kFewWaves >= b1) break;
+    load(b + 2 * kFewWaves, pages, raw[0]);
+    look(b + 3 * kFewWaves);
+    block(b + kFewWaves, raw[1]);
   }
 
   // Join the waves: common maximum, then sums.
@@ -274,6 +292,19 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 
 constexpr int kJoin = 8;  // shares that a wave reads at a time
 
+// A row's maximum and denominator out of its shares' (one a lane), and the lane's share's
+// weight among them.
+__device__ __forceinline__ float join_stats(float2 ml, float& m, float& den) {
+  m = ml.x;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float d = ml.x - (m == -INFINITY ? 0.f : m);
+  den = times_exp2(ml.y, d);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
+  return __builtin_amdgcn_exp2f(d);
+}
+
 // The sum of a row's shares, two dims a lane, at `at` + z * step of the shares z < n that
 // `ml` (lane z's) holds: to out, unnormalized sums times 2^-kWeight 2^E0 / denominator. W waves
 // a row; false: the wave has no part in what follows.
@@ -281,14 +312,7 @@ template <int W>
 __device__ __forceinline__ bool join(const Args& a, float2 ml, int64_t at, int64_t step, int n, int w,
                                      float& m, float& den, float& o0, float& o1) {
   const int l = threadIdx.x & 63;
-  m = ml.x;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  const float d = ml.x - (m == -INFINITY ? 0.f : m);
-  const float own = __builtin_amdgcn_exp2f(d);
-  den = times_exp2(ml.y, d);
-#pragma unroll
-  for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
+  const float own = join_stats(ml, m, den);
   o0 = 0.f, o1 = 0.f;
   for (int z0 = kJoin * (w % W); z0 < n; z0 += kJoin * W) {
     float2 v[kJoin];
@@ -319,7 +343,7 @@ __device__ __forceinline__ bool join(const Args& a, float2 ml, int64_t at, int64
 }
 
 template <class K, int RT, int W>
-__global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
+__device__ __forceinline__ void join_tiles(const Args& a) {
   const int l = threadIdx.x & 63, w = uniform((int)threadIdx.x >> 6);
   const int64_t i = (int64_t)blockIdx.x * (4 / W) + w / W;
   const int64_t th = i / RT;
@@ -338,6 +362,96 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
   reinterpret_cast<float2*>(a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd)[l] =
       float2{o0 * f, o1 * f};
   if (K::kStats && l == 0) a.stats[(t.row0 + tok) * a.heads + head] = stat_of(m, den);
+}
+
+template <class K, int RT, int W>
+__global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
+  join_tiles<K, RT, W>(a);
+}
+
+// ---- few rows: what each key was given ----
+//
+// The few-row form leaves its logits, t_rj of row r and key j; per key and cached head this
+// adds up   sum_r 2^(t_rj - m_r - e_j) / d_r   (sdq_kv_weights.hip forms the logits again where
+// rows are many). A thread has four keys, a row of logits is read once, and maxima and
+// denominators come from the shares themselves, so that the join of the outputs is the same
+// launch: its workgroups are the first `joins`.
+
+constexpr int kCountKeys = 1024;  // of a workgroup
+constexpr int kCountRows = 64;    // whose statistics LDS holds
+
+template <int W>
+__global__ void __launch_bounds__(256) kv_counts_kernel(Args a, float* __restrict__ sums,
+                                                        unsigned joins, int across) {
+  if (blockIdx.x < joins) {
+    join_tiles<Own, kFewRows, W>(a);
+    return;
+  }
+  __shared__ float2 stats[kCountRows];
+  __shared__ int sees[kCountRows];
+  const View& c = a.c;
+  const int tid = threadIdx.x, l = tid & 63, w = uniform(tid >> 6);
+  const unsigned i = blockIdx.x - joins;
+  const int sh = (int)(i / across);
+  const int h = sh % c.kv_heads, s = sh / c.kv_heads;
+  const Tile t = rows_of(a, s);
+  const int e0 = first_exp(c, t, h);
+  const int64_t tile0 = t.row0 * a.group / kFewRows + s;  // numbers as in find_tile
+  for (int k0 = (int)(i % across) * kCountKeys; k0 < t.len; k0 += across * kCountKeys) {
+    const int p = k0 + 4 * tid;
+    const int64_t at = p < t.len ? kv::place_of(c, s, p, h) : -1;
+    v4f e = v4f{0.f, 0.f, 0.f, 0.f}, sum = e;
+    if (at >= 0) {
+      const v4f vs = *reinterpret_cast<const v4f_any*>(c.vs + at);
+#pragma unroll
+      for (int j = 0; j < 4; j++) e[j] = key_terms(0.f, vs[j], p + j < t.len, 0.f, e0).e;
+    }
+    for (int64_t r0 = 0; r0 < t.rows; r0 += kCountRows) {
+      const int n = (int)(t.rows - r0 < kCountRows ? t.rows - r0 : kCountRows);
+      __syncthreads();  // the last rows' statistics are read
+      for (int r = w; r < n; r += 4) {
+        const int64_t row = r0 + r, tok = row / a.group;
+        float2 st;
+        if (a.splits == 1) {
+          st = a.stats[(t.row0 + tok) * a.heads + h * a.group + (row - tok * a.group)];
+        } else {
+          const int64_t th = (tile0 + row / kFewRows) * c.kv_heads + h;
+          const float2 ml = l < a.splits ? a.part_ml[(th * a.splits + l) * kFewRows + row % kFewRows]
+                                         : float2{-INFINITY, 0.f};
+          float m, den;
+          join_stats(ml, m, den);
+          st = stat_of(m, den);
+        }
+        if (l == 0) {
+          stats[r] = st;
+          sees[r] = st.y > 0.f ? keys_of(t, row, a.group, a.causal) : 0;
+        }
+      }
+      __syncthreads();
+      if (at >= 0) {
+        int64_t tok = r0 / a.group;
+        int qh = (int)(r0 - tok * a.group);
+        for (int r = 0; r < n; r++) {
+          const int see = sees[r];
+          if (p < see) {
+            const float2 st = stats[r];
+            const v4f x = *reinterpret_cast<const v4f*>(
+                a.logits + ((t.row0 + tok) * a.heads + h * a.group + qh) * a.keys + p);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float y = p + j < see ? x[j] - st.x - e[j] : -INFINITY;
+              sum[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(y), st.y, sum[j]);
+            }
+          }
+          if (++qh == a.group) qh = 0, tok++;
+        }
+      }
+    }
+    if (at < 0 || t.rows == 0) continue;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (p + j < t.len) sums[at + j] = p + j < t.first ? sums[at + j] + sum[j] : sum[j];
+  }
 }
 
 // The same for rows behind a shared part: shares z < z0 are its, the others the row's own.
@@ -410,8 +524,10 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   const View& c = a.c;
   const int nh = K::kByRow ? a.nh : c.kv_heads;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, r16 = l & 15, g = l >> 4;
-  const int z = (int)(blockIdx.x % a.splits);
-  const int64_t th = blockIdx.x / a.splits;
+  // causal: the last rows, which see most, first (4099 rows over themselves, 24 heads on 8: 329 us the other way round, 252 so)
+  const unsigned block = a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const int z = (int)(block % a.splits);
+  const int64_t th = block / a.splits;
   const int h = (K::kByRow ? a.h0 : 0) + (int)(th % nh);
   const Tile t = find_tile<K, kRows>(a, a.tile0 + th / nh);
   if (t.s < 0) return;
@@ -754,6 +870,36 @@ hipError_t launch_kv_counted(const View& c, const KvRows& r, const kvplan::Plan&
   Args a = args_of(c, r, scratch, p.part_bytes);
   a.stats = stats;
   return run<Counted>(a, p, s);
+}
+
+int64_t kv_logit_keys(const View& c) { return round_up(std::max<int64_t>(c.max_pages << c.page_log2, 1), 32); }
+
+hipError_t launch_kv_counted_few(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
+                                 float2* stats, float* logits, float* sums, int cu_count,
+                                 hipStream_t s) {
+  Args a = args_of(c, r, scratch, p.part_bytes);
+  a.stats = stats, a.logits = logits, a.keys = kv_logit_keys(c);
+  a.splits = p.splits;
+  hipError_t e;
+  for (int64_t tile = 0; tile < p.tiles; tile += p.tiles_per_launch) {
+    a.tile0 = tile;
+    if ((e = launch_tiles<Logits>(a, p, std::min(p.tiles_per_launch, p.tiles - tile), c.kv_heads,
+                                  s)) != hipSuccess)
+      return e;
+  }
+  // with shares, all tiles are one launch's: so is their join
+  a.tile0 = 0;
+  const int64_t rows = p.tiles * c.kv_heads * kFewRows;
+  const unsigned joins = p.splits == 1 ? 0 : (unsigned)(p.splits > kJoin ? rows : rows / 4);
+  const int64_t pairs = (int64_t)c.nseq * c.kv_heads;
+  const int64_t across = std::min(ceil_div(std::max<int64_t>(c.max_pages << c.page_log2, 1), kCountKeys),
+                                  ceil_div(4 * (int64_t)cu_count, pairs));
+  const dim3 grid((unsigned)(joins + across * pairs));
+  if (p.splits > kJoin)
+    hipLaunchKernelGGL((kv_counts_kernel<4>), grid, dim3(256), 0, s, a, sums, joins, (int)across);
+  else
+    hipLaunchKernelGGL((kv_counts_kernel<1>), grid, dim3(256), 0, s, a, sums, joins, (int)across);
+  return hipGetLastError();
 }
 
 hipError_t launch_kv_shared(const View& c, const kv::Shared& pre, const KvRows& r,

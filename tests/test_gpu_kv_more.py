@@ -496,6 +496,18 @@ def test_weights_at_any_float(sdq_dev):
         assert_bitexact(runs[-1], runs[0])
 
 
+@pytest.mark.parametrize("new", [1, 5])
+def test_weights_of_a_wide_table(sdq_dev, new):
+    """A table of 2^27 tokens, nearly all of it unused: the form that keeps no logits."""
+    c = More(sdq_dev, [new, new], [300, 4000], 1, 16, seed=18)
+    table = np.full((2, 1 << 23), -1, np.int32)
+    table[:, :c.most] = c.table
+    c.table, c.most = table, 1 << 23
+    c.up()
+    c.check_weights(2)
+    c.check_weights(2, causal=False)
+
+
 # ---- eviction ----
 
 def _weights(c, kind):
@@ -522,9 +534,14 @@ def test_evict(sdq_dev, lens, keep, first, last, kind):
     c.check_evict(_weights(c, kind), keep, first, last)
 
 
-def test_evict_long(sdq_dev):
-    c = More(sdq_dev, [0], [150001], 1, 256, seed=20)
-    c.check_evict(_weights(c, "spread"), 30000, 64, 4096)
+@pytest.mark.parametrize("kind", ["spread", "ties", "odd", "equal"])
+@pytest.mark.parametrize("lens,keep,first,last", [
+    ([150001], 30000, 64, 4096), ([70000, 0, 16384, 16385, 33000], 5000, 3, 100),
+    ([66000, 65999], 65999, 0, 1), ([100000], 1, 0, 0), ([65552, 1], 65552, 7, 9)])
+def test_evict_long(sdq_dev, lens, keep, first, last, kind):
+    """Tables of more tokens than a workgroup's registers hold."""
+    c = More(sdq_dev, [0] * len(lens), lens, 2, 256, seed=20)
+    c.check_evict(_weights(c, kind), keep, first, last)
 
 
 @pytest.mark.parametrize("kind", ["spread", "odd"])
