@@ -1077,6 +1077,8 @@ int kv_call(const sdq_kv_cache* c, const sdq_kv_batch* b, const KvRows& r, int64
   if (!(r.scale >= -3.4e38f && r.scale <= 3.4e38f))
     return set_error(SDQ_ERR_INVALID, tag + ": scale must be finite");
   if (out->view.T == 0) return SDQ_OK;
+  if (T * r.heads > int64_t(1) << 31)
+    return set_error(SDQ_ERR_INVALID, tag + ": T * heads must be at most 2^31");
   const int64_t C = (int64_t)r.heads * kv::kHd;
   if ((rc = kv_rows(tag, "q", r.q, r.ldq, C)) || (rc = kv_rows(tag, "out", r.out, r.ldo, C)))
     return rc;
@@ -1084,9 +1086,9 @@ int kv_call(const sdq_kv_cache* c, const sdq_kv_batch* b, const KvRows& r, int64
     return set_error(SDQ_ERR_INVALID, tag + ": out overlaps q");
   return SDQ_OK;
 }
-kvplan::Plan plan_of(const KvCall& k) {
+kvplan::Plan plan_of(const KvCall& k, int tall = 0) {
   return kvplan::plan(k.view.T, k.view.nseq, k.rows.heads / k.view.kv_heads, k.view.kv_heads,
-                      k.view.max_pages << k.view.page_log2, g_dev[k.dev].cu_count);
+                      k.view.max_pages << k.view.page_log2, g_dev[k.dev].cu_count, tall);
 }
 
 // Host -> device through the first two slots' pinned buffers, on the first

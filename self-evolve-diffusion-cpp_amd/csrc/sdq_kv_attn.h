@@ -32,7 +32,7 @@ constexpr float kNear = -10.f;
 // What the rows of a launch see, and where their sums go.
 struct Own {  // a sequence's last tokens, its own keys
   static constexpr bool kFree = false, kGroups = false, kByRow = false, kStats = false,
-                        kLogits = false;
+                        kLogits = false, kRest = false;
 };
 struct Cross : Own {  // any rows, all keys of their sequence
   static constexpr bool kFree = true;
@@ -47,7 +47,7 @@ struct Prefix : Cross {  // the rows of a run of sequences, the keys that those 
   static constexpr bool kGroups = true, kByRow = true;
 };
 struct Rest : Own {  // own keys behind shared ones
-  static constexpr bool kByRow = true;
+  static constexpr bool kByRow = true, kRest = true;
 };
 
 struct Args {
@@ -71,6 +71,8 @@ struct Args {
   // kByRow: cached heads h0 .. h0 + nh - 1 of this launch, shares z0 .. of `shares`; the
   // sums are [row][head of those][share][128]
   int h0, nh, z0, shares;
+  int want;  // Prefix: workgroups that the shares are to make
+  int least; // keys of a share
   kv::Shared pre;  // Prefix: c has its lens, table, max_pages and number of parts
 };
 
@@ -83,7 +85,15 @@ struct Tile {
   int64_t row0;   // the sequence's first row in q
   int len;        // keys, at most 2^30
   int first;      // position of the sequence's first row
+  int part, part_len;  // Rest: the shared part (-1: none) and its tokens
+  int tiles;           // Prefix: that hold rows, of all parts (0: not counted)
 };
+constexpr Tile kNoTile{-1, 0, 0, 0, 0, 0, -1, 0, 0};
+
+// A row's token. Rows times heads are at most 2^31 (sdq_api.hip).
+__device__ __forceinline__ int token_of(int64_t r, int group) {
+  return (int)((uint32_t)r / (uint32_t)group);
+}
 
 // A lane's value that is the same in the whole wave, as a scalar.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -112,25 +122,80 @@ __device__ __forceinline__ int last_upto(int most, F f, int64_t v) {
   return uniform(lo);
 }
 
+// The shared part that sequence s begins with, -1: none.
+__device__ __forceinline__ int part_of(const kv::Shared& p, int s) {
+  const int g = last_upto(p.n, [&](int i) { return (int64_t)p.seq_of(i); }, s);
+  return g >= 0 && s < p.seq_of(g + 1) ? g : -1;
+}
+__device__ __forceinline__ int64_t length_of(const View& c, const kv::Shared& p, int g) {
+  const int64_t n = p.lens[g], most = p.max_pages << c.page_log2;
+  return n < 0 ? 0 : n > most ? most : n;
+}
 // Tile number `tile`. Sequence s, whose rows start at row a and end before row b of all
 // (row: a token's head of the group), has the numbers from a / RT + s to b / RT + s, at
 // least as many as it has tiles of RT rows: a number without a tile is none. So the
 // sequence is found by search, with no sum over those before it
 // (a scan over them took a fifth of a microsecond for each 64). The same in every wave.
+//
+// Fewer than 64 sequences: a lane each has its rows and length, loaded side by side (the
+// search and what follows it would load one after the other).
 template <class K, int RT>
 __device__ __forceinline__ Tile find_tile(const Args& a, int64_t tile) {
   const View& c = a.c;
   const int group = a.group;
-  Tile t{-1, 0, 0, 0, 0, 0};
-  auto row_of = [&](int s) { return kv::row_of(c, K::kGroups ? a.pre.seq_of(s) : s); };
-  auto first = [&](int s) { return row_of(s) * group / RT + s; };
-  const int lo = last_upto(c.nseq, first, tile);
-  if (lo < 0) return t;
-  t.row0 = row_of(lo);
-  const int64_t tokens = row_of(lo + 1) - t.row0;
-  t.r0 = (tile - first(lo)) * RT;
+  Tile t = kNoTile;
+  constexpr bool kParts = K::kRest;
+  const bool near = c.nseq < 64 && (!K::kGroups || a.pre.nseq < 64) && (!kParts || a.pre.n < 64);
+  int lo;
+  int64_t tokens, at;
+  if (near) {
+    const int l = threadIdx.x & 63;
+    int row = (int)kv::row_of(c, min(l, K::kGroups ? a.pre.nseq : c.nseq));
+    const int len = (int)kv::length_of(c, min(l, c.nseq - 1));
+    int part_at = 0, part_len = 0;
+    if (kParts) {
+      part_at = a.pre.seq_of(min(l, a.pre.n));
+      part_len = (int)length_of(c, a.pre, min(l, a.pre.n - 1));
+    }
+    if (K::kGroups) row = __shfl(row, a.pre.seq_of(min(l, c.nseq)));
+    const uint64_t upto = __ballot(l < c.nseq && (int64_t)row * group / RT + l <= tile);
+    if (!upto) return t;
+    lo = uniform(63 - __builtin_clzll(upto));
+    t.row0 = __builtin_amdgcn_readlane(row, lo);
+    tokens = __builtin_amdgcn_readlane(row, lo + 1) - t.row0;
+    t.len = __builtin_amdgcn_readlane(len, lo);
+    if (kParts) {
+      const uint64_t begun = __ballot(l < a.pre.n && part_at <= lo);
+      const int g = begun ? uniform(63 - __builtin_clzll(begun)) : -1;
+      if (g >= 0 && lo < __builtin_amdgcn_readlane(part_at, g + 1)) {
+        t.part = g;
+        t.part_len = __builtin_amdgcn_readlane(part_len, g);
+      }
+    }
+    if (K::kGroups) {
+      const int n = __shfl_down(row, 1) - row;
+      int tiles = l < c.nseq && n > 0 ? (int)(((int64_t)n * group + RT - 1) / RT) : 0;
+#pragma unroll
+      for (int o = 32; o; o >>= 1) tiles += __shfl_xor(tiles, o);
+      t.tiles = uniform(tiles);
+    }
+    at = t.row0 * group / RT + lo;
+  } else {
+    auto row_of = [&](int s) { return kv::row_of(c, K::kGroups ? a.pre.seq_of(s) : s); };
+    auto first = [&](int s) { return row_of(s) * group / RT + s; };
+    lo = last_upto(c.nseq, first, tile);
+    if (lo < 0) return t;
+    t.row0 = row_of(lo);
+    tokens = row_of(lo + 1) - t.row0;
+    t.len = (int)kv::length_of(c, lo);
+    if (kParts) {
+      t.part = part_of(a.pre, lo);
+      if (t.part >= 0) t.part_len = (int)length_of(c, a.pre, t.part);
+    }
+    at = first(lo);
+  }
+  t.r0 = (tile - at) * RT;
   t.rows = tokens > 0 ? tokens * group : 0;
-  t.len = (int)kv::length_of(c, lo);
   t.first = K::kFree ? 0 : t.len - (int)(tokens > 0 ? tokens : 0);
   if (t.r0 < t.rows) t.s = lo;
   return t;
@@ -138,7 +203,9 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int64_t tile) {
 
 // All rows of sequence s.
 __device__ __forceinline__ Tile rows_of(const Args& a, int s) {
-  Tile t{s, 0, 0, kv::row_of(a.c, s), 0, 0};
+  Tile t = kNoTile;
+  t.s = s;
+  t.row0 = kv::row_of(a.c, s);
   const int64_t tokens = kv::row_of(a.c, s + 1) - t.row0;
   t.rows = tokens > 0 ? tokens * a.group : 0;
   t.len = (int)kv::length_of(a.c, s);
@@ -146,16 +213,47 @@ __device__ __forceinline__ Tile rows_of(const Args& a, int s) {
   return t;
 }
 
-// The sequence of row t, -1: none.
-__device__ __forceinline__ int seq_at(const View& c, int64_t t) {
-  const int s = last_upto(c.nseq, [&](int i) { return kv::row_of(c, i); }, t);
-  return s >= 0 && t < kv::row_of(c, s + 1) ? s : -1;
+// Row `row` of the call: its sequence (-1: none), that one's table row, length and shared part, and
+// in `first` the row's own position.
+__device__ __forceinline__ Tile find_row(const Args& a, int64_t row) {
+  const View& c = a.c;
+  Tile t = kNoTile;
+  int s, end;
+  if (c.nseq < 64 && a.pre.n < 64) {  // as in find_tile
+    const int l = threadIdx.x & 63;
+    const int at = (int)kv::row_of(c, min(l, c.nseq));
+    const int len = (int)kv::length_of(c, min(l, c.nseq - 1));
+    const int part_at = a.pre.seq_of(min(l, a.pre.n));
+    const int part_len = (int)length_of(c, a.pre, min(l, a.pre.n - 1));
+    const uint64_t upto = __ballot(l < c.nseq && at <= row);
+    if (!upto) return t;
+    s = uniform(63 - __builtin_clzll(upto));
+    end = __builtin_amdgcn_readlane(at, s + 1);
+    t.len = __builtin_amdgcn_readlane(len, s);
+    const uint64_t begun = __ballot(l < a.pre.n && part_at <= s);
+    const int g = begun ? uniform(63 - __builtin_clzll(begun)) : -1;
+    if (g >= 0 && s < __builtin_amdgcn_readlane(part_at, g + 1)) {
+      t.part = g;
+      t.part_len = __builtin_amdgcn_readlane(part_len, g);
+    }
+  } else {
+    s = last_upto(c.nseq, [&](int i) { return kv::row_of(c, i); }, row);
+    if (s < 0) return t;
+    end = (int)kv::row_of(c, s + 1);
+    t.len = (int)kv::length_of(c, s);
+    t.part = part_of(a.pre, s);
+    if (t.part >= 0) t.part_len = (int)length_of(c, a.pre, t.part);
+  }
+  if (row >= end) return t;
+  t.s = s;
+  t.first = t.len - (int)(end - row);
+  return t;
 }
 
 // Keys that row r sees (0: it has no position, or is none).
 __device__ __forceinline__ int keys_of(const Tile& t, int64_t r, int group, int causal) {
   if (r >= t.rows) return 0;
-  const int p = t.first + (int)(r / group);
+  const int p = t.first + token_of(r, group);
   return p < 0 ? 0 : causal ? (p + 1 < t.len ? p + 1 : t.len) : t.len;
 }
 // And the rows [r, r + n) at most: the last one.
@@ -239,7 +337,7 @@ __device__ __forceinline__ void load_q(const Args& a, const Tile& t, int h, int6
                                        float x[4][8]) {
   const bool ok = r < t.rows;
   const int64_t rr = ok ? r : 0;
-  const int64_t tok = rr / a.group;
+  const int64_t tok = token_of(rr, a.group);
   const float* p =
       a.q + (t.row0 + tok) * a.ldq + (int64_t)(h * a.group + (int)(rr - tok * a.group)) * kHd;
 #pragma unroll
@@ -301,36 +399,29 @@ __device__ __forceinline__ KeyTerms key_terms(float ks, float vs, bool ok, float
   k.f = !ok ? 0.f : fabsf(vs) >= top ? __builtin_nanf("") : __builtin_ldexpf(vs, kWeight - e - e0);
   return k;
 }
-// E0: the exponent of the sequence's first value scale; from kLeast on, so that a
-// first value of next to nothing leaves those after it their range. pages: the
-// sequence's.
-__device__ __forceinline__ int first_exp(const View& c, const int32_t* pages, int64_t len, int h) {
-  if (len <= 0) return 0;
-  const int64_t page = pages[0];
-  const float v =
-      page >= 0 && page < c.pages ? c.vs[(page * c.kv_heads + h) << c.page_log2] : 0.f;
+// E0: the exponent of the sequence's first value scale (0: no value); from kLeast on, so that a
+// first value of next to nothing leaves those after it their range.
+__device__ __forceinline__ int exp_of(float v) {
   const int e = v != 0.f ? __builtin_amdgcn_frexp_expf(v) : 0;
   return e < kLeast ? kLeast : e;
 }
-__device__ __forceinline__ int first_exp(const View& c, const Tile& t, int h) {
-  return first_exp(c, c.table + t.s * c.max_pages, t.len, h);
+// That scale: of the token that the first of `pages` begins with, 0 where there is none.
+__device__ __forceinline__ float first_value(const View& c, const int32_t* pages, int64_t len, int h) {
+  if (len <= 0) return 0.f;
+  const int64_t page = *scalar_ptr(pages);
+  return page >= 0 && page < c.pages ? *scalar_ptr(c.vs + ((page * c.kv_heads + h) << c.page_log2)) : 0.f;
 }
-
-// The shared part that sequence s begins with, -1: none.
-__device__ __forceinline__ int part_of(const kv::Shared& p, int s) {
-  const int g = last_upto(p.n, [&](int i) { return (int64_t)p.seq_of(i); }, s);
-  return g >= 0 && s < p.seq_of(g + 1) ? g : -1;
+// Of a tile's sequence: behind a shared part that part's first value, so that both passes' sums
+// have the same units.
+template <class K>
+__device__ __forceinline__ float first_value(const Args& a, const Tile& t, int h) {
+  if (K::kRest && t.part_len > 0)
+    return first_value(a.c, a.pre.table + t.part * a.pre.max_pages, t.part_len, h);
+  return first_value(a.c, a.c.table + t.s * a.c.max_pages, t.len, h);
 }
-__device__ __forceinline__ int64_t length_of(const View& c, const kv::Shared& p, int g) {
-  const int64_t n = p.lens[g], most = p.max_pages << c.page_log2;
-  return n < 0 ? 0 : n > most ? most : n;
-}
-// E0 of sequence s behind its part g of the shared ones: the first value of all, so that
-// both passes' sums have the same units.
-__device__ __forceinline__ int first_exp(const Args& a, int s, int g, int h) {
-  const int64_t n = g >= 0 ? length_of(a.c, a.pre, g) : 0;
-  return n > 0 ? first_exp(a.c, a.pre.table + g * a.pre.max_pages, n, h)
-               : first_exp(a.c, a.c.table + s * a.c.max_pages, kv::length_of(a.c, s), h);
+template <class K>
+__device__ __forceinline__ int first_exp(const Args& a, const Tile& t, int h) {
+  return exp_of(first_value<K>(a, t, h));
 }
 
 // One query's softmax state in a lane: the reference m (the maximum of t, or up

@@ -42,22 +42,30 @@ namespace {
 
 using namespace kvattn;
 
-template <class K>
-__device__ __forceinline__ int e0_of(const Args& a, const Tile& t, int h) {
-  if constexpr (std::is_same<K, Rest>::value)
-    return first_exp(a, t.s, part_of(a.pre, t.s), h);
-  else
-    return first_exp(a.c, t, h);
-}
-
 // Where a share of a tile's row keeps its sums (th: the workgroup's tile and head).
 template <class K>
 __device__ __forceinline__ int64_t share_at(const Args& a, const Tile& t, int64_t th, int h, int z,
                                             int rows, int row) {
   if (!K::kByRow) return (th * a.splits + z) * rows + row;
-  const int64_t r = t.r0 + row, tok = r / a.group;
+  const int64_t r = t.r0 + row, tok = token_of(r, a.group);
   const int64_t at = (t.row0 + tok) * (a.nh * a.group) + (h - a.h0) * a.group + (r - tok * a.group);
   return at * a.shares + a.z0 + z;
+}
+
+// Shares that a tile's keys are cut into. A shared part's rows are known here alone: as many
+// shares as make a.want workgroups of all parts' tiles. Where each has its own place among a
+// row's (kByRow), a share has a.least keys at least; one that is left out says so.
+template <class K>
+__device__ __forceinline__ int shares_of(const Args& a, const Tile& t, int keys) {
+  if (!K::kByRow) return a.splits;
+  int n = a.splits;
+  if (K::kGroups && t.tiles > 0) n = min(n, max(1, (int)((uint32_t)a.want / (uint32_t)(t.tiles * a.nh))));
+  return min(n, max(1, (keys + a.least - 1) / a.least));
+}
+template <class K>
+__device__ __forceinline__ void leave_out(const Args& a, const Tile& t, int64_t th, int h, int z, int rows) {
+  if ((int)threadIdx.x < rows && t.r0 + threadIdx.x < t.rows)
+    a.part_ml[share_at<K>(a, t, th, h, z, rows, threadIdx.x)] = float2{-INFINITY, 0.f};
 }
 
 // ---- few rows: a tile of 16, the workgroup's waves share out the keys ----
@@ -75,34 +83,25 @@ constexpr int kFewWaves = kvplan::kFewWaves;
 constexpr int kFewStride = kHd + 4;  // LDS row of a merged sum (bank spread)
 
 template <class K>
-__global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) {
+__device__ __forceinline__ void few_rows(const Args& a, unsigned wg) {
   const View& c = a.c;
   const int nh = K::kByRow ? a.nh : c.kv_heads;
   const int w = uniform((int)threadIdx.x >> 6), l = threadIdx.x & 63, r16 = l & 15, g = l >> 4;
-  const int z = (int)(blockIdx.x % a.splits);
-  const int64_t th = blockIdx.x / a.splits;
-  const int h = (K::kByRow ? a.h0 : 0) + (int)(th % nh);
-  const Tile t = find_tile<K, kFewRows>(a, a.tile0 + th / nh);
+  const int z = (int)(wg % (unsigned)a.splits);
+  const unsigned th = wg / (unsigned)a.splits;
+  const int h = (K::kByRow ? a.h0 : 0) + (int)(th % (unsigned)nh);
+  const Tile t = find_tile<K, kFewRows>(a, a.tile0 + th / (unsigned)nh);
   if (t.s < 0) return;
 
-  float x[4][8];
-  load_q(a, t, h, t.r0 + r16, g, x);
-  bool bad;
-  const int qe = q_exp(clean(x, bad));
-  v8h qh[4], ql[4];
-#pragma unroll
-  for (int kb = 0; kb < 4; kb++) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[kb][i] = __builtin_ldexpf(x[kb][i], qe);
-    parts8(x[kb], qh[kb], ql[kb]);
-  }
-  const float qk = __builtin_ldexpf(a.scale2, -qe);
-  const int e0 = e0_of<K>(a, t, h);
-
   const int keys = keys_of_rows(t, t.r0, kFewRows, a.group, a.causal);
+  const int splits = shares_of<K>(a, t, keys);
+  if (K::kByRow && z >= splits) {
+    leave_out<K>(a, t, th, h, z, kFewRows);
+    return;
+  }
   const int blocks = (keys + 31) / 32;
-  const int b0 = (int)((int64_t)blocks * z / a.splits);
-  const int b1 = (int)((int64_t)blocks * (z + 1) / a.splits);
+  const int b0 = (int)((int64_t)blocks * z / splits);
+  const int b1 = (int)((int64_t)blocks * (z + 1) / splits);
   // what this lane's row sees, and what every row of the tile does
   const int mine = keys_of(t, t.r0 + r16, a.group, a.causal);
   const int all = keys_of(t, t.r0, a.group, a.causal);  // the first row
@@ -112,17 +111,19 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 #pragma unroll
   for (int e = 0; e < 8; e++) acc[e] = v4f{0.f, 0.f, 0.f, 0.f};
 
+  __shared__ v4f terms[kFewWaves][32];
   float* row_logits = nullptr;  // of the lane's keys 4 g .. of a tile
   if (K::kLogits && t.r0 + r16 < t.rows) {
-    const int64_t tok = (t.r0 + r16) / a.group;
+    const int64_t tok = token_of(t.r0 + r16, a.group);
     const int head = h * a.group + (int)(t.r0 + r16 - tok * a.group);
     row_logits = a.logits + ((t.row0 + tok) * a.heads + head) * a.keys + 4 * g;
   }
-  // A block's codes and scales, loaded one block ahead, its pages another one.
+  // A block's codes and scales, loaded one block ahead, its pages another one. The first ones
+  // and the first value's scale are on their way before the queries are made ready.
   struct Raw {
     uint4 k[2][2];
     uint2 v[2][4];
-    v4f ks[2], vs[2];
+    float ks, vs;  // of key l % 32
     bool there[2];
   };
   // Every load is made whether or not there is a block (of the first page then): behind a branch
@@ -131,6 +132,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
   const int last = (keys - 1) >> c.page_log2;
   auto page_at = [&](int b, int kt) { return table[min((b * 32 + 16 * kt) >> c.page_log2, last)]; };
   auto load = [&](int b, const int pages[2], Raw& r) {
+    int64_t at_of[2];
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
       const int p = b * 32 + 16 * kt;
@@ -143,11 +145,45 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 #pragma unroll
       for (int i = 0; i < 4; i++)
         r.v[kt][i] = *reinterpret_cast<const uint2*>(c.v + (at + 4 * g + i) * kHd + 8 * r16);
-      r.ks[kt] = *reinterpret_cast<const v4f_any*>(c.ks + at + 4 * g);
-      r.vs[kt] = *reinterpret_cast<const v4f_any*>(c.vs + at + 4 * g);
+      at_of[kt] = at;
     }
+    const int64_t mine_at = (l & 16 ? at_of[1] : at_of[0]) + r16;
+    r.ks = c.ks[mine_at];
+    r.vs = c.vs[mine_at];
   };
+  // Two blocks in turn, each loaded while the other is at work (a copy from one to the other
+  // would wait for its loads).
+  Raw raw[2];
+  int pages[2];
+  auto look = [&](int b) { pages[0] = page_at(b, 0), pages[1] = page_at(b, 1); };
+  int b = b0 + w;
+  if (b < b1) look(b);
+  float x[4][8];
+  load_q(a, t, h, t.r0 + r16, g, x);
+  const float v0 = first_value<K>(a, t, h);
+  if (b < b1) {
+    load(b, pages, raw[0]);
+    look(b + kFewWaves);
+  }
+  bool bad;
+  const int qe = q_exp(clean(x, bad));
+  v8h qh[4], ql[4];
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[kb][i] = __builtin_ldexpf(x[kb][i], qe);
+    parts8(x[kb], qh[kb], ql[kb]);
+  }
+  const float qk = __builtin_ldexpf(a.scale2, -qe);
+  const int e0 = exp_of(v0);
+
   auto block = [&](int b, const Raw& cur) {
+    // Keys' terms: one key a lane, handed round in LDS (each lane for the eight keys that it needs
+    // was a quarter of a block's operations).
+    const KeyTerms own = key_terms(
+        cur.ks, cur.vs, (l & 16 ? cur.there[1] : cur.there[0]) && b * 32 + (l & 31) < t.len, 1.f, e0);
+    terms[w][l & 31] = v4f{own.c, own.e, own.w, own.f};
+    const bool far = __any(own.e < kNear);
     v4f s[2], kc[2], ke[2], kw[2], kf[2];
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
@@ -161,15 +197,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
       }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const KeyTerms k = key_terms(cur.ks[kt][i], cur.vs[kt][i],
-                                     cur.there[kt] && b * 32 + 16 * kt + 4 * g + i < t.len, qk, e0);
-        kc[kt][i] = k.c, ke[kt][i] = k.e, kw[kt][i] = k.w, kf[kt][i] = k.f;
+        const v4f k = terms[w][16 * kt + 4 * g + i];
+        kc[kt][i] = k[0] * qk, ke[kt][i] = k[1], kw[kt][i] = k[2], kf[kt][i] = k[3];
       }
     }
     v8h ph, pl;
-    float least = ke[0][0];
-#pragma unroll
-    for (int j = 1; j < 8; j++) least = fminf(least, ke[j >> 2][j & 3]);
     auto softmax = [&](auto mask, auto seen) {
       constexpr bool kMask = decltype(mask)::value;
       const float mx = logits<kMask>(s, kc, ke, seen);
@@ -179,7 +211,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
           *reinterpret_cast<v4f*>(row_logits + b * 32 + 16 * kt) = s[kt];
       }
       if (__any(rises(st, mx))) raise(st, mx, acc);
-      if (__any(least < kNear)) add_faint(s, ke, st);
+      if (far) add_faint(s, ke, st);
       weights<kMask>(s, kw, kf, st, seen, ph, pl);
     };
     if (b * 32 + 32 <= all && cur.there[0] && cur.there[1]) {
@@ -215,17 +247,6 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
     tile_e(std::integral_constant<int, 2>{}, vb, acc[6]);
     tile_e(std::integral_constant<int, 3>{}, vb, acc[7]);
   };
-  // Two blocks in turn, each loaded while the other is at work (a copy from one to the other
-  // would wait for its loads).
-  Raw raw[2];
-  int pages[2];
-  auto look = [&](int b) { pages[0] = page_at(b, 0), pages[1] = page_at(b, 1); };
-  int b = b0 + w;
-  if (b < b1) {
-    look(b);
-    load(b, pages, raw[0]);
-    look(b + kFewWaves);
-  }
   for (; b < b1; b += 2 * kFewWaves) {
     load(b + kFewWaves, pages, raw[1]);
     look(b + 2 * kFewWaves);
@@ -269,7 +290,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
     const float f = den == 0.f ? 0.f : __builtin_ldexpf(1.f, e0 - kWeight) / den;
 #pragma unroll
     for (int d = 0; d < kPer; d++) o[d] = o[d] * f;
-    const int64_t tok = r / a.group;
+    const int64_t tok = token_of(r, a.group);
     const int head = h * a.group + (int)(r - tok * a.group);
     dst = a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd + d0;
     if (K::kStats && d0 == 0) a.stats[(t.row0 + tok) * a.heads + head] = stat_of(m, den);
@@ -281,6 +302,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) 
 #pragma unroll
   for (int d = 0; d < kPer; d += 4)
     *reinterpret_cast<v4f*>(dst + d) = v4f{o[d], o[d + 1], o[d + 2], o[d + 3]};
+}
+template <class K>
+__global__ void __launch_bounds__(64 * kFewWaves, 2) kv_attn_few_kernel(Args a) {
+  few_rows<K>(a, blockIdx.x);
 }
 
 // ---- joining the shares of cut keys: W waves a row ----
@@ -350,14 +375,15 @@ __device__ __forceinline__ void join_tiles(const Args& a) {
   const int row = (int)(i % RT), h = (int)(th % a.c.kv_heads);
   const Tile t = find_tile<K, RT>(a, a.tile0 + th / a.c.kv_heads);
   if (t.s < 0 || t.r0 + row >= t.rows) return;  // with W = 4 for the whole workgroup
+  const float v0 = first_value<K>(a, t, h);
   // lane z holds share z's maximum and denominator (splits <= 64)
   const int64_t at = th * a.splits * RT + row;
   const float2 ml = l < a.splits ? a.part_ml[at + (int64_t)l * RT] : float2{-INFINITY, 0.f};
   float m, den, o0, o1;
   if (!join<W>(a, ml, at, RT, a.splits, w, m, den, o0, o1)) return;
   const float f =
-      den == 0.f ? 0.f : __builtin_ldexpf(1.f, first_exp(a.c, t, h) - kWeight) / den;
-  const int64_t r = t.r0 + row, tok = r / a.group;
+      den == 0.f ? 0.f : __builtin_ldexpf(1.f, exp_of(v0) - kWeight) / den;
+  const int64_t r = t.r0 + row, tok = token_of(r, a.group);
   const int head = h * a.group + (int)(r - tok * a.group);
   reinterpret_cast<float2*>(a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd)[l] =
       float2{o0 * f, o1 * f};
@@ -395,7 +421,7 @@ __global__ void __launch_bounds__(256) kv_counts_kernel(Args a, float* __restric
   const int sh = (int)(i / across);
   const int h = sh % c.kv_heads, s = sh / c.kv_heads;
   const Tile t = rows_of(a, s);
-  const int e0 = first_exp(c, t, h);
+  const int e0 = first_exp<Own>(a, t, h);
   const int64_t tile0 = t.row0 * a.group / kFewRows + s;  // numbers as in find_tile
   for (int k0 = (int)(i % across) * kCountKeys; k0 < t.len; k0 += across * kCountKeys) {
     const int p = k0 + 4 * tid;
@@ -454,28 +480,85 @@ __global__ void __launch_bounds__(256) kv_counts_kernel(Args a, float* __restric
   }
 }
 
-// The same for rows behind a shared part: shares z < z0 are its, the others the row's own.
+// The same for rows behind a shared part, whose shares lie side by side: z < z0 are the part's, the
+// others the row's own, up to 128 of them, two a lane. Those that were left out are not read.
 template <int W>
 __global__ void __launch_bounds__(256) kv_attn_join_rows_kernel(Args a, int64_t i0) {
   const int l = threadIdx.x & 63, w = uniform((int)threadIdx.x >> 6);
   const int64_t i = i0 + (int64_t)blockIdx.x * (4 / W) + w / W;
   const int per = a.nh * a.group;
-  const int64_t t = i / per;
-  if (t >= a.c.T) return;
-  const int s = seq_at(a.c, t);
-  if (s < 0) return;
-  const int g = part_of(a.pre, s);
-  const int head = a.h0 * a.group + (int)(i - t * per);
-  // a sequence without a shared part has none of its shares, a row without a position none
-  const bool placed = kv::length_of(a.c, s) - kv::row_of(a.c, s + 1) + t >= 0;
-  const int z0 = g < 0 ? a.z0 : 0, n = placed ? a.shares - z0 : 0;
-  const int64_t at = i * a.shares + z0;
-  const float2 ml = l < n ? a.part_ml[at + l] : float2{-INFINITY, 0.f};
-  float m, den, o0, o1;
-  if (!join<W>(a, ml, at, 1, n, w, m, den, o0, o1)) return;
-  const float f = den == 0.f ? 0.f
-                             : __builtin_ldexpf(1.f, first_exp(a, s, g, head / a.group) - kWeight) / den;
-  reinterpret_cast<float2*>(a.out + t * a.ldo + (int64_t)head * kHd)[l] = float2{o0 * f, o1 * f};
+  const int64_t row = i / per;
+  if (row >= a.c.T) return;
+  const int head = (int)(i - row * per);
+  const int64_t at = i * a.shares;
+  float2 ml[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+    ml[j] = l + 64 * j < a.shares ? a.part_ml[at + l + 64 * j] : float2{-INFINITY, 0.f};
+  const Tile t = find_row(a, row);
+  if (t.s < 0) return;
+  const float v0 = first_value<Rest>(a, t, a.h0 + head / a.group);
+  // a row without a position sees nothing; a sequence without a shared part has none of its shares
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+    if (t.first < 0 || (t.part < 0 && l + 64 * j < a.z0)) ml[j].x = -INFINITY;
+  float m = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float own[2], den = 0.f;
+  uint64_t live[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    live[j] = __ballot(ml[j].x != -INFINITY);
+    own[j] = __builtin_amdgcn_exp2f(ml[j].x - ref);
+    den += ml[j].x != -INFINITY ? times_exp2(ml[j].y, ml[j].x - ref) : 0.f;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);
+  const float2* part = reinterpret_cast<const float2*>(a.part + at * kHd) + l;
+  float o0 = 0.f, o1 = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    // wave w of the row takes every W-th of the live ones, kJoin of them at a time
+    uint64_t rest = live[j];
+    while (rest) {
+      float2 v[kJoin];
+      int z[kJoin];
+#pragma unroll
+      for (int k = 0; k < kJoin; k++) {
+        z[k] = -1;
+#pragma unroll
+        for (int u = 0; u < W; u++) {
+          const int n = rest ? __builtin_ctzll(rest) : -1;
+          rest &= rest - 1;
+          if (u == w % W) z[k] = n;
+        }
+        if (z[k] >= 0) v[k] = part[(int64_t)(z[k] + 64 * j) * 64];
+      }
+#pragma unroll
+      for (int k = 0; k < kJoin; k++)
+        if (z[k] >= 0) {
+          const float f = __shfl(own[j], z[k]);
+          o0 = __builtin_fmaf(v[k].x, f, o0);
+          o1 = __builtin_fmaf(v[k].y, f, o1);
+        }
+    }
+  }
+  if (W > 1) {
+    __shared__ float2 sums[W][64];
+    sums[w][l] = float2{o0, o1};
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int k = 1; k < W; k++) {
+      o0 += sums[k][l].x;
+      o1 += sums[k][l].y;
+    }
+  }
+  const float f = den == 0.f ? 0.f : __builtin_ldexpf(1.f, exp_of(v0) - kWeight) / den;
+  reinterpret_cast<float2*>(a.out + row * a.ldo + (int64_t)(a.h0 * a.group + head) * kHd)[l] =
+      float2{o0 * f, o1 * f};
 }
 
 // ---- chunks: NW waves of 16 QT rows over the same keys ----
@@ -516,7 +599,7 @@ struct Block {
 };
 
 template <class K, int NW, int QT>
-__global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
+__device__ __forceinline__ void chunk_rows(const Args& a, unsigned wg) {
   constexpr int kRows = 16 * QT * NW;
   using Blk = Block<NW>;
   constexpr int KB = Blk::kKeys;
@@ -524,14 +607,19 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   const View& c = a.c;
   const int nh = K::kByRow ? a.nh : c.kv_heads;
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, r16 = l & 15, g = l >> 4;
-  // causal: the last rows, which see most, first (4099 rows over themselves, 24 heads on 8: 329 us the other way round, 252 so)
-  const unsigned block = a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const int z = (int)(block % a.splits);
-  const int64_t th = block / a.splits;
-  const int h = (K::kByRow ? a.h0 : 0) + (int)(th % nh);
-  const Tile t = find_tile<K, kRows>(a, a.tile0 + th / nh);
+  const int z = (int)(wg % (unsigned)a.splits);
+  const unsigned th = wg / (unsigned)a.splits;
+  const int h = (K::kByRow ? a.h0 : 0) + (int)(th % (unsigned)nh);
+  const Tile t = find_tile<K, kRows>(a, a.tile0 + th / (unsigned)nh);
   if (t.s < 0) return;
 
+  const int keys = keys_of_rows(t, t.r0, kRows, a.group, a.causal);
+  const int splits = shares_of<K>(a, t, keys);
+  if (K::kByRow && z >= splits) {
+    leave_out<K>(a, t, th, h, z, kRows);
+    return;
+  }
+  const float v0 = first_value<K>(a, t, h);
   v8h qh[QT][4], ql[QT][4];
   int mine[QT];
   float qk[QT];
@@ -551,11 +639,10 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     }
     qk[qt] = __builtin_ldexpf(a.scale2, -qe);
   }
-  const int e0 = e0_of<K>(a, t, h);
-  const int keys = keys_of_rows(t, t.r0, kRows, a.group, a.causal);
+  const int e0 = exp_of(v0);
   const int blocks = (keys + KB - 1) / KB;
-  const int b0 = (int)((int64_t)blocks * z / a.splits);
-  const int b1 = (int)((int64_t)blocks * (z + 1) / a.splits);
+  const int b0 = (int)((int64_t)blocks * z / splits);
+  const int b1 = (int)((int64_t)blocks * (z + 1) / splits);
   // keys that the wave's rows see at most, and all of them see (the first row)
   const int64_t wr = t.r0 + w * QT * 16;
   const int wmost = wr < t.rows ? keys_of_rows(t, wr, QT * 16, a.group, a.causal) : 0;
@@ -779,7 +866,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
     float* dst;
     if (!K::kByRow && a.splits == 1) {
       f = den == 0.f ? 0.f : __builtin_ldexpf(1.f, e0 - kWeight) / den;
-      const int64_t tok = r / a.group;
+      const int64_t tok = token_of(r, a.group);
       const int head = h * a.group + (int)(r - tok * a.group);
       dst = a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd + 32 * g;
       if (K::kStats && g == 0)
@@ -799,6 +886,30 @@ __global__ void __launch_bounds__(64 * NW) kv_attn_chunk_kernel(Args a) {
   }
 }
 
+template <class K, int NW, int QT>
+__global__ void __launch_bounds__(64 * NW, NW == 4 && QT == 2 ? 2 : 1) kv_attn_chunk_kernel(Args a) {
+  // causal: the last rows, which see most, first (4099 rows over themselves, 24 heads on 8: 329 us
+  // the other way round, 252 so)
+  chunk_rows<K, NW, QT>(a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+template <class K, int ROWS>
+__device__ __forceinline__ void tile_rows(const Args& a, unsigned wg) {
+  if constexpr (ROWS == kFewRows)
+    few_rows<K>(a, wg);
+  else
+    chunk_rows<K, 4, ROWS / 64>(a, wg);
+}
+// Shared parts and own keys in one launch, the parts' `shared` workgroups first: the own keys'
+// are short and fill what those leave.
+template <int PR, int OR>
+__global__ void __launch_bounds__(256, 2) kv_attn_shared_kernel(Args pre, Args own, unsigned shared) {
+  if (blockIdx.x < shared)
+    tile_rows<Prefix, PR>(pre, blockIdx.x);
+  else
+    tile_rows<Rest, OR>(own, blockIdx.x - shared);
+}
+
 // Workgroups for n tiles (from a.tile0 on) of nh heads.
 template <class K>
 hipError_t launch_tiles(const Args& a, const kvplan::Plan& p, int64_t n, int nh, hipStream_t s) {
@@ -807,6 +918,8 @@ hipError_t launch_tiles(const Args& a, const kvplan::Plan& p, int64_t n, int nh,
     hipLaunchKernelGGL(kv_attn_few_kernel<K>, grid, dim3(64 * kFewWaves), 0, s, a);
   else if (p.rows == 64)
     hipLaunchKernelGGL((kv_attn_chunk_kernel<K, 4, 1>), grid, dim3(256), 0, s, a);
+  else if constexpr (K::kGroups)  // rows of a part are 128 at most
+    hipLaunchKernelGGL((kv_attn_chunk_kernel<K, 4, 2>), grid, dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((kv_attn_chunk_kernel<K, 8, 2>), grid, dim3(512), 0, s, a);
   return hipGetLastError();
@@ -883,9 +996,9 @@ hipError_t launch_kv_counted_few(const View& c, const KvRows& r, const kvplan::P
   hipError_t e;
   for (int64_t tile = 0; tile < p.tiles; tile += p.tiles_per_launch) {
     a.tile0 = tile;
-    if ((e = launch_tiles<Logits>(a, p, std::min(p.tiles_per_launch, p.tiles - tile), c.kv_heads,
-                                  s)) != hipSuccess)
-      return e;
+    const int64_t n = std::min(p.tiles_per_launch, p.tiles - tile) * c.kv_heads * p.splits;
+    hipLaunchKernelGGL(kv_attn_few_kernel<Logits>, dim3((unsigned)n), dim3(64 * kFewWaves), 0, s, a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   // with shares, all tiles are one launch's: so is their join
   a.tile0 = 0;
@@ -902,37 +1015,58 @@ hipError_t launch_kv_counted_few(const View& c, const KvRows& r, const kvplan::P
   return hipGetLastError();
 }
 
-hipError_t launch_kv_shared(const View& c, const kv::Shared& pre, const KvRows& r,
+template <int PR>
+void launch_both(const Args& pre, const Args& own, int own_rows, unsigned shared, unsigned all,
+                 hipStream_t s) {
+  if (own_rows == kFewRows)
+    hipLaunchKernelGGL((kv_attn_shared_kernel<PR, kFewRows>), dim3(all), dim3(256), 0, s, pre, own,
+                       shared);
+  else
+    hipLaunchKernelGGL((kv_attn_shared_kernel<PR, 64>), dim3(all), dim3(256), 0, s, pre, own, shared);
+}
+
+hipError_t launch_kv_shared(const View& c, const kv::Shared& parts, const KvRows& r,
                             const kvplan::SharedPlan& p, void* scratch, hipStream_t s) {
   Args own = args_of(c, r, scratch, p.part_bytes);
-  own.pre = pre;
+  own.pre = parts;
   own.shares = p.pre.splits + p.own.splits;
-  Args shared = own;
-  own.z0 = p.pre.splits, own.splits = p.own.splits;
-  shared.z0 = 0, shared.splits = p.pre.splits, shared.causal = 0;
-  shared.c.lens = pre.lens, shared.c.table = pre.table;
-  shared.c.nseq = pre.n, shared.c.max_pages = pre.max_pages;
+  Args pre = own;
+  own.z0 = p.pre.splits, own.splits = p.own.splits, own.least = p.own_least;
+  pre.z0 = 0, pre.splits = p.pre.splits, pre.least = p.pre_least, pre.want = p.want, pre.causal = 0;
+  pre.c.lens = parts.lens, pre.c.table = parts.table;
+  pre.c.nseq = parts.n, pre.c.max_pages = parts.max_pages;
   for (int h0 = 0; h0 < c.kv_heads; h0 += p.heads) {
-    own.h0 = shared.h0 = h0;
-    own.nh = shared.nh = std::min(p.heads, c.kv_heads - h0);
+    own.h0 = pre.h0 = h0;
+    own.nh = pre.nh = std::min(p.heads, c.kv_heads - h0);
     hipError_t e;
-    for (int64_t t = 0; t < p.pre.tiles; t += p.pre.tiles_per_launch) {
-      shared.tile0 = t;
-      if ((e = launch_tiles<Prefix>(shared, p.pre, std::min(p.pre.tiles_per_launch, p.pre.tiles - t),
-                                    own.nh, s)) != hipSuccess)
-        return e;
-    }
-    for (int64_t t = 0; t < p.own.tiles; t += p.own.tiles_per_launch) {
-      own.tile0 = t;
-      if ((e = launch_tiles<Rest>(own, p.own, std::min(p.own.tiles_per_launch, p.own.tiles - t),
-                                  own.nh, s)) != hipSuccess)
-        return e;
+    if (p.own.rows <= 64 && p.pre.tiles <= p.pre.tiles_per_launch && p.own.tiles <= p.own.tiles_per_launch) {
+      own.tile0 = pre.tile0 = 0;
+      const unsigned shared = (unsigned)(p.pre.tiles * own.nh * p.pre.splits);
+      const unsigned all = shared + (unsigned)(p.own.tiles * own.nh * p.own.splits);
+      if (p.pre.rows == kFewRows)
+        launch_both<kFewRows>(pre, own, p.own.rows, shared, all, s);
+      else if (p.pre.rows == 64)
+        launch_both<64>(pre, own, p.own.rows, shared, all, s);
+      else
+        launch_both<128>(pre, own, p.own.rows, shared, all, s);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    } else {
+      for (int64_t t = 0; t < p.pre.tiles; t += p.pre.tiles_per_launch) {
+        pre.tile0 = t;
+        e = launch_tiles<Prefix>(pre, p.pre, std::min(p.pre.tiles_per_launch, p.pre.tiles - t), own.nh, s);
+        if (e != hipSuccess) return e;
+      }
+      for (int64_t t = 0; t < p.own.tiles; t += p.own.tiles_per_launch) {
+        own.tile0 = t;
+        e = launch_tiles<Rest>(own, p.own, std::min(p.own.tiles_per_launch, p.own.tiles - t), own.nh, s);
+        if (e != hipSuccess) return e;
+      }
     }
     // rows a launch: a grid's threads are a 32-bit number
     const int64_t rows = c.T * own.nh * own.group, most = int64_t(1) << 22;
     for (int64_t i = 0; i < rows; i += most) {
       const int64_t n = std::min(most, rows - i);
-      if (own.shares > kJoin)
+      if (own.shares > 2 * kJoin)
         hipLaunchKernelGGL((kv_attn_join_rows_kernel<4>), dim3((unsigned)n), dim3(256), 0, s, own, i);
       else
         hipLaunchKernelGGL((kv_attn_join_rows_kernel<1>), dim3((unsigned)ceil_div(n, 4)), dim3(256),

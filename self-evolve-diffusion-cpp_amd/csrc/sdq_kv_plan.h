@@ -25,7 +25,7 @@ struct Plan {
 
 // T rows of nseq sequences, group query heads to each of kv_heads cached ones,
 // most: the keys a sequence can have.
-inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count) {
+inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count, int tall = 0) {
   Plan p{};
   const int64_t rows = T * group;
   // Rows of a sequence, on average: only their sum is known here. Any choice is
@@ -35,6 +35,7 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   // rows 30 and 39, 48 rows 38 and 40, 72 rows 42 and 41, 144 rows 68 and 49.
   const int64_t mean = (rows + nseq - 1) / nseq;
   p.rows = mean <= 32 ? kFewRows : mean <= 128 ? 64 : 256;
+  if (p.rows == 256 && tall) p.rows = tall;
   // Numbers of tiles: rows / height and one a sequence (csrc/sdq_kv_attn.hip); those that
   // hold one are at most the sum of ceil(rows_s / height) over the sequences that have any.
   p.tiles = rows / p.rows + nseq;
@@ -62,29 +63,39 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   return p;
 }
 
-// Attention over shared parts and own keys: both as plan() cuts them, their shares' sums one
-// beside the other for every row, cached heads at a time that the scratch takes.
+// Attention over shared parts and own keys: their shares' sums one beside the other for every
+// row, cached heads at a time that the scratch takes.
 struct SharedPlan {
   Plan pre, own;
-  int heads;              // cached heads at a time
-  int64_t part_bytes;     // partial sums; maxima and denominators follow
+  int want;                 // workgroups that the parts' shares are to make
+  int pre_least, own_least; // keys of a share
+  int heads;                // cached heads at a time
+  int64_t part_bytes;       // partial sums; maxima and denominators follow
   int64_t scratch_bytes;
 };
+constexpr int kMaxShares = 128, kMaxOwnShares = 16;
 
 // n shared parts of up to most_pre tokens.
 inline SharedPlan shared_plan(int64_t T, int nseq, int n, int group, int kv_heads, int64_t most,
                               int64_t most_pre, int cu_count) {
   SharedPlan p{};
   p.own = plan(T, nseq, group, kv_heads, most, cu_count);
-  p.pre = plan(T, n, group, kv_heads, most_pre, cu_count);
-  p.own.splits = std::min(p.own.splits, 16);  // a wave of the join has a share a lane
-  p.pre.splits = std::min(p.pre.splits, kMaxSplits - 16);
+  p.own.splits = std::min(p.own.splits, kMaxOwnShares);
+  p.pre = plan(T, n, group, kv_heads, most_pre, cu_count, 128);
+  // How many tiles the parts' rows make is known on the device, which cuts their keys into that
+  // many shares that two workgroups a CU are at work; here the most that can be. Rows of no
+  // sequence, and tiles that a part does not fill, leave room for one more than the rows say.
+  p.want = 2 * cu_count;
+  p.pre_least = p.own_least = 256;
+  const int64_t tiles = std::max<int64_t>(1, T * group / p.pre.rows);
+  const int64_t s = std::min<int64_t>(p.want / std::max<int64_t>(tiles * kv_heads, 1), most_pre / p.pre_least);
+  p.pre.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, kMaxShares - kMaxOwnShares));
   const int shares = p.own.splits + p.pre.splits;
   const int64_t head = T * group * shares * (128 + 2) * 4;
   p.heads = (int)std::max<int64_t>(1, std::min<int64_t>(kv_heads, kMaxScratch / std::max<int64_t>(head, 1)));
   for (Plan* q : {&p.pre, &p.own})
     q->tiles_per_launch = std::max<int64_t>(
-        1, ((int64_t(1) << 31) - 1) / ((int64_t)p.heads * q->splits * 512));
+        1, ((int64_t(1) << 30) - 1) / ((int64_t)p.heads * q->splits * 512));
   p.part_bytes = T * group * p.heads * shares * 128 * 4;
   p.scratch_bytes = p.part_bytes / 128 * 130;
   return p;

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
   if (t.rows == 0) return;
   const Cut cut = cut_of(t, wk);
   const int32_t* table = c.table + s * c.max_pages;
-  const int e0 = first_exp(c, t, h);
+  const int e0 = first_exp<Own>(a, t, h);
   const int step_tok = kRows / a.group, step_qh = kRows % a.group;
 
   // Items (block, range) in order, those that no row sees left out: every across-th is ours.

@@ -30,7 +30,7 @@ int main() {
     const int64_t most = i % 50 ? log_size(30) : 0, pre = i % 49 ? log_size(30) : 0;
     const kp::SharedPlan p = kp::shared_plan(T, nseq, n, group, kvh, most, pre, 256);
     const int shares = p.pre.splits + p.own.splits;
-    REQUIRE(p.pre.splits >= 1 && p.own.splits >= 1 && shares <= kp::kMaxSplits);
+    REQUIRE(p.pre.splits >= 1 && p.own.splits >= 1 && shares <= kp::kMaxShares);
     REQUIRE(p.heads >= 1 && p.heads <= kvh);
     REQUIRE(p.part_bytes == T * group * p.heads * shares * 512);
     REQUIRE(p.scratch_bytes >= p.part_bytes + T * group * p.heads * shares * 8);
