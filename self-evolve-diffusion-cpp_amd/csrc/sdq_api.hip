@@ -2565,7 +2565,7 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
   std::unique_lock<std::mutex> turn;
   char* base;
   // the shares' sums, two numbers a row and head, and few rows' logits
-  size_t stats_at = (size_t)round_up(plan.scratch_bytes, 16);
+  const size_t stats_at = (size_t)round_up(plan.scratch_bytes, 16);
   const size_t stats_bytes = (size_t)round_up(T * heads * (int64_t)sizeof(float2), 16);
   const int64_t row = kv_logit_keys(call.view) * 4;
   if (plan.rows == kvplan::kFewRows && row <= kvplan::kMaxScratch / (T * heads) &&
@@ -2583,16 +2583,17 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
   const KvWeightsPlan wplan =
       plan_kv_weights(T, call.view.nseq, heads / c->kv_heads, c->kv_heads,
                       call.view.max_pages << call.view.page_log2, cus);
-  // the shares' sums or, once they are joined, the ranges'
-  stats_at = (size_t)round_up(std::max(plan.scratch_bytes, wplan.scratch_bytes), 16);
-  if ((rc = shared_scratch(call.dev, s, stats_at + stats_bytes, &scratch, &turn))) return rc;
-  float2* stats = reinterpret_cast<float2*>(reinterpret_cast<char*>(scratch) + stats_at);
+  // the shares' sums or, once they are joined, the ranges', and the rows' parts and statistics
+  const size_t kept_at = (size_t)round_up(std::max(plan.scratch_bytes, wplan.scratch_bytes), 16);
+  if ((rc = shared_scratch(call.dev, s, kept_at + (size_t)wplan.kept_bytes, &scratch, &turn)))
+    return rc;
+  void* kept = reinterpret_cast<char*>(scratch) + kept_at;
   rc = timed("kv_attention_weights", s, [&] {
-    return launch_kv_counted(call.view, call.rows, plan, scratch, stats, s);
+    return launch_kv_counted(call.view, call.rows, plan, scratch, wplan, kept, s);
   });
   if (rc) return rc;
   return timed("kv_weights", s, [&] {
-    return launch_kv_weights(call.view, call.rows, stats, weights, wplan, scratch, s);
+    return launch_kv_weights(call.view, call.rows, wplan, kept, weights, scratch, s);
   });
 }
 

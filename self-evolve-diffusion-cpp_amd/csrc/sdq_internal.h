@@ -292,26 +292,27 @@ hipError_t launch_kv_cross(const kv::View& c, const KvRows& r, const kvplan::Pla
                            void* scratch, hipStream_t s);
 hipError_t launch_kv_shared(const kv::View& c, const kv::Shared& pre, const KvRows& r,
                             const kvplan::SharedPlan& plan, void* scratch, hipStream_t s);
-// launch_kv_attn that keeps each row's maximum and reciprocal denominator, and the sums of
-// the weights by key that go by them: w as the cache's scales.
+// launch_kv_attn that keeps in `kept` what the sums of the weights by key go by, and those:
+// w as the cache's scales.
+struct KvWeightsPlan {
+  int across;  // workgroups of a sequence and head
+  int cut;     // its rows may be cut into ranges
+  int seqs;    // sequences at a time
+  int64_t n16;  // numbers of tiles of 16 rows
+  int64_t kept_bytes, scratch_bytes;
+};
+KvWeightsPlan plan_kv_weights(int64_t T, int nseq, int group, int kv_heads, int64_t most,
+                              int cu_count);
 hipError_t launch_kv_counted(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
-                             void* scratch, float2* stats, hipStream_t s);
+                             void* scratch, const KvWeightsPlan& p, void* kept, hipStream_t s);
+hipError_t launch_kv_weights(const kv::View& c, const KvRows& r, const KvWeightsPlan& p, void* kept,
+                             float* w, void* scratch, hipStream_t s);
 // Both at once for few rows (the plan's tiles of 16), whose logits are kept in between:
 // kv_logit_keys floats a row and head.
 int64_t kv_logit_keys(const kv::View& c);
 hipError_t launch_kv_counted_few(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
                                  void* scratch, float2* stats, float* logits, float* sums,
                                  int cu_count, hipStream_t s);
-struct KvWeightsPlan {
-  int across;  // workgroups of a sequence and head
-  int cut;     // its rows may be cut into ranges
-  int seqs;    // sequences at a time
-  int64_t scratch_bytes;
-};
-KvWeightsPlan plan_kv_weights(int64_t T, int nseq, int group, int kv_heads, int64_t most,
-                              int cu_count);
-hipError_t launch_kv_weights(const kv::View& c, const KvRows& r, const float2* stats, float* w,
-                             const KvWeightsPlan& p, void* scratch, hipStream_t s);
 struct KvEvictPlan {
   int seqs;       // sequences at a time
   int chunks;     // of a sequence, 0: it fits a workgroup

@@ -37,10 +37,10 @@ struct Own {  // a sequence's last tokens, its own keys
 struct Cross : Own {  // any rows, all keys of their sequence
   static constexpr bool kFree = true;
 };
-struct Counted : Own {  // each row's maximum and denominator are kept
+struct Counted : Own {  // rows' parts, maxima and denominators are kept
   static constexpr bool kStats = true;
 };
-struct Logits : Counted {  // and the logits
+struct Logits : Own {  // few rows' logits, maxima and denominators
   static constexpr bool kLogits = true;
 };
 struct Prefix : Cross {  // the rows of a run of sequences, the keys that those share
@@ -49,6 +49,12 @@ struct Prefix : Cross {  // the rows of a run of sequences, the keys that those 
 struct Rest : Own {  // own keys behind shared ones
   static constexpr bool kByRow = true, kRest = true;
 };
+
+struct RowInfo {
+  float qk, m, inv;
+  int see;  // keys; 0: the row adds nothing
+};
+constexpr int kQTile = 8192;  // bytes of a tile's parts
 
 struct Args {
   View c;
@@ -63,11 +69,16 @@ struct Args {
   int64_t tile0;     // first tile of this launch
   float* part;       // [tile][kv head][split][row][128], unscaled sums
   float2* part_ml;   // the same without dims: maximum, denominator
-  // kStats: [row][head] maximum and reciprocal denominator (infinity and 0: adds nothing)
+  // kLogits: [row][head] maximum and reciprocal denominator (infinity and 0: adds nothing), and
+  // [row][head][key] logits, `keys` of them a row
   float2* stats;
-  // kLogits: [row][head][key], `keys` of them a row
   float* logits;
   int64_t keys;
+  // kStats: [cached head][tile of 16 rows] their parts, [hi, lo][kb][lane 16 B], and what else
+  // their weights ask for. n16 numbers of tiles, as in find_tile.
+  char* qparts;
+  RowInfo* info;
+  int64_t n16;
   // kByRow: cached heads h0 .. h0 + nh - 1 of this launch, shares z0 .. of `shares`; the
   // sums are [row][head of those][share][128]
   int h0, nh, z0, shares;
@@ -502,6 +513,28 @@ __device__ __forceinline__ void raise(State& st, float mx, v4f acc[8]) {
 // A row's entry of Args::stats.
 __device__ __forceinline__ float2 stat_of(float m, float den) {
   return den > 0.f ? float2{m, 1.f / den} : float2{INFINITY, 0.f};
+}
+
+// The tile of 16 rows that row r (a multiple of 16 or within the tile) of t's sequence is in.
+__device__ __forceinline__ int64_t tile16(const Args& a, const Tile& t, int h, int64_t r) {
+  return h * a.n16 + t.row0 * a.group / 16 + t.s + (r >> 4);
+}
+__device__ __forceinline__ RowInfo info_of(const Args& a, const Tile& t, int64_t r, float qk, float m,
+                                           float den) {
+  const float2 st = stat_of(m, den);
+  const int see = st.y > 0.f ? keys_of(t, r, a.group, a.causal) : 0;
+  return RowInfo{qk, st.x, st.y, see};
+}
+// The wave's 16 rows from r0 on: their parts, as the lanes hold them.
+__device__ __forceinline__ void keep_parts(const Args& a, const Tile& t, int h, int64_t r0,
+                                           const v8h qh[4], const v8h ql[4]) {
+  if (r0 >= t.rows) return;
+  char* p = a.qparts + tile16(a, t, h, r0) * kQTile + (threadIdx.x & 63) * 16;
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++) {
+    *reinterpret_cast<v8h*>(p + 1024 * kb) = qh[kb];
+    *reinterpret_cast<v8h*>(p + 4096 + 1024 * kb) = ql[kb];
+  }
 }
 
 }  // namespace kvattn

@@ -112,6 +112,7 @@ __device__ __forceinline__ void few_rows(const Args& a, unsigned wg) {
   for (int e = 0; e < 8; e++) acc[e] = v4f{0.f, 0.f, 0.f, 0.f};
 
   __shared__ v4f terms[kFewWaves][32];
+  __shared__ float qks[kFewRows];
   float* row_logits = nullptr;  // of the lane's keys 4 g .. of a tile
   if (K::kLogits && t.r0 + r16 < t.rows) {
     const int64_t tok = token_of(t.r0 + r16, a.group);
@@ -176,6 +177,13 @@ __device__ __forceinline__ void few_rows(const Args& a, unsigned wg) {
   }
   const float qk = __builtin_ldexpf(a.scale2, -qe);
   const int e0 = exp_of(v0);
+  if (K::kStats && z == 0 && w == 0) {
+    keep_parts(a, t, h, t.r0, qh, ql);
+    // a row that is none, or whose shares are joined later
+    if (g == 0 && (a.splits > 1 || t.r0 + r16 >= t.rows))
+      a.info[tile16(a, t, h, t.r0) * 16 + r16] = RowInfo{qk, INFINITY, 0.f, 0};
+    if (g == 0) qks[r16] = qk;
+  }
 
   auto block = [&](int b, const Raw& cur) {
     // Keys' terms: one key a lane, handed round in LDS (each lane for the eight keys that it needs
@@ -293,7 +301,9 @@ __device__ __forceinline__ void few_rows(const Args& a, unsigned wg) {
     const int64_t tok = token_of(r, a.group);
     const int head = h * a.group + (int)(r - tok * a.group);
     dst = a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd + d0;
-    if (K::kStats && d0 == 0) a.stats[(t.row0 + tok) * a.heads + head] = stat_of(m, den);
+    if (K::kLogits && d0 == 0) a.stats[(t.row0 + tok) * a.heads + head] = stat_of(m, den);
+    if (K::kStats && d0 == 0)
+      a.info[tile16(a, t, h, t.r0) * 16 + row] = info_of(a, t, r, qks[row], m, den);
   } else {
     const int64_t at = share_at<K>(a, t, th, h, z, kFewRows, row);
     if (d0 == 0) a.part_ml[at] = float2{m, den};
@@ -387,7 +397,10 @@ __device__ __forceinline__ void join_tiles(const Args& a) {
   const int head = h * a.group + (int)(r - tok * a.group);
   reinterpret_cast<float2*>(a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd)[l] =
       float2{o0 * f, o1 * f};
-  if (K::kStats && l == 0) a.stats[(t.row0 + tok) * a.heads + head] = stat_of(m, den);
+  if (K::kStats && l == 0) {
+    RowInfo& info = a.info[tile16(a, t, h, r) * 16 + (r & 15)];
+    info = info_of(a, t, r, info.qk, m, den);
+  }
 }
 
 template <class K, int RT, int W>
@@ -638,6 +651,12 @@ __device__ __forceinline__ void chunk_rows(const Args& a, unsigned wg) {
       parts8(x[kb], qh[qt][kb], ql[qt][kb]);
     }
     qk[qt] = __builtin_ldexpf(a.scale2, -qe);
+    if (K::kStats && z == 0) {
+      keep_parts(a, t, h, t.r0 + (w * QT + qt) * 16, qh[qt], ql[qt]);
+      const int64_t r0 = t.r0 + (w * QT + qt) * 16;
+      if (g == 0 && r0 < t.rows && (a.splits > 1 || r >= t.rows))
+        a.info[tile16(a, t, h, r0) * 16 + r16] = RowInfo{qk[qt], INFINITY, 0.f, 0};
+    }
   }
   const int e0 = exp_of(v0);
   const int blocks = (keys + KB - 1) / KB;
@@ -870,7 +889,7 @@ __device__ __forceinline__ void chunk_rows(const Args& a, unsigned wg) {
       const int head = h * a.group + (int)(r - tok * a.group);
       dst = a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd + 32 * g;
       if (K::kStats && g == 0)
-        a.stats[(t.row0 + tok) * a.heads + head] = stat_of(st[qt].m, den);
+        a.info[tile16(a, t, h, r) * 16 + r16] = info_of(a, t, r, qk[qt], st[qt].m, den);
     } else {
       const int64_t at = share_at<K>(a, t, th, h, z, kRows, row);
       if (g == 0) a.part_ml[at] = float2{st[qt].m, den};
@@ -979,9 +998,11 @@ hipError_t launch_kv_cross(const View& c, const KvRows& r, const kvplan::Plan& p
 }
 
 hipError_t launch_kv_counted(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
-                             float2* stats, hipStream_t s) {
+                             const KvWeightsPlan& wp, void* kept, hipStream_t s) {
   Args a = args_of(c, r, scratch, p.part_bytes);
-  a.stats = stats;
+  a.qparts = static_cast<char*>(kept);
+  a.info = reinterpret_cast<RowInfo*>(a.qparts + wp.n16 * c.kv_heads * kQTile);
+  a.n16 = wp.n16;
   return run<Counted>(a, p, s);
 }
 

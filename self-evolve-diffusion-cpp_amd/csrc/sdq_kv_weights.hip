@@ -6,10 +6,16 @@
 //   sum_r 2^(t_rj - m_r - e_j) / d_r.
 //
 // The logits are formed again, bit for bit as the attention forms them (a row's weights then
-// sum to 1 however large they are), two MFMA products each: half of the attention's. A wave keeps 64 keys in registers, the workgroup 256, and the rows pass by in
-// LDS, 32 at a time in two buffers; a lane sums the weights of 16 of its keys for one row of
-// 16, the lanes' sums are joined once a block of keys. One workgroup sums a key over all
-// rows, in their order: no atomics, the same bits every time.
+// sum to 1 however large they are), two MFMA products each: half of the attention's. That
+// left the rows' two fp16 parts in the order of the MFMA operands, so that this kernel moves
+// them by LDS-DMA and its loop holds MFMAs, LDS reads and exponentials only.
+// A wave keeps 64 keys in registers, the workgroup 512, and the rows pass by in LDS, 64 at a
+// time in a ring of three; a lane sums the weights of 16 of its keys for one row of 16, the
+// lanes' sums are joined once a block of keys. The products of the next 16 rows stand beside
+// the exponentials of the last ones. Few blocks of many rows are cut into ranges of
+// rows, whose sums a second kernel adds up in order: no atomics, the same bits every time.
+//
+// 4099 rows over themselves, 24 heads on 8: MEASURED.
 #include <algorithm>
 
 #include "sdq_kv_attn.h"
@@ -24,15 +30,13 @@ using namespace kvattn;
 constexpr int kWaves = 8;
 constexpr int kTiles = 4;                     // of 16 keys, a wave
 constexpr int kBlock = 16 * kTiles * kWaves;  // keys of a workgroup
-constexpr int kRows = 32;                     // in LDS
-constexpr int kLeastLog = 8;                  // of a range's rows
+constexpr int kRows = 64;                     // of a stage in LDS
+constexpr int kRing = 3;
+constexpr int kLeastLog = 10;                 // of a range's rows
+constexpr int kDma = 5;                       // a wave's, a stage: 4 of the parts, one of the rest
 
-struct RowInfo {
-  float qk, m, inv;
-  int see;  // keys; 0: the row adds nothing
-};
 struct Stage {
-  __attribute__((aligned(16))) char q[2][kRows / 16][4][1024];  // [hi, lo][tile][kb][lane 16 B]
+  __attribute__((aligned(16))) char q[kRows / 16][kQTile];
   RowInfo row[kRows];
 };
 
@@ -41,6 +45,7 @@ struct Work {
   float* part;  // [sequence, head][block, range][kBlock] where rows are cut
   int across;   // workgroups of a sequence and head
   int cut;      // rows may be cut
+  int s0;       // the launch's first sequence
 };
 
 // How the blocks of keys of a sequence and head, and ranges of 2^log of its rows, are shared out.
@@ -64,7 +69,8 @@ __device__ __forceinline__ int64_t first_row(const Args& a, const Tile& t, int b
   return tok > 0 ? tok * a.group / kRows * kRows : 0;
 }
 __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk) {
-  __shared__ Stage buf[2];
+  __shared__ Stage ring[kRing];
+  __shared__ __attribute__((aligned(16))) float terms[kWaves][2][64];
   const View& c = a.c;
   const int tid = threadIdx.x, w = uniform(tid >> 6), l = tid & 63, r16 = l & 15, g = l >> 4;
   const int x = (int)(blockIdx.x % wk.across);
@@ -73,9 +79,10 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
   const Tile t = rows_of(a, s);
   if (t.rows == 0) return;
   const Cut cut = cut_of(t, wk);
-  const int32_t* table = c.table + s * c.max_pages;
+  const auto* table = scalar_ptr(c.table + s * c.max_pages);
   const int e0 = first_exp<Own>(a, t, h);
-  const int step_tok = kRows / a.group, step_qh = kRows % a.group;
+  const int64_t tile0 = h * a.n16 + t.row0 * a.group / 16 + wk.s0 + s;
+  const uint32_t lds = uniform((int)dev::lds_addr32(ring));
 
   // Items (block, range) in order, those that no row sees left out: every across-th is ours.
   const bool whole = cut.ranges == 1;
@@ -92,110 +99,87 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
     const int k0 = b * kBlock + 16 * kTiles * w;
     v8h key[kTiles][4];
     v4f kc[kTiles], ke[kTiles];
-    bool far = false;
+    int page[kTiles];
+#pragma unroll
+    for (int kt = 0; kt < kTiles; kt++) page[kt] = table[min(k0 + 16 * kt, t.len - 1) >> c.page_log2];
+    int64_t at[kTiles];
+    uint4 raw[kTiles][2];
+#pragma unroll
+    for (int kt = 0; kt < kTiles; kt++) {  // of the first page where there is none
+      if (k0 + 16 * kt >= t.len || page[kt] >= c.pages) page[kt] = -1;
+      at[kt] = (((page[kt] < 0 ? 0 : page[kt]) * (int64_t)c.kv_heads + h) << c.page_log2) +
+               ((k0 + 16 * kt) & ((1 << c.page_log2) - 1));
+      const int8_t* kp = c.k + (at[kt] + r16) * kHd + 16 * g;
+      raw[kt][0] = *reinterpret_cast<const uint4*>(kp);
+      raw[kt][1] = *reinterpret_cast<const uint4*>(kp + 64);
+    }
+    // scales: a key a lane, what follows from them handed round in LDS
+    const int64_t own = (g == 0 ? at[0] : g == 1 ? at[1] : g == 2 ? at[2] : at[3]) + r16;
+    const int own_page = g == 0 ? page[0] : g == 1 ? page[1] : g == 2 ? page[2] : page[3];
+    const float ks = c.ks[own], vs = c.vs[own];
+    const KeyTerms k = key_terms(ks, vs, own_page >= 0 && k0 + l < t.len, 1.f, e0);
+    terms[w][0][l] = k.c, terms[w][1][l] = k.e;
+    const bool any_far = __any(k.e < kNear);
 #pragma unroll
     for (int kt = 0; kt < kTiles; kt++) {
-      const int p = k0 + 16 * kt;
-      const int page = p < t.len ? table[p >> c.page_log2] : -1;
-      const bool there = page >= 0 && page < c.pages;
-      const int64_t at = (((there ? page : 0) * (int64_t)c.kv_heads + h) << c.page_log2) +
-                         (p & ((1 << c.page_log2) - 1));
-      const int8_t* kp = c.k + (at + r16) * kHd + 16 * g;
 #pragma unroll
       for (int j = 0; j < 2; j++) {
-        const uint4 r = *reinterpret_cast<const uint4*>(kp + 64 * j);
-        key[kt][2 * j] = codes8(r.x, r.y);
-        key[kt][2 * j + 1] = codes8(r.z, r.w);
+        key[kt][2 * j] = codes8(raw[kt][j].x, raw[kt][j].y);
+        key[kt][2 * j + 1] = codes8(raw[kt][j].z, raw[kt][j].w);
       }
-      const v4f ks = *reinterpret_cast<const v4f_any*>(c.ks + at + 4 * g);
-      const v4f vs = *reinterpret_cast<const v4f_any*>(c.vs + at + 4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const KeyTerms k =
-            key_terms(ks[i], vs[i], there && p + 4 * g + i < t.len, 1.f, e0);
-        kc[kt][i] = k.c, ke[kt][i] = k.e;
-        far |= k.e < kNear;
-      }
+      kc[kt] = *reinterpret_cast<const v4f*>(&terms[w][0][16 * kt + 4 * g]);
+      ke[kt] = *reinterpret_cast<const v4f*>(&terms[w][1][16 * kt + 4 * g]);
     }
-    const bool any_far = __any(far);
 
     for (; skip < n; skip += wk.across) {
-      const int64_t z = z0 + skip;
-      const int64_t begin = lead > z << cut.log ? lead : z << cut.log;
-      const int64_t end = (z + 1) << cut.log < t.rows ? (z + 1) << cut.log : t.rows;
+      const int z = z0 + skip;
+      const int64_t begin = lead > (int64_t)z << cut.log ? lead : (int64_t)z << cut.log;
+      const int64_t end = (int64_t)(z + 1) << cut.log < t.rows ? (int64_t)(z + 1) << cut.log : t.rows;
       v4f sum[kTiles];
 #pragma unroll
       for (int kt = 0; kt < kTiles; kt++) sum[kt] = v4f{0.f, 0.f, 0.f, 0.f};
 
-      // A stage's rows: 8 dims a thread, loaded one stage ahead of their turn to fp16. The row's
-      // token and query head go on by what kRows rows are.
-      const int row = tid >> 4, j = tid & 15;
-      int tok = (int)((begin + row) / a.group), qh = (int)(begin + row - (int64_t)tok * a.group);
-      const int rows = (int)(end - begin);
-      v4f raw[2];
-      float2 st;
-      int see;
-      auto load = [&](int r0) {
-        const bool ok = r0 + row < rows;
-        const int64_t at = t.row0 + (ok ? tok : 0);
-        const int head = h * a.group + (ok ? qh : 0);
-        const float* q = a.q + at * a.ldq + (int64_t)head * kHd + 8 * j;
+      // Stages of 64 rows from `begin` (a multiple of 64); behind the last tile that one again. A
+      // wave moves half a tile of parts and an eighth of the rest.
+      const int tiles = (int)((end - begin + 15) >> 4), stages = (tiles + 3) >> 2;
+      const int64_t first = tile0 + (begin >> 4);
+      auto issue = [&](int i, int slot) {
+        const uint32_t to = lds + (uint32_t)slot * (uint32_t)sizeof(Stage);
+        const int64_t tile = first + min(4 * i + (w >> 1), tiles - 1);
+        const dev::v4u parts = dev::raw_rsrc(a.qparts + tile * kQTile, kQTile);
 #pragma unroll
-        for (int i = 0; i < 2; i++) raw[i] = *reinterpret_cast<const v4f*>(q + 4 * i);
-        st = a.stats[at * a.heads + head];
-        const int p = t.first + tok;
-        see = !ok || p < 0 ? 0 : a.causal && p < t.len ? p + 1 : t.len;
-        tok += step_tok, qh += step_qh;
-        if (qh >= a.group) qh -= a.group, tok++;
-      };
-      auto stage = [&](Stage& d) {
-        float v[8], mx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float f = raw[i >> 2][i & 3];
-          v[i] = fabsf(f) <= 3.402823466e38f ? f : 0.f;
-          mx = fmaxf(mx, fabsf(v[i]));
+        for (int k = 0; k < 4; k++) {
+          const uint32_t at = (uint32_t)(w & 1) * 4096 + 1024 * k;
+          dev::dma16<4>(parts, l * 16, at, to + (w >> 1) * kQTile + at);
         }
-#pragma unroll
-        for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        const int e = q_exp(mx);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = __builtin_ldexpf(v[i], e);
-        // dims 8 j ..: k slots 8 (j / 2 % 4) + i of step 2 (j / 8) + j % 2
-        v8h hi, lo;
-        parts8(v, hi, lo);
-        const int off = (16 * ((j >> 1) & 3) + (row & 15)) * 16, kb = 2 * (j >> 3) + (j & 1);
-        *reinterpret_cast<v8h*>(d.q[0][row >> 4][kb] + off) = hi;
-        *reinterpret_cast<v8h*>(d.q[1][row >> 4][kb] + off) = lo;
-        if (j == 0)
-          d.row[row] = RowInfo{__builtin_ldexpf(a.scale2, -e), st.x, st.y, st.y > 0.f ? see : 0};
-      };
-      auto compute = [&](const Stage& d, auto faint) {
-        constexpr bool kFaint = decltype(faint)::value;
-        constexpr int kRt = kRows / 16;
-        RowInfo ri[kRt];
-        bool some = false, every = true;
-#pragma unroll
-        for (int rt = 0; rt < kRt; rt++) {
-          ri[rt] = d.row[16 * rt + r16];
-          some |= ri[rt].see > k0;
-          every &= ri[rt].see >= k0 + 16 * kTiles;
+        if (l < 8) {
+          const uint32_t at = (uint32_t)(w & 1) * 128;
+          dev::dma16<4>(dev::raw_rsrc(a.info + tile * 16, 256), l * 16, at,
+                        to + 4 * kQTile + (w >> 1) * 256 + at);
         }
-        if (!__any(some)) return;
-        v4f sc[kRt][kTiles];
-#pragma unroll
-        for (int rt = 0; rt < kRt; rt++)
-#pragma unroll
-          for (int kt = 0; kt < kTiles; kt++) sc[rt][kt] = v4f{0.f, 0.f, 0.f, 0.f};
-        // a step's operands are read before the products of the step ahead of it
-        v8h op[2][2][kRt];
+      };
+      // Of tiles in order, the first that sees any of the wave's keys and the first that sees all.
+      auto from = [&](int key) {
+        const int64_t r = a.causal ? (int64_t)(key - t.first) * a.group - begin : 0;
+        return r;  // the first row that sees the key
+      };
+      const int64_t some = from(k0) >> 4, every = (from(k0 + 16 * kTiles - 1) + 15) >> 4;
+      struct Scores {
+        v4f s[kTiles];
+        RowInfo ri;
+      };
+      // The scores of tile `nx` beside the weights of the tile ahead of it.
+      auto step = [&](const Stage& d, int nx, bool live, Scores& to, const Scores& of, auto faint,
+                      auto mask) {
+        constexpr bool kFaint = decltype(faint)::value, kMask = decltype(mask)::value;
+        v8h op[2][2];
         auto read = [&](int kb) {
 #pragma unroll
           for (int part = 0; part < 2; part++)
-#pragma unroll
-            for (int rt = 0; rt < kRt; rt++)
-              op[kb & 1][part][rt] = *reinterpret_cast<const v8h*>(d.q[part][rt][kb] + l * 16);
+            op[kb & 1][part] = *reinterpret_cast<const v8h*>(d.q[nx] + 4096 * part + 1024 * kb + l * 16);
         };
+        to.ri = d.row[16 * nx + r16];
+        if (!live) to.ri.m = INFINITY, to.ri.inv = 0.f, to.ri.see = 0;
         read(0);
 #pragma unroll
         for (int kb = 0; kb < 4; kb++) {
@@ -204,47 +188,56 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
 #pragma unroll
           for (int part = 1; part >= 0; part--)
 #pragma unroll
-            for (int rt = 0; rt < kRt; rt++)
+            for (int kt = 0; kt < kTiles; kt++)
+              to.s[kt] = mma(key[kt][kb], op[kb & 1][part],
+                             kb == 0 && part == 1 ? v4f{0.f, 0.f, 0.f, 0.f} : to.s[kt]);
+          const v4f ck = kc[kb] * of.ri.qk;
 #pragma unroll
-              for (int kt = 0; kt < kTiles; kt++)
-                sc[rt][kt] = mma(key[kt][kb], op[kb & 1][part][rt], sc[rt][kt]);
+          for (int i = 0; i < 4; i++) {
+            float y = __builtin_fmaf(of.s[kb][i], ck[i], ke[kb][i]) - of.ri.m;
+            if (kFaint) y -= ke[kb][i];
+            if (kMask) y = k0 + 16 * kb + 4 * g + i < of.ri.see ? y : -INFINITY;
+            sum[kb][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(y), of.ri.inv, sum[kb][i]);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
-        auto add = [&](auto mask) {
-#pragma unroll
-          for (int rt = 0; rt < kRt; rt++)
-#pragma unroll
-            for (int kt = 0; kt < kTiles; kt++) {
-              const v4f ck = kc[kt] * ri[rt].qk;
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                float y = __builtin_fmaf(sc[rt][kt][i], ck[i], ke[kt][i]) - ri[rt].m;
-                if (kFaint) y -= ke[kt][i];
-                if (decltype(mask)::value) y = k0 + 16 * kt + 4 * g + i < ri[rt].see ? y : -INFINITY;
-                sum[kt][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(y), ri[rt].inv, sum[kt][i]);
-              }
-            }
-        };
-        if (__all(every))
-          add(std::false_type{});
-        else
-          add(std::true_type{});
       };
       auto pass = [&](auto faint) {
-        load(0);
-        __syncthreads();  // the last item's rows are read
-        stage(buf[0]);
-        load(kRows);
-        __syncthreads();
-        int n = 0;
-        for (int r0 = 0; r0 < rows; r0 += kRows, n ^= 1) {
-          if (r0 + kRows < rows) {
-            stage(buf[n ^ 1]);
-            load(r0 + 2 * kRows);
-          }
-          compute(buf[n], faint);
-          __syncthreads();
+        Scores sc[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {  // before the first tile: adds nothing
+          sc[j].ri = RowInfo{0.f, INFINITY, 0.f, 0};
+#pragma unroll
+          for (int kt = 0; kt < kTiles; kt++) sc[j].s[kt] = v4f{0.f, 0.f, 0.f, 0.f};
         }
+        // tile 4 i + nx, and the weights of the one ahead of it
+        auto one = [&](const Stage& d, int i, int nx, Scores& to, const Scores& of, auto mask) {
+          if (4 * i + nx >= some) step(d, nx, 4 * i + nx < tiles, to, of, faint, mask);
+        };
+        auto four = [&](const Stage& d, int i, auto mask) {
+          one(d, i, 0, sc[1], sc[0], mask);
+          one(d, i, 1, sc[0], sc[1], mask);
+          one(d, i, 2, sc[1], sc[0], mask);
+          one(d, i, 3, sc[0], sc[1], mask);
+        };
+        __builtin_amdgcn_s_waitcnt(dev::waitcnt_vm(0));
+        asm volatile("s_barrier" ::: "memory");  // the last item's rows are read
+        issue(0, 0), issue(1, 1);
+        int slot = 0, ahead = 2;
+        for (int i = 0; i < stages; i++) {
+          __builtin_amdgcn_s_waitcnt(dev::waitcnt_vm(kDma));
+          asm volatile("s_barrier" ::: "memory");
+          issue(i + 2, ahead);
+          const Stage& d = ring[slot];
+          // a row that adds nothing has an infinite maximum: only keys ahead of a row are masked
+          if (4 * i - 1 >= every)
+            four(d, i, std::false_type{});
+          else
+            four(d, i, std::true_type{});
+          slot = slot == kRing - 1 ? 0 : slot + 1;
+          ahead = ahead == kRing - 1 ? 0 : ahead + 1;
+        }
+        one(ring[0], stages, 0, sc[1], sc[0], std::true_type{});  // the last tile's weights
       };
       if (any_far)
         pass(std::true_type{});
@@ -274,6 +267,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
     }
     skip = whole ? 0 : skip - n;
   }
+  __builtin_amdgcn_s_waitcnt(dev::waitcnt_vm(0));
 }
 
 // Where rows were cut: the ranges' sums of a key, in order, to its place.
@@ -301,8 +295,10 @@ __global__ void __launch_bounds__(kBlock) kv_weights_join_kernel(Args a, Work wk
 
 KvWeightsPlan plan_kv_weights(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count) {
   KvWeightsPlan p{};
-  // One workgroup to a CU at once, four rounds of them.
-  const int64_t pairs = (int64_t)nseq * kv_heads, want = 4 * (int64_t)cu_count;
+  p.n16 = T * group / 16 + nseq;
+  p.kept_bytes = p.n16 * kv_heads * (kQTile + 16 * (int64_t)sizeof(RowInfo));
+  // One workgroup to a CU at once, two rounds of them.
+  const int64_t pairs = (int64_t)nseq * kv_heads, want = 2 * (int64_t)cu_count;
   p.cut = T * group / nseq >= 128;
   const int64_t blocks = ceil_div(std::max<int64_t>(most, 1), kBlock);
   p.across = (int)std::max<int64_t>(1, std::min(p.cut ? want : blocks, ceil_div(want, pairs)));
@@ -312,20 +308,20 @@ KvWeightsPlan plan_kv_weights(int64_t T, int nseq, int group, int kv_heads, int6
   return p;
 }
 
-hipError_t launch_kv_weights(const View& c, const KvRows& r, const float2* stats, float* w,
-                             const KvWeightsPlan& p, void* scratch, hipStream_t s) {
+hipError_t launch_kv_weights(const View& c, const KvRows& r, const KvWeightsPlan& p, void* kept, float* w,
+                             void* scratch, hipStream_t s) {
   Args a{};
-  a.c = c;
-  a.q = r.q, a.ldq = r.ldq;
   a.heads = r.heads, a.group = r.heads / c.kv_heads;
-  a.scale2 = r.scale * 1.44269504088896341f;
   a.causal = r.causal;
-  a.stats = const_cast<float2*>(stats);
-  const Work wk{w, static_cast<float*>(scratch), p.across, p.cut};
+  a.qparts = static_cast<char*>(kept);
+  a.info = reinterpret_cast<RowInfo*>(a.qparts + p.n16 * c.kv_heads * kQTile);
+  a.n16 = p.n16;
+  Work wk{w, static_cast<float*>(scratch), p.across, p.cut, 0};
   for (int s0 = 0; s0 < c.nseq; s0 += p.seqs) {
     a.c = c;
     a.c.q_start += s0, a.c.lens += s0, a.c.table += s0 * c.max_pages;
     a.c.nseq = std::min(p.seqs, c.nseq - s0);
+    wk.s0 = s0;
     const dim3 grid((unsigned)((int64_t)p.across * a.c.nseq * c.kv_heads));
     hipLaunchKernelGGL(kv_weights_kernel, grid, dim3(64 * kWaves), 0, s, a, wk);
     hipError_t e = hipGetLastError();
