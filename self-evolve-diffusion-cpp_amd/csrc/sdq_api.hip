@@ -1091,6 +1091,17 @@ kvplan::Plan plan_of(const KvCall& k, int tall = 0) {
                       k.view.max_pages << k.view.page_log2, g_dev[k.dev].cu_count, tall);
 }
 
+// The scratch of a call's plan, and behind it that of its packed keys (null: none).
+int kv_scratch(const KvCall& k, const kvplan::Plan& plan, hipStream_t s, float** scratch, void** packed,
+               std::unique_lock<std::mutex>* turn) {
+  const int64_t at = round_up(plan.scratch_bytes, 16);
+  const int64_t more = kv_packed_bytes(k.view, k.rows.heads / k.view.kv_heads, plan);
+  if (at + more == 0) return SDQ_OK;
+  const int rc = shared_scratch(k.dev, s, (size_t)(at + more), scratch, turn);
+  if (rc == SDQ_OK && more) *packed = reinterpret_cast<char*>(*scratch) + at;
+  return rc;
+}
+
 // Host -> device through the first two slots' pinned buffers, on the first
 // one's stream. A buffer is refilled only
 // after the DMA that read it finished.
@@ -2486,11 +2497,11 @@ int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* 
   const kvplan::Plan plan = plan_of(call);
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
-  if (plan.scratch_bytes > 0 &&
-      (rc = shared_scratch(call.dev, s, (size_t)plan.scratch_bytes, &scratch, &turn)))
-    return rc;
-  return timed("kv_attention", s,
-               [&] { return launch_kv_attn(call.view, call.rows, plan, scratch, s); });
+  void* packed = nullptr;
+  if ((rc = kv_scratch(call, plan, s, &scratch, &packed, &turn))) return rc;
+  return timed("kv_attention", s, [&] {
+    return launch_kv_attn(call.view, call.rows, plan, scratch, packed, s);
+  });
 }
 
 int sdq_kv_cross_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
@@ -2504,11 +2515,11 @@ int sdq_kv_cross_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const f
   const kvplan::Plan plan = plan_of(call);
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
-  if (plan.scratch_bytes > 0 &&
-      (rc = shared_scratch(call.dev, s, (size_t)plan.scratch_bytes, &scratch, &turn)))
-    return rc;
-  return timed("kv_cross_attention", s,
-               [&] { return launch_kv_cross(call.view, call.rows, plan, scratch, s); });
+  void* packed = nullptr;
+  if ((rc = kv_scratch(call, plan, s, &scratch, &packed, &turn))) return rc;
+  return timed("kv_cross_attention", s, [&] {
+    return launch_kv_cross(call.view, call.rows, plan, scratch, packed, s);
+  });
 }
 
 int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, const sdq_kv_batch* b,
@@ -2583,17 +2594,20 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
   const KvWeightsPlan wplan =
       plan_kv_weights(T, call.view.nseq, heads / c->kv_heads, c->kv_heads,
                       call.view.max_pages << call.view.page_log2, cus);
-  // the shares' sums or, once they are joined, the ranges', and the rows' parts and statistics
+  // the shares' sums or, once they are joined, the ranges', the rows' parts and statistics, and
+  // the keys as operands
   const size_t kept_at = (size_t)round_up(std::max(plan.scratch_bytes, wplan.scratch_bytes), 16);
-  if ((rc = shared_scratch(call.dev, s, kept_at + (size_t)wplan.kept_bytes, &scratch, &turn)))
-    return rc;
-  void* kept = reinterpret_cast<char*>(scratch) + kept_at;
+  const size_t packed_at = kept_at + (size_t)round_up(wplan.kept_bytes, 16);
+  const int64_t more = kv_packed_bytes(call.view, heads / c->kv_heads, plan);
+  if ((rc = shared_scratch(call.dev, s, packed_at + (size_t)more, &scratch, &turn))) return rc;
+  base = reinterpret_cast<char*>(scratch);
   rc = timed("kv_attention_weights", s, [&] {
-    return launch_kv_counted(call.view, call.rows, plan, scratch, wplan, kept, s);
+    return launch_kv_counted(call.view, call.rows, plan, scratch, wplan, base + kept_at,
+                             more ? base + packed_at : nullptr, s);
   });
   if (rc) return rc;
   return timed("kv_weights", s, [&] {
-    return launch_kv_weights(call.view, call.rows, wplan, kept, weights, scratch, s);
+    return launch_kv_weights(call.view, call.rows, wplan, base + kept_at, weights, scratch, s);
   });
 }
 

@@ -285,11 +285,13 @@ struct KvRows {
   float scale;
   int causal;
 };
-// plan: kvplan::plan's for this call; scratch: its scratch_bytes.
+// plan: kvplan::plan's for this call; scratch: its scratch_bytes; packed: kv_packed_bytes of
+// memory for the keys as operands, where that is not 0.
+int64_t kv_packed_bytes(const kv::View& c, int group, const kvplan::Plan& plan);
 hipError_t launch_kv_attn(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
-                          void* scratch, hipStream_t s);
+                          void* scratch, void* packed, hipStream_t s);
 hipError_t launch_kv_cross(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
-                           void* scratch, hipStream_t s);
+                           void* scratch, void* packed, hipStream_t s);
 hipError_t launch_kv_shared(const kv::View& c, const kv::Shared& pre, const KvRows& r,
                             const kvplan::SharedPlan& plan, void* scratch, hipStream_t s);
 // launch_kv_attn that keeps in `kept` what the sums of the weights by key go by, and those:
@@ -304,7 +306,8 @@ struct KvWeightsPlan {
 KvWeightsPlan plan_kv_weights(int64_t T, int nseq, int group, int kv_heads, int64_t most,
                               int cu_count);
 hipError_t launch_kv_counted(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
-                             void* scratch, const KvWeightsPlan& p, void* kept, hipStream_t s);
+                             void* scratch, const KvWeightsPlan& p, void* kept, void* packed,
+                             hipStream_t s);
 hipError_t launch_kv_weights(const kv::View& c, const KvRows& r, const KvWeightsPlan& p, void* kept,
                              float* w, void* scratch, hipStream_t s);
 // Both at once for few rows (the plan's tiles of 16), whose logits are kept in between:

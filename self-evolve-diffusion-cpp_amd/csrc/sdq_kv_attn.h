@@ -537,5 +537,22 @@ __device__ __forceinline__ void keep_parts(const Args& a, const Tile& t, int h, 
   }
 }
 
+// Where a share of a tile's row keeps its sums (th: the workgroup's tile and head).
+template <class K>
+__device__ __forceinline__ int64_t share_at(const Args& a, const Tile& t, int64_t th, int h, int z,
+                                            int rows, int row) {
+  if (!K::kByRow) return (th * a.splits + z) * rows + row;
+  const int64_t r = t.r0 + row, tok = token_of(r, a.group);
+  const int64_t at = (t.row0 + tok) * (a.nh * a.group) + (h - a.h0) * a.group + (r - tok * a.group);
+  return at * a.shares + a.z0 + z;
+}
+
 }  // namespace kvattn
+
+// Keys as MFMA operands, of all sequences and heads (sdq_kv_packed.hip): once a call, then tiles
+// of 256 rows in `grid` workgroups over them.
+hipError_t launch_kv_pack(const kvattn::Args& a, void* packed, hipStream_t s);
+template <class K>
+hipError_t launch_kv_packed(const kvattn::Args& a, void* packed, unsigned grid, hipStream_t s);
+
 }  // namespace sdq

@@ -42,16 +42,6 @@ namespace {
 
 using namespace kvattn;
 
-// Where a share of a tile's row keeps its sums (th: the workgroup's tile and head).
-template <class K>
-__device__ __forceinline__ int64_t share_at(const Args& a, const Tile& t, int64_t th, int h, int z,
-                                            int rows, int row) {
-  if (!K::kByRow) return (th * a.splits + z) * rows + row;
-  const int64_t r = t.r0 + row, tok = token_of(r, a.group);
-  const int64_t at = (t.row0 + tok) * (a.nh * a.group) + (h - a.h0) * a.group + (r - tok * a.group);
-  return at * a.shares + a.z0 + z;
-}
-
 // Shares that a tile's keys are cut into. A shared part's rows are known here alone: as many
 // shares as make a.want workgroups of all parts' tiles. Where each has its own place among a
 // row's (kByRow), a share has a.least keys at least; one that is left out says so.
@@ -955,13 +945,18 @@ hipError_t launch_join(const Args& a, int64_t n, hipStream_t s) {
 }
 
 template <class K>
-hipError_t run(Args a, const kvplan::Plan& p, hipStream_t s) {
+hipError_t run(Args a, const kvplan::Plan& p, void* packed, hipStream_t s) {
   a.splits = p.splits;
+  if (packed) {
+    const hipError_t e = launch_kv_pack(a, packed, s);
+    if (e != hipSuccess) return e;
+  }
   // launches of as many tiles as a grid's 32-bit thread count takes
   for (int64_t tile = 0; tile < p.tiles; tile += p.tiles_per_launch) {
     const int64_t n = std::min(p.tiles_per_launch, p.tiles - tile);
     a.tile0 = tile;
-    hipError_t e = launch_tiles<K>(a, p, n, a.c.kv_heads, s);
+    hipError_t e = packed ? launch_kv_packed<K>(a, packed, (unsigned)(n * a.c.kv_heads * p.splits), s)
+                          : launch_tiles<K>(a, p, n, a.c.kv_heads, s);
     if (e != hipSuccess) return e;
     if (p.splits > 1) {
       e = p.rows == kFewRows ? launch_join<K, kFewRows>(a, n * a.c.kv_heads, s)
@@ -988,22 +983,22 @@ Args args_of(const View& c, const KvRows& r, void* scratch, int64_t part_bytes) 
 }  // namespace
 
 hipError_t launch_kv_attn(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
-                          hipStream_t s) {
-  return run<Own>(args_of(c, r, scratch, p.part_bytes), p, s);
+                          void* packed, hipStream_t s) {
+  return run<Own>(args_of(c, r, scratch, p.part_bytes), p, packed, s);
 }
 
 hipError_t launch_kv_cross(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
-                           hipStream_t s) {
-  return run<Cross>(args_of(c, r, scratch, p.part_bytes), p, s);
+                           void* packed, hipStream_t s) {
+  return run<Cross>(args_of(c, r, scratch, p.part_bytes), p, packed, s);
 }
 
 hipError_t launch_kv_counted(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
-                             const KvWeightsPlan& wp, void* kept, hipStream_t s) {
+                             const KvWeightsPlan& wp, void* kept, void* packed, hipStream_t s) {
   Args a = args_of(c, r, scratch, p.part_bytes);
   a.qparts = static_cast<char*>(kept);
   a.info = reinterpret_cast<RowInfo*>(a.qparts + wp.n16 * c.kv_heads * kQTile);
   a.n16 = wp.n16;
-  return run<Counted>(a, p, s);
+  return run<Counted>(a, p, packed, s);
 }
 
 int64_t kv_logit_keys(const View& c) { return round_up(std::max<int64_t>(c.max_pages << c.page_log2, 1), 32); }

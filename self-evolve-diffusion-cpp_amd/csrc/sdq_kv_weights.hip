@@ -169,21 +169,25 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
         RowInfo ri;
       };
       // The scores of tile `nx` beside the weights of the tile ahead of it.
+      v8h op[2][2];
       auto step = [&](const Stage& d, int nx, bool live, Scores& to, const Scores& of, auto faint,
                       auto mask) {
         constexpr bool kFaint = decltype(faint)::value, kMask = decltype(mask)::value;
-        v8h op[2][2];
-        auto read = [&](int kb) {
+        // operands are read a step of eight products ahead, the next tile's first ones too
+        auto read = [&](int tile, int kb) {
 #pragma unroll
           for (int part = 0; part < 2; part++)
-            op[kb & 1][part] = *reinterpret_cast<const v8h*>(d.q[nx] + 4096 * part + 1024 * kb + l * 16);
+            op[kb & 1][part] = *reinterpret_cast<const v8h*>(d.q[tile] + 4096 * part + 1024 * kb + l * 16);
         };
         to.ri = d.row[16 * nx + r16];
         if (!live) to.ri.m = INFINITY, to.ri.inv = 0.f, to.ri.see = 0;
-        read(0);
+        if (kMask || nx == 0) read(nx, 0);  // masked tiles may be left out
 #pragma unroll
         for (int kb = 0; kb < 4; kb++) {
-          if (kb < 3) read(kb + 1);
+          if (kb < 3)
+            read(nx, kb + 1);
+          else if (!kMask && nx < 3)
+            read(nx + 1, 0);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int part = 1; part >= 0; part--)
@@ -214,29 +218,29 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
         auto one = [&](const Stage& d, int i, int nx, Scores& to, const Scores& of, auto mask) {
           if (4 * i + nx >= some) step(d, nx, 4 * i + nx < tiles, to, of, faint, mask);
         };
-        auto four = [&](const Stage& d, int i, auto mask) {
-          one(d, i, 0, sc[1], sc[0], mask);
-          one(d, i, 1, sc[0], sc[1], mask);
-          one(d, i, 2, sc[1], sc[0], mask);
-          one(d, i, 3, sc[0], sc[1], mask);
-        };
         __builtin_amdgcn_s_waitcnt(dev::waitcnt_vm(0));
         asm volatile("s_barrier" ::: "memory");  // the last item's rows are read
         issue(0, 0), issue(1, 1);
         int slot = 0, ahead = 2;
-        for (int i = 0; i < stages; i++) {
-          __builtin_amdgcn_s_waitcnt(dev::waitcnt_vm(kDma));
-          asm volatile("s_barrier" ::: "memory");
-          issue(i + 2, ahead);
-          const Stage& d = ring[slot];
-          // a row that adds nothing has an infinite maximum: only keys ahead of a row are masked
-          if (4 * i - 1 >= every)
-            four(d, i, std::false_type{});
-          else
-            four(d, i, std::true_type{});
-          slot = slot == kRing - 1 ? 0 : slot + 1;
-          ahead = ahead == kRing - 1 ? 0 : ahead + 1;
-        }
+        auto run = [&](int i, int to, auto mask) {
+          for (; i < to; i++) {
+            __builtin_amdgcn_s_waitcnt(dev::waitcnt_vm(kDma));
+            asm volatile("s_barrier" ::: "memory");
+            issue(i + 2, ahead);
+            const Stage& d = ring[slot];
+            one(d, i, 0, sc[1], sc[0], mask);
+            one(d, i, 1, sc[0], sc[1], mask);
+            one(d, i, 2, sc[1], sc[0], mask);
+            one(d, i, 3, sc[0], sc[1], mask);
+            slot = slot == kRing - 1 ? 0 : slot + 1;
+            ahead = ahead == kRing - 1 ? 0 : ahead + 1;
+          }
+        };
+        // Stages whose rows may not see all of the wave's keys, then the others (a row that adds
+        // nothing has an infinite maximum: only keys ahead of a row are masked).
+        const int first = (int)max((int64_t)0, min((int64_t)stages, (every + 4) >> 2));
+        run(0, first, std::true_type{});
+        run(first, stages, std::false_type{});
         one(ring[0], stages, 0, sc[1], sc[0], std::true_type{});  // the last tile's weights
       };
       if (any_far)

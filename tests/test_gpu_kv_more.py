@@ -261,6 +261,26 @@ def test_cross(sdq_dev, rows, lens, heads, kvh):
     c.check_cross(heads)
 
 
+@pytest.mark.parametrize("rows,lens", [([1100], [1]), ([1024], [64]), ([2500], [577]),
+                                       ([1030, 2000, 900], [300, 0, 4099]), ([3000, 1100], [65, 127])])
+@pytest.mark.parametrize("heads,kvh", [(2, 2), (3, 1)])
+def test_cross_of_thousands(sdq_dev, rows, lens, heads, kvh):
+    """Rows enough for keys that are turned to operands once; their first rows alone, which take
+    the other form, have the same bits."""
+    import torch
+
+    c = More(sdq_dev, rows, lens, kvh, (16, 64, 32)[len(rows) % 3], seed=sum(rows), first=1, behind=2)
+    c.vs[c.table[0, 0], :, 0] *= F(2.0**14)  # the others' exponents far below the first one's
+    c.up()
+    q = c.queries(heads)
+    got = c.check_cross(heads, q=q)
+    if len(rows) == 1:
+        few = c.sdq.KvBatch(c.t(np.array([0, 700], np.int32)), c.batch.lens, c.batch.table)
+        out = torch.zeros((700, heads * HD), device=sdq_dev)
+        c.sdq.kv_cross_attention(c.cache, few, c.t(q[1:701]), out, heads)
+        assert_bitexact(out.cpu().numpy(), got[1:701])
+
+
 @pytest.mark.parametrize("rows", [1, 40, 300])
 def test_cross_scale_strides_missing_pages(sdq_dev, rows):
     import torch
@@ -423,7 +443,7 @@ def test_shared_many_sequences(sdq_dev, nseq, n):
 @pytest.mark.parametrize("new,lens", [
     ([1], [1]), ([1], [257]), ([1] * 6, [3, 0, 700, 64, 129, 2050]), ([2], [2]), ([17], [40]),
     ([33, 0, 1], [100, 50, 16]), ([130], [131]), ([300, 7], [300, 2000]), ([31, 1, 128], [0, 1, 500]),
-    ([64, 65], [64, 1000])])
+    ([64, 65], [64, 1000]), ([1100], [1100]), ([600, 500], [700, 4099])])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("heads,kvh", [(2, 2), (4, 1), (6, 2)])
 def test_weights(sdq_dev, new, lens, causal, heads, kvh):
