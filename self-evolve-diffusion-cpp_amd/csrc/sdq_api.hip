@@ -1091,17 +1091,6 @@ kvplan::Plan plan_of(const KvCall& k, int tall = 0) {
                       k.view.max_pages << k.view.page_log2, g_dev[k.dev].cu_count, tall);
 }
 
-// The scratch of a call's plan, and behind it that of its packed keys (null: none).
-int kv_scratch(const KvCall& k, const kvplan::Plan& plan, hipStream_t s, float** scratch, void** packed,
-               std::unique_lock<std::mutex>* turn) {
-  const int64_t at = round_up(plan.scratch_bytes, 16);
-  const int64_t more = kv_packed_bytes(k.view, k.rows.heads / k.view.kv_heads, plan);
-  if (at + more == 0) return SDQ_OK;
-  const int rc = shared_scratch(k.dev, s, (size_t)(at + more), scratch, turn);
-  if (rc == SDQ_OK && more) *packed = reinterpret_cast<char*>(*scratch) + at;
-  return rc;
-}
-
 // Host -> device through the first two slots' pinned buffers, on the first
 // one's stream. A buffer is refilled only
 // after the DMA that read it finished.
@@ -2497,10 +2486,11 @@ int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* 
   const kvplan::Plan plan = plan_of(call);
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
-  void* packed = nullptr;
-  if ((rc = kv_scratch(call, plan, s, &scratch, &packed, &turn))) return rc;
+  if (plan.scratch_bytes > 0 &&
+      (rc = shared_scratch(call.dev, s, (size_t)plan.scratch_bytes, &scratch, &turn)))
+    return rc;
   return timed("kv_attention", s, [&] {
-    return launch_kv_attn(call.view, call.rows, plan, scratch, packed, s);
+    return launch_kv_attn(call.view, call.rows, plan, scratch, s);
   });
 }
 
@@ -2515,8 +2505,13 @@ int sdq_kv_cross_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const f
   const kvplan::Plan plan = plan_of(call);
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
-  void* packed = nullptr;
-  if ((rc = kv_scratch(call, plan, s, &scratch, &packed, &turn))) return rc;
+  // the shares' sums, and the keys as operands
+  const int64_t packed_at = round_up(plan.scratch_bytes, 16);
+  const int64_t more = kv_packed_bytes(call.view, heads / c->kv_heads, plan);
+  if (packed_at + more > 0 &&
+      (rc = shared_scratch(call.dev, s, (size_t)(packed_at + more), &scratch, &turn)))
+    return rc;
+  void* packed = more ? reinterpret_cast<char*>(scratch) + packed_at : nullptr;
   return timed("kv_cross_attention", s, [&] {
     return launch_kv_cross(call.view, call.rows, plan, scratch, packed, s);
   });

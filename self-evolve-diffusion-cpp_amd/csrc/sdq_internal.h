@@ -289,7 +289,7 @@ struct KvRows {
 // memory for the keys as operands, where that is not 0.
 int64_t kv_packed_bytes(const kv::View& c, int group, const kvplan::Plan& plan);
 hipError_t launch_kv_attn(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
-                          void* scratch, void* packed, hipStream_t s);
+                          void* scratch, hipStream_t s);
 hipError_t launch_kv_cross(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
                            void* scratch, void* packed, hipStream_t s);
 hipError_t launch_kv_shared(const kv::View& c, const kv::Shared& pre, const KvRows& r,

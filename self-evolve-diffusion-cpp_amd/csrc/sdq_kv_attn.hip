@@ -947,7 +947,9 @@ hipError_t launch_join(const Args& a, int64_t n, hipStream_t s) {
 template <class K>
 hipError_t run(Args a, const kvplan::Plan& p, void* packed, hipStream_t s) {
   a.splits = p.splits;
-  if (packed) {
+  // sdq_kv_attention goes without: it has to run where scratch cannot be had
+  constexpr bool kPacks = !std::is_same<K, Own>::value;
+  if (kPacks && packed) {
     const hipError_t e = launch_kv_pack(a, packed, s);
     if (e != hipSuccess) return e;
   }
@@ -955,8 +957,12 @@ hipError_t run(Args a, const kvplan::Plan& p, void* packed, hipStream_t s) {
   for (int64_t tile = 0; tile < p.tiles; tile += p.tiles_per_launch) {
     const int64_t n = std::min(p.tiles_per_launch, p.tiles - tile);
     a.tile0 = tile;
-    hipError_t e = packed ? launch_kv_packed<K>(a, packed, (unsigned)(n * a.c.kv_heads * p.splits), s)
-                          : launch_tiles<K>(a, p, n, a.c.kv_heads, s);
+    hipError_t e;
+    if constexpr (kPacks)
+      e = packed ? launch_kv_packed<K>(a, packed, (unsigned)(n * a.c.kv_heads * p.splits), s)
+                 : launch_tiles<K>(a, p, n, a.c.kv_heads, s);
+    else
+      e = launch_tiles<K>(a, p, n, a.c.kv_heads, s);
     if (e != hipSuccess) return e;
     if (p.splits > 1) {
       e = p.rows == kFewRows ? launch_join<K, kFewRows>(a, n * a.c.kv_heads, s)
@@ -983,8 +989,8 @@ Args args_of(const View& c, const KvRows& r, void* scratch, int64_t part_bytes) 
 }  // namespace
 
 hipError_t launch_kv_attn(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
-                          void* packed, hipStream_t s) {
-  return run<Own>(args_of(c, r, scratch, p.part_bytes), p, packed, s);
+                          hipStream_t s) {
+  return run<Own>(args_of(c, r, scratch, p.part_bytes), p, nullptr, s);
 }
 
 hipError_t launch_kv_cross(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,

@@ -432,7 +432,6 @@ hipError_t launch_kv_packed(const Args& a, void* packed, unsigned grid, hipStrea
                      pack_of(a.c, packed));
   return hipGetLastError();
 }
-template hipError_t launch_kv_packed<Own>(const Args&, void*, unsigned, hipStream_t);
 template hipError_t launch_kv_packed<Cross>(const Args&, void*, unsigned, hipStream_t);
 template hipError_t launch_kv_packed<Counted>(const Args&, void*, unsigned, hipStream_t);
 
