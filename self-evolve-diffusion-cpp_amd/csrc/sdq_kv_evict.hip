@@ -73,12 +73,28 @@ struct Tokens {
   }
 };
 
+constexpr int kCopies = 2;
 struct Lds {
-  uint32_t hist[2048];
+  __attribute__((aligned(16))) uint32_t hist[2048 * kCopies];  // [digit][lane % kCopies]
   uint32_t wave[kWaves];
   uint32_t rounds[16][kWaves];
   uint32_t found[3];
 };
+
+// The counts of 2 digits from `first` on, of all copies.
+__device__ __forceinline__ uint2 counts_of(const Lds& s, int first) {
+  uint32_t n[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int c = 0; c < kCopies; c++) n[i] += s.hist[(first + i) * kCopies + c];
+  return uint2{n[0], n[1]};
+}
+__device__ __forceinline__ void clear_counts(Lds& s) {
+#pragma unroll
+  for (int c = 0; c < 2 * kCopies; c += 4)
+    *reinterpret_cast<uint4*>(&s.hist[c * kThreads + 4 * threadIdx.x]) = uint4{0, 0, 0, 0};
+}
 
 // Inclusive sum over the lanes of a wave.
 __device__ __forceinline__ uint32_t scan(uint32_t v) {
@@ -160,15 +176,46 @@ struct Border {
   }
 };
 
+// Lists tokens p .. p + 3 of N rounds, behind a above the border and e on it, and counts on.
+template <int N>
+__device__ __forceinline__ void list(Border b, const uint32_t (&r)[N][kRun], int p, uint32_t& a,
+                                     uint32_t& e, int32_t* kept, Lds& s) {
+  const int wave = threadIdx.x >> 6;
+  uint32_t upto[N];
+#pragma unroll
+  for (int j = 0; j < N; j++) {
+    upto[j] = scan(b.count(r[j]));
+    if ((threadIdx.x & 63) == 63) s.rounds[j][wave] = upto[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < N; j++) {
+    // Compared again: the masks of all rounds kept from above are more than the scalar registers.
+    asm volatile("" : "+v"(b.border));
+    // the counts of a round are at most 4096 each: no carry
+    uint32_t v = upto[j] - b.count(r[j]), total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) {
+      const uint32_t u = s.rounds[j][i];
+      v += i < wave ? u : 0;
+      total += u;
+    }
+    b.put(kept, p + j * kRound, r[j], a + (v & 0xffff), e + (v >> 16));
+    a += total & 0xffff;
+    e += total >> 16;
+  }
+}
+
 template <int N>
 __device__ __forceinline__ void count_digits(const uint32_t (&r)[N][kRun], int shift, int bits,
                                              uint32_t prefix, Lds& s) {
+  const int copy = threadIdx.x % kCopies;
 #pragma unroll
   for (int j = 0; j < N; j++)
 #pragma unroll
     for (int i = 0; i < kRun; i++)
       if (r[j][i] != kAbsent && (shift == 21 || r[j][i] >> (shift + bits) == prefix))
-        atomicAdd(&s.hist[(r[j][i] >> shift) & ((1u << bits) - 1)], 1u);
+        atomicAdd(&s.hist[((r[j][i] >> shift) & ((1u << bits) - 1)) * kCopies + copy], 1u);
 }
 
 // A sequence of up to N rounds, in registers.
@@ -183,13 +230,16 @@ __device__ __forceinline__ void select(const Tokens& t, int64_t most, int32_t* k
   Border b{0, 0};
   uint32_t keep = (uint32_t)most, need = keep, prefix = 0;
   int shift = 32;
-  for (int bits : {11, 11, 10}) {
+#pragma unroll 1
+  for (int level = 0; level < 3; level++) {
+    const int bits = level < 2 ? 11 : 10;
     shift -= bits;
-    s.hist[tid] = s.hist[tid + kThreads] = 0;
+    clear_counts(s);
     __syncthreads();
     count_digits<N>(r, shift, bits, prefix, s);
     __syncthreads();
-    const Digit d = find_digit(s.hist[2047 - 2 * tid], s.hist[2046 - 2 * tid], need, s);
+    const uint2 n = counts_of(s, 2046 - 2 * tid);
+    const Digit d = find_digit(n.y, n.x, need, s);
     if (shift == 21 && d.total <= keep) {  // all that hold a token
       keep = d.total;
       break;
@@ -204,27 +254,8 @@ __device__ __forceinline__ void select(const Tokens& t, int64_t most, int32_t* k
   }
   if (len && tid == 0) *len = (int32_t)keep;
 
-  uint32_t upto[N];
-#pragma unroll
-  for (int j = 0; j < N; j++) {
-    upto[j] = scan(b.count(r[j]));
-    if ((tid & 63) == 63) s.rounds[j][wave] = upto[j];
-  }
-  __syncthreads();
   uint32_t a = 0, e = 0;
-#pragma unroll
-  for (int j = 0; j < N; j++) {
-#pragma unroll
-    for (int i = 0; i < kWaves; i++) {
-      const uint32_t u = s.rounds[j][i];
-      if (i == wave) {
-        const uint32_t v = upto[j] - b.count(r[j]);
-        b.put(kept, j * kRound + tid * kRun, r[j], a + (v & 0xffff), e + (v >> 16));
-      }
-      a += u & 0xffff;
-      e += u >> 16;
-    }
-  }
+  list<N>(b, r, tid * kRun, a, e, kept, s);
   for (int64_t i = keep + tid; i < most; i += kThreads) kept[i] = -1;
 }
 
@@ -257,7 +288,8 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(View c, const float
 // Launch `level` counts the chunks' tokens by digit `level` below the digits that are known by
 // then, which every workgroup of a sequence and head finds from all chunks' counts of the
 // launch before; the fourth launch lists. What a chunk has to list before its own is in the
-// counts of those ahead of it.
+// counts of those ahead of it. The first launch leaves the ranks side by side for the others:
+// in the pages a head's weights are 64 bytes apiece.
 struct Found {
   uint32_t prefix, need, keep;
   uint32_t digit[3];
@@ -267,12 +299,28 @@ struct Found {
 struct Long {
   uint32_t* hist;  // [pair][chunk][level][2048]
   Found* found;    // [pair][level]
+  uint32_t* ranks; // [pair][chunks * chunk]
   int chunks;      // a pair has at most
-  int64_t chunk;   // tokens, whole rounds
+  int64_t chunk;   // tokens, whole times 4 rounds
+
+  // Tokens p .. p + 3 of 4 rounds, absent from `end` on.
+  __device__ __forceinline__ void load(int64_t pair, int64_t p, int64_t end, uint32_t (&r)[4][kRun]) const {
+    const uint32_t* of = ranks + pair * chunks * chunk + p;
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint4*>(of + (p + j * kRound < end ? j * kRound : 0));
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t x[kRun] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int i = 0; i < kRun; i++) r[j][i] = p + j * kRound < end ? x[i] : kAbsent;
+    }
+  }
 };
 
+template <int level>
 __global__ void __launch_bounds__(kThreads)
-kv_select_long_kernel(View c, const float* __restrict__ w, Kept k, Long g, int level) {
+kv_select_long_kernel(View c, const float* __restrict__ w, Kept k, Long g) {
   __shared__ Lds lds;
   const int tid = threadIdx.x;
   const int chunk = (int)(blockIdx.x % g.chunks);
@@ -288,7 +336,7 @@ kv_select_long_kernel(View c, const float* __restrict__ w, Kept k, Long g, int l
 
   Found f{0, (uint32_t)k.keep, (uint32_t)k.keep, {0, 0, 0}, 0, 0};
   if (level > 0) {
-    if (level > 1) f = g.found[pair * 3 + level - 2];
+    if constexpr (level > 1) f = g.found[pair * 3 + level - 2];
     if (!f.done) {
       const int lv = level - 1;
       uint32_t hi = 0, lo = 0;
@@ -310,22 +358,30 @@ kv_select_long_kernel(View c, const float* __restrict__ w, Kept k, Long g, int l
         f.done = d.count == d.need;
       }
     }
-    if (level < 3 && chunk == 0 && tid == 0) g.found[pair * 3 + level - 1] = f;
+    if constexpr (level < 3)
+      if (chunk == 0 && tid == 0) g.found[pair * 3 + level - 1] = f;
   }
   const int64_t end = begin + g.chunk < t.len ? begin + g.chunk : t.len;
-  if (level < 3) {
+  if constexpr (level < 3) {
     if (f.done) return;
-    lds.hist[tid] = lds.hist[tid + kThreads] = 0;
+    clear_counts(lds);
     __syncthreads();
     for (int64_t p = begin + tid * kRun; p < end; p += 4 * kRound) {
       uint32_t r[4][kRun];
-      t.load<4>(p, end, r);
+      if constexpr (level == 0) {
+        t.load<4>(p, end, r);
+        uint32_t* of = g.ranks + pair * g.chunks * g.chunk + p;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (p + j * kRound < end)
+            *reinterpret_cast<uint4*>(of + j * kRound) = uint4{r[j][0], r[j][1], r[j][2], r[j][3]};
+      } else {
+        g.load(pair, p, end, r);
+      }
       count_digits<4>(r, shift(level), bits(level), f.prefix, lds);
     }
     __syncthreads();
-    uint32_t* out = hist(chunk, level);
-    out[tid] = lds.hist[tid];
-    out[tid + kThreads] = lds.hist[tid + kThreads];
+    *reinterpret_cast<uint2*>(hist(chunk, level) + 2 * tid) = counts_of(lds, 2 * tid);
     return;
   }
 
@@ -334,15 +390,17 @@ kv_select_long_kernel(View c, const float* __restrict__ w, Kept k, Long g, int l
   const Border b = f.done == 2 ? Border{0, 0} : f.done ? Border{edge - 1, 0} : Border{edge, f.need};
   // what the chunks ahead list: tokens of higher digits, and of the last one where all are kept
   uint32_t a = 0, e = 0;
+#pragma unroll 1
   for (int lv = 0; lv < f.levels; lv++) {
-#pragma unroll 8
+    const uint32_t at = lv == 0 ? f.digit[0] : lv == 1 ? f.digit[1] : f.digit[2];
+#pragma unroll 4
     for (int ch = 0; ch < chunk; ch++) {
       const uint2 u = *reinterpret_cast<const uint2*>(hist(ch, lv) + 2 * tid);
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const uint32_t digit = 2 * tid + i, n = i ? u.y : u.x;
-        a += f.done == 2 || digit > f.digit[lv] || (f.done && lv == last && digit == f.digit[lv]) ? n : 0;
-        e += !f.done && lv == last && digit == f.digit[lv] ? n : 0;
+        a += f.done == 2 || digit > at || (f.done && lv == last && digit == at) ? n : 0;
+        e += !f.done && lv == last && digit == at ? n : 0;
       }
     }
   }
@@ -353,15 +411,10 @@ kv_select_long_kernel(View c, const float* __restrict__ w, Kept k, Long g, int l
   a = all_a, e = all_e;
   for (int64_t base = begin; base < end; base += 4 * kRound) {
     uint32_t r[4][kRun];
-    t.load<4>(base + tid * kRun, end, r);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      uint32_t total;
-      const uint32_t v = before_me(b.count(r[j]), total, lds);
-      b.put(kept, (int)(base + j * kRound + tid * kRun), r[j], a + (v & 0xffff), e + (v >> 16));
-      a += total & 0xffff;
-      e += total >> 16;
-    }
+    const int64_t p = base + tid * kRun;
+    g.load(pair, p < end ? p : base, p < end ? end : 0, r);
+    __syncthreads();
+    list<4>(b, r, (int)(base + tid * kRun), a, e, kept, lds);
   }
   if (chunk == 0) {
     if (h == 0 && tid == 0) k.lens[s] = (int32_t)f.keep;
@@ -406,9 +459,9 @@ KvEvictPlan plan_kv_evict(int nseq, int kv_heads, int64_t most) {
   p.seqs = std::max(1, (1 << 21) / kv_heads);  // a grid's threads are a 32-bit number
   if (most > 16 * kRound) {
     const int64_t chunks = std::min<int64_t>(64, std::max(1, (1 << 20) / kv_heads));
-    p.chunk = std::max<int64_t>(4 * kRound, round_up(ceil_div(most, chunks), kRound));
+    p.chunk = round_up(ceil_div(most, chunks), 4 * kRound);
     p.chunks = (int)ceil_div(most, p.chunk);
-    const int64_t pair = (int64_t)p.chunks * 3 * 2048 * 4 + 3 * (int64_t)sizeof(Found);
+    const int64_t pair = p.chunks * (3 * 2048 + p.chunk) * 4 + 3 * (int64_t)sizeof(Found);
     p.seqs = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t(1) << 28) / (pair * kv_heads),
                                                          (1 << 20) / ((int64_t)p.chunks * kv_heads)));
     p.seqs = std::min(p.seqs, nseq);
@@ -428,13 +481,13 @@ hipError_t launch_kv_evict(const View& c, float* w, const Kept& k, const KvEvict
     const unsigned pairs = (unsigned)(v.nseq * c.kv_heads);
     hipError_t e;
     if (p.chunks) {
-      const Long g{static_cast<uint32_t*>(scratch),
-                   reinterpret_cast<Found*>(static_cast<char*>(scratch) +
-                                            (int64_t)pairs * p.chunks * 3 * 2048 * 4),
-                   p.chunks, p.chunk};
-      for (int level = 0; level < 4; level++) {
-        hipLaunchKernelGGL(kv_select_long_kernel, dim3(pairs * p.chunks), dim3(kThreads), 0, s, v, w, q,
-                           g, level);
+      uint32_t* hist = static_cast<uint32_t*>(scratch);
+      uint32_t* ranks = hist + (int64_t)pairs * p.chunks * 3 * 2048;
+      const Long g{hist, reinterpret_cast<Found*>(ranks + pairs * p.chunks * p.chunk), ranks, p.chunks,
+                   p.chunk};
+      for (auto kernel : {kv_select_long_kernel<0>, kv_select_long_kernel<1>, kv_select_long_kernel<2>,
+                          kv_select_long_kernel<3>}) {
+        hipLaunchKernelGGL(kernel, dim3(pairs * p.chunks), dim3(kThreads), 0, s, v, w, q, g);
         if ((e = hipGetLastError()) != hipSuccess) return e;
       }
     } else {
