@@ -572,7 +572,7 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
  * are and their positions (-1 behind the last). Of b, lens and table are read. The pages left
  * are as they were; what goes to a page id outside the pool is lost. A page of to_table may
  * be in no sequence's table and in to_table once only. first + last <= keep; no output may
- * overlap another array (to_lens is not b's lens). Stream-ordered; tables of more than 65536
+ * overlap another array (to_lens is not b's lens). Stream-ordered; tables of more than 16384
  * tokens take scratch from the stream's workspace (a capture then needs one call of the same
  * shape before it). */
 int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, int64_t first,

@@ -73,11 +73,12 @@ struct Tokens {
   }
 };
 
+// Many weights have the same high digit, and lanes that count the same digit wait for each other.
 constexpr int kCopies = 2;
 struct Lds {
   __attribute__((aligned(16))) uint32_t hist[2048 * kCopies];  // [digit][lane % kCopies]
   uint32_t wave[kWaves];
-  uint32_t rounds[16][kWaves];
+  uint32_t rounds[4][kWaves];
   uint32_t found[3];
 };
 
@@ -277,10 +278,8 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(View c, const float
     for (int64_t i = threadIdx.x; i < k.keep; i += kThreads) kept[i] = -1;
   } else if (t.len <= kRound)
     select<1>(t, k.keep, kept, to, lds);
-  else if (t.len <= 4 * kRound)
-    select<4>(t, k.keep, kept, to, lds);
   else
-    select<16>(t, k.keep, kept, to, lds);
+    select<4>(t, k.keep, kept, to, lds);
 }
 
 // ---- sequences that may be longer: their tokens in chunks, a workgroup each ----
@@ -457,7 +456,7 @@ __global__ void __launch_bounds__(256) kv_move_kernel(View c, float* __restrict_
 KvEvictPlan plan_kv_evict(int nseq, int kv_heads, int64_t most) {
   KvEvictPlan p{};
   p.seqs = std::max(1, (1 << 21) / kv_heads);  // a grid's threads are a 32-bit number
-  if (most > 16 * kRound) {
+  if (most > 4 * kRound) {
     const int64_t chunks = std::min<int64_t>(64, std::max(1, (1 << 20) / kv_heads));
     p.chunk = round_up(ceil_div(most, chunks), 4 * kRound);
     p.chunks = (int)ceil_div(most, p.chunk);
