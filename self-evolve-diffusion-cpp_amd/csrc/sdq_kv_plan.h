@@ -24,8 +24,9 @@ struct Plan {
 };
 
 // T rows of nseq sequences, group query heads to each of kv_heads cached ones,
-// most: the keys a sequence can have.
-inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count, int tall = 0) {
+// most: the keys a sequence can have; few rows over up to `whole` of them are not cut.
+inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count, int tall = 0,
+                 int64_t whole = 0) {
   Plan p{};
   const int64_t rows = T * group;
   // Rows of a sequence, on average: only their sum is known here. Any choice is
@@ -49,6 +50,7 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   const int64_t least = p.rows == kFewRows ? 256 : 512;  // keys of a share
   int64_t s = std::min<int64_t>(want / std::max<int64_t>(groups, 1), most / least);
   s = std::max<int64_t>(1, std::min<int64_t>(s, kMaxSplits));
+  if (p.rows == kFewRows && most <= whole) s = 1;
   const int64_t per = (int64_t)kv_heads * p.rows * (128 + 2) * 4;  // bytes a tile and share
   while (s > 1 && p.tiles * per * s > kMaxScratch) s--;
   p.splits = (int)s;

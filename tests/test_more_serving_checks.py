@@ -166,7 +166,7 @@ def test_every_shared_plan_fits(tmp_path):
 
 
 @pytest.mark.slow
-@pytest.mark.parametrize("src", ["sdq_kv_weights.hip", "sdq_kv_evict.hip"])
+@pytest.mark.parametrize("src", ["sdq_kv_packed.hip", "sdq_kv_weights.hip", "sdq_kv_evict.hip"])
 def test_no_hazard(tmp_path, src):
     if not os.path.exists(HIPCC):
         pytest.skip("hipcc not available")
