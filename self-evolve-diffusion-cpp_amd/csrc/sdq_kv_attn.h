@@ -312,18 +312,20 @@ __device__ __forceinline__ float quad_sum(float v) {
   return quad(v, [](float a, float b) { return a + b; });
 }
 
-// x - hi of either half of a pair of fp16, exact, in one operation.
+// x - hi of either half of a pair of fp16, exact, in one operation. The factor is hidden from
+// the compiler, which makes a conversion and a subtraction of the plain form. Written by hand the
+// operation would not be seen as one that may not yet write over an operand of a matrix
+// instruction.
+__device__ __forceinline__ float minus_one() {
+  float m = -1.f;
+  asm("" : "+s"(m));
+  return m;
+}
 __device__ __forceinline__ float less_low(v2h hi, float x) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(hi), "v"(x));
-  return r;
+  return __builtin_fmaf((float)hi[0], minus_one(), x);
 }
 __device__ __forceinline__ float less_high(v2h hi, float x) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-      : "=v"(r)
-      : "v"(hi), "v"(x));
-  return r;
+  return __builtin_fmaf((float)hi[1], minus_one(), x);
 }
 // fp32 to two fp16 parts, both rounded (two conversions at a time): the high
 // part's remainder is exact, so the pair is off by at most 2^-22.
