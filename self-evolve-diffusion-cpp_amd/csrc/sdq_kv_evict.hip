@@ -287,8 +287,7 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(View c, const float
 // Launch `level` counts the chunks' tokens by digit `level` below the digits that are known by
 // then, which every workgroup of a sequence and head finds from all chunks' counts of the
 // launch before; the fourth launch lists. What a chunk has to list before its own is in the
-// counts of those ahead of it. The first launch leaves the ranks side by side for the others:
-// in the pages a head's weights are 64 bytes apiece.
+// counts of those ahead of it.
 struct Found {
   uint32_t prefix, need, keep;
   uint32_t digit[3];
@@ -298,23 +297,8 @@ struct Found {
 struct Long {
   uint32_t* hist;  // [pair][chunk][level][2048]
   Found* found;    // [pair][level]
-  uint32_t* ranks; // [pair][chunks * chunk]
   int chunks;      // a pair has at most
   int64_t chunk;   // tokens, whole times 4 rounds
-
-  // Tokens p .. p + 3 of 4 rounds, absent from `end` on.
-  __device__ __forceinline__ void load(int64_t pair, int64_t p, int64_t end, uint32_t (&r)[4][kRun]) const {
-    const uint32_t* of = ranks + pair * chunks * chunk + p;
-    uint4 v[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint4*>(of + (p + j * kRound < end ? j * kRound : 0));
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const uint32_t x[kRun] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-      for (int i = 0; i < kRun; i++) r[j][i] = p + j * kRound < end ? x[i] : kAbsent;
-    }
-  }
 };
 
 template <int level>
@@ -367,16 +351,7 @@ kv_select_long_kernel(View c, const float* __restrict__ w, Kept k, Long g) {
     __syncthreads();
     for (int64_t p = begin + tid * kRun; p < end; p += 4 * kRound) {
       uint32_t r[4][kRun];
-      if constexpr (level == 0) {
-        t.load<4>(p, end, r);
-        uint32_t* of = g.ranks + pair * g.chunks * g.chunk + p;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (p + j * kRound < end)
-            *reinterpret_cast<uint4*>(of + j * kRound) = uint4{r[j][0], r[j][1], r[j][2], r[j][3]};
-      } else {
-        g.load(pair, p, end, r);
-      }
+      t.load<4>(p, end, r);
       count_digits<4>(r, shift(level), bits(level), f.prefix, lds);
     }
     __syncthreads();
@@ -411,9 +386,9 @@ kv_select_long_kernel(View c, const float* __restrict__ w, Kept k, Long g) {
   for (int64_t base = begin; base < end; base += 4 * kRound) {
     uint32_t r[4][kRun];
     const int64_t p = base + tid * kRun;
-    g.load(pair, p < end ? p : base, p < end ? end : 0, r);
-    __syncthreads();
-    list<4>(b, r, (int)(base + tid * kRun), a, e, kept, lds);
+    t.load<4>(p, end, r);
+    __syncthreads();  // the last rounds' counts are read
+    list<4>(b, r, (int)p, a, e, kept, lds);
   }
   if (chunk == 0) {
     if (h == 0 && tid == 0) k.lens[s] = (int32_t)f.keep;
@@ -460,7 +435,7 @@ KvEvictPlan plan_kv_evict(int nseq, int kv_heads, int64_t most) {
     const int64_t chunks = std::min<int64_t>(64, std::max(1, (1 << 20) / kv_heads));
     p.chunk = round_up(ceil_div(most, chunks), 4 * kRound);
     p.chunks = (int)ceil_div(most, p.chunk);
-    const int64_t pair = p.chunks * (3 * 2048 + p.chunk) * 4 + 3 * (int64_t)sizeof(Found);
+    const int64_t pair = p.chunks * 3 * 2048 * 4 + 3 * (int64_t)sizeof(Found);
     p.seqs = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t(1) << 28) / (pair * kv_heads),
                                                          (1 << 20) / ((int64_t)p.chunks * kv_heads)));
     p.seqs = std::min(p.seqs, nseq);
@@ -481,8 +456,7 @@ hipError_t launch_kv_evict(const View& c, float* w, const Kept& k, const KvEvict
     hipError_t e;
     if (p.chunks) {
       uint32_t* hist = static_cast<uint32_t*>(scratch);
-      uint32_t* ranks = hist + (int64_t)pairs * p.chunks * 3 * 2048;
-      const Long g{hist, reinterpret_cast<Found*>(ranks + pairs * p.chunks * p.chunk), ranks, p.chunks,
+      const Long g{hist, reinterpret_cast<Found*>(hist + (int64_t)pairs * p.chunks * 3 * 2048), p.chunks,
                    p.chunk};
       for (auto kernel : {kv_select_long_kernel<0>, kv_select_long_kernel<1>, kv_select_long_kernel<2>,
                           kv_select_long_kernel<3>}) {
