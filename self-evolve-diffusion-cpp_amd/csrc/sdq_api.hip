@@ -1059,6 +1059,13 @@ int kv_rows(const std::string& tag, const char* name, const float* p, int64_t ld
 // Scales of a cache's keys (or values).
 size_t kv_scales(const kv::View& v) { return ((size_t)v.pages * v.kv_heads) << v.page_log2; }
 
+// Memory that meets the cache's, whose scales take `scales` bytes.
+bool kv_overlaps(const sdq_kv_cache* c, const void* p, size_t n, size_t scales) {
+  const size_t codes = scales / 4 * kv::kHd;
+  return bytes_overlap(p, n, c->ks, scales) || bytes_overlap(p, n, c->vs, scales) ||
+         bytes_overlap(p, n, c->k, codes) || bytes_overlap(p, n, c->v, codes);
+}
+
 // A checked call of one of the paged attentions (view.T == 0: nothing to do).
 struct KvCall {
   kv::View view;
@@ -2563,7 +2570,7 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
   const size_t nw = kv_scales(call.view) * 4;
   if (bytes_overlap(weights, nw, out, (size_t)((T - 1) * ldo + (int64_t)heads * kv::kHd) * 4) ||
       bytes_overlap(weights, nw, q, (size_t)((T - 1) * ldq + (int64_t)heads * kv::kHd) * 4) ||
-      bytes_overlap(weights, nw, c->ks, nw))
+      kv_overlaps(c, weights, nw, nw))
     return set_error(SDQ_ERR_INVALID, tag + ": weights overlaps another array");
   if ((rc = usable_device(&call.dev))) return rc;
   const hipStream_t s = stream_of(stream);
@@ -2638,7 +2645,7 @@ int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, i
            bytes_overlap(p, n, to_table, nto) || bytes_overlap(p, n, weights, nw);
   };
   if (meets(to_lens, nl) || meets(kept, nk) || bytes_overlap(to_lens, nl, kept, nk) ||
-      bytes_overlap(weights, nw, c->ks, nw) || bytes_overlap(weights, nw, c->vs, nw))
+      kv_overlaps(c, weights, nw, nw) || kv_overlaps(c, to_lens, nl, nw) || kv_overlaps(c, kept, nk, nw))
     return set_error(SDQ_ERR_INVALID, tag + ": an output overlaps another array");
   int dev = -1;
   if ((rc = usable_device(&dev))) return rc;

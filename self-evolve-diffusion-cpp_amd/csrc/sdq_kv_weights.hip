@@ -256,6 +256,9 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           float v = any_far ? sum[kt][i] : __builtin_ldexpf(sum[kt][i], -(int)ke[kt][i]);
+          // A row that sees a scale of infinity or NaN gives it no weight or has none itself, but
+          // makes a NaN here.
+          if (!(fabsf(kc[kt][i]) <= 3.402823466e38f)) v = 0.f;
 #pragma unroll
           for (int o = 8; o; o >>= 1) v += __shfl_xor(v, o);
           mine = r16 == 4 * kt + i ? v : mine;
@@ -306,8 +309,9 @@ KvWeightsPlan plan_kv_weights(int64_t T, int nseq, int group, int kv_heads, int6
   p.cut = T * group / nseq >= 128;
   const int64_t blocks = ceil_div(std::max<int64_t>(most, 1), kBlock);
   p.across = (int)std::max<int64_t>(1, std::min(p.cut ? want : blocks, ceil_div(want, pairs)));
-  // sequences at a time that a grid's 32-bit thread count takes
-  p.seqs = (int)std::min<int64_t>(nseq, std::max<int64_t>(1, (int64_t(1) << 22) / ((int64_t)p.across * kv_heads)));
+  // sequences at a time that a grid's 32-bit thread count takes, and 512 MiB of ranges' sums
+  p.seqs = (int)std::min<int64_t>(
+      nseq, std::max<int64_t>(1, (int64_t(1) << (p.cut ? 15 : 22)) / ((int64_t)p.across * kv_heads)));
   if (p.cut) p.scratch_bytes = (int64_t)p.seqs * kv_heads * 8 * p.across * kBlock * 4;
   return p;
 }

@@ -484,6 +484,36 @@ def test_weights_bad_rows_and_pages(sdq_dev, new):
     assert_bitexact(runs[1], runs[0], "twice")
 
 
+@pytest.mark.parametrize("scale", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("new,L", [(12, 40), (90, 700), (1100, 1100)])
+def test_weights_bad_scale(sdq_dev, new, L, scale):
+    """A key whose scale is no number: rows whose logit of it is NaN or infinity add nothing, the
+    others what they add without it, and itself gets nothing."""
+    c = More(sdq_dev, [new], [L], 1, 16, seed=21)
+    key = L - new // 2
+    at = c.table[0, key // 16], 0, key % 16
+    q, w = c.queries(2), c.rng.uniform(0, 0.1, (c.pages, 1, 16)).astype(F)
+    k, v, see = c.own(0, 0, True)
+    want, tol = np.zeros(L), np.zeros(L)
+    for j in range(2):
+        x = q[:, j * HD:(j + 1) * HD]
+        dot = (x.astype(np.float64) @ k[key]) * scale
+        lost = see[:, key] & ~(dot < 0)
+        rest = see.copy()
+        rest[:, key] = False
+        _, _, wt, rel = soft(x, k, v, rest, HD**-0.5)
+        want += (wt * ~lost[:, None]).sum(0)
+        tol += (wt * rel * ~lost[:, None]).sum(0)
+    p = np.arange(L)
+    place = c.table[0, p // 16], 0, p % 16
+    want += np.where(p < L - new, w[place], 0)
+    c.ks[at] = scale
+    c.up()
+    tw, out = c.t(w), c.torch.zeros((c.T, 256), device=sdq_dev)
+    c.sdq.kv_attention_weights(c.cache, c.batch, tw, c.t(q), out, 2)
+    c.close(tw.cpu().numpy()[place], want, tol + (new / 8 + 16) * 2.0**-24 * want + 1e-37)
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_weights_range(sdq_dev, new):
     """Value scales 2^60 apart do not enter the weights; sharp and huge logits."""

@@ -81,6 +81,9 @@ def test_weights():
     _refused("null weights", "sdq_kv_attention_weights", c, b, None, *rows)
     for w in (Q, Q + 512, O - 64, P):
         _refused("overlaps", "sdq_kv_attention_weights", c, b, w, *rows)
+    c, b = _kv(k=P, ks=P << 1, v=P << 2, vs=P << 3)
+    for w in (P, P << 1, P << 2, P << 3, (P << 2) + 4096):
+        _refused("overlaps", "sdq_kv_attention_weights", c, b, w, *rows)
 
 
 def test_evict():
@@ -100,7 +103,9 @@ def test_evict():
                       ("null", dict(kept=None)), ("overlaps", dict(lens=P << 4)),
                       ("overlaps", dict(lens=(P << 5) + 28)), ("overlaps", dict(kept=TO - 4)),
                       ("overlaps", dict(lens=K + 16)), ("overlaps", dict(kept=W - 4)),
-                      ("overlaps", dict(w=P << 1)), ("overlaps", dict(w=(P << 3) + 64))):
+                      ("overlaps", dict(w=P << 1)), ("overlaps", dict(w=(P << 3) + 64)),
+                      ("overlaps", dict(w=P)), ("overlaps", dict(lens=P << 3)),
+                      ("overlaps", dict(kept=P << 2))):
         _refused(match, "sdq_kv_evict", *call(**kw))
     _refused("null cache or batch", "sdq_kv_evict", None, *call()[1:])
     _refused("null cache or batch", "sdq_kv_evict", c, None, *call()[2:])
