@@ -510,7 +510,7 @@ int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t 
  * rows a sequence, and chunks too few for the machine, cut the keys into shares joined
  * by a second kernel, their scratch from the stream's workspace: a capture needs one call
  * of the same shape before it (SDQ_ERR_INVALID otherwise, the capture stays usable).
- * A row's result depends on no other row's contents, nor on timing. */
+ * A row's result depends on no other row's contents, nor on timing. T * heads is at most 2^31. */
 int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
                      float* out, int64_t ldo, int64_t T, int heads, float scale, int causal,
                      void* stream);
@@ -519,8 +519,10 @@ int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* 
  * context over all denoising steps, the other branch's tokens): rows [q_start[s],
  * q_start[s+1]) see all lens[s] tokens of sequence s, however many rows there are;
  *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / (heads/kv_heads)]) v[j, ...].
- * Rows of a sequence without tokens get 0. Everything else as sdq_kv_attention.
- * Cached counterpart of sdq_sdpa_batched, whose sequences have one length
+ * Rows of a sequence without tokens get 0. Everything else as sdq_kv_attention; besides, where
+ * the sequences have 1024 rows a cached head and more, on average, the scratch holds the keys as
+ * MFMA operands, 528 bytes a token of the table and cached head, if they fit 512 MiB (the same
+ * bits as without). Cached counterpart of sdq_sdpa_batched, whose sequences have one length
  * (src/model/ovi_dit.cpp:241, 249). */
 int sdq_kv_cross_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
                            float* out, int64_t ldo, int64_t T, int heads, float scale,
@@ -556,10 +558,13 @@ int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, 
  *                                                   the call's rows (whose places are new)
  *   weights[place of j] = weights[place of j] + sum for the tokens before them
  * weights: device memory of the caller, [pages, kv_heads, page_size] f32 as the cache's
- * scales, with a float's alignment. fp32 sums in the order of rows; the same bits every time.
- * Rows that hold a NaN or an infinity add nothing. No two of the call's sequences may have a
- * page in common (their sums would be lost in part). Scratch from the stream's workspace in
- * every call. */
+ * scales, with a float's alignment; it overlaps no other array. fp32 sums, each row's weights
+ * added in a fixed order: the same bits every time. Rows whose softmax is no number (a NaN or an
+ * infinity in q, in the scale of a key that they see) add nothing. No page may stand twice in the
+ * tables of the call's sequences (sums would be lost in part). Scratch from the stream's
+ * workspace in every call (a capture needs one call of the same shape before it): up to 32 rows
+ * of q a sequence and cached head, on average, their logits, if they fit 512 MiB, else 528 bytes a
+ * row of q and head, and what sdq_kv_cross_attention takes. */
 int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights,
                              const float* q, int64_t ldq, float* out, int64_t ldo, int64_t T,
                              int heads, float scale, int causal, void* stream);
@@ -572,9 +577,9 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
  * are and their positions (-1 behind the last). Of b, lens and table are read. The pages left
  * are as they were; what goes to a page id outside the pool is lost. A page of to_table may
  * be in no sequence's table and in to_table once only. first + last <= keep; no output may
- * overlap another array (to_lens is not b's lens). Stream-ordered; tables of more than 16384
- * tokens take scratch from the stream's workspace (a capture then needs one call of the same
- * shape before it). */
+ * overlap another array (to_lens is not b's lens), nor weights the cache. Stream-ordered;
+ * tables of more than 16384 tokens take scratch from the stream's workspace (a capture then
+ * needs one call of the same shape before it). */
 int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, int64_t first,
                  int64_t last, int64_t keep, const int32_t* to_table, int64_t to_max_pages,
                  int32_t* to_lens, int32_t* kept, void* stream);

@@ -1093,9 +1093,9 @@ int kv_call(const sdq_kv_cache* c, const sdq_kv_batch* b, const KvRows& r, int64
     return set_error(SDQ_ERR_INVALID, tag + ": out overlaps q");
   return SDQ_OK;
 }
-kvplan::Plan plan_of(const KvCall& k, int tall = 0, int64_t whole = 0) {
+kvplan::Plan plan_of(const KvCall& k, kvplan::Kind kind = kvplan::kOwn) {
   return kvplan::plan(k.view.T, k.view.nseq, k.rows.heads / k.view.kv_heads, k.view.kv_heads,
-                      k.view.max_pages << k.view.page_log2, g_dev[k.dev].cu_count, tall, whole);
+                      k.view.max_pages << k.view.page_log2, g_dev[k.dev].cu_count, kind);
 }
 
 // Host -> device through the first two slots' pinned buffers, on the first
@@ -2509,9 +2509,7 @@ int sdq_kv_cross_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const f
   if (rc || call.view.T == 0) return rc;
   if ((rc = usable_device(&call.dev))) return rc;
   const hipStream_t s = stream_of(stream);
-  // Joining costs a launch, 3 us and more: 512 keys 12.6 us for 15.9 in two shares (8 rows, 24
-  // heads), 700 keys 15.0 for 16.9, 1024 keys 17.7 for 21.5, but 17.3 for 15.8 of 4 rows.
-  const kvplan::Plan plan = plan_of(call, 0, 768);
+  const kvplan::Plan plan = plan_of(call, kvplan::kCross);
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
   // the shares' sums, and the keys as operands

@@ -23,10 +23,15 @@ struct Plan {
   int64_t scratch_bytes;     // 0: none
 };
 
+// Whose plan: a sequence's last tokens over its own keys; rows over other keys; shared parts'
+// rows over those, and over the keys behind them.
+enum Kind { kOwn, kCross, kPart, kRest };
+constexpr int kWhole = 768;  // keys that cross attention's few rows take in one share
+
 // T rows of nseq sequences, group query heads to each of kv_heads cached ones,
-// most: the keys a sequence can have; few rows over up to `whole` of them are not cut.
-inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count, int tall = 0,
-                 int64_t whole = 0) {
+// most: the keys a sequence can have.
+inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count,
+                 Kind kind = kOwn) {
   Plan p{};
   const int64_t rows = T * group;
   // Rows of a sequence, on average: only their sum is known here. Any choice is
@@ -36,7 +41,20 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   // rows 30 and 39, 48 rows 38 and 40, 72 rows 42 and 41, 144 rows 68 and 49.
   const int64_t mean = (rows + nseq - 1) / nseq;
   p.rows = mean <= 32 ? kFewRows : mean <= 128 ? 64 : 256;
-  if (p.rows == 256 && tall) p.rows = tall;
+  if (p.rows == 256 && kind == kPart) p.rows = 128;
+  // Few rows' tiles have the shorter way from a call to its result, and one for each 16 rows has
+  // more of the CUs (us, cross attention): 512 keys, 8 cached heads, one sequence of 256 rows 11.6
+  // for 26.8 with 64 and 38.9 with 256; 24 heads, four of 128 rows 23.7, 33.2 and 31.2, but
+  // sixteen of 64 rows 42.9, 37.2 and 58.7. 4099 keys: 24 heads, four of 96 rows 100, 115, 121;
+  // sixteen 303, 434, 411; 8 heads, four of 128 rows 44.3, 44.2, 43.8, one of 256 rows 33, 36 and
+  // 48. Shared parts of 8209 keys, 8 heads: 256 rows 47 for 57 with 128, 512 rows 78 for 77; 300 keys
+  // behind them, four of 48 rows 42 for 48 with 64. From 1024 rows on cross attention's chunks have
+  // an order of their own (sdq_kv_packed.hip). Own keys keep the heights above, and their bits.
+  const int64_t few = (mean + kFewRows - 1) / kFewRows * nseq * kv_heads;  // workgroups
+  const bool whole = kind == kCross && most <= kWhole;
+  if (whole ? mean < 1024 && few <= 4 * cu_count
+            : (kind == kCross && mean <= 96) || (kind != kOwn && mean <= 256 && few <= cu_count / 2))
+    p.rows = kFewRows;
   // Numbers of tiles: rows / height and one a sequence (csrc/sdq_kv_attn.hip); those that
   // hold one are at most the sum of ceil(rows_s / height) over the sequences that have any.
   p.tiles = rows / p.rows + nseq;
@@ -50,7 +68,9 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   const int64_t least = p.rows == kFewRows ? 256 : 512;  // keys of a share
   int64_t s = std::min<int64_t>(want / std::max<int64_t>(groups, 1), most / least);
   s = std::max<int64_t>(1, std::min<int64_t>(s, kMaxSplits));
-  if (p.rows == kFewRows && most <= whole) s = 1;
+  // Joining costs a launch, 3 us and more: 512 keys 12.6 us for 15.9 in two shares (8 rows, 24
+  // heads), 700 keys 15.0 for 16.9, 1024 keys 17.7 for 21.5, but 17.3 for 15.8 of 4 rows.
+  if (p.rows == kFewRows && whole) s = 1;
   const int64_t per = (int64_t)kv_heads * p.rows * (128 + 2) * 4;  // bytes a tile and share
   while (s > 1 && p.tiles * per * s > kMaxScratch) s--;
   p.splits = (int)s;
@@ -81,9 +101,9 @@ constexpr int kMaxShares = 128, kMaxOwnShares = 16;
 inline SharedPlan shared_plan(int64_t T, int nseq, int n, int group, int kv_heads, int64_t most,
                               int64_t most_pre, int cu_count) {
   SharedPlan p{};
-  p.own = plan(T, nseq, group, kv_heads, most, cu_count);
+  p.own = plan(T, nseq, group, kv_heads, most, cu_count, kRest);
   p.own.splits = std::min(p.own.splits, kMaxOwnShares);
-  p.pre = plan(T, n, group, kv_heads, most_pre, cu_count, 128);
+  p.pre = plan(T, n, group, kv_heads, most_pre, cu_count, kPart);
   // How many tiles the parts' rows make is known on the device, which cuts their keys into that
   // many shares that two workgroups a CU are at work; here the most that can be. Rows of no
   // sequence, and tiles that a part does not fill, leave room for one more than the rows say.

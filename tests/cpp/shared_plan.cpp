@@ -1,5 +1,6 @@
-// Sweeps the plan of attention over shared parts (csrc/sdq_kv_plan.h): every launch's grid
-// and the scratch within bounds, and the shares of a row as many as a wave's lanes at most.
+// Sweeps the plans of attention over shared parts and of cross attention (csrc/sdq_kv_plan.h):
+// every launch's grid and the scratch within bounds, and the shares of a row as many as a wave's
+// lanes take.
 #include <cstdio>
 #include <random>
 
@@ -42,6 +43,14 @@ int main() {
       REQUIRE(at_once * p.heads * q->splits * block <= 0xffffffffll);
       REQUIRE(q->tiles >= T * group / q->rows);
     }
+    const kp::Plan c = kp::plan(T, nseq, group, kvh, most, 256, kp::kCross);
+    const int64_t at_once = std::min(c.tiles, c.tiles_per_launch) * kvh * c.splits;
+    REQUIRE(c.rows == 16 || c.rows == 64 || c.rows == 256);
+    REQUIRE(c.splits >= 1 && c.splits <= kp::kMaxSplits && c.tiles_per_launch >= 1);
+    REQUIRE(c.tiles >= T * group / c.rows + nseq);
+    REQUIRE(at_once * 512 <= 0xffffffffll && c.scratch_bytes <= kp::kMaxScratch);
+    REQUIRE(c.splits == 1 || (c.tiles_per_launch >= c.tiles && c.scratch_bytes > c.part_bytes));
+    REQUIRE(c.splits == 1 || at_once / c.splits * c.rows * 256 <= 0xffffffffll);
   }
   return 0;
 }

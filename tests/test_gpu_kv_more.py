@@ -266,7 +266,7 @@ def test_cross(sdq_dev, rows, lens, heads, kvh):
 @pytest.mark.parametrize("heads,kvh", [(2, 2), (3, 1)])
 def test_cross_of_thousands(sdq_dev, rows, lens, heads, kvh):
     """Rows enough for keys that are turned to operands once; their first rows alone, which take
-    the other form, have the same bits."""
+    the other form beside a table of more keys, have the same bits."""
     import torch
 
     c = More(sdq_dev, rows, lens, kvh, (16, 64, 32)[len(rows) % 3], seed=sum(rows), first=1, behind=2)
@@ -275,7 +275,9 @@ def test_cross_of_thousands(sdq_dev, rows, lens, heads, kvh):
     q = c.queries(heads)
     got = c.check_cross(heads, q=q)
     if len(rows) == 1:
-        few = c.sdq.KvBatch(c.t(np.array([0, 700], np.int32)), c.batch.lens, c.batch.table)
+        table = np.full((1, 800 // c.page + 1), -1, np.int32)
+        table[:, :c.table.shape[1]] = c.table
+        few = c.sdq.KvBatch(c.t(np.array([0, 700], np.int32)), c.batch.lens, c.t(table))
         out = torch.zeros((700, heads * HD), device=sdq_dev)
         c.sdq.kv_cross_attention(c.cache, few, c.t(q[1:701]), out, heads)
         assert_bitexact(out.cpu().numpy(), got[1:701])
@@ -301,9 +303,19 @@ def test_cross_scale_strides_missing_pages(sdq_dev, rows):
     assert (got[:, :256] == -2).all() and (got[:, 768:896] == -2).all() and (got[:, 1408:] == -2).all()
 
 
-@pytest.mark.parametrize("n", [1, 33, 200])
+@pytest.mark.parametrize("rows,lens", [([110] * 5, [900, 0, 1500, 33, 800]), ([100] * 20, [90, 700] * 10),
+                                       ([300] * 8, [500, 1, 64, 127] * 2)])
+@pytest.mark.parametrize("heads", [8, 16])
+def test_cross_of_many_sequences(sdq_dev, rows, lens, heads):
+    """Work enough for the taller tiles."""
+    c = More(sdq_dev, rows, lens, 8, 32, seed=len(rows) + heads, first=1, behind=2)
+    c.check_cross(heads)
+
+
+@pytest.mark.parametrize("n", [1, 16, 600])
 def test_cross_of_as_many_rows(sdq_dev, n):
-    """As many rows as keys: the bits of kv_attention without its causal mask."""
+    """As many rows as keys: the bits of kv_attention without its causal mask, where both take tiles
+    of the same height."""
     import torch
 
     c = More(sdq_dev, [n, n], [n, n], 2, 32, seed=n)
@@ -436,6 +448,18 @@ def test_shared_many_sequences(sdq_dev, nseq, n):
     c = More(sdq_dev, new, new + rng.integers(0, 30, nseq), 1, 16, seed=13, first=2, behind=1)
     c.share(np.sort(rng.integers(0, nseq + 1, n + 1)), rng.integers(0, 90, n))
     c.check_shared(3)
+
+
+@pytest.mark.parametrize("new,parts", [(20, 6), (50, 3), (140, 2)])
+@pytest.mark.parametrize("heads", [8, 16])
+def test_shared_of_many_rows(sdq_dev, new, parts, heads):
+    """Work enough for the parts' taller tiles."""
+    rng = np.random.default_rng(new)
+    nseq = 18 // parts * parts // (1 if new < 50 else 2)
+    rows = rng.integers(new - 10, new + 1, nseq)
+    c = More(sdq_dev, rows, rows + rng.integers(0, 70, nseq), 8, 16, seed=15, first=1, behind=1)
+    c.share([nseq * g // parts for g in range(parts + 1)], rng.integers(100, 900, parts))
+    c.check_shared(heads)
 
 
 # ---- counted weights ----
