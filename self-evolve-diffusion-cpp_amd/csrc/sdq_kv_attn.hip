@@ -60,13 +60,14 @@ __device__ __forceinline__ void leave_out(const Args& a, const Tile& t, int64_t 
 
 // ---- few rows: a tile of 16, the workgroup's waves share out the keys ----
 //
-// Bound by the cache's bytes, 264 a key and cached head, each read once by the wave
-// that uses it, straight into the MFMA operands' lanes, a block of 32 keys ahead: 1
-// token x 262145 keys, 8 cached heads, 111 us, 5.0 TB/s, the rate of a large copy.
-// 8 tokens of ragged sequences up to 4099 keys, 24 heads: 34 us, 3.4 TB/s; there a wave
-// has eight blocks at most, and every sequence has the same number of shares: the longest
-// has shares of 1025 keys, where the mean is 652. Two tiles read their keys twice (8
-// sequences of up to 24 rows 45 us).
+// Bound by the cache's bytes, 264 a key and cached head, each read once by the wave that uses
+// it, straight into the MFMA operands' lanes, two blocks of 32 keys on their way (in turn: a
+// wait for the older one leaves the other in flight). The keys' terms are worked out one key a
+// lane and handed round in LDS. 1 token x 262145 keys, 8 cached heads, 103 us, 5.4 TB/s, the rate
+// of a large copy. 8 tokens of ragged sequences up to 4099 keys, 24 heads: 27 us, 4.3 TB/s; there
+// a wave has eight blocks at most, and every sequence has the same number of shares: the longest
+// has shares of 1025 keys, where the mean is 652. Tiles of one sequence read its keys each (one of
+// 131072 keys, 8 heads: 16 rows 50 us, 64 rows 150).
 
 constexpr int kFewRows = kvplan::kFewRows;
 constexpr int kFewWaves = kvplan::kFewWaves;
@@ -404,7 +405,10 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(Args a) {
 // adds up   sum_r 2^(t_rj - m_r - e_j) / d_r   (sdq_kv_weights.hip forms the logits again where
 // rows are many). A thread has four keys, a row of logits is read once, and maxima and
 // denominators come from the shares themselves, so that the join of the outputs is the same
-// launch: its workgroups are the first `joins`.
+// launch: its workgroups are the first `joins`. 8 tokens over up to 4099 keys, 24 heads: 7.4 us beside
+// the attention's 29; one over 131073 keys, 32 heads on 8, 14 beside 64. Both wait for the logits, 4
+// bytes a row and key. From 33 rows on the chunks and sdq_kv_weights.hip are faster (one sequence
+// over 4099 keys, 24 heads: 32 rows 47 us for 48, 64 rows 72 for 49).
 
 constexpr int kCountKeys = 1024;  // of a workgroup
 constexpr int kCountRows = 64;    // whose statistics LDS holds
@@ -910,7 +914,12 @@ __device__ __forceinline__ void tile_rows(const Args& a, unsigned wg) {
     chunk_rows<K, 4, ROWS / 64>(a, wg);
 }
 // Shared parts and own keys in one launch, the parts' `shared` workgroups first: the own keys'
-// are short and fill what those leave.
+// are short and fill what those leave (16 tokens of 24 heads behind 4099 shared keys 20 us, two
+// launches 16 + 9; 297 rows behind 8209 and 5026 125, 123 + 20). 128 rows a part and head:
+// bound by the products and the softmax beside them, 131073 keys x 8 heads 183 us of 116 at a large
+// library product's rate; turning the keys to fp16 is shared by half as many rows as in the chunks
+// of 256. Blocks on their way in LDS by LDS-DMA, four of them, made it slower (220 us): what they
+// cost in LDS reads is more than the loads' latency.
 template <int PR, int OR>
 __global__ void __launch_bounds__(256, 2) kv_attn_shared_kernel(Args pre, Args own, unsigned shared) {
   if (blockIdx.x < shared)
@@ -1088,7 +1097,8 @@ hipError_t launch_kv_shared(const View& c, const kv::Shared& parts, const KvRows
     const int64_t rows = c.T * own.nh * own.group, most = int64_t(1) << 22;
     for (int64_t i = 0; i < rows; i += most) {
       const int64_t n = std::min(most, rows - i);
-      if (own.shares > 2 * kJoin)
+      // 16 rows of 113 shares 12 us with four waves a row, 15 with one; 1120 of 70 14.5 and 12.8
+      if (own.shares > 4 * kJoin && rows < 1024)
         hipLaunchKernelGGL((kv_attn_join_rows_kernel<4>), dim3((unsigned)n), dim3(256), 0, s, own, i);
       else
         hipLaunchKernelGGL((kv_attn_join_rows_kernel<1>), dim3((unsigned)ceil_div(n, 4)), dim3(256),

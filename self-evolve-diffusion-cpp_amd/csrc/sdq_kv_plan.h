@@ -35,25 +35,28 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   Plan p{};
   const int64_t rows = T * group;
   // Rows of a sequence, on average: only their sum is known here. Any choice is
-  // right for any lengths. Where the taller tile is faster (us, four sequences over 4099
-  // keys): 24 cached heads, 32 rows 54 with 16 and 68 with 64, 48 rows 78 and 77, 96 rows 115
-  // with 64 and 121 with 256, 160 rows 156 and 169, 256 rows 209 and 189; 8 cached heads, 24
-  // rows 30 and 39, 48 rows 38 and 40, 72 rows 42 and 41, 144 rows 68 and 49.
+  // right for any lengths (us, four sequences over 4099 keys): 24 cached heads, 32 rows 47 with
+  // 16 and 68 with 64, 48 rows 63 and 76, 96 rows 99, 114 with 64 and 117 with 256, 160 rows 131,
+  // 151 and 165, 256 rows 184, 209 and 185; 8 cached heads, 24 rows 26 and 39, 48 rows 33 and 41,
+  // 72 rows 39 and 42, 144 rows 61, 68 and 48.
   const int64_t mean = (rows + nseq - 1) / nseq;
   p.rows = mean <= 32 ? kFewRows : mean <= 128 ? 64 : 256;
-  if (p.rows == 256 && kind == kPart) p.rows = 128;
+  // parts of 32768 keys, 24 heads, 64 rows 91 with 64 and 119 with 128, 96 rows 171 and 126
+  if (mean > 64 && kind == kPart) p.rows = 128;
   // Few rows' tiles have the shorter way from a call to its result, and one for each 16 rows has
   // more of the CUs (us, cross attention): 512 keys, 8 cached heads, one sequence of 256 rows 11.6
   // for 26.8 with 64 and 38.9 with 256; 24 heads, four of 128 rows 23.7, 33.2 and 31.2, but
   // sixteen of 64 rows 42.9, 37.2 and 58.7. 4099 keys: 24 heads, four of 96 rows 100, 115, 121;
   // sixteen 303, 434, 411; 8 heads, four of 128 rows 44.3, 44.2, 43.8, one of 256 rows 33, 36 and
   // 48. Shared parts of 8209 keys, 8 heads: 256 rows 47 for 57 with 128, 512 rows 78 for 77; 300 keys
-  // behind them, four of 48 rows 42 for 48 with 64. From 1024 rows on cross attention's chunks have
+  // behind them, four of 48 rows 42 for 48 with 64. Each tile reads its keys, which over long ones
+  // is what it waits for: shared parts of 8 heads, 64 rows over 32768 keys 46 for 52 with 64, over
+  // 131072 137 for 116, 128 rows 250 for 169 with 128. From 1024 rows on cross attention's chunks have
   // an order of their own (sdq_kv_packed.hip). Own keys keep the heights above, and their bits.
   const int64_t few = (mean + kFewRows - 1) / kFewRows * nseq * kv_heads;  // workgroups
   const bool whole = kind == kCross && most <= kWhole;
-  if (whole ? mean < 1024 && few <= 4 * cu_count
-            : (kind == kCross && mean <= 96) || (kind != kOwn && mean <= 256 && few <= cu_count / 2))
+  const bool small = mean <= 256 && few <= cu_count / 2 && few * most <= int64_t(1) << 21;
+  if (whole ? mean < 1024 && few <= 4 * cu_count : (kind == kCross && mean <= 96) || (kind != kOwn && small))
     p.rows = kFewRows;
   // Numbers of tiles: rows / height and one a sequence (csrc/sdq_kv_attn.hip); those that
   // hold one are at most the sum of ceil(rows_s / height) over the sequences that have any.
@@ -61,8 +64,8 @@ inline Plan plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int
   const int64_t groups =  // workgroups without a cut
       (rows + std::min<int64_t>(nseq, T) * (p.rows - 1)) / p.rows * kv_heads;
   // Enough workgroups for every CU. A few-row one is four waves that wait for memory, and
-  // two fit a CU at once: three to a CU (8 sequences x 24 heads x 4099 keys: two 52 us,
-  // three 42, four 45, six 47). A chunk's of 256 rows takes a CU's registers, and the
+  // two fit a CU at once: three to a CU (8 ragged sequences x 24 heads up to 4099 keys: two 36
+  // us, three 27, four 29, six 32). A chunk's of 256 rows takes a CU's registers, and the
   // second round evens out what the first leaves idle.
   const int64_t want = (p.rows == kFewRows ? 3 : p.rows == 64 ? 4 : 2) * (int64_t)cu_count;
   const int64_t least = p.rows == kFewRows ? 256 : 512;  // keys of a share
