@@ -828,3 +828,106 @@ def test_empty_calls(sdq_dev):
     c.sdq.kv_attention_weights(c.cache, empty, w, x, o, 2)
     c.sdq.kv_evict(c.cache, empty, w, i32(0, 1), i32(0), i32(0, 2, 5))
     assert (o == 3).all() and (w == 0).all()
+
+
+@pytest.mark.parametrize("rows", [([3, 60]), ([1100, 90])])
+def test_far_pages(sdq_dev, rows):
+    """Pages behind 4 GiB of codes: the bits of the same pages at the pool's beginning."""
+    import torch
+
+    c = More(sdq_dev, rows, [n + 700 for n in rows], 8, 256, seed=33, extra=4)
+    c.share([0, 2], [600])
+    n, far = c.pages, 20000
+    pool = c.sdq.KvCache.empty(far, 256, 8)
+    for name in ("k", "v", "ks", "vs"):
+        getattr(pool, name)[far - n:] = getattr(c.cache, name)
+    move = lambda t: c.t(np.where(t >= 0, t + far - n, -1).astype(np.int32))  # noqa: E731
+    there = (pool, c.sdq.KvBatch(c.batch.q_start, c.batch.lens, move(c.table)),
+             c.sdq.KvShared(c.shared.s_start, c.shared.lens, move(c.s_table)), move)
+    to, q = c.free[:2].reshape(2, 1), c.t(c.queries(16))
+    w = c.t(c.rng.uniform(0, 0.1, (n, 8, 256)).astype(F))
+
+    def step(cache, batch, shared, place):
+        outs = [torch.zeros((c.T, 2048), device=sdq_dev) for _ in range(3)]
+        ws = torch.zeros((cache.pages, 8, 256), device=sdq_dev)
+        ws[-n:] = w
+        lens = torch.zeros(2, dtype=torch.int32, device=sdq_dev)
+        kept = torch.zeros((2, 8, 200), dtype=torch.int32, device=sdq_dev)
+        c.sdq.kv_cross_attention(cache, batch, q, outs[0], 16)
+        c.sdq.kv_attention_shared(cache, shared, batch, q, outs[1], 16)
+        c.sdq.kv_attention_weights(cache, batch, ws, q, outs[2], 16)
+        c.sdq.kv_evict(cache, batch, ws, place(to), lens, kept, first=3, last=20)
+        return [x.cpu().numpy() for x in outs + [ws[-n:], lens, kept, cache.k[-n:], cache.v[-n:]]]
+
+    for got, want in zip(step(*there), step(c.cache, c.batch, c.shared, lambda t: c.t(t))):
+        assert_bitexact(got, want)
+
+
+def test_pool_without_pages(sdq_dev):
+    """Tables that name pages of an empty pool: rows see nothing, nothing is kept."""
+    import torch
+
+    c = More(sdq_dev, [2, 40], [20, 40], 2, 16, seed=34)
+    c.share([0, 2], [30])
+    cache = c.sdq.KvCache.empty(0, 16, 2)
+    w, q = torch.zeros((0, 2, 16), device=sdq_dev), c.t(c.queries(4))
+    for call in (lambda o: c.sdq.kv_cross_attention(cache, c.batch, q, o, 4),
+                 lambda o: c.sdq.kv_attention_shared(cache, c.shared, c.batch, q, o, 4),
+                 lambda o: c.sdq.kv_attention_weights(cache, c.batch, w, q, o, 4)):
+        out = torch.full((c.T, 512), 3.0, device=sdq_dev)
+        call(out)
+        assert (out == 0).all()
+    lens = torch.full((2,), 9, dtype=torch.int32, device=sdq_dev)
+    kept = torch.full((2, 2, 16), 9, dtype=torch.int32, device=sdq_dev)
+    c.sdq.kv_evict(cache, c.batch, w, c.t(c.table[:, :1]), lens, kept)
+    assert (lens == 0).all() and (kept == -1).all()
+
+
+def test_captured_large(sdq_dev):
+    """Keys as operands, rows counted by their parts and a table of many chunks in one graph, replayed
+    over other weights with eager calls between."""
+    import torch
+
+    c = More(sdq_dev, [1100], [1200], 2, 16, seed=35)
+    wide = np.full((1, 20000 // 16), -1, np.int32)
+    wide[:, :c.table.shape[1]] = c.table
+    long = c.sdq.KvBatch(c.batch.q_start, c.batch.lens, c.t(wide))
+    q = c.t(c.queries(4))
+    to = c.t(np.full((1, 4), c.pages, np.int32))  # nowhere: only what is kept counts
+    w = torch.zeros((c.pages, 2, 16), device=sdq_dev)
+    outs = [torch.zeros((c.T, 512), device=sdq_dev) for _ in range(2)]
+    lens = torch.zeros(1, dtype=torch.int32, device=sdq_dev)
+    kept = torch.zeros((1, 2, 64), dtype=torch.int32, device=sdq_dev)
+
+    def step():
+        c.sdq.kv_cross_attention(c.cache, c.batch, q, outs[0], 4)
+        c.sdq.kv_attention_weights(c.cache, c.batch, w, q, outs[1], 4)
+        c.sdq.kv_evict(c.cache, long, w, to, lens, kept, first=2, last=5)
+        return outs + [w, lens, kept]
+
+    def fresh(seed):
+        g = torch.Generator(device=sdq_dev).manual_seed(seed)
+        q.copy_(torch.randn(q.shape, generator=g, device=sdq_dev))
+        w.copy_(torch.rand(w.shape, generator=g, device=sdq_dev))
+
+    side = torch.cuda.Stream()
+    fresh(0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for seed in (1, 2, 3):
+        fresh(seed)
+        want = [x.cpu().numpy() for x in step()]
+        fresh(seed)
+        for x in outs + [lens, kept]:
+            x.fill_(-1)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.synchronize()
+        for got, x in zip(outs + [w, lens, kept], want):
+            assert_bitexact(got.cpu().numpy(), x)
