@@ -345,26 +345,66 @@ __device__ __forceinline__ void parts8(const float x[8], v8h& hi, v8h& lo) {
   }
 }
 
-// The lane's slice of a query row (head of a token), zeros where it is none.
+// r[c] of the lanes g (l >> 4) of a row: that of lane c, r[g], comes to lane g in r[c].
+__device__ __forceinline__ void swap_quads(v4f (&r)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    uint32_t x[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) x[c] = __float_as_uint(r[c][k]);
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      const auto p = __builtin_amdgcn_permlane32_swap(x[c], x[c + 2], false, false);
+      x[c] = p[0], x[c + 2] = p[1];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c += 2) {
+      const auto p = __builtin_amdgcn_permlane16_swap(x[c], x[c + 1], false, false);
+      x[c] = p[0], x[c + 1] = p[1];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) r[c][k] = __uint_as_float(x[c]);
+  }
+}
+
+// The lane's slice of a query row (head of a token), zeros where it is none. Four lanes load 64
+// bytes that lie side by side and exchange them for what each needs.
 __device__ __forceinline__ void load_q(const Args& a, const Tile& t, int h, int64_t r, int g,
                                        float x[4][8]) {
   const bool ok = r < t.rows;
   const int64_t rr = ok ? r : 0;
   const int64_t tok = token_of(rr, a.group);
   const float* p =
-      a.q + (t.row0 + tok) * a.ldq + (int64_t)(h * a.group + (int)(rr - tok * a.group)) * kHd;
+      a.q + (t.row0 + tok) * a.ldq + (int64_t)(h * a.group + (int)(rr - tok * a.group)) * kHd + 4 * g;
 #pragma unroll
-  for (int kb = 0; kb < 4; kb++)
+  for (int half = 0; half < 2; half++) {
+    v4f v[4];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const float4 v =
-          ok ? *reinterpret_cast<const float4*>(p + 64 * (kb >> 1) + 16 * g + 8 * (kb & 1) + 4 * j)
-             : make_float4(0.f, 0.f, 0.f, 0.f);
-      x[kb][4 * j] = v.x;
-      x[kb][4 * j + 1] = v.y;
-      x[kb][4 * j + 2] = v.z;
-      x[kb][4 * j + 3] = v.w;
+    for (int c = 0; c < 4; c++)
+      v[c] = ok ? *reinterpret_cast<const v4f*>(p + 64 * half + 16 * c) : v4f{0.f, 0.f, 0.f, 0.f};
+    swap_quads(v);
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[2 * half + (c >> 1)][4 * (c & 1) + i] = v[c][i];
+  }
+}
+// A row's sums times f: the lane has dims 32 g + 8 i + e in acc[e][i]. As they were loaded, 64 bytes
+// of a row by four lanes (a lane's own 16 bytes apart from the others' were partial lines).
+__device__ __forceinline__ void store_row(float* row, const v4f acc[8], float f, int g, bool ok) {
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    v4f v[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const int e = 4 * (c & 1), i = 2 * u + (c >> 1);
+      v[c] = v4f{acc[e][i] * f, acc[e + 1][i] * f, acc[e + 2][i] * f, acc[e + 3][i] * f};
     }
+    swap_quads(v);
+    if (ok)
+#pragma unroll
+      for (int c = 0; c < 4; c++) *reinterpret_cast<v4f*>(row + 32 * c + 16 * u + 4 * g) = v[c];
+  }
 }
 // The largest magnitude of a row's slice. NaN and infinities become zeros, and the row (of
 // four lanes) is `bad`: its denominator is NaN once it has seen a key, and 0 before.

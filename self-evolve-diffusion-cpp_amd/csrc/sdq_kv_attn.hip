@@ -873,29 +873,25 @@ __device__ __forceinline__ void chunk_rows(const Args& a, unsigned wg) {
   for (int qt = 0; qt < QT; qt++) {
     const int row = (w * QT + qt) * 16 + r16;
     const int64_t r = t.r0 + row;
-    if (r >= t.rows) continue;
+    const bool ok = r < t.rows;
     const float den = den_of(st[qt].l, bad[qt]);
     float f = 1.f;
-    float* dst;
-    if (!K::kByRow && a.splits == 1) {
+    float* dst = a.out;
+    if (!ok) {
+      // its lanes take part in the exchange below
+    } else if (!K::kByRow && a.splits == 1) {
       f = den == 0.f ? 0.f : __builtin_ldexpf(1.f, e0 - kWeight) / den;
       const int64_t tok = token_of(r, a.group);
       const int head = h * a.group + (int)(r - tok * a.group);
-      dst = a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd + 32 * g;
+      dst = a.out + (t.row0 + tok) * a.ldo + (int64_t)head * kHd;
       if (K::kStats && g == 0)
         a.info[tile16(a, t, h, r) * 16 + r16] = info_of(a, t, r, qk[qt], st[qt].m, den);
     } else {
       const int64_t at = share_at<K>(a, t, th, h, z, kRows, row);
       if (g == 0) a.part_ml[at] = float2{st[qt].m, den};
-      dst = a.part + at * kHd + 32 * g;
+      dst = a.part + at * kHd;
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      *reinterpret_cast<v4f*>(dst + 8 * i) =
-          v4f{acc[qt][0][i] * f, acc[qt][1][i] * f, acc[qt][2][i] * f, acc[qt][3][i] * f};
-      *reinterpret_cast<v4f*>(dst + 8 * i + 4) =
-          v4f{acc[qt][4][i] * f, acc[qt][5][i] * f, acc[qt][6][i] * f, acc[qt][7][i] * f};
-    }
+    store_row(dst, acc[qt], f, g, ok);
   }
 }
 
