@@ -8,7 +8,7 @@
 // the softmax only, and there is room to put a block's exponentials beside the next block's
 // scores, and the next block's logits beside this one's sums: neither waits for the other.
 //
-// 24 heads: 27280 rows over 512 keys 427 us (8 of them the pass), 509 in chunks; 2048 rows over 4099
+// 24 heads: 27280 rows over 512 keys 419 us (8 of them the pass), 509 in chunks; 2048 rows over 4099
 // 254 and 288, 8192 over 4099 709 and 720, 1024 over 4099 162 and 158, over 512 39 and 45: taken
 // from 1024 rows a sequence on. Bound by the matrix units and the softmax beside them: 8192 rows
 // over as many keys at 1.17 PFLOP/s, the rate of a large library product. Over 512 keys what

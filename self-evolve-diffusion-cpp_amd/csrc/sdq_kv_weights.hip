@@ -35,6 +35,7 @@ constexpr int kBlock = 16 * kTiles * kWaves;  // keys of a workgroup
 constexpr int kRows = 64;                     // of a stage in LDS
 constexpr int kRing = 3;
 constexpr int kLeastLog = 10;                 // of a range's rows (2^8 157 us, 2^12 223, see above)
+constexpr int kShortLog = 7;                  // the same where there are workgroups to spare
 constexpr int kDma = 5;                       // a wave's, a stage: 4 of the parts, one of the rest
 
 struct Stage {
@@ -59,7 +60,12 @@ __device__ __forceinline__ Cut cut_of(const Tile& t, const Work& wk) {
   if (wk.cut && c.blocks > 0) {
     // up to 4 items a workgroup: a pair's items are fewer than 8 * across
     const int64_t want = (4 * wk.across + c.blocks - 1) / c.blocks;
-    c.log = kLeastLog;
+    // one a CU (half of across) of short ranges, if there are no more: 1100 keys, 8 heads, 1000 rows
+    // 111 -> 78 us of the call
+    c.log = kShortLog;
+    while (c.log < kLeastLog &&
+           2 * ((t.rows + (int64_t(1) << c.log) - 1) >> c.log) * c.blocks > wk.across)
+      c.log++;
     while ((t.rows + (int64_t(1) << c.log) - 1) >> c.log > want) c.log++;
     c.ranges = (int)((t.rows + (int64_t(1) << c.log) - 1) >> c.log);
   }
