@@ -560,7 +560,7 @@ int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, 
  * weights: device memory of the caller, [pages, kv_heads, page_size] f32 as the cache's
  * scales, with a float's alignment; it overlaps no other array. fp32 sums, each row's weights
  * added in a fixed order: the same bits every time. Rows whose softmax is no number (a NaN or an
- * infinity in q, in the scale of a key that they see) add nothing. No page may stand twice in the
+ * infinity in q, in the scale of a key that they see, a logit past fp32's range) add nothing. No page may stand twice in the
  * tables of the call's sequences (sums would be lost in part). Scratch from the stream's
  * workspace in every call (a capture needs one call of the same shape before it): up to 32 rows
  * of q a sequence and cached head, on average, their logits, if they fit 512 MiB, else 528 bytes a

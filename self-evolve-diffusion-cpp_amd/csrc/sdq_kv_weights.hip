@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
             op[kb & 1][part] = *reinterpret_cast<const v8h*>(d.q[tile] + 4096 * part + 1024 * kb + l * 16);
         };
         to.ri = d.row[16 * nx + r16];
-        if (!live) to.ri.m = INFINITY, to.ri.inv = 0.f, to.ri.see = 0;
+        if (!live) to.ri = kNoRow;
         if (kMask || nx == 0) read(nx, 0);  // masked tiles may be left out
 #pragma unroll
         for (int kb = 0; kb < 4; kb++) {
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
         Scores sc[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {  // before the first tile: adds nothing
-          sc[j].ri = RowInfo{0.f, INFINITY, 0.f, 0};
+          sc[j].ri = kNoRow;
 #pragma unroll
           for (int kt = 0; kt < kTiles; kt++) sc[j].s[kt] = v4f{0.f, 0.f, 0.f, 0.f};
         }
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
           }
         };
         // Stages whose rows may not see all of the wave's keys, then the others (a row that adds
-        // nothing has an infinite maximum: only keys ahead of a row are masked).
+        // nothing has finite logits and an infinite maximum: only keys ahead of a row are masked).
         const int first = (int)max((int64_t)0, min((int64_t)stages, (every + 4) >> 2));
         run(0, first, std::true_type{});
         run(first, stages, std::false_type{});
