@@ -510,7 +510,8 @@ int sdq_kv_read(const sdq_kv_cache* c, const sdq_kv_batch* b, float* k, int64_t 
  * rows a sequence, and chunks too few for the machine, cut the keys into shares joined
  * by a second kernel, their scratch from the stream's workspace: a capture needs one call
  * of the same shape before it (SDQ_ERR_INVALID otherwise, the capture stays usable).
- * A row's result depends on no other row's contents, nor on timing. T * heads is at most 2^31. */
+ * A row's result depends on no other row's contents, nor on timing. T * heads is at most 2^31.
+ * out overlaps neither q nor the cache's and the batch's arrays. */
 int sdq_kv_attention(const sdq_kv_cache* c, const sdq_kv_batch* b, const float* q, int64_t ldq,
                      float* out, int64_t ldo, int64_t T, int heads, float scale, int causal,
                      void* stream);
@@ -546,7 +547,8 @@ typedef struct sdq_kv_shared {
  * all of its sequences' rows together. The range of value scales counts from the shared
  * part's first token (the sequence's own where that part is empty). Scratch from the
  * stream's workspace in every call, 1040 bytes and up for a row and head (of as many heads
- * at a time as 512 MiB take): a capture needs one call of the same shape before it. */
+ * at a time as 512 MiB take): a capture needs one call of the same shape before it.
+ * out overlaps none of shared's arrays either. */
 int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, const sdq_kv_batch* b,
                             const float* q, int64_t ldq, float* out, int64_t ldo, int64_t T,
                             int heads, float scale, int causal, void* stream);

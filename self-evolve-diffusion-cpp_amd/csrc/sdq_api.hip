@@ -962,6 +962,15 @@ bool rows_overlap(const float* a, int64_t lda, const float* b, int64_t ldb, int6
   return by < C || by > lda - C;
 }
 
+// Whether n bytes at p share any with M rows of C floats, ld apart (what lies between rows is none).
+bool meets_rows(const void* p, size_t n, const float* a, int64_t ld, int64_t M, int64_t C) {
+  if (M < 1 || !bytes_overlap(p, n, a, (size_t)((M - 1) * ld + C) * 4)) return false;
+  const auto x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(a);
+  // the first row that ends behind p
+  const int64_t row = x < y + (size_t)C * 4 ? 0 : (int64_t)((x - y - (size_t)C * 4) / ((size_t)ld * 4)) + 1;
+  return row < M && y + (size_t)(row * ld) * 4 < x + n;
+}
+
 // One timed launch: a record of its own between sdq_profile_begin / _end.
 template <class F>
 int timed(const char* name, hipStream_t s, F launch) {
@@ -1059,11 +1068,18 @@ int kv_rows(const std::string& tag, const char* name, const float* p, int64_t ld
 // Scales of a cache's keys (or values).
 size_t kv_scales(const kv::View& v) { return ((size_t)v.pages * v.kv_heads) << v.page_log2; }
 
-// Memory that meets the cache's, whose scales take `scales` bytes.
-bool kv_overlaps(const sdq_kv_cache* c, const void* p, size_t n, size_t scales) {
-  const size_t codes = scales / 4 * kv::kHd;
-  return bytes_overlap(p, n, c->ks, scales) || bytes_overlap(p, n, c->vs, scales) ||
-         bytes_overlap(p, n, c->k, codes) || bytes_overlap(p, n, c->v, codes);
+// Whether any of the cache's arrays, or of the batch's (without q_start where the call does not
+// read that one), meet what `meets` stands for.
+template <class F>
+bool kv_arrays(const sdq_kv_cache* c, const kv::View& v, F meets) {
+  const size_t scales = kv_scales(v) * 4, codes = kv_scales(v) * kv::kHd;
+  return meets(c->ks, scales) || meets(c->vs, scales) || meets(c->k, codes) || meets(c->v, codes);
+}
+template <class F>
+bool kv_arrays(const sdq_kv_batch* b, bool starts, F meets) {
+  const size_t n = (size_t)b->nseq;
+  return (starts && meets(b->q_start, (n + 1) * 4)) || meets(b->lens, n * 4) ||
+         meets(b->table, n * (size_t)b->max_pages * 4);
 }
 
 // A checked call of one of the paged attentions (view.T == 0: nothing to do).
@@ -1091,6 +1107,9 @@ int kv_call(const sdq_kv_cache* c, const sdq_kv_batch* b, const KvRows& r, int64
     return rc;
   if (rows_overlap(r.out, r.ldo, r.q, r.ldq, T, C))
     return set_error(SDQ_ERR_INVALID, tag + ": out overlaps q");
+  auto meets = [&](const void* p, size_t n) { return meets_rows(p, n, r.out, r.ldo, T, C); };
+  if (kv_arrays(c, out->view, meets) || kv_arrays(b, true, meets))
+    return set_error(SDQ_ERR_INVALID, tag + ": out overlaps the cache or the batch's arrays");
   return SDQ_OK;
 }
 kvplan::Plan plan_of(const KvCall& k, kvplan::Kind kind = kvplan::kOwn) {
@@ -2541,6 +2560,13 @@ int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, 
     return set_error(SDQ_ERR_INVALID, tag + ": null arrays of the shared parts");
   if (shared->n == 0)
     return sdq_kv_attention(c, b, q, ldq, out, ldo, T, heads, scale, causal, stream);
+  const size_t n = (size_t)shared->n;
+  auto meets = [&](const void* p, size_t bytes) {
+    return meets_rows(p, bytes, out, ldo, T, (int64_t)heads * kv::kHd);
+  };
+  if (meets(shared->s_start, (n + 1) * 4) || meets(shared->lens, n * 4) ||
+      meets(shared->table, n * (size_t)shared->max_pages * 4))
+    return set_error(SDQ_ERR_INVALID, tag + ": out overlaps the shared parts' arrays");
   const kv::Shared parts{shared->s_start, shared->lens, shared->table, shared->n,
                          c->pages > 0 ? shared->max_pages : 0, call.view.nseq};
   if ((rc = usable_device(&call.dev))) return rc;
@@ -2566,9 +2592,10 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
   if (rc || call.view.T == 0) return rc;
   if (c->pages > 0 && !weights) return set_error(SDQ_ERR_INVALID, tag + ": null weights");
   const size_t nw = kv_scales(call.view) * 4;
-  if (bytes_overlap(weights, nw, out, (size_t)((T - 1) * ldo + (int64_t)heads * kv::kHd) * 4) ||
-      bytes_overlap(weights, nw, q, (size_t)((T - 1) * ldq + (int64_t)heads * kv::kHd) * 4) ||
-      kv_overlaps(c, weights, nw, nw))
+  const int64_t C = (int64_t)heads * kv::kHd;
+  auto meets = [&](const void* p, size_t n) { return bytes_overlap(p, n, weights, nw); };
+  if (meets_rows(weights, nw, out, ldo, T, C) || meets_rows(weights, nw, q, ldq, T, C) ||
+      kv_arrays(c, call.view, meets) || kv_arrays(b, true, meets))
     return set_error(SDQ_ERR_INVALID, tag + ": weights overlaps another array");
   if ((rc = usable_device(&call.dev))) return rc;
   const hipStream_t s = stream_of(stream);
@@ -2637,13 +2664,19 @@ int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, i
     return set_error(SDQ_ERR_INVALID, tag + ": null pointer");
   const size_t nw = kv_scales(view) * 4, nl = (size_t)b->nseq * 4;
   const size_t nk = (size_t)b->nseq * c->kv_heads * keep * 4;
-  const size_t nt = (size_t)b->nseq * b->max_pages * 4, nto = (size_t)b->nseq * to_max_pages * 4;
-  auto meets = [&](const void* p, size_t n) {  // an output on an input
-    return bytes_overlap(p, n, b->lens, nl) || bytes_overlap(p, n, b->table, nt) ||
-           bytes_overlap(p, n, to_table, nto) || bytes_overlap(p, n, weights, nw);
+  const size_t nto = (size_t)b->nseq * to_max_pages * 4;
+  // what is written (the cache and weights are read too) on anything else
+  auto onto = [&](const void* p, size_t n) {
+    auto meets = [&](const void* x, size_t nx) { return bytes_overlap(x, nx, p, n); };
+    return kv_arrays(b, false, meets) || meets(to_table, nto);
   };
-  if (meets(to_lens, nl) || meets(kept, nk) || bytes_overlap(to_lens, nl, kept, nk) ||
-      kv_overlaps(c, weights, nw, nw) || kv_overlaps(c, to_lens, nl, nw) || kv_overlaps(c, kept, nk, nw))
+  auto on_cache = [&](const void* p, size_t n) {
+    return kv_arrays(c, view, [&](const void* x, size_t nx) { return bytes_overlap(x, nx, p, n); });
+  };
+  if (onto(to_lens, nl) || onto(kept, nk) || onto(weights, nw) || kv_arrays(c, view, onto) ||
+      bytes_overlap(to_lens, nl, kept, nk) || bytes_overlap(to_lens, nl, weights, nw) ||
+      bytes_overlap(kept, nk, weights, nw) || on_cache(weights, nw) || on_cache(to_lens, nl) ||
+      on_cache(kept, nk))
     return set_error(SDQ_ERR_INVALID, tag + ": an output overlaps another array");
   int dev = -1;
   if ((rc = usable_device(&dev))) return rc;
