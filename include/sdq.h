@@ -580,8 +580,9 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
  * are as they were; what goes to a page id outside the pool is lost. A page of to_table may
  * be in no sequence's table and in to_table once only. first + last <= keep; no output may
  * overlap another array (to_lens is not b's lens), nor weights the cache. Stream-ordered;
- * tables of more than 16384 tokens take scratch from the stream's workspace (a capture then
- * needs one call of the same shape before it). */
+ * tables of more than 16384 tokens take scratch from the stream's workspace, up to 256 MiB or
+ * 24.1 KiB a cached head, whichever is more (a capture then needs one call of the same shape
+ * before it). */
 int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, int64_t first,
                  int64_t last, int64_t keep, const int32_t* to_table, int64_t to_max_pages,
                  int32_t* to_lens, int32_t* kept, void* stream);

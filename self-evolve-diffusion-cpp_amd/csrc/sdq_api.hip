@@ -2620,8 +2620,8 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
                                    reinterpret_cast<float*>(base + stats_bytes), weights, cus, s);
     });
   }
-  const KvWeightsPlan wplan =
-      plan_kv_weights(T, call.view.nseq, heads / c->kv_heads, c->kv_heads,
+  const kvplan::WeightsPlan wplan =
+      kvplan::weights_plan(T, call.view.nseq, heads / c->kv_heads, c->kv_heads,
                       call.view.max_pages << call.view.page_log2, cus);
   // the shares' sums or, once they are joined, the ranges', the rows' parts and statistics, and
   // the keys as operands
@@ -2682,8 +2682,8 @@ int sdq_kv_evict(const sdq_kv_cache* c, const sdq_kv_batch* b, float* weights, i
   if ((rc = usable_device(&dev))) return rc;
   const hipStream_t s = stream_of(stream);
   const kv::Kept k{first, last, keep, to_table, to_max_pages, to_lens, kept};
-  const KvEvictPlan plan =
-      plan_kv_evict(view.nseq, view.kv_heads, view.max_pages << view.page_log2);
+  const kvplan::EvictPlan plan =
+      kvplan::evict_plan(view.nseq, view.kv_heads, view.max_pages << view.page_log2);
   float* scratch = nullptr;
   std::unique_lock<std::mutex> turn;
   if (plan.scratch_bytes > 0 &&

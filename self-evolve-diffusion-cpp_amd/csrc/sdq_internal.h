@@ -270,6 +270,8 @@ struct Kept;
 namespace kvplan {
 struct Plan;
 struct SharedPlan;
+struct WeightsPlan;
+struct EvictPlan;
 }
 hipError_t launch_kv_write(const kv::View& c, const float* k, int64_t ldk, const float* v,
                            int64_t ldv, hipStream_t s);
@@ -296,19 +298,10 @@ hipError_t launch_kv_shared(const kv::View& c, const kv::Shared& pre, const KvRo
                             const kvplan::SharedPlan& plan, void* scratch, hipStream_t s);
 // launch_kv_attn that keeps in `kept` what the sums of the weights by key go by, and those:
 // w as the cache's scales.
-struct KvWeightsPlan {
-  int across;  // workgroups of a sequence and head
-  int cut;     // its rows may be cut into ranges
-  int seqs;    // sequences at a time
-  int64_t n16;  // numbers of tiles of 16 rows
-  int64_t kept_bytes, scratch_bytes;
-};
-KvWeightsPlan plan_kv_weights(int64_t T, int nseq, int group, int kv_heads, int64_t most,
-                              int cu_count);
 hipError_t launch_kv_counted(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
-                             void* scratch, const KvWeightsPlan& p, void* kept, void* packed,
+                             void* scratch, const kvplan::WeightsPlan& p, void* kept, void* packed,
                              hipStream_t s);
-hipError_t launch_kv_weights(const kv::View& c, const KvRows& r, const KvWeightsPlan& p, void* kept,
+hipError_t launch_kv_weights(const kv::View& c, const KvRows& r, const kvplan::WeightsPlan& p, void* kept,
                              float* w, void* scratch, hipStream_t s);
 // Both at once for few rows (the plan's tiles of 16), whose logits are kept in between:
 // kv_logit_keys floats a row and head.
@@ -316,14 +309,7 @@ int64_t kv_logit_keys(const kv::View& c);
 hipError_t launch_kv_counted_few(const kv::View& c, const KvRows& r, const kvplan::Plan& plan,
                                  void* scratch, float2* stats, float* logits, float* sums,
                                  int cu_count, hipStream_t s);
-struct KvEvictPlan {
-  int seqs;       // sequences at a time
-  int chunks;     // of a sequence, 0: it fits a workgroup
-  int64_t chunk;  // tokens
-  int64_t scratch_bytes;
-};
-KvEvictPlan plan_kv_evict(int nseq, int kv_heads, int64_t most);
-hipError_t launch_kv_evict(const kv::View& c, float* w, const kv::Kept& k, const KvEvictPlan& p,
+hipError_t launch_kv_evict(const kv::View& c, float* w, const kv::Kept& k, const kvplan::EvictPlan& p,
                            void* scratch, hipStream_t s);
 
 // GEMM tile configurations.

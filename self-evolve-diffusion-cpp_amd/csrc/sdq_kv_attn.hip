@@ -1004,7 +1004,7 @@ hipError_t launch_kv_cross(const View& c, const KvRows& r, const kvplan::Plan& p
 }
 
 hipError_t launch_kv_counted(const View& c, const KvRows& r, const kvplan::Plan& p, void* scratch,
-                             const KvWeightsPlan& wp, void* kept, void* packed, hipStream_t s) {
+                             const kvplan::WeightsPlan& wp, void* kept, void* packed, hipStream_t s) {
   Args a = args_of(c, r, scratch, p.part_bytes);
   a.qparts = static_cast<char*>(kept);
   a.info = reinterpret_cast<RowInfo*>(a.qparts + wp.n16 * c.kv_heads * kQTile);

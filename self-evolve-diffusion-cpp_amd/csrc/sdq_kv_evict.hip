@@ -1,16 +1,18 @@
 // Eviction from the paged int8 cache by a weight for each token and head (gfx950).
 //
-// select: one workgroup a sequence and head. Every token gets a number whose order is the
+// select: one workgroup a sequence and head, for tables of up to 16384 tokens. Every token gets a number whose order is the
 // order of keeping (tokens that stay whatever their weight, then weights from the largest, NaN
 // last, then places without a token); the keep-th largest number is found digit by digit (11,
 // 11 and 10 bits, counted in LDS), and the tokens from it on are listed in order of their
-// position, of those that equal it the first ones. Up to 65536 tokens stay in registers, four
-// that lie side by side to a load; longer sequences are read again for each digit.
+// position, of those that equal it the first ones. The tokens stay in registers, four that lie
+// side by side to a load. Wider tables: chunks of whole times 16384 tokens, a workgroup each, and four
+// launches (three that count a digit, one that lists), each of which reads the weights again.
 // move: 32 kept rows of codes a workgroup, 8 lanes a row.
 #include <algorithm>
 
 #include "sdq_device.h"
 #include "sdq_kv.h"
+#include "sdq_kv_plan.h"
 
 #pragma clang fp contract(off)
 
@@ -27,6 +29,7 @@ constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kRun = 4;  // tokens of a thread that lie side by side
 constexpr int kRound = kThreads * kRun;
+static_assert(4 * kRound == kvplan::kEvictRegisters);
 
 constexpr uint32_t kAlways = 0xffffffffu, kAbsent = 0u;
 // Weights in order as numbers 2 .. 0xfffffffe - 1, zeros of either sign the same; NaN 1.
@@ -224,7 +227,7 @@ __device__ __forceinline__ void count_digits(const uint32_t (&r)[N][kRun], int s
 template <int N>
 __device__ __forceinline__ void select(const Tokens& t, int64_t most, int32_t* kept, int32_t* len,
                                        Lds& s) {
-  const int tid = threadIdx.x, wave = tid >> 6;
+  const int tid = threadIdx.x;
   uint32_t r[N][kRun];
   t.load<N>(tid * kRun, t.len, r);
   // The border's digits from the highest; as soon as a digit's tokens are all kept the rest
@@ -295,6 +298,7 @@ struct Found {
   int levels;  // digits that matter
   int done;    // 1: all of the last digit's tokens are kept, 2: all tokens are
 };
+static_assert(3 * sizeof(Found) == kvplan::kEvictFound);
 struct Long {
   uint32_t* hist;  // [pair][chunk][level][2048]
   Found* found;    // [pair][level]
@@ -428,24 +432,7 @@ __global__ void __launch_bounds__(256) kv_move_kernel(View c, float* __restrict_
 
 }  // namespace
 
-// Longer than a workgroup's registers: chunks of 16384 tokens, at most 64 of them.
-KvEvictPlan plan_kv_evict(int nseq, int kv_heads, int64_t most) {
-  KvEvictPlan p{};
-  p.seqs = std::max(1, (1 << 21) / kv_heads);  // a grid's threads are a 32-bit number
-  if (most > 4 * kRound) {
-    const int64_t chunks = std::min<int64_t>(64, std::max(1, (1 << 20) / kv_heads));
-    p.chunk = round_up(ceil_div(most, chunks), 4 * kRound);
-    p.chunks = (int)ceil_div(most, p.chunk);
-    const int64_t pair = p.chunks * 3 * 2048 * 4 + 3 * (int64_t)sizeof(Found);
-    p.seqs = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t(1) << 28) / (pair * kv_heads),
-                                                         (1 << 20) / ((int64_t)p.chunks * kv_heads)));
-    p.seqs = std::min(p.seqs, nseq);
-    p.scratch_bytes = pair * kv_heads * p.seqs;
-  }
-  return p;
-}
-
-hipError_t launch_kv_evict(const View& c, float* w, const Kept& k, const KvEvictPlan& p, void* scratch,
+hipError_t launch_kv_evict(const View& c, float* w, const Kept& k, const kvplan::EvictPlan& p, void* scratch,
                            hipStream_t s) {
   for (int s0 = 0; s0 < c.nseq; s0 += p.seqs) {
     View v = c;

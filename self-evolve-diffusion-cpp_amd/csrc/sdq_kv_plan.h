@@ -1,5 +1,5 @@
-// Host arithmetic of the paged attention: tile height, share count and scratch
-// of a call, from sizes alone (plain C++, no device code).
+// Host arithmetic of the paged attention, of the sums of its weights and of eviction: tile height,
+// share count and scratch of a call, from sizes alone (plain C++, no device code).
 #pragma once
 
 #include <algorithm>
@@ -123,6 +123,63 @@ inline SharedPlan shared_plan(int64_t T, int nseq, int n, int group, int kv_head
         1, ((int64_t(1) << 30) - 1) / ((int64_t)p.heads * q->splits * 512));
   p.part_bytes = T * group * p.heads * shares * 128 * 4;
   p.scratch_bytes = p.part_bytes / 128 * 130;
+  return p;
+}
+
+// The sums of weights by key that form the logits again (sdq_kv_weights.hip).
+constexpr int kCountBlock = 512;            // keys of a workgroup
+constexpr int kCountKept = 8192 + 16 * 16;  // bytes that the attention leaves of a tile of 16 rows
+struct WeightsPlan {
+  int across;   // workgroups of a sequence and head
+  int cut;      // its rows may be cut into ranges
+  int seqs;     // sequences at a time
+  int64_t n16;  // numbers of tiles of 16 rows
+  int64_t kept_bytes, scratch_bytes;
+};
+inline WeightsPlan weights_plan(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count) {
+  WeightsPlan p{};
+  p.n16 = T * group / 16 + nseq;
+  p.kept_bytes = p.n16 * kv_heads * kCountKept;
+  // One workgroup to a CU at once, two rounds of them.
+  const int64_t pairs = (int64_t)nseq * kv_heads, want = 2 * (int64_t)cu_count;
+  const int64_t many = (want + pairs - 1) / pairs;
+  // sequences at a time that a grid's 32-bit thread count takes, and 512 MiB of ranges' sums
+  const int64_t ranges = kMaxScratch / (8 * kCountBlock * 4);
+  p.cut = T * group / nseq >= 128 && many * kv_heads <= ranges;
+  const int64_t blocks = (std::max<int64_t>(most, 1) + kCountBlock - 1) / kCountBlock;
+  p.across = (int)std::max<int64_t>(1, std::min(p.cut ? want : blocks, many));
+  p.seqs = (int)std::min<int64_t>(
+      nseq, std::max<int64_t>(1, (p.cut ? ranges : int64_t(1) << 22) / ((int64_t)p.across * kv_heads)));
+  if (p.cut) p.scratch_bytes = (int64_t)p.seqs * kv_heads * 8 * p.across * kCountBlock * 4;
+  return p;
+}
+
+// Eviction (sdq_kv_evict.hip). Tables longer than a workgroup's registers: chunks of whole times
+// 16384 tokens, at most 64 of them, and fewer where the cached heads are so many that a sequence's
+// counts would pass 256 MiB (from 171 heads on; one chunk has 24.1 KiB a head).
+constexpr int kEvictRegisters = 16384;  // tokens
+constexpr int64_t kEvictCounts = 3 * 2048 * 4, kEvictFound = 3 * 32, kEvictScratch = int64_t(1) << 28;
+struct EvictPlan {
+  int seqs;       // sequences at a time
+  int chunks;     // of a sequence, 0: it fits a workgroup
+  int64_t chunk;  // tokens
+  int64_t scratch_bytes;
+};
+inline EvictPlan evict_plan(int nseq, int kv_heads, int64_t most) {
+  EvictPlan p{};
+  p.seqs = std::max(1, (1 << 21) / kv_heads);  // a grid's threads are a 32-bit number
+  if (most > kEvictRegisters) {
+    const int64_t fit = (kEvictScratch / kv_heads - kEvictFound) / kEvictCounts;
+    const int64_t chunks =
+        std::max<int64_t>(1, std::min<int64_t>({64, (1 << 20) / kv_heads, fit}));
+    p.chunk = ((most + chunks - 1) / chunks + kEvictRegisters - 1) / kEvictRegisters * kEvictRegisters;
+    p.chunks = (int)((most + p.chunk - 1) / p.chunk);
+    const int64_t pair = p.chunks * kEvictCounts + kEvictFound;
+    p.seqs = (int)std::max<int64_t>(1, std::min<int64_t>(kEvictScratch / (pair * kv_heads),
+                                                         (1 << 20) / ((int64_t)p.chunks * kv_heads)));
+    p.seqs = std::min(p.seqs, nseq);
+    p.scratch_bytes = pair * kv_heads * p.seqs;
+  }
   return p;
 }
 

@@ -21,6 +21,7 @@
 #include <algorithm>
 
 #include "sdq_kv_attn.h"
+#include "sdq_kv_plan.h"
 
 #pragma clang fp contract(off)
 
@@ -34,6 +35,7 @@ constexpr int kTiles = 4;                     // of 16 keys, a wave
 constexpr int kBlock = 16 * kTiles * kWaves;  // keys of a workgroup
 constexpr int kRows = 64;                     // of a stage in LDS
 constexpr int kRing = 3;
+static_assert(kBlock == kvplan::kCountBlock && kQTile + 16 * sizeof(RowInfo) == kvplan::kCountKept);
 constexpr int kLeastLog = 10;                 // of a range's rows (2^8 157 us, 2^12 223, see above)
 constexpr int kShortLog = 7;                  // the same where there are workgroups to spare
 constexpr int kDma = 5;                       // a wave's, a stage: 4 of the parts, one of the rest
@@ -308,23 +310,7 @@ __global__ void __launch_bounds__(kBlock) kv_weights_join_kernel(Args a, Work wk
 
 }  // namespace
 
-KvWeightsPlan plan_kv_weights(int64_t T, int nseq, int group, int kv_heads, int64_t most, int cu_count) {
-  KvWeightsPlan p{};
-  p.n16 = T * group / 16 + nseq;
-  p.kept_bytes = p.n16 * kv_heads * (kQTile + 16 * (int64_t)sizeof(RowInfo));
-  // One workgroup to a CU at once, two rounds of them.
-  const int64_t pairs = (int64_t)nseq * kv_heads, want = 2 * (int64_t)cu_count;
-  p.cut = T * group / nseq >= 128;
-  const int64_t blocks = ceil_div(std::max<int64_t>(most, 1), kBlock);
-  p.across = (int)std::max<int64_t>(1, std::min(p.cut ? want : blocks, ceil_div(want, pairs)));
-  // sequences at a time that a grid's 32-bit thread count takes, and 512 MiB of ranges' sums
-  p.seqs = (int)std::min<int64_t>(
-      nseq, std::max<int64_t>(1, (int64_t(1) << (p.cut ? 15 : 22)) / ((int64_t)p.across * kv_heads)));
-  if (p.cut) p.scratch_bytes = (int64_t)p.seqs * kv_heads * 8 * p.across * kBlock * 4;
-  return p;
-}
-
-hipError_t launch_kv_weights(const View& c, const KvRows& r, const KvWeightsPlan& p, void* kept, float* w,
+hipError_t launch_kv_weights(const View& c, const KvRows& r, const kvplan::WeightsPlan& p, void* kept, float* w,
                              void* scratch, hipStream_t s) {
   Args a{};
   a.heads = r.heads, a.group = r.heads / c.kv_heads;

@@ -1,11 +1,11 @@
-"""The paged cache's operators at the ends of their ranges: logits past fp32, against the
-definitions in 64 bits. Tolerances as in tests/test_gpu_kv_more.py."""
+"""The paged cache's operators at the ends of their ranges: logits past fp32, long chunks and many
+heads, against the definitions in 64 bits. Tolerances as in tests/test_gpu_kv_more.py."""
 import numpy as np
 import pytest
 
 from conftest import assert_bitexact
 from test_gpu_kv_cache import F, HD
-from test_gpu_kv_more import More
+from test_gpu_kv_more import More, _weights
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,55 @@ def test_weights_of_a_huge_scale(sdq_dev, new):
     want = 2 * new / 700
     # logits within 1e-45 * 127 * 128 * 3e37 * 10 * log2(e) < 0.01 of 0, the others' exactly 0 here
     assert (np.abs(got - want) <= 0.01 * want).all(), (got.min(), got.max(), want)
+
+
+# ---- eviction: chunks of more tokens than a workgroup's registers, and many heads ----
+
+@pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
+def test_evict_longer_chunks(sdq_dev, kind):
+    """A table of 2^22 tokens, most of it unused: chunks of 65536, read in several rounds."""
+    c = More(sdq_dev, [0] * 3, [150001, 65536, 70000], 2, 256, seed=47)
+    table = np.full((3, 1 << 14), -1, np.int32)
+    table[:, :c.most] = c.table
+    c.table, c.most = table, 1 << 14
+    c.up()
+    c.check_evict(_weights(c, kind), 20000, 3, 100)
+
+
+class Sparse(More):
+    def evict64(self, w, keep, first, last):
+        """More.evict64 where few tokens have a page."""
+        kept = np.full((len(self.lens), self.kvh, keep), -1, np.int32)
+        lens = np.zeros(len(self.lens), np.int32)
+        for s, L in enumerate(self.lens):
+            pages = np.flatnonzero((self.table[s] >= 0) & (self.table[s] < self.pages))
+            p = (pages[:, None] * self.page + np.arange(self.page)).ravel()
+            p = p[p < L]
+            lens[s] = min(keep, len(p))
+            must = (p < first) | (p >= L - last)
+            x = w[self.table[s, p // self.page], :, p % self.page].astype(np.float64)
+            for h in range(self.kvh):
+                order = np.lexsort((p, np.where(must, 0, -x[:, h]), ~must))[:keep]
+                kept[s, h, :len(order)] = np.sort(p[order])
+        return kept, lens
+
+
+def test_evict_many_heads(sdq_dev):
+    """1024 cached heads over a table of 2^20 tokens: fewer and longer chunks, and scratch of no more
+    than 256 MiB."""
+    import torch
+
+    c = Sparse(sdq_dev, [0, 0], [90, 40], 1024, 16, seed=48)
+    table = np.full((2, 1 << 16), -1, np.int32)
+    for s, at in ((0, [0, 1, 1023, 1024, 9000, 20001]), (1, [0, 7168, 14336])):  # tokens far apart
+        table[s, at] = c.table[s, :len(at)]
+    c.table, c.most, c.lens = table, 1 << 16, [20001 * 16 + 10, 14336 * 16 + 3]
+    c.up()
+    w = _weights(c, "ties")
+    with torch.cuda.stream(torch.cuda.Stream()):  # a workspace of its own
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0] + torch.cuda.memory_reserved()
+        c.check_evict(w, 33, 2, 15)
+        torch.cuda.synchronize()
+        used = before - torch.cuda.mem_get_info()[0] - torch.cuda.memory_reserved()
+    assert used <= 2**28 + 2**24, used
