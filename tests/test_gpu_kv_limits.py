@@ -1,11 +1,12 @@
 """The paged cache's operators at the ends of their ranges: logits past fp32, long chunks and many
-heads, against the definitions in 64 bits. Tolerances as in tests/test_gpu_kv_more.py."""
+heads, and calls that the host cuts into several launches (cached heads, sequences or rows at a time), against
+the definitions in 64 bits. Tolerances as in tests/test_gpu_kv_more.py."""
 import numpy as np
 import pytest
 
 from conftest import assert_bitexact
 from test_gpu_kv_cache import F, HD
-from test_gpu_kv_more import More, _weights
+from test_gpu_kv_more import More, _weights, soft
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +107,163 @@ def test_evict_many_heads(sdq_dev):
         torch.cuda.synchronize()
         used = before - torch.cuda.mem_get_info()[0] - torch.cuda.memory_reserved()
     assert used <= 2**28 + 2**24, used
+
+
+# ---- calls of several launches ----
+
+def _shared_case(dev, new, lens, kvh, s_start, parts, seed):
+    c = More(dev, new, lens, kvh, 16, seed=seed, first=1, behind=1)
+    c.share(s_start, parts)
+    return c
+
+
+def _check_shared_rows(c, heads, places):
+    """kv_attention_shared, causal, at (sequence, its row, query head)."""
+    import torch
+
+    g = torch.Generator(device=c.dev).manual_seed(c.T)
+    q = torch.randn((c.T, heads * HD), generator=g, device=c.dev).mul_(1.5)
+    out = torch.full((c.T, heads * HD), -3.0, device=c.dev)
+    c.sdq.kv_attention_shared(c.cache, c.shared, c.batch, q, out, heads)
+    assert (out[0] == -3).all() and (out[-1] == -3).all()
+    assert bool(torch.isfinite(out).all())
+    for s, r, h in places:
+        kh, n = h // (heads // c.kvh), c.new[s]
+        k, v, ok = c.values(s, kh)
+        pk, pv, pok = c.part(s, kh)
+        see = np.concatenate([pok, ok & (np.arange(len(k)) <= len(k) - n + r)])[None]
+        at = c.start[s] + r, slice(h * HD, (h + 1) * HD)
+        want, tol, _, _ = soft(q[at].cpu().numpy()[None], np.concatenate([pk, k]),
+                               np.concatenate([pv, v]), see, HD**-0.5)
+        c.close(out[at].cpu().numpy()[None], want, tol)
+
+
+@pytest.mark.parametrize("nseq,new,parts", [(2, 8500, [300, 4099]), (1000, 17, [2050, 0, 33])])
+def test_shared_heads_at_a_time(sdq_dev, nseq, new, parts):
+    """More rows than 512 MiB of shares hold for all heads: seven of eight cached heads, then one."""
+    rng = np.random.default_rng(nseq)
+    rows = [new] * nseq if nseq < 3 else list(rng.integers(new - 3, new + 4, nseq))
+    lens = [int(n + rng.integers(0, 60)) for n in rows]
+    s_start = [0, 1, 2] if nseq < 3 else [0, 500, 600, 990]
+    c = _shared_case(sdq_dev, rows, lens, 8, s_start, parts, seed=42)
+    assert 7 * sum(rows) * 4 * 2 * 520 <= 2**29 < 8 * sum(rows) * 4 * 2 * 520
+    places = [(s, r, h) for s in (0, nseq // 2, nseq - 1) for r in (0, rows[s] // 2, rows[s] - 1)
+              for h in (0, 1, 26, 27, 28, 31)]
+    _check_shared_rows(c, 32, places)
+
+
+def test_shared_rows_of_one_head(sdq_dev):
+    """Query heads of one cached head, more than 2^22 rows: the join takes several launches."""
+    rng = np.random.default_rng(3)
+    rows = list(rng.integers(60, 141, 1400))
+    c = _shared_case(sdq_dev, rows, [int(n + rng.integers(0, 20)) for n in rows], 1, [0, 700, 1390],
+                     [60, 17], seed=43)
+    assert sum(rows) * 32 > 2**22
+    places = [(s, r, h) for s in (0, 699, 700, 1300, 1395, 1399) for r in (0, rows[s] - 1) for h in (0, 31)]
+    _check_shared_rows(c, 32, places)
+
+
+def test_weights_sequences_at_a_time(sdq_dev):
+    """More pairs of a sequence and cached head than a grid takes: 512 sequences of 64 heads, then the
+    others, long ones (whose rows are cut into ranges) on both sides."""
+    import torch
+
+    nseq, kvh, G = 516, 64, 2
+    new = [64] * nseq
+    for s in (0, 511, 512, 515):
+        new[s] = 1100
+    new[514] = 0
+    lens = [n + 9 if s % 2 else n for s, n in enumerate(new)]
+    need = [-(-n // 32) for n in lens]
+    pages = sum(need) + 1
+    g = torch.Generator(device=sdq_dev).manual_seed(44)
+    codes = lambda: torch.randint(-127, 128, (pages, kvh, 32, HD), generator=g, device=sdq_dev,  # noqa: E731
+                                  dtype=torch.int8)
+    rand = lambda *s: torch.rand(s, generator=g, device=sdq_dev)  # noqa: E731
+    c = More(sdq_dev, [1], [1], 1, 16)  # the definitions' home
+    cache = c.sdq.KvCache(codes(), 0.012 * (0.5 + rand(pages, kvh, 32)), codes(),
+                          0.02 * (0.5 + rand(pages, kvh, 32)))
+    table = np.full((nseq, max(need)), -1, np.int32)
+    ids = np.random.default_rng(44).permutation(pages)
+    at = 0
+    for s, n in enumerate(need):
+        table[s, :n] = ids[at:at + n]
+        at += n
+    start = np.concatenate([[0], np.cumsum(new)])
+    T = int(start[-1])
+    batch = c.sdq.KvBatch(c.t(start.astype(np.int32)), c.t(np.array(lens, np.int32)), c.t(table))
+    q = torch.randn((T, kvh * G * HD), generator=g, device=sdq_dev).mul_(1.5)
+    w = rand(pages, kvh, 32)
+    before = w.clone()
+    out = torch.empty_like(q)
+    c.sdq.kv_attention_weights(cache, batch, w, q, out, kvh * G)
+    assert bool(torch.isfinite(w).all())
+    assert torch.equal(w[ids[-1]], before[ids[-1]])  # no sequence's page
+    same = torch.empty_like(q)
+    c.sdq.kv_attention(cache, batch, q, same, kvh * G)
+    assert torch.equal(out, same)
+    for s in (0, 1, 300, 511, 512, 513, 515):
+        n, L = new[s], lens[s]
+        p = np.arange(L)
+        see = p[None] <= (L - n + np.arange(n))[:, None]
+        for h in (0, 31, 63):
+            pg, slot = torch.from_numpy(table[s, p // 32].astype(np.int64)), torch.from_numpy(p % 32)
+            host = lambda t: t[pg.to(sdq_dev), h, slot.to(sdq_dev)].cpu().numpy().astype(np.float64)  # noqa: E731
+            k, v = host(cache.k) * host(cache.ks)[:, None], host(cache.v) * host(cache.vs)[:, None]
+            total, off = np.zeros(L), np.zeros(L)
+            for j in range(G * h, G * h + G):
+                x = q[start[s]:start[s + 1], j * HD:(j + 1) * HD].cpu().numpy()
+                _, _, wt, rel = soft(x, k, v, see, HD**-0.5)
+                total += wt.sum(0)
+                off += (wt * rel).sum(0)
+            total += np.where(p < L - n, host(before), 0)
+            c.close(host(w), total, off + (n * G / 16 + 16) * 2.0**-24 * total + 1e-37)
+
+
+def test_evict_long_sequences_at_a_time(sdq_dev):
+    """Tables of 2^20 tokens, nearly all unused, of 64 heads: two sequences of three at a time."""
+    c = More(sdq_dev, [0] * 3, [3000, 17000, 700], 64, 256, seed=45)
+    table = np.full((3, 4096), -1, np.int32)
+    table[:, :c.most] = c.table
+    c.table, c.most = table, 4096
+    c.up()
+    w = np.exp(2 * c.rng.standard_normal((c.pages, 64, 256))).astype(F)
+    c.check_evict(w, 500, 3, 40)
+
+
+def test_evict_sequences_at_a_time(sdq_dev):
+    """33000 sequences of 64 heads, the same few pages' tokens: 32768 of them, then the others."""
+    import torch
+
+    nseq, kvh, keep = 33000, 64, 6
+    c = More(sdq_dev, [0] * 5, [16, 9, 0, 31, 6], kvh, 16, seed=46)
+    w = c.rng.integers(0, 4, (c.pages, kvh, 16)).astype(F)
+    want, want_lens = c.evict64(w, keep, 1, 2)
+    which = np.random.default_rng(46).integers(0, 5, nseq)
+    i32 = lambda a: c.t(np.asarray(a, np.int32))  # noqa: E731
+    batch = c.sdq.KvBatch(i32(np.zeros(nseq + 1)), i32(np.array(c.lens)[which]), i32(c.table[which]))
+    free = 10
+    shape = (c.pages + free, kvh, 16)
+    pool = c.sdq.KvCache.empty(shape[0], 16, kvh)
+    for name in ("k", "v", "ks", "vs"):
+        getattr(pool, name).zero_()
+        getattr(pool, name)[:c.pages] = getattr(c.cache, name)
+    tw = torch.zeros(shape, device=sdq_dev)
+    tw[:c.pages] = c.t(w)
+    # most go nowhere; ten sequences on either side of the launches' border have a page
+    live = [0, 1, 2, 32766, 32767, 32768, 32769, 32770, 32998, 32999]
+    to = np.full((nseq, 1), -1, np.int32)
+    to[live, 0] = c.pages + np.arange(free)
+    lens = torch.full((nseq,), -9, dtype=torch.int32, device=sdq_dev)
+    kept = torch.full((nseq, kvh, keep), -9, dtype=torch.int32, device=sdq_dev)
+    c.sdq.kv_evict(pool, batch, tw, i32(to), lens, kept, first=1, last=2)
+    assert_bitexact(lens.cpu().numpy(), want_lens[which], "lens")
+    assert_bitexact(kept.cpu().numpy(), want[which], "kept")
+    for i, s in enumerate(live):
+        n, src = want_lens[which[s]], which[s]
+        for h in (0, 63):
+            pos = want[src, h, :n]
+            at = c.table[src, pos // 16], h, pos % 16
+            for got, x in ((pool.k, c.k), (pool.vs, c.vs), (tw, w)):
+                assert_bitexact(got[c.pages + i, h, :n].cpu().numpy(), x[at])
+    assert torch.equal(tw[:c.pages], c.t(w))
