@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(256) kv_attn_join_rows_kernel(Args a, int64_t 
   // a row without a position sees nothing; a sequence without a shared part has none of its shares
 #pragma unroll
   for (int j = 0; j < 2; j++)
-    if (t.first < 0 || (t.part < 0 && l + 64 * j < a.z0)) ml[j].x = -INFINITY;
+    if (t.first < 0 || (t.part < 0 && l + 64 * j < a.z0)) ml[j] = float2{-INFINITY, 0.f};
   float m = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -517,9 +517,11 @@ __global__ void __launch_bounds__(256) kv_attn_join_rows_kernel(Args a, int64_t 
   uint64_t live[2];
 #pragma unroll
   for (int j = 0; j < 2; j++) {
-    live[j] = __ballot(ml[j].x != -INFINITY);
+    // a share whose only keys have logits of NaN has no maximum, but a denominator
+    const bool has = ml[j].x != -INFINITY || ml[j].y != 0.f;
+    live[j] = __ballot(has);
     own[j] = __builtin_amdgcn_exp2f(ml[j].x - ref);
-    den += ml[j].x != -INFINITY ? times_exp2(ml[j].y, ml[j].x - ref) : 0.f;
+    den += has ? times_exp2(ml[j].y, ml[j].x - ref) : 0.f;
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) den += __shfl_xor(den, o);

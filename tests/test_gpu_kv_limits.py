@@ -57,6 +57,42 @@ def test_weights_of_a_huge_scale(sdq_dev, new):
     assert (np.abs(got - want) <= 0.01 * want).all(), (got.min(), got.max(), want)
 
 
+# ---- keys whose scale is no number ----
+
+@pytest.mark.parametrize("new", [1, 40, 300])
+@pytest.mark.parametrize("where", ["own", "part"])
+@pytest.mark.parametrize("scale", [np.nan, np.inf])
+def test_shared_bad_scale(sdq_dev, new, where, scale):
+    """A key whose scale is NaN makes the rows NaN that see it, be it alone in its part or among the
+    rows' own keys: as kv_attention of the same tokens through one table. An infinite one does where the
+    logit is not -infinity."""
+    c = More(sdq_dev, [new, new], [new if where == "part" else 1, new + 3], 2, 16, seed=49)
+    c.share([0, 1, 2], [16, 16])
+    if where == "own":
+        c.table[0, 1:] = -1
+        c.ks[c.table[0, 0], :, 0] = scale
+    else:  # alone: the other fifteen have no page
+        c.s_lens[0] = 1
+        c.ks[c.s_table[0, 0], :, 0] = scale
+    c.up_shared()
+    q = c.queries(4)
+    key = (c.k[c.table[0, 0], :, 0] if where == "own" else c.k[c.s_table[0, 0], :, 0]).astype(np.float64)
+    got, same = (c.torch.full((c.T, 512), -3.0, device=c.dev) for _ in range(2))
+    c.sdq.kv_attention_shared(c.cache, c.shared, c.batch, c.t(q), got, 4)
+    got = got.cpu().numpy().reshape(-1, 4, HD)
+    for r in range(new):
+        placed = c.lens[0] - new + r >= 0
+        for h in range(4):
+            dot = q[r, h * HD:(h + 1) * HD].astype(np.float64) @ key[h // 2]
+            lost = placed and (np.isnan(scale) or dot >= 0)
+            assert np.isnan(got[r, h]).all() if lost else np.isfinite(got[r, h]).all(), (r, h, dot)
+    c.s_lens[0] = 0 if where == "part" else 16
+    c.ks[~np.isfinite(c.ks)] = F(0.01)
+    c.up_shared()
+    c.sdq.kv_attention_shared(c.cache, c.shared, c.batch, c.t(q), same, 4)
+    assert_bitexact(got.reshape(-1, 512)[new:], same.cpu().numpy()[new:], "the other sequence")
+
+
 # ---- eviction: chunks of more tokens than a workgroup's registers, and many heads ----
 
 @pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
