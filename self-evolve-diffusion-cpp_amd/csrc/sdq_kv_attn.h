@@ -50,13 +50,10 @@ struct Rest : Own {  // own keys behind shared ones
   static constexpr bool kByRow = true, kRest = true;
 };
 
-// A row that adds nothing has qk = 0 too: its logits, formed again, are then finite (one past
-// fp32's range less the infinite maximum would be NaN).
 struct RowInfo {
   float qk, m, inv;
   int see;  // keys; 0: the row adds nothing
 };
-constexpr RowInfo kNoRow{0.f, INFINITY, 0.f, 0};
 constexpr int kQTile = 8192;  // bytes of a tile's parts
 
 struct Args {
@@ -567,11 +564,8 @@ __device__ __forceinline__ int64_t tile16(const Args& a, const Tile& t, int h, i
 __device__ __forceinline__ RowInfo info_of(const Args& a, const Tile& t, int64_t r, float qk, float m,
                                            float den) {
   const float2 st = stat_of(m, den);
-  return st.y > 0.f ? RowInfo{qk, st.x, st.y, keys_of(t, r, a.group, a.causal)} : kNoRow;
-}
-// Of a row whose shares are joined later (which fills in the rest), or that is none.
-__device__ __forceinline__ RowInfo unjoined(float qk, bool row) {
-  return RowInfo{row ? qk : 0.f, INFINITY, 0.f, 0};
+  const int see = st.y > 0.f ? keys_of(t, r, a.group, a.causal) : 0;
+  return RowInfo{qk, st.x, st.y, see};
 }
 // The wave's 16 rows from r0 on: their parts, as the lanes hold them.
 __device__ __forceinline__ void keep_parts(const Args& a, const Tile& t, int h, int64_t r0,

@@ -172,7 +172,7 @@ __device__ __forceinline__ void few_rows(const Args& a, unsigned wg) {
     keep_parts(a, t, h, t.r0, qh, ql);
     // a row that is none, or whose shares are joined later
     if (g == 0 && (a.splits > 1 || t.r0 + r16 >= t.rows))
-      a.info[tile16(a, t, h, t.r0) * 16 + r16] = unjoined(qk, t.r0 + r16 < t.rows);
+      a.info[tile16(a, t, h, t.r0) * 16 + r16] = RowInfo{qk, INFINITY, 0.f, 0};
     if (g == 0) qks[r16] = qk;
   }
 
@@ -651,7 +651,7 @@ __device__ __forceinline__ void chunk_rows(const Args& a, unsigned wg) {
       keep_parts(a, t, h, t.r0 + (w * QT + qt) * 16, qh[qt], ql[qt]);
       const int64_t r0 = t.r0 + (w * QT + qt) * 16;
       if (g == 0 && r0 < t.rows && (a.splits > 1 || r >= t.rows))
-        a.info[tile16(a, t, h, r0) * 16 + r16] = unjoined(qk[qt], r < t.rows);
+        a.info[tile16(a, t, h, r0) * 16 + r16] = RowInfo{qk[qt], INFINITY, 0.f, 0};
     }
   }
   const int e0 = exp_of(v0);

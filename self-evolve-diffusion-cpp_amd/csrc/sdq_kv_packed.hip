@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv_attn_packed_kernel(Args a, 
       keep_parts(a, t, h, t.r0 + r_half + (w * QT + qt) * 16, qh[qt], ql[qt]);
       const int64_t r0 = t.r0 + r_half + (w * QT + qt) * 16;
       if (g == 0 && r0 < t.rows && (a.splits > 1 || r >= t.rows))
-        a.info[tile16(a, t, h, r0) * 16 + r16] = unjoined(qk[qt], r < t.rows);
+        a.info[tile16(a, t, h, r0) * 16 + r16] = RowInfo{qk[qt], INFINITY, 0.f, 0};
     }
   }
   const int e0 = exp_of(v0);

@@ -190,7 +190,10 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
             op[kb & 1][part] = *reinterpret_cast<const v8h*>(d.q[tile] + 4096 * part + 1024 * kb + l * 16);
         };
         to.ri = d.row[16 * nx + r16];
-        if (!live) to.ri = kNoRow;
+        if (!live) to.ri.m = INFINITY, to.ri.inv = 0.f, to.ri.see = 0;
+        // A row that adds nothing: its logits are formed as 0, since one past fp32's range, less the
+        // infinite maximum, would be NaN.
+        if (to.ri.inv == 0.f) to.ri.qk = 0.f;
         if (kMask || nx == 0) read(nx, 0);  // masked tiles may be left out
 #pragma unroll
         for (int kb = 0; kb < 4; kb++) {
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(64 * kWaves) kv_weights_kernel(Args a, Work wk
         Scores sc[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {  // before the first tile: adds nothing
-          sc[j].ri = kNoRow;
+          sc[j].ri = RowInfo{0.f, INFINITY, 0.f, 0};
 #pragma unroll
           for (int kt = 0; kt < kTiles; kt++) sc[j].s[kt] = v4f{0.f, 0.f, 0.f, 0.f};
         }
