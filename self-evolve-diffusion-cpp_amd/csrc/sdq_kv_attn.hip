@@ -166,7 +166,7 @@ __device__ __forceinline__ void few_rows(const Args& a, unsigned wg) {
     for (int i = 0; i < 8; i++) x[kb][i] = __builtin_ldexpf(x[kb][i], qe);
     parts8(x[kb], qh[kb], ql[kb]);
   }
-  const float qk = __builtin_ldexpf(a.scale2, -qe);
+  const float qk = bad ? 0.f : __builtin_ldexpf(a.scale2, -qe);
   const int e0 = exp_of(v0);
   if (K::kStats && z == 0 && w == 0) {
     keep_parts(a, t, h, t.r0, qh, ql);
@@ -646,7 +646,7 @@ __device__ __forceinline__ void chunk_rows(const Args& a, unsigned wg) {
       for (int i = 0; i < 8; i++) x[kb][i] = __builtin_ldexpf(x[kb][i], qe);
       parts8(x[kb], qh[qt][kb], ql[qt][kb]);
     }
-    qk[qt] = __builtin_ldexpf(a.scale2, -qe);
+    qk[qt] = bad[qt] ? 0.f : __builtin_ldexpf(a.scale2, -qe);
     if (K::kStats && z == 0) {
       keep_parts(a, t, h, t.r0 + (w * QT + qt) * 16, qh[qt], ql[qt]);
       const int64_t r0 = t.r0 + (w * QT + qt) * 16;

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) kv_attn_packed_kernel(Args a, 
       for (int i = 0; i < 8; i++) x[kb][i] = __builtin_ldexpf(x[kb][i], qe);
       parts8(x[kb], qh[qt][kb], ql[qt][kb]);
     }
-    qk[qt] = __builtin_ldexpf(a.scale2, -qe);
+    qk[qt] = bad[qt] ? 0.f : __builtin_ldexpf(a.scale2, -qe);
     if (K::kStats && z == 0) {
       keep_parts(a, t, h, t.r0 + r_half + (w * QT + qt) * 16, qh[qt], ql[qt]);
       const int64_t r0 = t.r0 + r_half + (w * QT + qt) * 16;

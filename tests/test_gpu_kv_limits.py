@@ -93,6 +93,26 @@ def test_shared_bad_scale(sdq_dev, new, where, scale):
     assert_bitexact(got.reshape(-1, 512)[new:], same.cpu().numpy()[new:], "the other sequence")
 
 
+@pytest.mark.parametrize("new", [1, 40, 70, 300, 1100])
+def test_bad_row_over_an_infinite_scale(sdq_dev, new):
+    """A row of NaN that sees a single key is NaN, also where that key's scale is infinite and what is
+    left of the row would have a logit of -infinity."""
+    c = More(sdq_dev, [new], [1], 1, 16, seed=50)
+    c.share([0, 1], [0])
+    key = c.k[c.table[0, 0], 0, 0]
+    c.ks[c.table[0, 0], 0, 0] = np.inf
+    c.up_shared()
+    q = np.repeat(np.where(key > 0, -1, 1)[None], new, 0).astype(F)
+    q[-1, 5] = np.nan
+    for call in (lambda o: c.sdq.kv_attention(c.cache, c.batch, c.t(q), o, 1),
+                 lambda o: c.sdq.kv_cross_attention(c.cache, c.batch, c.t(q), o, 1),
+                 lambda o: c.sdq.kv_attention_shared(c.cache, c.shared, c.batch, c.t(q), o, 1)):
+        out = c.torch.full((new, HD), -3.0, device=c.dev)
+        call(out)
+        got = out.cpu().numpy()
+        assert np.isnan(got[-1]).all() and (got[:-1] == 0).all()
+
+
 # ---- eviction: chunks of more tokens than a workgroup's registers, and many heads ----
 
 @pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
