@@ -546,8 +546,9 @@ typedef struct sdq_kv_shared {
  * a position among its own tokens sees nothing and gets 0. A part's keys are read once for
  * all of its sequences' rows together. The range of value scales counts from the shared
  * part's first token (the sequence's own where that part is empty). Scratch from the
- * stream's workspace in every call, 1040 bytes and up for a row and head (of as many heads
- * at a time as 512 MiB take): a capture needs one call of the same shape before it.
+ * stream's workspace in every call, 1040 bytes and up for a row and head, of as many cached
+ * heads at a time as 512 MiB take, one at least: a capture needs one call of the same shape
+ * before it.
  * out overlaps none of shared's arrays either. */
 int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, const sdq_kv_batch* b,
                             const float* q, int64_t ldq, float* out, int64_t ldo, int64_t T,
@@ -562,8 +563,9 @@ int sdq_kv_attention_shared(const sdq_kv_cache* c, const sdq_kv_shared* shared, 
  * weights: device memory of the caller, [pages, kv_heads, page_size] f32 as the cache's
  * scales, with a float's alignment; it overlaps no other array. fp32 sums, each row's weights
  * added in a fixed order: the same bits every time. Rows whose softmax is no number (a NaN or an
- * infinity in q, in the scale of a key that they see, a logit past fp32's range) add nothing. No page may stand twice in the
- * tables of the call's sequences (sums would be lost in part). Scratch from the stream's
+ * infinity in q, in the scale of a key that they see, a logit past fp32's range) add nothing.
+ * No page may stand twice in the tables of the call's sequences (sums would be lost in part);
+ * out overlaps the weights as little as what sdq_kv_attention names. Scratch from the stream's
  * workspace in every call (a capture needs one call of the same shape before it): up to 32 rows
  * of q a sequence and cached head, on average, their logits, if they fit 512 MiB, else 528 bytes a
  * row of q and head, and what sdq_kv_cross_attention takes. */

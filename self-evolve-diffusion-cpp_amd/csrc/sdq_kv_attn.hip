@@ -914,8 +914,9 @@ __device__ __forceinline__ void tile_rows(const Args& a, unsigned wg) {
 // Shared parts and own keys in one launch, the parts' `shared` workgroups first: the own keys'
 // are short and fill what those leave (16 tokens of 24 heads behind 4099 shared keys 20 us, two
 // launches 16 + 9; 297 rows behind 8209 and 5026 125, 123 + 20). 128 rows a part and head:
-// bound by the products and the softmax beside them, 131073 keys x 8 heads 183 us of 116 at a large
-// library product's rate; turning the keys to fp16 is shared by half as many rows as in the chunks
+// 131073 keys x 8 heads 183 us of 116 at a large library product's rate. Vector operations take 57% of
+// the cycles (the softmax, turning the keys), the products 39%; waves wait for a counter or barrier 30%
+// of their life; turning the keys to fp16 is shared by half as many rows as in the chunks
 // of 256. Blocks on their way in LDS by LDS-DMA, four of them, made it slower (220 us): what they
 // cost in LDS reads is more than the loads' latency.
 template <int PR, int OR>

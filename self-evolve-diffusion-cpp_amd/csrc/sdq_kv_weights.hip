@@ -15,9 +15,10 @@
 // the exponentials of the last ones. Few blocks of many rows are cut into ranges of
 // rows, whose sums a second kernel adds up in order: no atomics, the same bits every time.
 //
-// 4099 rows over themselves, 24 heads on 8: 138 us and 4.5 of the join, where the products are 87
+// 4099 rows over themselves, 24 heads on 8: 139 us and 4.6 of the join, where the products are 87
 // at a large library product's rate; the exponentials beside them and the diagonal's half-used
-// blocks are the rest.
+// blocks are the rest (CUs busy 85% of the time, the matrix units 42% of that, waves waiting for a
+// counter or barrier 38% of their life).
 #include <algorithm>
 
 #include "sdq_kv_attn.h"
