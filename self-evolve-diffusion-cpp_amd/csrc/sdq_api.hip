@@ -2622,7 +2622,7 @@ int sdq_kv_attention_weights(const sdq_kv_cache* c, const sdq_kv_batch* b, float
   }
   const kvplan::WeightsPlan wplan =
       kvplan::weights_plan(T, call.view.nseq, heads / c->kv_heads, c->kv_heads,
-                      call.view.max_pages << call.view.page_log2, cus);
+                           call.view.max_pages << call.view.page_log2, cus);
   // the shares' sums or, once they are joined, the ranges', the rows' parts and statistics, and
   // the keys as operands
   const size_t kept_at = (size_t)round_up(std::max(plan.scratch_bytes, wplan.scratch_bytes), 16);

@@ -8,15 +8,14 @@
 // the softmax only, and there is room to put a block's exponentials beside the next block's
 // scores, and the next block's logits beside this one's sums: neither waits for the other.
 //
-// 24 heads: 27280 rows over 512 keys 419 us (8 of them the pass), 509 in chunks, in turn on one box
-// (385 to 422 on others); 2048 rows over 4099
-// 254 and 288, 8192 over 4099 709 and 720, 1024 over 4099 162 and 158, over 512 39 and 45: taken
-// from 1024 rows a sequence on. Bound by the matrix units and the softmax beside them: 8192 rows
-// over as many keys at 1.17 PFLOP/s, the rate of a large library product. Over 512 keys the matrix
-// units are busy 42% of the cycles and the vector units 49%, waves wait for a counter or barrier 29% of
-// their life and for their turn to issue 33%; what
-// stands beside the loop, 670 MB of queries and output, is not overlapped with it. A tile is two
-// workgroups of four waves, two workgroups a CU: eight waves at one ring were slower.
+// 24 heads: 27280 rows over 512 keys 419 us (8 of them the pass), 509 in chunks, in turn on one card
+// (385 to 422 on others); 2048 rows over 4099 254 and 288, 8192 over 4099 709 and 720, 1024 over
+// 4099 162 and 158, over 512 39 and 45: taken from 1024 rows a sequence on. Bound by the matrix
+// units and the softmax beside them: 8192 rows over as many keys at 1.17 PFLOP/s, the rate of a
+// large library product. Over 512 keys the matrix units are busy 42% of the cycles and the vector
+// units 49%, waves wait for a counter or barrier 29% of their life and for their turn to issue 33%;
+// what stands beside the loop, 670 MB of queries and output, is not overlapped with it. A tile is
+// two workgroups of four waves, two workgroups a CU: eight waves at one ring were slower.
 #include <algorithm>
 
 #include "sdq_kv_attn.h"
